@@ -26,6 +26,14 @@ GLA_KV_F32 = 0
 GLA_KV_Q8_0 = 1
 GLA_PREC_F32 = 0
 GLA_PREC_BF16 = 1
+GLA_ROPE_INTERLEAVED = 0
+GLA_ROPE_HALF = 1
+GLA_ROPE_NONE = 0
+GLA_ROPE_LINEAR = 1
+GLA_ROPE_BANDS = 2
+GLA_ROPE_YARN = 3
+GLA_Q4_0 = 0
+GLA_Q4_K = 1
 
 # GlintError variant each status code stands for (src/error.rs:41-52, :78-82).
 ERROR_NAMES = {
@@ -89,6 +97,46 @@ class PrefillArgs(C.Structure):
     ]
 
 
+class RopeSpec(C.Structure):
+    _fields_ = [
+        ("head_dim", C.c_int),
+        ("rot_dim", C.c_int),
+        ("freq_dim", C.c_int),
+        ("layout", C.c_int),
+        ("scaling", C.c_int),
+        ("original_ctx", C.c_int),
+        ("freq_base", C.c_double),
+        ("factor", C.c_double),
+        ("low", C.c_double),
+        ("high", C.c_double),
+        ("amplitude", C.c_double),
+        ("divisors", C.c_void_p),
+    ]
+
+
+class AppendArgs(C.Structure):
+    _fields_ = [
+        ("kv", C.c_void_p),
+        ("layer", C.c_int),
+        ("n_seqs", C.c_int),
+        ("seq_slot", C.c_void_p),
+        ("page_table", C.c_void_p),
+        ("page_table_stride", C.c_int),
+        ("q_start", C.c_void_p),
+        ("pos_offset", C.c_void_p),
+        ("max_q_len", C.c_int),
+        ("rope", C.c_void_p),
+        ("k", C.c_void_p),
+        ("k_stride", C.c_int64),
+        ("v", C.c_void_p),
+        ("v_stride", C.c_int64),
+        ("q", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("q_out", C.c_void_p),
+        ("n_heads", C.c_int),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/glint_attn.h declares.
 _P = C.c_void_p
 _I = C.c_int
@@ -115,6 +163,7 @@ SIGNATURES = {
     "gla_kv_row_id": (_I64, [_P, _I, _I, _I]),
     "gla_kv_write_rows": (_I, [_P, _P, _P, _P, _P, _I]),
     "gla_kv_write_rows_host": (_I, [_P, _P, _P, _P, _P, _I]),
+    "gla_kv_read_rows": (_I, [_P, _P, _P, _P, _P, _I]),
     "gla_kv_export_rows_host": (_I, [_P, _P, _P, _I, _P, _P]),
     "gla_kv_import_rows_host": (_I, [_P, _P, _P, _I, _P, _P]),
     "gla_kv_row_bytes": (_I64, [_P]),
@@ -132,6 +181,16 @@ SIGNATURES = {
     "gla_q8w_rows": (_I, [_P]),
     "gla_q8w_cols": (_I, [_P]),
     "gla_matvec_q8_0": (_I, [_P, _P, _P, _I, _P]),
+    "gla_rope_freqs": (_I, [C.POINTER(RopeSpec), _P, _P]),
+    "gla_rope_plan_create": (_I, [_P, C.POINTER(RopeSpec), C.POINTER(_P)]),
+    "gla_rope_plan_destroy": (_I, [_P]),
+    "gla_rope_rows": (_I, [_P, _P, _P, _I64, _P, _I64, _I, _I, _P]),
+    "gla_kv_append": (_I, [_P, C.POINTER(AppendArgs)]),
+    "gla_q4w_create": (_I, [_P, _I, _P, _I, _I, C.POINTER(_P)]),
+    "gla_q4w_destroy": (_I, [_P]),
+    "gla_q4w_rows": (_I, [_P]),
+    "gla_q4w_cols": (_I, [_P]),
+    "gla_matvec_q4": (_I, [_P, _P, _P, _I, _P]),
 }
 
 _lib = None

@@ -107,6 +107,10 @@ class _KvBase:
     def write_rows_device(self, rows: DeviceBuffer, k: DeviceBuffer, v: DeviceBuffer, n_rows: int) -> None:
         check(_lib.lib().gla_kv_write_rows(self.backend.ctx, self.handle, rows.ptr, k.ptr, v.ptr, n_rows))
 
+    def read_rows_device(self, rows: DeviceBuffer, k: DeviceBuffer, v: DeviceBuffer, n_rows: int) -> None:
+        """The f32 values the storage holds of rows (gla_kv_read_rows), into device k and v [n_rows][kv_dim]."""
+        check(_lib.lib().gla_kv_read_rows(self.backend.ctx, self.handle, rows.ptr, k.ptr, v.ptr, n_rows))
+
     def export_rows(self, rows: Sequence[int]) -> tuple[np.ndarray, np.ndarray]:
         """Rows in KvStore::export_raw byte format: ([n][row_bytes], [n][row_bytes]) uint8."""
         rows = np.ascontiguousarray(rows, dtype=np.int64)
@@ -214,6 +218,76 @@ class Q8Weights:
     def destroy(self) -> None:
         if self.handle:
             check(_lib.lib().gla_q8w_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+class Q4Weights:
+    """GGML Q4_0 or Q4_K weights uploaded once and repacked for the device (gla_q4w_create)."""
+
+    def __init__(self, backend: "GpuBackend", handle: C.c_void_p, rows: int, cols: int, fmt: str):
+        self.backend, self.handle, self.rows, self.cols, self.fmt = backend, handle, rows, cols, fmt
+
+    def destroy(self) -> None:
+        if self.handle:
+            check(_lib.lib().gla_q4w_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+_LAYOUTS = {"interleaved": _lib.GLA_ROPE_INTERLEAVED, "half": _lib.GLA_ROPE_HALF}
+_SCALINGS = {"none": _lib.GLA_ROPE_NONE, "linear": _lib.GLA_ROPE_LINEAR, "bands": _lib.GLA_ROPE_BANDS,
+             "yarn": _lib.GLA_ROPE_YARN}
+_Q4_FORMATS = {"q4_0": (_lib.GLA_Q4_0, 32, 18), "q4_k": (_lib.GLA_Q4_K, 256, 144)}
+
+
+def rope_spec(head_dim: int, freq_base: float = 10000.0, layout: str = "interleaved", rot_dim: int = 0,
+              freq_dim: int = 0, scaling: str = "none", factor: float = 1.0, original_ctx: int = 0, low: float = 1.0,
+              high: float = 32.0, amplitude: float = 0.0, divisors: Optional[np.ndarray] = None) -> "_lib.RopeSpec":
+    """gla_rope_spec: what include/glint_attn.h says of each field."""
+    s = _lib.RopeSpec()
+    s.head_dim, s.rot_dim, s.freq_dim = head_dim, rot_dim, freq_dim
+    s.layout, s.scaling = _LAYOUTS[layout], _SCALINGS[scaling]
+    s.original_ctx, s.freq_base, s.factor, s.low, s.high = original_ctx, freq_base, factor, low, high
+    s.amplitude = amplitude
+    if divisors is not None:
+        d = np.ascontiguousarray(divisors, dtype=np.float32)
+        if d.shape != ((rot_dim or head_dim) // 2,):
+            raise ValueError("divisors must be float32[rot_dim / 2]")
+        s.divisors = d.ctypes.data
+        s._divisors = d  # alive as long as the specification
+    return s
+
+
+def rope_freqs(**spec) -> tuple[np.ndarray, float]:
+    """The frequencies (float64[rot_dim / 2], radians a position) and the amplitude of a specification
+    (gla_rope_freqs; needs no device). Arguments as GpuBackend.create_rope_plan."""
+    s = rope_spec(**spec)
+    f = np.empty((s.rot_dim if s.rot_dim > 0 else max(s.head_dim, 0)) // 2, dtype=np.float64)
+    amp = C.c_double()
+    check(_lib.lib().gla_rope_freqs(C.byref(s), _ptr(f), C.byref(amp)))
+    return f, amp.value
+
+
+class RopePlan:
+    """A rotary specification's frequencies on the device (gla_rope_plan_create)."""
+
+    def __init__(self, backend: "GpuBackend", handle: C.c_void_p, head_dim: int):
+        self.backend, self.handle, self.head_dim = backend, handle, head_dim
+
+    def destroy(self) -> None:
+        if self.handle:
+            check(_lib.lib().gla_rope_plan_destroy(self.handle))
             self.handle = None
 
     def __del__(self):
@@ -532,3 +606,51 @@ class GpuBackend:
     def matvec_q8_0(self, w: Q8Weights, x: DeviceBuffer, n_vec: int, y: DeviceBuffer) -> None:
         """y[v] = W x[v] for n_vec device vectors (QuantizedTensor::matvec, src/tensor/quantized.rs:247-346)."""
         check(_lib.lib().gla_matvec_q8_0(self.ctx, w.handle, x.ptr, n_vec, y.ptr))
+
+    def create_rope_plan(self, head_dim: int, freq_base: float = 10000.0, **spec) -> RopePlan:
+        """Rotary positions (gla_rope_plan_create). Keywords: layout ("interleaved", "half"), rot_dim, freq_dim,
+        scaling ("none", "linear", "bands", "yarn"), factor, original_ctx, low, high, amplitude, divisors."""
+        s = rope_spec(head_dim, freq_base, **spec)
+        h = C.c_void_p()
+        check(_lib.lib().gla_rope_plan_create(self.ctx, C.byref(s), C.byref(h)))
+        return RopePlan(self, h, head_dim)
+
+    def rope_rows(self, plan: RopePlan, x: DeviceBuffer, n_rows: int, n_heads: int, pos: DeviceBuffer,
+                  out: Optional[DeviceBuffer] = None, x_stride: int = 0, out_stride: int = 0) -> None:
+        """gla_rope_rows: device rows x [n_rows][n_heads][head_dim] rotated into `out` (None: in place)."""
+        check(_lib.lib().gla_rope_rows(self.ctx, plan.handle, x.ptr, x_stride, x.ptr if out is None else out.ptr,
+                                       x_stride if out is None else out_stride, n_rows, n_heads, pos.ptr))
+
+    def append(self, kv: _KvBase, k: DeviceBuffer, v: DeviceBuffer, q_start: DeviceBuffer, pos_offset: DeviceBuffer,
+               n_seqs: int, max_q_len: int, rope: Optional[RopePlan] = None, q: Optional[DeviceBuffer] = None,
+               q_out: Optional[DeviceBuffer] = None, n_heads: int = 0, k_stride: int = 0, v_stride: int = 0,
+               q_stride: int = 0, layer: int = 0, seq_slot: Optional[DeviceBuffer] = None,
+               page_table: Optional[DeviceBuffer] = None, page_table_stride: int = 0) -> None:
+        """gla_kv_append on device buffers (asynchronous on the backend's stream)."""
+        a = _lib.AppendArgs()
+        a.kv = kv.handle
+        a.layer = layer
+        a.n_seqs = n_seqs
+        a.seq_slot = seq_slot.ptr if seq_slot is not None else None
+        a.page_table = page_table.ptr if page_table is not None else None
+        a.page_table_stride = page_table_stride
+        a.q_start, a.pos_offset, a.max_q_len = q_start.ptr, pos_offset.ptr, max_q_len
+        a.rope = rope.handle if rope is not None else None
+        a.k, a.k_stride, a.v, a.v_stride = k.ptr, k_stride, v.ptr, v_stride
+        if q is not None:
+            a.q, a.q_stride, a.n_heads = q.ptr, q_stride, n_heads
+            a.q_out = q_out.ptr if q_out is not None else q.ptr
+        check(_lib.lib().gla_kv_append(self.ctx, C.byref(a)))
+
+    def create_q4_weights(self, ggml: np.ndarray, rows: int, cols: int, fmt: str = "q4_0") -> Q4Weights:
+        """Upload GGML Q4_0 ("q4_0") or Q4_K ("q4_k") bytes (gla_q4w_create)."""
+        code, group, size = _Q4_FORMATS[fmt]
+        raw = np.ascontiguousarray(ggml, dtype=np.uint8).reshape(-1)
+        assert raw.size == rows * (cols // group) * size
+        h = C.c_void_p()
+        check(_lib.lib().gla_q4w_create(self.ctx, code, _ptr(raw), rows, cols, C.byref(h)))
+        return Q4Weights(self, h, rows, cols, fmt)
+
+    def matvec_q4(self, w: Q4Weights, x: DeviceBuffer, n_vec: int, y: DeviceBuffer) -> None:
+        """y[v] = W x[v] for n_vec device vectors (gla_matvec_q4)."""
+        check(_lib.lib().gla_matvec_q4(self.ctx, w.handle, x.ptr, n_vec, y.ptr))

@@ -48,7 +48,7 @@ HIP_FLAGS = [
     f"-I{ROOT / 'include'}",
 ]
 HIP_SOURCES = ["gla_capi.hip", "gla_kvstore.hip", "gla_decode.hip", "gla_decode_q8.hip", "gla_prefill.hip",
-               "gla_ops.hip"]
+               "gla_ops.hip", "gla_rope.hip", "gla_q4.hip"]
 
 
 def _run(cmd: list[str], cwd: Path | None = None) -> None:

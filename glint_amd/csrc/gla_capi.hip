@@ -223,29 +223,44 @@ struct SyncOnExit {
     }
 };
 
+// A storage or weight handle used with `ctx` must have been created on it (and
+// not be detached by the context's destruction).
+int check_owner(const gla_ctx *ctx, const gla_kv *kv, const char *fn) {
+    if (kv->ctx != ctx)
+        return set_error(GLA_ERR_INVALID, "%s: the KV storage belongs to %s", fn,
+                         kv->ctx ? "another context" : "a destroyed context");
+    return GLA_OK;
+}
+
+int page_map_of(const gla_kv *kv, int layer, const int32_t *seq_slot, const int32_t *page_table, int pt_stride,
+                PageMap *pm) {
+    memset(pm, 0, sizeof(*pm));
+    if (kv->is_pool) {
+        GLA_REQUIRE(page_table != nullptr, "a pool needs a page table");
+        GLA_REQUIRE(pt_stride > 0, "page_table_stride must be positive");
+        pm->page_table = page_table;
+        pm->pt_stride = pt_stride;
+        pm->n_pages = kv->n_pages;
+        pm->pos_limit = pt_stride * GLA_PAGE_SIZE;
+        pm->n_slots = 1;
+    } else {
+        GLA_REQUIRE(page_table == nullptr, "contiguous caches take no page table");
+        GLA_REQUIRE(layer >= 0 && layer < kv->n_layers, "layer %d out of range [0, %d)", layer, kv->n_layers);
+        pm->seq_slot = seq_slot;
+        pm->seq_page_stride = (int64_t)kv->n_layers * kv->pages_per_layer;
+        pm->layer_page_off = (int64_t)layer * kv->pages_per_layer;
+        pm->n_pages = kv->n_pages;
+        pm->pos_limit = kv->max_seq;
+        pm->n_slots = kv->n_seqs;
+    }
+    return GLA_OK;
+}
+
 static size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 }  // namespace gla
 
 using namespace gla;
-
-#define GLA_GUARD_BEGIN try {
-#define GLA_GUARD_END                                                         \
-    }                                                                         \
-    catch (const std::bad_alloc &) {                                          \
-        return set_error(GLA_ERR_BUFFER, "host allocation failed");           \
-    }                                                                         \
-    catch (const std::exception &ex) {                                        \
-        return set_error(GLA_ERR_DEVICE, "internal error: %s", ex.what());    \
-    }                                                                         \
-    catch (...) {                                                             \
-        return set_error(GLA_ERR_DEVICE, "internal error at the C boundary"); \
-    }
-
-#define GLA_REQUIRE(cond, ...)                                        \
-    do {                                                              \
-        if (!(cond)) return set_error(GLA_ERR_INVALID, __VA_ARGS__); \
-    } while (0)
 
 extern "C" {
 
@@ -294,6 +309,8 @@ int gla_destroy(gla_ctx *ctx) {
         kv->ctx = nullptr;
     }
     for (gla_q8w *w : ctx->q8ws) detach_q8w(w);
+    for (gla_q4w *w : ctx->q4ws) detach_q4w(w);
+    for (gla_rope_plan *r : ctx->ropes) detach_rope(r);
     if (ctx->dstage) (void)hipFree(ctx->dstage);
     if (ctx->hstage) (void)hipHostFree(ctx->hstage);
     for (const auto &r : ctx->retired) {
@@ -374,15 +391,6 @@ int gla_memcpy_dtoh(gla_ctx *ctx, void *dst_host, const void *src_dev, size_t by
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
     GLA_CHECK_HIP(hipMemcpyAsync(dst_host, src_dev, bytes, hipMemcpyDeviceToHost, ctx->stream), GLA_ERR_BUFFER);
     GLA_CHECK_HIP(hipStreamSynchronize(ctx->stream), GLA_ERR_BUFFER);
-    return GLA_OK;
-}
-
-// A storage or weight handle used with `ctx` must have been created on it (and
-// not be detached by the context's destruction).
-static int check_owner(const gla_ctx *ctx, const gla_kv *kv, const char *fn) {
-    if (kv->ctx != ctx)
-        return set_error(GLA_ERR_INVALID, "%s: the KV storage belongs to %s", fn,
-                         kv->ctx ? "another context" : "a destroyed context");
     return GLA_OK;
 }
 
@@ -548,6 +556,19 @@ int gla_kv_write_rows_host(gla_ctx *ctx, gla_kv *kv, const int64_t *rows, const 
     GLA_GUARD_END
 }
 
+int gla_kv_read_rows(gla_ctx *ctx, const gla_kv *kv, const int64_t *rows_dev, float *k_dev, float *v_dev,
+                     int n_rows) {
+    GLA_GUARD_BEGIN
+    GLA_REQUIRE(ctx && kv && n_rows >= 0, "gla_kv_read_rows: bad argument");
+    if (int rc = check_owner(ctx, kv, "gla_kv_read_rows")) return rc;
+    if (n_rows == 0) return GLA_OK;
+    GLA_REQUIRE(rows_dev && k_dev && v_dev, "gla_kv_read_rows: NULL buffer");
+    GLA_REQUIRE((((uintptr_t)k_dev | (uintptr_t)v_dev) & 15) == 0, "gla_kv_read_rows: k and v must be 16-byte aligned");
+    GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
+    return launch_read_rows(ctx, kv, rows_dev, k_dev, v_dev, n_rows);
+    GLA_GUARD_END
+}
+
 int gla_kv_export_rows_host(gla_ctx *ctx, const gla_kv *kv, const int64_t *rows, int n_rows, uint8_t *k_out,
                             uint8_t *v_out) {
     GLA_GUARD_BEGIN
@@ -638,30 +659,6 @@ long gla_window_start(long pos, long sliding_window, int alternating, int layer)
     if (sliding_window <= 0) return 0;
     long w = pos - sliding_window + 1;
     return w > 0 ? w : 0;
-}
-
-static int page_map_of(const gla_kv *kv, int layer, const int32_t *seq_slot, const int32_t *page_table,
-                       int pt_stride, PageMap *pm) {
-    memset(pm, 0, sizeof(*pm));
-    if (kv->is_pool) {
-        GLA_REQUIRE(page_table != nullptr, "a pool needs a page table");
-        GLA_REQUIRE(pt_stride > 0, "page_table_stride must be positive");
-        pm->page_table = page_table;
-        pm->pt_stride = pt_stride;
-        pm->n_pages = kv->n_pages;
-        pm->pos_limit = pt_stride * GLA_PAGE_SIZE;
-        pm->n_slots = 1;
-    } else {
-        GLA_REQUIRE(page_table == nullptr, "contiguous caches take no page table");
-        GLA_REQUIRE(layer >= 0 && layer < kv->n_layers, "layer %d out of range [0, %d)", layer, kv->n_layers);
-        pm->seq_slot = seq_slot;
-        pm->seq_page_stride = (int64_t)kv->n_layers * kv->pages_per_layer;
-        pm->layer_page_off = (int64_t)layer * kv->pages_per_layer;
-        pm->n_pages = kv->n_pages;
-        pm->pos_limit = kv->max_seq;
-        pm->n_slots = kv->n_seqs;
-    }
-    return GLA_OK;
 }
 
 // Validate gla_decode_args and fill the launch; *nothing = true when the

@@ -35,6 +35,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <exception>
+#include <new>
 #include <string>
 #include <utility>
 #include <vector>
@@ -45,6 +47,24 @@
     do {                                                                                            \
         hipError_t _e = (expr);                                                                     \
         if (_e != hipSuccess) return gla::set_error((code), "%s: %s", #expr, hipGetErrorString(_e)); \
+    } while (0)
+
+#define GLA_GUARD_BEGIN try {
+#define GLA_GUARD_END                                                         \
+    }                                                                         \
+    catch (const std::bad_alloc &) {                                          \
+        return set_error(GLA_ERR_BUFFER, "host allocation failed");           \
+    }                                                                         \
+    catch (const std::exception &ex) {                                        \
+        return set_error(GLA_ERR_DEVICE, "internal error: %s", ex.what());    \
+    }                                                                         \
+    catch (...) {                                                             \
+        return set_error(GLA_ERR_DEVICE, "internal error at the C boundary"); \
+    }
+
+#define GLA_REQUIRE(cond, ...)                                        \
+    do {                                                              \
+        if (!(cond)) return set_error(GLA_ERR_INVALID, __VA_ARGS__); \
     } while (0)
 
 namespace gla {
@@ -212,6 +232,8 @@ struct gla_ctx {
     // after its context frees only itself.
     std::vector<gla_kv *> kvs;
     std::vector<gla_q8w *> q8ws;
+    std::vector<gla_q4w *> q4ws;
+    std::vector<gla_rope_plan *> ropes;
     // RoPE inverse frequencies 1 / powf(base, 2p / head_dim) of the last
     // (base, head_dim) rotated on this context, computed on the host
     float rope_base = 0.0f;
@@ -240,12 +262,20 @@ struct gla_kv {
 namespace gla {
 
 KvLayout layout_of(const gla_kv *kv);
+// A storage used with `ctx` must have been created on it (and not be detached
+// by the context's destruction).
+int check_owner(const gla_ctx *ctx, const gla_kv *kv, const char *fn);
+// Where the pages of a batch's sequences are, from the arguments that say so.
+int page_map_of(const gla_kv *kv, int layer, const int32_t *seq_slot, const int32_t *page_table, int pt_stride,
+                PageMap *pm);
 // At least `bytes` of device scratch for work on ctx->stream (grown by
 // doubling; a replaced buffer stays allocated until gla_destroy).
 int ensure_scratch(gla_ctx *ctx, size_t bytes, void **out);
 int ensure_dstage(gla_ctx *ctx, size_t bytes);
 // Free a weight handle's device memory and detach it from its context.
 void detach_q8w(gla_q8w *w);
+void detach_q4w(gla_q4w *w);
+void detach_rope(gla_rope_plan *r);
 int ensure_hstage(gla_ctx *ctx, size_t bytes);
 
 // Pages the window of one sequence spans, with the decode kernels' clamping
@@ -321,6 +351,7 @@ struct PrefillLaunch {
 int launch_prefill(gla_ctx *ctx, const PrefillLaunch &p);
 
 int launch_write_rows(gla_ctx *ctx, gla_kv *kv, const int64_t *rows, const float *k, const float *v, int n);
+int launch_read_rows(gla_ctx *ctx, const gla_kv *kv, const int64_t *rows, float *k, float *v, int n);
 int launch_export_rows(gla_ctx *ctx, const gla_kv *kv, const int64_t *rows, int n, uint8_t *k_out,
                        uint8_t *v_out);
 int launch_import_rows(gla_ctx *ctx, gla_kv *kv, const int64_t *rows, int n, const uint8_t *k_in,

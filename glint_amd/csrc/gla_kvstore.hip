@@ -1,75 +1,13 @@
-// gla_kvstore.hip -- device side of KvStore::write / export_raw / import_raw
-// and of the page pool's copy-on-write and recycle wipe.
-//
-// Quantize-on-write reproduces KvCacheQ8::quantize_into (src/cache/mod.rs:296-315)
-// bit for bit: d = max|x| / 127 (1.0 for an all-zero block), q = clamp(round
-// half away from zero(x * (1/d)), -127, 127) computed from the f32 d, NaN -> 0,
-// and the stored scale is f16(d) rounded to nearest even.
+// gla_kvstore.hip -- device side of KvStore::write / export_raw / import_raw,
+// of reading rows back as f32 and of the page pool's copy-on-write and recycle
+// wipe. Quantize-on-write (gla_rows.h) is KvCacheQ8::quantize_into's, bit for bit.
 #include <algorithm>
 
-#include "gla_internal.h"
+#include "gla_rows.h"
 
 namespace gla {
 
 namespace {
-
-struct RowOps {
-    KvLayout L;
-    int64_t n_rows_total;  // valid row ids are [0, n_rows_total)
-    int head_dim;
-    int kv_dim;
-    int n_blocks;  // kv_dim / 32
-    bool q8;
-};
-
-RowOps row_ops(const gla_kv *kv) {
-    RowOps o;
-    o.L = layout_of(kv);
-    o.n_rows_total = kv->n_pages * GLA_PAGE_SIZE;
-    o.head_dim = kv->head_dim;
-    o.kv_dim = kv->kv_dim;
-    o.n_blocks = kv->kv_dim / 32;
-    o.q8 = kv->dtype == GLA_KV_Q8_0;
-    return o;
-}
-
-// Byte offset of element `gi` (0 .. kv_dim-1) of row `row`, and of its scale.
-__device__ __forceinline__ int64_t elem_off(const RowOps &o, int64_t row, int gi, int esize) {
-    const int64_t page = row >> 4;
-    const int slot = (int)(row & 15);
-    const int h = gi / o.head_dim;
-    const int e = gi - h * o.head_dim;
-    return page * o.L.page_stride + (int64_t)h * o.L.head_stride + (int64_t)slot * o.L.row_stride +
-           (int64_t)e * esize;
-}
-// Byte offset of the Q8_0 scale of (row, element gi) from L.ks (which = 0,
-// parity-grouped) or L.vs (which = 1, row-major).
-__device__ __forceinline__ int64_t scale_off(const RowOps &o, int64_t row, int gi, int which) {
-    const int64_t page = row >> 4;
-    const int slot = (int)(row & 15);
-    const int h = gi / o.head_dim;
-    const int e = gi - h * o.head_dim;
-    const int idx = which ? slot * (o.head_dim >> 5) + (e >> 5) : q8ks_off(slot, e >> 5, o.head_dim);
-    return page * o.L.page_stride + (int64_t)h * o.L.head_stride + (int64_t)idx * 2;
-}
-
-// Byte offset of Q8_0 quant (row, element gi) of K (which = 0) or V (1); the
-// quants of a (page, head) are stored in MFMA operand order (q8k_off / q8v_off).
-__device__ __forceinline__ int64_t q8_off(const RowOps &o, int64_t row, int gi, int which) {
-    const int64_t page = row >> 4;
-    const int slot = (int)(row & 15);
-    const int h = gi / o.head_dim;
-    const int e = gi - h * o.head_dim;
-    const int in_head = which ? q8v_off(slot, e, o.head_dim) : q8k_off(slot, e, o.head_dim);
-    return page * o.L.page_stride + (int64_t)h * o.L.head_stride + in_head;
-}
-
-__device__ __forceinline__ int8_t quantize_one(float x, float inv_d) {
-    float r = roundf(x * inv_d);
-    if (r < -127.0f) r = -127.0f;
-    if (r > 127.0f) r = 127.0f;
-    return (r != r) ? (int8_t)0 : (int8_t)r;
-}
 
 // One thread per 8 elements of a row's K or V, so a wave reads 2 KiB of a source
 // row at once and a Q8_0 block is four neighbouring lanes, which find its
@@ -103,34 +41,41 @@ __global__ __launch_bounds__(256) void write_rows_kernel(const RowOps o, const i
             d[1] = c;
             continue;
         }
-        const float x[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
-        float max_abs = 0.0f;
+        const float e[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+        store_q8(o, row, gi, which, e);
+    }
+}
+
+// The f32 values of a row's K and V: threads as write_rows_kernel deals them.
+// A Q8_0 value is quant times f16 scale, exact in f32 but for its last rounding.
+__global__ __launch_bounds__(256) void read_rows_kernel(const RowOps o, const int64_t *rows, float *k, float *v, int n,
+                                                        int per) {
+    const int units = o.kv_dim / 4;
+    const int first = blockIdx.x * per;
+    for (int t = threadIdx.x; t < units * per; t += 256) {
+        const int rr = t / units;
+        const int r = first + rr;
+        const int u = t - rr * units;
+        const int which = u >= units / 2;
+        const int gi = (which ? u - units / 2 : u) * 8;
+        if (r >= n) continue;
+        const int64_t row = rows[r];
+        if (row < 0 || row >= o.n_rows_total) continue;
+        const uint8_t *src = which ? o.L.v : o.L.k;
+        float x[8];
+        if (!o.q8) {
+            const float4 *s = reinterpret_cast<const float4 *>(src + elem_off(o, row, gi, 4));
+            *reinterpret_cast<float4 *>(x) = s[0];
+            *reinterpret_cast<float4 *>(x + 4) = s[1];
+        } else {
+            const uint8_t *sc = (which ? o.L.vs : o.L.ks) + scale_off(o, row, gi, which);
+            const float d = __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t *>(sc)));
 #pragma unroll
-        for (int j = 0; j < 8; j++) max_abs = fmaxf(max_abs, fabsf(x[j]));
-        // quad_perm [1 0 3 2], then [2 3 0 1]
-        max_abs = fmaxf(max_abs, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(max_abs), 0xB1, 0xf, 0xf, true)));
-        max_abs = fmaxf(max_abs, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(max_abs), 0x4E, 0xf, 0xf, true)));
-        const float dsc = max_abs > 0.0f ? max_abs / 127.0f : 1.0f;
-        const float inv_d = 1.0f / dsc;
-        uint32_t w[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const uint32_t b0 = (uint8_t)quantize_one(x[4 * j + 0], inv_d);
-            const uint32_t b1 = (uint8_t)quantize_one(x[4 * j + 1], inv_d);
-            const uint32_t b2 = (uint8_t)quantize_one(x[4 * j + 2], inv_d);
-            const uint32_t b3 = (uint8_t)quantize_one(x[4 * j + 3], inv_d);
-            w[j] = (b0 | (b1 << 8) | (b2 << 16) | (b3 << 24)) ^ 0x80808080u;  // stored as x + 128
+            for (int j = 0; j < 8; j++) x[j] = (float)(int8_t)(src[q8_off(o, row, gi + j, which)] ^ 0x80) * d;
         }
-        if (!which) {  // K: 8 dims of a slot are 8 consecutive bytes
-            *reinterpret_cast<uint2 *>(dst + q8_off(o, row, gi, 0)) = make_uint2(w[0], w[1]);
-        } else {  // V: one byte per element, 4-position columns
-#pragma unroll
-            for (int j = 0; j < 8; j++) dst[q8_off(o, row, gi + j, 1)] = (uint8_t)(w[j >> 2] >> ((j & 3) * 8));
-        }
-        if ((gi & 31) == 0) {
-            uint8_t *sb = const_cast<uint8_t *>(which ? o.L.vs : o.L.ks);
-            *reinterpret_cast<uint16_t *>(sb + scale_off(o, row, gi, which)) = __half_as_ushort(__float2half_rn(dsc));
-        }
+        float4 *dst = reinterpret_cast<float4 *>((which ? v : k) + (int64_t)r * o.kv_dim + gi);
+        dst[0] = *reinterpret_cast<const float4 *>(x);
+        dst[1] = *reinterpret_cast<const float4 *>(x + 4);
     }
 }
 
@@ -226,6 +171,14 @@ int launch_write_rows(gla_ctx *ctx, gla_kv *kv, const int64_t *rows, const float
     const int per = std::max(1, 256 / (o.kv_dim / 4));
     hipLaunchKernelGGL(write_rows_kernel, dim3((n - 1) / per + 1), dim3(256), 0, ctx->stream, o, rows, k, v, n, per);
     return check_launch("write_rows_kernel");
+}
+
+int launch_read_rows(gla_ctx *ctx, const gla_kv *kv, const int64_t *rows, float *k, float *v, int n) {
+    if (n <= 0) return GLA_OK;
+    const RowOps o = row_ops(kv);
+    const int per = std::max(1, 256 / (o.kv_dim / 4));
+    hipLaunchKernelGGL(read_rows_kernel, dim3((n - 1) / per + 1), dim3(256), 0, ctx->stream, o, rows, k, v, n, per);
+    return check_launch("read_rows_kernel");
 }
 
 int launch_export_rows(gla_ctx *ctx, const gla_kv *kv, const int64_t *rows, int n, uint8_t *k_out,

@@ -9,8 +9,9 @@
  *   - PagePool page recycle and copy-on-write       src/cache/paged.rs:79-82, :433-444
  *   - attn_heads_cpu over a batch (decode)          src/transformer/forward.rs:1468-1502
  *   - prefill attention loop                        src/transformer/forward.rs:927-958
- * and, beside it on a decode step, RoPE (src/tensor/ops.rs:212-245) and the
- * Q8_0 weight matvec (src/tensor/quantized.rs:247-346, :587-610).
+ * and, beside it on a decode step, RoPE (src/tensor/ops.rs:212-245), the
+ * Q8_0 weight matvec (src/tensor/quantized.rs:247-346, :587-610), the 4-bit
+ * one and the append of rotated rows to a storage.
  * The numerics follow flash_attn_1d_ext (src/tensor/flash.rs:46-124).
  *
  * Conventions (the same as Glint's outbound C API, include/glint.h:21-35):
@@ -157,6 +158,14 @@ int gla_kv_write_rows(gla_ctx *ctx, gla_kv *kv, const int64_t *rows_dev, const f
 /* The same with host pointers; returns when the rows are written. */
 int gla_kv_write_rows_host(gla_ctx *ctx, gla_kv *kv, const int64_t *rows, const float *k, const float *v,
                            int n_rows);
+
+/* Read rows back as the f32 values the storage holds of them (Q8_0: quant
+ * times its block's f16 scale): the inverse of gla_kv_write_rows, for rows
+ * that move to another storage or are rotated to other positions. Device
+ * pointers, k and v 16-byte aligned; asynchronous. rows: int64[n_rows]; k, v:
+ * [n_rows][kv_dim]. The outputs of ids outside the storage are left as they were. */
+int gla_kv_read_rows(gla_ctx *ctx, const gla_kv *kv, const int64_t *rows_dev, float *k_dev, float *v_dev,
+                     int n_rows);
 
 /* Export rows as the bytes KvStore::export_raw produces for them
  * (src/cache/mod.rs:68-84, :219-241, :390-395): f32 rows are kv_dim native
@@ -332,6 +341,102 @@ int gla_attention_resident(gla_ctx *ctx, const float *q, const gla_kv *cache, in
 int gla_rope(gla_ctx *ctx, float *x, int n_rows, int n_heads, int head_dim, const int32_t *pos, float freq_base,
              float scaling_factor, int rot_dim);
 
+/* Rotary positions beyond gla_rope's: both layouts, part of the head, and
+ * frequencies stretched for contexts longer than the model was trained on.
+ * Pair p < rot_dim / 2 of a head at position pos is turned by the angle
+ * pos * f[p]:
+ *     (a, b) -> amplitude * (a cos - b sin, a sin + b cos),
+ * (a, b) = dimensions (2p, 2p + 1) in the interleaved layout and
+ * (p, p + rot_dim / 2) in the half layout; dimensions from rot_dim on are left
+ * as they are. Angles, cos, sin and the products are 64-bit; the result is
+ * rounded once. Positions may be negative (turning back). */
+typedef enum gla_rope_layout { GLA_ROPE_INTERLEAVED = 0, GLA_ROPE_HALF = 1 } gla_rope_layout;
+/* From the frequency g = freq_base^(-2p / freq_dim) / divisors[p]:
+ *   NONE    f = g
+ *   LINEAR  f = g / factor
+ *   BANDS   by the turns t = original_ctx * g / 2 pi a pair makes in the
+ *           original context: f = g / factor below `low` turns, g above
+ *           `high`, between them (1 - w) g / factor + w g,
+ *           w = (t - low) / (high - low)
+ *   YARN    by the pair: w falls linearly from 1 at pair
+ *           max(floor(e(high)), 0) to 0 at pair min(ceil(e(low)),
+ *           freq_dim - 1) (0.001 pairs later where the two are equal), where
+ *           e(t) is the pair that would make t turns,
+ *           freq_dim * ln(original_ctx / (2 pi t)) / (2 ln freq_base);
+ *           f = (1 - w) g / factor + w g; the amplitude's default is
+ *           0.1 ln(factor) + 1 (for factor > 1) */
+typedef enum gla_rope_scaling {
+    GLA_ROPE_NONE = 0,
+    GLA_ROPE_LINEAR = 1,
+    GLA_ROPE_BANDS = 2,
+    GLA_ROPE_YARN = 3
+} gla_rope_scaling;
+typedef struct gla_rope_spec {
+    int head_dim; /* 1 .. 512 */
+    int rot_dim;  /* rotated dimensions of a head, even, <= head_dim; 0: all (head_dim even) */
+    int freq_dim; /* the exponent's denominator; 0: rot_dim (gla_rope's is head_dim) */
+    gla_rope_layout layout;
+    gla_rope_scaling scaling;
+    int original_ctx;      /* BANDS, YARN: positions the model was trained on */
+    double freq_base;      /* > 0; for YARN not 1 */
+    double factor;         /* LINEAR, BANDS, YARN: > 0 */
+    double low, high;      /* BANDS, YARN: turns, 0 < low < high */
+    double amplitude;      /* of cos and sin; 0: the rule's own (1, for YARN see above) */
+    const float *divisors; /* host [rot_dim / 2], none of them 0 (a GGUF file's rope_freqs), or NULL */
+} gla_rope_spec;
+/* The frequencies f[rot_dim / 2] and the amplitude a specification gives
+ * (either output may be NULL). Host only: needs no device. */
+int gla_rope_freqs(const gla_rope_spec *spec, double *freqs, double *amplitude);
+
+/* A specification's frequencies on the device, made once per model. Freed
+ * with its context or by gla_rope_plan_destroy, like the weights below. */
+typedef struct gla_rope_plan gla_rope_plan;
+int gla_rope_plan_create(gla_ctx *ctx, const gla_rope_spec *spec, gla_rope_plan **out);
+int gla_rope_plan_destroy(gla_rope_plan *plan);
+
+/* Rotate device rows: x [n_rows] rows of [n_heads][head_dim] floats, x_stride
+ * floats apart (0: n_heads * head_dim), into out likewise; row r at position
+ * pos[r] (device int32). out may be x with the same stride (in place); other
+ * overlaps are not allowed. Asynchronous; allocates nothing. */
+int gla_rope_rows(gla_ctx *ctx, const gla_rope_plan *plan, const float *x, int64_t x_stride, float *out,
+                  int64_t out_stride, int n_rows, int n_heads, const int32_t *pos);
+
+/* Append new positions to the caches or page tables of a batch, from the rows
+ * a fused Q/K/V projection gives: K rotated on the way, V as it is, both
+ * quantised for Q8_0 storage as gla_kv_write_rows does (bit for bit), and the
+ * queries rotated beside them into the dense rows gla_decode and gla_prefill
+ * take. Sequence b's new rows are q_start[b] .. q_start[b+1]-1 of k, v and q,
+ * row r at position pos_offset[b] + (r - q_start[b]), as in gla_prefill; a
+ * decode step has one row per sequence.
+ * K and V of a row whose position is outside the storage (a cache's max_seq, a
+ * pool's page_table_stride * 16 positions), whose seq_slot is no sequence or
+ * whose page id is no page are not stored (the reference panics; a clamped
+ * write would overwrite another row); its query is rotated all the same. Rows
+ * of one call that meet at one place of the storage (a page in two tables) leave
+ * one of them, which one is unspecified. Rows past max_q_len of a sequence and
+ * rows outside every sequence are left alone. Asynchronous; allocates nothing. */
+typedef struct gla_append_args {
+    gla_kv *kv;
+    int layer;                 /* caches */
+    int n_seqs;
+    const int32_t *seq_slot;   /* caches: device int32[B] or NULL */
+    const int32_t *page_table; /* pools: device int32[B][page_table_stride] */
+    int page_table_stride;
+    const int32_t *q_start;    /* device int32[B + 1] */
+    const int32_t *pos_offset; /* device int32[B] */
+    int max_q_len;             /* host: >= every q_start[b+1] - q_start[b] */
+    const gla_rope_plan *rope; /* NULL: no rotation; else its head_dim is the storage's */
+    const float *k;            /* device rows of [n_kv_heads][head_dim], k_stride floats apart (0: dense) */
+    int64_t k_stride;
+    const float *v;            /* the same */
+    int64_t v_stride;
+    const float *q;            /* device rows of [n_heads][head_dim], q_stride floats apart (0: dense), or NULL */
+    int64_t q_stride;
+    float *q_out;              /* device [rows][n_heads][head_dim]; may be q where that is dense */
+    int n_heads;               /* of q */
+} gla_append_args;
+int gla_kv_append(gla_ctx *ctx, const gla_append_args *args);
+
 /* Q8_0 weights on the device, uploaded once: the GpuBackend::upload_buffer of
  * a GGML Q8_0 tensor (src/backend/gpu.rs:111-121), repacked for the MFMA
  * matvec. ggml_host: rows x (cols / 32) blocks of [f16 scale LE][32 x i8]
@@ -350,6 +455,26 @@ int gla_q8w_cols(const gla_q8w *w);
  * once, more share them in tiles through LDS. n_vec above 262,128 is refused
  * (GLA_ERR_INVALID): split the call. */
 int gla_matvec_q8_0(gla_ctx *ctx, const gla_q8w *w, const float *x, int n_vec, float *y);
+
+/* 4-bit weights on the device, uploaded once from a GGML tensor and repacked:
+ *   Q4_0  rows x (cols / 32) blocks of 18 bytes, [f16 d][16 bytes: low nibbles
+ *         values 0-15, high nibbles 16-31], value d * (nibble - 8)
+ *   Q4_K  rows x (cols / 256) blocks of 144 bytes, [f16 d][f16 dmin][12 bytes:
+ *         eight 6-bit scales and eight 6-bit minima][128 bytes of nibbles],
+ *         value (d * scale) * nibble - dmin * minimum in groups of 32
+ * cols a multiple of 32 (Q4_0) or 256 (Q4_K). Returns when the weights are on
+ * the device; handles behave as gla_q8w's do. */
+typedef enum gla_q4_format { GLA_Q4_0 = 0, GLA_Q4_K = 1 } gla_q4_format;
+typedef struct gla_q4w gla_q4w;
+int gla_q4w_create(gla_ctx *ctx, gla_q4_format format, const uint8_t *ggml_host, int rows, int cols, gla_q4w **out);
+int gla_q4w_destroy(gla_q4w *w);
+int gla_q4w_rows(const gla_q4w *w);
+int gla_q4w_cols(const gla_q4w *w);
+
+/* y[v][r] = sum_c W[r][c] * x[v][c] for n_vec vectors, as gla_matvec_q8_0:
+ * x device [n_vec][cols], y device [n_vec][rows], f32, y apart from x.
+ * Asynchronous. n_vec above 262,128 is refused (split the call). */
+int gla_matvec_q4(gla_ctx *ctx, const gla_q4w *w, const float *x, int n_vec, float *y);
 
 #ifdef __cplusplus
 }
