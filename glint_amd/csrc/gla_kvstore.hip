@@ -67,11 +67,30 @@ __global__ __launch_bounds__(256) void read_rows_kernel(const RowOps o, const in
             const float4 *s = reinterpret_cast<const float4 *>(src + elem_off(o, row, gi, 4));
             *reinterpret_cast<float4 *>(x) = s[0];
             *reinterpret_cast<float4 *>(x + 4) = s[1];
-        } else {
-            const uint8_t *sc = (which ? o.L.vs : o.L.ks) + scale_off(o, row, gi, which);
+        } else if (!which) {
+            const uint8_t *sc = o.L.ks + scale_off(o, row, gi, 0);
             const float d = __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t *>(sc)));
+            const uint2 q = *reinterpret_cast<const uint2 *>(src + q8_off(o, row, gi, 0));
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = (float)(int8_t)(src[q8_off(o, row, gi + j, which)] ^ 0x80) * d;
+            for (int j = 0; j < 8; j++)
+                x[j] = (float)(int8_t)(((j < 4 ? q.x : q.y) >> (8 * (j & 3))) ^ 0x80u) * d;
+        } else {
+            // a column of the page's V holds dimensions j, j + 16, j + 32, j + 48 of
+            // four positions in 16 bytes: the thread takes two columns of the row
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int col = (u - units / 2) + c * (units / 2);  // 16 to 64 dimensions
+                const int g = (col >> 4) * 64 + (col & 15);
+                const uint4 q = *reinterpret_cast<const uint4 *>(src + (q8_off(o, row, g, 1) & ~(int64_t)15));
+                const uint32_t sc = *reinterpret_cast<const uint32_t *>(o.L.vs + scale_off(o, row, g, 1));
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    v[(int64_t)r * o.kv_dim + g + 16 * i] =
+                        (float)(int8_t)((w[i] >> (8 * (row & 3))) ^ 0x80u) *
+                        __half2float(__ushort_as_half((unsigned short)(i < 2 ? sc : sc >> 16)));
+            }
+            continue;
         }
         float4 *dst = reinterpret_cast<float4 *>((which ? v : k) + (int64_t)r * o.kv_dim + gi);
         dst[0] = *reinterpret_cast<const float4 *>(x);

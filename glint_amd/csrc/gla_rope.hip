@@ -83,34 +83,46 @@ __device__ __forceinline__ void cos_sin(double t, double amp, double &c, double 
     s = (q == 2 || q == 3) ? -ss * amp : ss * amp;
 }
 
-// The factors of a lane's elements e0 .. e0 + 7: x -> own * c + partner * s.
+// A wave's LDS: cos and sin of its row's pairs, then (kHalf) the heads of a group.
+__host__ __device__ constexpr size_t wave_lds(int mode, int pairs) {
+    return mode == kCopy ? 0 : (size_t)pairs * sizeof(double2) + (mode == kHalf ? kMaxHeadDim * sizeof(float) : 0);
+}
+
+// The factors of a lane's elements e0 .. e0 + 7 of a head, elements from
+// 2 * pairs on left alone. The wave's lanes evaluate one pair each and read the
+// factors they need from LDS: eight evaluations a lane cost a call of one row
+// 1.4 us of its 4.4.
 template <int MODE>
 struct Turn {
     double c[MODE == kAdjacent ? 4 : 8], s[MODE == kAdjacent ? 4 : 8];
+    const Rope &r;
+    int e0, head_dim;
+    float *stage;  // kHalf: the head's place in LDS, filled by the wave's lanes of this head
 
-    __device__ __forceinline__ void set(const Rope &r, int e0, double pos) {
-        if constexpr (MODE == kAdjacent) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int p = e0 / 2 + j;
-                if (p < r.pairs) cos_sin(pos * r.turns[p], r.amplitude, c[j], s[j]);
+    __device__ __forceinline__ Turn(const Rope &rope, int lane, int e0, int h, int head_dim, double pos, double2 *lds)
+        : r(rope), e0(e0), head_dim(head_dim) {
+        if constexpr (MODE != kCopy) {
+            stage = reinterpret_cast<float *>(lds + r.pairs) + h * head_dim;
+            for (int p = lane; p < r.pairs; p += 64) {
+                double2 t;
+                cos_sin(pos * r.turns[p], r.amplitude, t.x, t.y);
+                lds[p] = t;
             }
-        } else if constexpr (MODE == kHalf) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            constexpr int N = MODE == kAdjacent ? 4 : 8;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int e = e0 + j;
-                if (e < 2 * r.pairs) {
-                    const bool second = e >= r.pairs;
-                    cos_sin(pos * r.turns[second ? e - r.pairs : e], r.amplitude, c[j], s[j]);
-                    if (!second) s[j] = -s[j];
-                }
+            for (int j = 0; j < N; j++) {
+                const int e = MODE == kAdjacent ? e0 / 2 + j : e0 + j;
+                const bool second = MODE == kHalf && e >= r.pairs;
+                const double2 t = lds[min(second ? e - r.pairs : e, r.pairs - 1)];
+                c[j] = t.x;
+                s[j] = MODE == kHalf && !second ? -t.y : t.y;
             }
         }
     }
 
-    // x: elements e0 .. +7 of a head; `stage` the head's place in LDS (kHalf),
-    // which the wave's lanes of this head fill together.
-    __device__ __forceinline__ void apply(const Rope &r, int e0, int head_dim, float (&x)[8], float *stage) const {
+    __device__ __forceinline__ void apply(float (&x)[8]) const {
         if constexpr (MODE == kAdjacent) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -164,35 +176,43 @@ __device__ __forceinline__ void store8(float *p, const float (&x)[8], int n) {
 }
 
 constexpr int kWaves = 4;
+constexpr int kVByPage = 16;
 
 // A wave takes heads of one row: `lanes` = ceil(head_dim / 8) lanes a head,
-// 64 / lanes heads at a time.
+// 64 / lanes heads at a time, the next ones' loads in flight.
 template <int MODE, bool V>
 __global__ __launch_bounds__(kWaves * 64) void rope_rows_kernel(const Rope r, const float *x, int64_t x_stride,
                                                                 float *out, int64_t out_stride, int n_rows,
                                                                 int n_heads, int head_dim, int lanes, int parts,
                                                                 const int32_t *pos) {
-    __shared__ __attribute__((aligned(16))) float lds[kWaves][kMaxHeadDim];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
-    const int64_t row = item / parts;
-    const int part = (int)(item - row * parts);
+    extern __shared__ double2 lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t item = blockIdx.x * kWaves + wave;
+    const int row = (int)(item / (uint32_t)parts);
+    const int part = (int)(item - (uint32_t)row * parts);
     if (row >= n_rows) return;
     const int per = 64 / lanes;  // heads at a time
-    const int h = lane / lanes;
-    if (h >= per) return;
-    const int e0 = (lane - h * lanes) * 8;
+    // lanes past the last whole head repeat its first one's work (they take part
+    // in the pairs' evaluation) and store nothing
+    const bool spare = lane >= per * lanes;
+    const int h = spare ? per - 1 : lane / lanes;
+    const int e0 = spare ? 0 : (lane - h * lanes) * 8;
     const int groups = (n_heads + per - 1) / per;
-    const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
-    Turn<MODE> t;
-    t.set(r, e0, pos[row]);
+    const int g0 = groups * part / parts, g1 = groups * (part + 1) / parts;
+    const float *src = x + row * x_stride + e0;
+    float *dst = out + row * out_stride + e0;
+    float next[8];
+    const auto load = [&](int g) { load8<V>(next, src + (int64_t)min(g * per + h, n_heads - 1) * head_dim, head_dim - e0); };
+    load(g0);
+    const Turn<MODE> t(r, lane, e0, h, head_dim, (double)pos[row], lds + wave * (wave_lds(MODE, r.pairs) / sizeof(double2)));
     for (int g = g0; g < g1; g++) {
         const int head = g * per + h;
-        if (head >= n_heads) continue;
         float e[8];
-        load8<V>(e, x + row * x_stride + (int64_t)head * head_dim + e0, head_dim - e0);
-        t.apply(r, e0, head_dim, e, lds[wave] + h * head_dim);
-        store8<V>(out + row * out_stride + (int64_t)head * head_dim + e0, e, head_dim - e0);
+#pragma unroll
+        for (int j = 0; j < 8; j++) e[j] = next[j];
+        if (g + 1 < g1) load(g + 1);
+        t.apply(e);
+        if (head < n_heads && !spare) store8<V>(dst + (int64_t)head * head_dim, e, head_dim - e0);
     }
 }
 
@@ -204,74 +224,175 @@ struct Append {
     Rope rope;
     const int32_t *q_start, *pos_offset;
     int n_seqs, max_q_len, parts;
+    int row_blocks;   // blocks of a sequence that take rows; the others take pages of V
+    int v_by_page;
     const float *k, *v, *q;
     float *q_out;
     int64_t k_stride, v_stride, q_stride;
     int n_heads, n_kv;
 };
 
-// The storage row of (b, pos), or -1 where there is none.
-__device__ __forceinline__ int64_t storage_row(const PageMap &pm, int b, int64_t pos) {
-    if (pos < 0 || pos >= pm.pos_limit) return -1;
+constexpr int kMaxGridY = 32768;  // sequences along y, the rest along z
+
+// The storage page of (b, page lp of the sequence), or -1 where there is none.
+__device__ __forceinline__ int64_t storage_page(const PageMap &pm, int b, int64_t lp) {
     int64_t page;
     if (pm.page_table) {
-        page = pm.page_table[(int64_t)b * pm.pt_stride + (pos >> 4)];
+        page = pm.page_table[(int64_t)b * pm.pt_stride + lp];
     } else {
         const int s = pm.seq_slot ? pm.seq_slot[b] : b;
         if (s < 0 || s >= pm.n_slots) return -1;
-        page = (int64_t)s * pm.seq_page_stride + pm.layer_page_off + (pos >> 4);
+        page = (int64_t)s * pm.seq_page_stride + pm.layer_page_off + lp;
     }
-    return page < 0 || page >= pm.n_pages ? -1 : page * GLA_PAGE_SIZE + (pos & 15);
+    return page < 0 || page >= pm.n_pages ? -1 : page;
+}
+
+// Maximum over the 16 lanes of a row: rotations by 8, 4, 2 and 1.
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xf, 0xf, true)));
+    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x124, 0xf, 0xf, true)));
+    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x122, 0xf, 0xf, true)));
+    return fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x121, 0xf, 0xf, true)));
+}
+
+// V of a Q8_0 page: a wave takes 64 dimensions of one head's 16 positions, the
+// kilobyte that lies together in the page (q8v_off), so lane (sg, j) makes the 16
+// bytes of positions 4 sg .. +3 and dimensions j, j + 16, j + 32, j + 48 and
+// stores them at once; row by row each byte is a store of its own. Positions of
+// the page that are not new stay: a group of four with such is stored byte by byte.
+__device__ __forceinline__ void append_v_page(const Append &a, int b, int idx, int lane) {
+    const int pieces = a.o.head_dim >> 6;
+    const int piece = idx % pieces;
+    const int head = idx / pieces % a.n_kv;
+    const int chunk = idx / pieces / a.n_kv;
+    const int first = a.q_start[b], last = a.q_start[b + 1];
+    const int64_t p0 = a.pos_offset[b];
+    const int64_t p1 = min(p0 + min(last - first, a.max_q_len), (int64_t)a.pm.pos_limit);
+    const int64_t lp = (p0 >> 4) + chunk;
+    if (p1 <= p0 || lp < 0 || lp * GLA_PAGE_SIZE >= p1) return;  // no new row in this page
+    const int64_t page = storage_page(a.pm, b, lp);
+    if (page < 0) return;
+    const int sg = lane >> 4, j = lane & 15;
+    const int64_t pos = lp * GLA_PAGE_SIZE + sg * 4;
+    float x[4][4];
+    bool in[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        in[i] = pos + i >= p0 && pos + i < p1;
+        const float *src = a.v + (in[i] ? first + (pos + i - p0) : (int64_t)first) * a.v_stride + head * a.o.head_dim + piece * 64 + j;
+#pragma unroll
+        for (int c = 0; c < 4; c++) x[i][c] = src[c * 16];
+    }
+    uint32_t w[4] = {0, 0, 0, 0};
+    float scale = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int c2 = 0; c2 < 2; c2++) {  // the two blocks of 32 dimensions
+            const float top = row_max(fmaxf(fmaxf(0.0f, fabsf(x[i][2 * c2])), fabsf(x[i][2 * c2 + 1])));
+            const float d = top > 0.0f ? top / 127.0f : 1.0f;
+            const float inv = 1.0f / d;
+            w[2 * c2] |= (uint32_t)(uint8_t)quantize_one(x[i][2 * c2], inv) << (8 * i);
+            w[2 * c2 + 1] |= (uint32_t)(uint8_t)quantize_one(x[i][2 * c2 + 1], inv) << (8 * i);
+            if (j == 2 * i + c2) scale = d;
+        }
+    uint8_t *dst = const_cast<uint8_t *>(a.o.L.v) + page * a.o.L.page_stride + head * a.o.L.head_stride + piece * 1024 +
+                   lane * 16;
+    if (in[0] && in[1] && in[2] && in[3]) {
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0] ^ 0x80808080u, w[1] ^ 0x80808080u, w[2] ^ 0x80808080u,
+                                                     w[3] ^ 0x80808080u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (in[i])
+#pragma unroll
+                for (int c = 0; c < 4; c++) dst[4 * c + i] = (uint8_t)(w[c] >> (8 * i)) ^ 0x80;
+    }
+    // lane 2 i + c2 of a row of lanes holds the scale of position i, block c2
+    const bool mine = j < 8 && pos + (j >> 1) >= p0 && pos + (j >> 1) < p1;
+    if (mine) {
+        uint8_t *vs = const_cast<uint8_t *>(a.o.L.vs) + page * a.o.L.page_stride + head * a.o.L.head_stride;
+        reinterpret_cast<uint16_t *>(vs)[(sg * 4 + (j >> 1)) * (a.o.head_dim >> 5) + piece * 2 + (j & 1)] =
+            __half_as_ushort(__float2half_rn(scale));
+    }
 }
 
 // A wave takes a part of one new row: its groups of 64 * 8 elements are those
-// of q, of K and of V in turn (head_dim / 8 lanes a head).
+// of q, of K and (unless V goes page by page) of V in turn, head_dim / 8 lanes a
+// head, the next group's loads in flight.
 template <int MODE, bool V>
 __global__ __launch_bounds__(kWaves * 64) void kv_append_kernel(const Append a) {
-    __shared__ __attribute__((aligned(16))) float lds[kWaves][kMaxHeadDim];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
-    const int64_t place = item / a.parts;
-    const int part = (int)(item - place * a.parts);
-    const int b = (int)(place / a.max_q_len);
-    const int i = (int)(place - (int64_t)b * a.max_q_len);
+    extern __shared__ double2 lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int b = blockIdx.z * kMaxGridY + blockIdx.y;
     if (b >= a.n_seqs) return;
+    if ((int)blockIdx.x >= a.row_blocks) {
+        append_v_page(a, b, (blockIdx.x - a.row_blocks) * kWaves + wave, lane);
+        return;
+    }
+    const uint32_t item = blockIdx.x * kWaves + wave;
+    const int i = (int)(item / (uint32_t)a.parts);
+    const int part = (int)(item - (uint32_t)i * a.parts);
     const int first = a.q_start[b], last = a.q_start[b + 1];
-    if (i >= last - first) return;
+    if (i >= min(last - first, a.max_q_len)) return;
     const int64_t r = (int64_t)first + i;
     const int64_t pos = (int64_t)a.pos_offset[b] + i;
-    const int64_t row = storage_row(a.pm, b, pos);
 
     const int head_dim = a.o.head_dim;
     const int lanes = head_dim >> 3, per = 64 / lanes;
     const int h = lane / lanes;
     const int e0 = (lane - h * lanes) * 8;
     const int gq = a.q ? (a.n_heads + per - 1) / per : 0, gk = (a.n_kv + per - 1) / per;
-    const int groups = gq + 2 * gk;
-    const int g0 = (int)((int64_t)groups * part / a.parts), g1 = (int)((int64_t)groups * (part + 1) / a.parts);
-    Turn<MODE> t;
-    if (MODE != kCopy && g0 < gq + gk) t.set(a.rope, e0, (double)pos);
-    for (int g = g0; g < g1; g++) {
-        float e[8];
+    const int groups = gq + (a.v_by_page ? gk : 2 * gk);
+    const int g0 = groups * part / a.parts, g1 = groups * (part + 1) / a.parts;
+    float next[8];
+    const auto load = [&](int g) {
+        const float *src;
         if (g < gq) {
-            const int head = g * per + h;
-            if (head >= a.n_heads) continue;
-            load8<V>(e, a.q + r * a.q_stride + head * head_dim + e0, 8);
-            t.apply(a.rope, e0, head_dim, e, lds[wave] + h * head_dim);
-            store8<V>(a.q_out + (r * a.n_heads + head) * head_dim + e0, e, 8);
-            continue;
+            src = a.q + r * a.q_stride + min(g * per + h, a.n_heads - 1) * head_dim;
+        } else {
+            const bool v = g >= gq + gk;
+            const int head = min((g - gq - (v ? gk : 0)) * per + h, a.n_kv - 1);
+            src = (v ? a.v + r * a.v_stride : a.k + r * a.k_stride) + head * head_dim;
         }
-        const int which = g >= gq + gk;
-        const int head = (g - gq - which * gk) * per + h;
-        if (head >= a.n_kv || row < 0) continue;
-        const int gi = head * head_dim + e0;
-        load8<V>(e, which ? a.v + r * a.v_stride + gi : a.k + r * a.k_stride + gi, 8);
-        if (!which) t.apply(a.rope, e0, head_dim, e, lds[wave] + h * head_dim);
-        if (a.o.q8)
-            store_q8(a.o, row, gi, which, e);
-        else
-            store8<true>(reinterpret_cast<float *>(const_cast<uint8_t *>(which ? a.o.L.v : a.o.L.k) +
-                                                   elem_off(a.o, row, gi, 4)), e, 8);
+        load8<V>(next, src + e0, 8);
+    };
+    load(g0);
+    int64_t row = -1;
+    if (g1 > gq && pos >= 0 && pos < a.pm.pos_limit) {
+        const int64_t page = storage_page(a.pm, b, pos >> 4);
+        if (page >= 0) row = page * GLA_PAGE_SIZE + (pos & 15);
+    }
+    const auto rest = [&](auto &t) {
+        for (int g = g0; g < g1; g++) {
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) e[j] = next[j];
+            if (g + 1 < g1) load(g + 1);
+            if (g < gq + gk) t.apply(e);
+            if (g < gq) {
+                const int head = g * per + h;
+                if (head < a.n_heads) store8<V>(a.q_out + (r * a.n_heads + head) * head_dim + e0, e, 8);
+                continue;
+            }
+            const int which = g >= gq + gk;
+            const int head = (g - gq - which * gk) * per + h;
+            if (head >= a.n_kv || row < 0) continue;
+            const int gi = head * head_dim + e0;
+            if (a.o.q8)
+                store_q8(a.o, row, gi, which, e);
+            else
+                store8<true>(reinterpret_cast<float *>(const_cast<uint8_t *>(which ? a.o.L.v : a.o.L.k) +
+                                                       elem_off(a.o, row, gi, 4)), e, 8);
+        }
+    };
+    if (MODE == kCopy || g0 >= gq + gk) {
+        const Turn<kCopy> t(a.rope, lane, e0, h, head_dim, 0.0, nullptr);
+        rest(t);
+    } else {
+        const Turn<MODE> t(a.rope, lane, e0, h, head_dim, (double)pos,
+                           lds + wave * (wave_lds(MODE, a.rope.pairs) / sizeof(double2)));
+        rest(t);
     }
 }
 
@@ -436,13 +557,12 @@ int gla_rope_rows(gla_ctx *ctx, const gla_rope_plan *plan, const float *x, int64
     const int d = plan->head_dim;
     const int lanes = (d + 7) / 8, per = 64 / lanes;
     const int parts = parts_of(n_rows, (n_heads + per - 1) / per);
-    const int64_t blocks = ((int64_t)n_rows * parts + kWaves - 1) / kWaves;
-    GLA_REQUIRE(blocks <= INT32_MAX, "gla_rope_rows: %d rows are too many for one call", n_rows);
+    const unsigned blocks = (unsigned)(((int64_t)n_rows * parts + kWaves - 1) / kWaves);
     const bool vec = d % 8 == 0 && aligned16(x, x_stride) && aligned16(out, out_stride);
     auto kernel = plan->half ? (vec ? rope_rows_kernel<kHalf, true> : rope_rows_kernel<kHalf, false>)
                              : (vec ? rope_rows_kernel<kAdjacent, true> : rope_rows_kernel<kAdjacent, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kWaves * 64), 0, ctx->stream, rope_of(plan), x, x_stride, out,
-                       out_stride, n_rows, n_heads, d, lanes, parts, pos);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kWaves * 64), kWaves * wave_lds(plan->half ? kHalf : kAdjacent, plan->pairs),
+                       ctx->stream, rope_of(plan), x, x_stride, out, out_stride, n_rows, n_heads, d, lanes, parts, pos);
     return launched("rope_rows_kernel");
     GLA_GUARD_END
 }
@@ -490,21 +610,31 @@ int gla_kv_append(gla_ctx *ctx, const gla_append_args *a) {
     p.q_out = a->q_out;
     p.n_heads = a->n_heads;
     p.n_kv = kv->n_kv_heads;
+    // V of a Q8_0 storage page by page where a sequence's rows fill pages, else
+    // with its row
+    p.v_by_page = p.o.q8 && p.max_q_len >= kVByPage;
     const int per = 64 / (kv->head_dim / 8);
-    const int groups = (a->q ? (a->n_heads + per - 1) / per : 0) + 2 * ((p.n_kv + per - 1) / per);
-    const int64_t places = (int64_t)a->n_seqs * a->max_q_len;
-    p.parts = parts_of(places, groups);
-    const int64_t blocks = (places * p.parts + kWaves - 1) / kWaves;
-    GLA_REQUIRE(blocks <= INT32_MAX, "gla_kv_append: %d sequences of %d rows are too many for one call", a->n_seqs,
+    const int gk = (p.n_kv + per - 1) / per;
+    const int groups = (a->q ? (a->n_heads + per - 1) / per : 0) + (p.v_by_page ? gk : 2 * gk);
+    p.parts = parts_of((int64_t)a->n_seqs * a->max_q_len, groups);
+    const int64_t row_blocks = ((int64_t)p.max_q_len * p.parts + kWaves - 1) / kWaves;
+    const int64_t chunks = ((int64_t)p.max_q_len + GLA_PAGE_SIZE - 2) / GLA_PAGE_SIZE + 1;  // pages a sequence may touch
+    const int64_t v_blocks = p.v_by_page ? (chunks * p.n_kv * (kv->head_dim / 64) + kWaves - 1) / kWaves : 0;
+    GLA_REQUIRE(row_blocks + v_blocks <= INT32_MAX / (kWaves * 64), "gla_kv_append: sequences of %d rows are too long for one call",
                 a->max_q_len);
+    p.row_blocks = (int)row_blocks;
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
     const bool vec = aligned16(p.k, p.k_stride) && aligned16(p.v, p.v_stride) &&
                      (!p.q || (aligned16(p.q, p.q_stride) && aligned16(p.q_out, 0)));
+    int mode = kCopy;
     auto kernel = vec ? kv_append_kernel<kCopy, true> : kv_append_kernel<kCopy, false>;
-    if (a->rope)
+    if (a->rope) {
+        mode = a->rope->half ? kHalf : kAdjacent;
         kernel = a->rope->half ? (vec ? kv_append_kernel<kHalf, true> : kv_append_kernel<kHalf, false>)
                                : (vec ? kv_append_kernel<kAdjacent, true> : kv_append_kernel<kAdjacent, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kWaves * 64), 0, ctx->stream, p);
+    }
+    const dim3 grid((unsigned)(row_blocks + v_blocks), std::min(a->n_seqs, kMaxGridY), (a->n_seqs + kMaxGridY - 1) / kMaxGridY);
+    hipLaunchKernelGGL(kernel, grid, dim3(kWaves * 64), kWaves * wave_lds(mode, p.rope.pairs), ctx->stream, p);
     return launched("kv_append_kernel");
     GLA_GUARD_END
 }

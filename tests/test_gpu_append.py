@@ -290,7 +290,7 @@ def test_refusals(backend):
                dict(v_stride=-1), dict(q_stride=100), dict(q_stride=256), dict(layer=2), dict(layer=-1),
                dict(page_table=ints.ptr), dict(kv=pool.handle), dict(kv=pool.handle, page_table=ints.ptr),
                dict(kv=pool.handle, page_table=ints.ptr, page_table_stride=-1),
-               dict(kv=pool.handle, page_table=ints.ptr, page_table_stride=1 << 28), dict(n_seqs=1 << 30, max_q_len=1 << 30)):
+               dict(kv=pool.handle, page_table=ints.ptr, page_table_stride=1 << 28), dict(max_q_len=(1 << 31) - 1)):
         assert call(**kw) == _lib.GLA_ERR_INVALID, kw
     assert call(q=None, q_out=None, n_heads=0) == _lib.GLA_OK
     for args in ((None, buf.ptr, buf.ptr, 1), (ints.ptr, None, buf.ptr, 1), (ints.ptr, buf.ptr, None, 1),
