@@ -38,7 +38,10 @@ void detach_rope(gla_rope_plan *r) {
 
 namespace {
 
-constexpr int kMaxHeadDim = 512;
+constexpr int kMaxHeadDim = 256;
+constexpr int kWaves = 4;   // waves of a workgroup, each on its own
+constexpr int kAhead = 4;   // groups whose loads a wave has in flight
+constexpr int kVByPage = 16;
 
 // ---- rotating ------------------------------------------------------------------
 
@@ -48,11 +51,11 @@ struct Rope {
     double amplitude;
 };
 
-// How a lane's 8 consecutive elements of a head find their pairs.
+// How a lane's 4 consecutive elements of a head find their pairs.
 enum Mode {
     kCopy = 0,       // no rotation
     kAdjacent = 1,   // interleaved: in the lane's own registers
-    kHalf = 2        // half: the partner is pairs elements away, in another lane's
+    kHalf = 2        // half: the partner is `pairs` elements away, in another lane's
 };
 
 __device__ __forceinline__ void cos_sin(double t, double amp, double &c, double &s) {
@@ -83,24 +86,24 @@ __device__ __forceinline__ void cos_sin(double t, double amp, double &c, double 
     s = (q == 2 || q == 3) ? -ss * amp : ss * amp;
 }
 
-// A wave's LDS: cos and sin of its row's pairs, then (kHalf) the heads of a group.
+// A wave's LDS: cos and sin of its row's pairs, then (kHalf) a group's heads.
 __host__ __device__ constexpr size_t wave_lds(int mode, int pairs) {
     return mode == kCopy ? 0 : (size_t)pairs * sizeof(double2) + (mode == kHalf ? kMaxHeadDim * sizeof(float) : 0);
 }
 
-// The factors of a lane's elements e0 .. e0 + 7 of a head, elements from
-// 2 * pairs on left alone. The wave's lanes evaluate one pair each and read the
-// factors they need from LDS: eight evaluations a lane cost a call of one row
-// 1.4 us of its 4.4.
-template <int MODE>
+// The factors of a lane's elements e0 .. e0 + 3 of a head; elements from
+// 2 * pairs on are left alone. The wave's lanes evaluate one pair each and read
+// the factors they need from LDS: evaluations of a lane's own eight elements cost
+// a call of one row 1.1 us of its 4.4.
+template <int MODE, bool V>
 struct Turn {
-    double c[MODE == kAdjacent ? 4 : 8], s[MODE == kAdjacent ? 4 : 8];
-    const Rope &r;
-    int e0, head_dim;
+    static constexpr int N = MODE == kAdjacent ? 2 : 4;
+    double c[N], s[N];
+    const int pairs, e0, head_dim;
     float *stage;  // kHalf: the head's place in LDS, filled by the wave's lanes of this head
 
-    __device__ __forceinline__ Turn(const Rope &rope, int lane, int e0, int h, int head_dim, double pos, double2 *lds)
-        : r(rope), e0(e0), head_dim(head_dim) {
+    __device__ __forceinline__ Turn(const Rope &r, int lane, int e0, int h, int head_dim, double pos, double2 *lds)
+        : pairs(r.pairs), e0(e0), head_dim(head_dim) {
         if constexpr (MODE != kCopy) {
             stage = reinterpret_cast<float *>(lds + r.pairs) + h * head_dim;
             for (int p = lane; p < r.pairs; p += 64) {
@@ -110,7 +113,6 @@ struct Turn {
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            constexpr int N = MODE == kAdjacent ? 4 : 8;
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 const int e = MODE == kAdjacent ? e0 / 2 + j : e0 + j;
@@ -122,64 +124,88 @@ struct Turn {
         }
     }
 
-    __device__ __forceinline__ void apply(float (&x)[8]) const {
+    __device__ __forceinline__ void apply(float (&x)[4]) const {
         if constexpr (MODE == kAdjacent) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < 2; j++) {
                 const double a = x[2 * j], b = x[2 * j + 1];
-                if (e0 / 2 + j < r.pairs) {
+                if (e0 / 2 + j < pairs) {
                     x[2 * j] = (float)fma(a, c[j], -(b * s[j]));
                     x[2 * j + 1] = (float)fma(a, s[j], b * c[j]);
                 }
             }
         } else if constexpr (MODE == kHalf) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the last head's reads
+            if constexpr (V) {
+                *reinterpret_cast<float4 *>(stage + e0) = make_float4(x[0], x[1], x[2], x[3]);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (e0 + j < head_dim) stage[e0 + j] = x[j];
+                for (int j = 0; j < 4; j++)
+                    if (e0 + j < head_dim) stage[e0 + j] = x[j];
+            }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
+            if (V && pairs % 4 == 0) {  // the four are of one half, their partners together
+                if (e0 < 2 * pairs) {
+                    const float4 b = *reinterpret_cast<const float4 *>(stage + (e0 < pairs ? e0 + pairs : e0 - pairs));
+                    x[0] = (float)fma((double)x[0], c[0], (double)b.x * s[0]);
+                    x[1] = (float)fma((double)x[1], c[1], (double)b.y * s[1]);
+                    x[2] = (float)fma((double)x[2], c[2], (double)b.z * s[2]);
+                    x[3] = (float)fma((double)x[3], c[3], (double)b.w * s[3]);
+                }
+            } else {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int e = e0 + j;
-                if (e < 2 * r.pairs) {
-                    const double b = stage[e < r.pairs ? e + r.pairs : e - r.pairs];
-                    x[j] = (float)fma((double)x[j], c[j], b * s[j]);
+                for (int j = 0; j < 4; j++) {
+                    const int e = e0 + j;
+                    if (e < 2 * pairs) {
+                        const double b = stage[e < pairs ? e + pairs : e - pairs];
+                        x[j] = (float)fma((double)x[j], c[j], b * s[j]);
+                    }
                 }
             }
         }
     }
 };
 
-// 8 elements of a head, `n` of them inside it (at least one); V: all 8, 16-byte aligned
+// 4 elements of a head, `n` of them inside it (at least one); V: all 4, 16-byte aligned
 template <bool V>
-__device__ __forceinline__ void load8(float (&x)[8], const float *p, int n) {
+__device__ __forceinline__ void load4(float (&x)[4], const float *p, int n) {
     if constexpr (V) {
-        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+        const float4 a = *reinterpret_cast<const float4 *>(p);
         x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-        x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = j < n ? p[j] : 0.0f;
+        for (int j = 0; j < 4; j++) x[j] = j < n ? p[j] : 0.0f;
     }
 }
 template <bool V>
-__device__ __forceinline__ void store8(float *p, const float (&x)[8], int n) {
+__device__ __forceinline__ void store4(float *p, const float (&x)[4], int n) {
     if constexpr (V) {
-        reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++)
+        for (int j = 0; j < 4; j++)
             if (j < n) p[j] = x[j];
     }
 }
 
-constexpr int kWaves = 4;
-constexpr int kVByPage = 16;
+// Groups g0 .. g1 - 1 through load(x, g) and then use(x, g), kAhead loads in flight.
+template <class Load, class Use>
+__device__ __forceinline__ void stream_groups(float (&x)[kAhead][4], int g0, int g1, const Load &load, const Use &use) {
+    for (int g = g0; g < g1; g += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            if (g + i >= g1) break;
+            float e[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
+            if (g + i + kAhead < g1) load(x[i], g + i + kAhead);
+            use(e, g + i);
+        }
+    }
+}
 
-// A wave takes heads of one row: `lanes` = ceil(head_dim / 8) lanes a head,
-// 64 / lanes heads at a time, the next ones' loads in flight.
+// A wave takes heads of one row: `lanes` = ceil(head_dim / 4) lanes a head,
+// 64 / lanes heads (a group) at a time. Bound: memory for many rows (7,993 rows
+// of 32 x 128, 262 MB, at the rate of a large copy), launch and latency for few.
 template <int MODE, bool V>
 __global__ __launch_bounds__(kWaves * 64) void rope_rows_kernel(const Rope r, const float *x, int64_t x_stride,
                                                                 float *out, int64_t out_stride, int n_rows,
@@ -196,24 +222,24 @@ __global__ __launch_bounds__(kWaves * 64) void rope_rows_kernel(const Rope r, co
     // in the pairs' evaluation) and store nothing
     const bool spare = lane >= per * lanes;
     const int h = spare ? per - 1 : lane / lanes;
-    const int e0 = spare ? 0 : (lane - h * lanes) * 8;
+    const int e0 = spare ? 0 : (lane - h * lanes) * 4;
     const int groups = (n_heads + per - 1) / per;
-    const int g0 = groups * part / parts, g1 = groups * (part + 1) / parts;
+    const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
     const float *src = x + row * x_stride + e0;
     float *dst = out + row * out_stride + e0;
-    float next[8];
-    const auto load = [&](int g) { load8<V>(next, src + (int64_t)min(g * per + h, n_heads - 1) * head_dim, head_dim - e0); };
-    load(g0);
-    const Turn<MODE> t(r, lane, e0, h, head_dim, (double)pos[row], lds + wave * (wave_lds(MODE, r.pairs) / sizeof(double2)));
-    for (int g = g0; g < g1; g++) {
-        const int head = g * per + h;
-        float e[8];
+    const auto load = [&](float (&e)[4], int g) {
+        load4<V>(e, src + (int64_t)min(g * per + h, n_heads - 1) * head_dim, head_dim - e0);
+    };
+    float ring[kAhead][4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) e[j] = next[j];
-        if (g + 1 < g1) load(g + 1);
+    for (int i = 0; i < kAhead; i++)
+        if (g0 + i < g1) load(ring[i], g0 + i);
+    const Turn<MODE, V> t(r, lane, e0, h, head_dim, (double)pos[row], lds + wave * (wave_lds(MODE, r.pairs) / sizeof(double2)));
+    stream_groups(ring, g0, g1, load, [&](float (&e)[4], int g) {
         t.apply(e);
-        if (head < n_heads && !spare) store8<V>(dst + (int64_t)head * head_dim, e, head_dim - e0);
-    }
+        const int head = g * per + h;
+        if (head < n_heads && !spare) store4<V>(dst + (int64_t)head * head_dim, e, head_dim - e0);
+    });
 }
 
 // ---- append ---------------------------------------------------------------------
@@ -317,9 +343,9 @@ __device__ __forceinline__ void append_v_page(const Append &a, int b, int idx, i
     }
 }
 
-// A wave takes a part of one new row: its groups of 64 * 8 elements are those
-// of q, of K and (unless V goes page by page) of V in turn, head_dim / 8 lanes a
-// head, the next group's loads in flight.
+// A wave takes a part of one new row: its groups of 64 * 4 elements are those
+// of q, of K and (unless V goes page by page) of V in turn, head_dim / 4 lanes a
+// head.
 template <int MODE, bool V>
 __global__ __launch_bounds__(kWaves * 64) void kv_append_kernel(const Append a) {
     extern __shared__ double2 lds[];
@@ -339,14 +365,13 @@ __global__ __launch_bounds__(kWaves * 64) void kv_append_kernel(const Append a) 
     const int64_t pos = (int64_t)a.pos_offset[b] + i;
 
     const int head_dim = a.o.head_dim;
-    const int lanes = head_dim >> 3, per = 64 / lanes;
+    const int lanes = head_dim >> 2, per = 64 / lanes;
     const int h = lane / lanes;
-    const int e0 = (lane - h * lanes) * 8;
+    const int e0 = (lane - h * lanes) * 4;
     const int gq = a.q ? (a.n_heads + per - 1) / per : 0, gk = (a.n_kv + per - 1) / per;
     const int groups = gq + (a.v_by_page ? gk : 2 * gk);
-    const int g0 = groups * part / a.parts, g1 = groups * (part + 1) / a.parts;
-    float next[8];
-    const auto load = [&](int g) {
+    const int g0 = (int)((int64_t)groups * part / a.parts), g1 = (int)((int64_t)groups * (part + 1) / a.parts);
+    const auto load = [&](float (&e)[4], int g) {
         const float *src;
         if (g < gq) {
             src = a.q + r * a.q_stride + min(g * per + h, a.n_heads - 1) * head_dim;
@@ -355,45 +380,40 @@ __global__ __launch_bounds__(kWaves * 64) void kv_append_kernel(const Append a) 
             const int head = min((g - gq - (v ? gk : 0)) * per + h, a.n_kv - 1);
             src = (v ? a.v + r * a.v_stride : a.k + r * a.k_stride) + head * head_dim;
         }
-        load8<V>(next, src + e0, 8);
+        load4<V>(e, src + e0, 4);
     };
-    load(g0);
+    float ring[kAhead][4];
+#pragma unroll
+    for (int n = 0; n < kAhead; n++)
+        if (g0 + n < g1) load(ring[n], g0 + n);
     int64_t row = -1;
     if (g1 > gq && pos >= 0 && pos < a.pm.pos_limit) {
         const int64_t page = storage_page(a.pm, b, pos >> 4);
         if (page >= 0) row = page * GLA_PAGE_SIZE + (pos & 15);
     }
-    const auto rest = [&](auto &t) {
-        for (int g = g0; g < g1; g++) {
-            float e[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) e[j] = next[j];
-            if (g + 1 < g1) load(g + 1);
+    const auto rest = [&](const auto &t) {
+        stream_groups(ring, g0, g1, load, [&](float (&e)[4], int g) {
             if (g < gq + gk) t.apply(e);
             if (g < gq) {
                 const int head = g * per + h;
-                if (head < a.n_heads) store8<V>(a.q_out + (r * a.n_heads + head) * head_dim + e0, e, 8);
-                continue;
+                if (head < a.n_heads) store4<V>(a.q_out + (r * a.n_heads + head) * head_dim + e0, e, 4);
+                return;
             }
             const int which = g >= gq + gk;
             const int head = (g - gq - which * gk) * per + h;
-            if (head >= a.n_kv || row < 0) continue;
+            if (head >= a.n_kv || row < 0) return;
             const int gi = head * head_dim + e0;
             if (a.o.q8)
                 store_q8(a.o, row, gi, which, e);
             else
-                store8<true>(reinterpret_cast<float *>(const_cast<uint8_t *>(which ? a.o.L.v : a.o.L.k) +
-                                                       elem_off(a.o, row, gi, 4)), e, 8);
-        }
+                store4<true>(reinterpret_cast<float *>(const_cast<uint8_t *>(which ? a.o.L.v : a.o.L.k) +
+                                                       elem_off(a.o, row, gi, 4)), e, 4);
+        });
     };
-    if (MODE == kCopy || g0 >= gq + gk) {
-        const Turn<kCopy> t(a.rope, lane, e0, h, head_dim, 0.0, nullptr);
-        rest(t);
-    } else {
-        const Turn<MODE> t(a.rope, lane, e0, h, head_dim, (double)pos,
-                           lds + wave * (wave_lds(MODE, a.rope.pairs) / sizeof(double2)));
-        rest(t);
-    }
+    if (MODE == kCopy || g0 >= gq + gk)
+        rest(Turn<kCopy, V>(a.rope, lane, e0, h, head_dim, 0.0, nullptr));
+    else
+        rest(Turn<MODE, V>(a.rope, lane, e0, h, head_dim, (double)pos, lds + wave * (wave_lds(MODE, a.rope.pairs) / sizeof(double2))));
 }
 
 bool aligned16(const void *p, int64_t stride) { return ((uintptr_t)p & 15) == 0 && stride % 4 == 0; }
@@ -407,11 +427,15 @@ int check_plan(const gla_ctx *ctx, const gla_rope_plan *r, const char *fn) {
 
 Rope rope_of(const gla_rope_plan *p) { return Rope{p->turns, p->pairs, p->amplitude}; }
 
-// Parts of a row's `groups` that waves take: enough waves to fill the chip's
-// 1,024 SIMDs a few times over, at most one group each.
-int parts_of(int64_t rows, int groups) {
-    const int64_t want = (4096 + rows - 1) / rows;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(groups, want));
+// Parts of a row's `groups` that waves take: about `waves` of them in all, at
+// most one group each. Short waves keep the last round of a long call short;
+// waves of rows that ragged sequences do not have cost an append a little. us
+// for 4,096 / 16,384 / 32,768 / 65,536 / 131,072: 7,993 query rows 55.3 / 51.6 /
+// 50.3 / 49.5 / 48.9, ragged prompts into a Q8_0 pool (append and read) 96 / 90 /
+// 92 / 96 / 107, into f32 caches 68.7 / 60.9 / 58.8 / 64.2 / 70.5.
+constexpr int kRopeWaves = 65536, kAppendWaves = 24576;
+int parts_of(int64_t rows, int groups, int waves) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(groups, (waves + rows - 1) / rows));
 }
 
 // The frequencies and the amplitude of a specification, or an error.
@@ -555,10 +579,10 @@ int gla_rope_rows(gla_ctx *ctx, const gla_rope_plan *plan, const float *x, int64
     GLA_REQUIRE(x != out || x_stride == out_stride, "gla_rope_rows: in place needs one stride");
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
     const int d = plan->head_dim;
-    const int lanes = (d + 7) / 8, per = 64 / lanes;
-    const int parts = parts_of(n_rows, (n_heads + per - 1) / per);
+    const int lanes = (d + 3) / 4, per = 64 / lanes;
+    const int parts = parts_of(n_rows, (n_heads + per - 1) / per, kRopeWaves);
     const unsigned blocks = (unsigned)(((int64_t)n_rows * parts + kWaves - 1) / kWaves);
-    const bool vec = d % 8 == 0 && aligned16(x, x_stride) && aligned16(out, out_stride);
+    const bool vec = d % 4 == 0 && aligned16(x, x_stride) && aligned16(out, out_stride);
     auto kernel = plan->half ? (vec ? rope_rows_kernel<kHalf, true> : rope_rows_kernel<kHalf, false>)
                              : (vec ? rope_rows_kernel<kAdjacent, true> : rope_rows_kernel<kAdjacent, false>);
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kWaves * 64), kWaves * wave_lds(plan->half ? kHalf : kAdjacent, plan->pairs),
@@ -613,10 +637,10 @@ int gla_kv_append(gla_ctx *ctx, const gla_append_args *a) {
     // V of a Q8_0 storage page by page where a sequence's rows fill pages, else
     // with its row
     p.v_by_page = p.o.q8 && p.max_q_len >= kVByPage;
-    const int per = 64 / (kv->head_dim / 8);
+    const int per = 64 / (kv->head_dim / 4);
     const int gk = (p.n_kv + per - 1) / per;
     const int groups = (a->q ? (a->n_heads + per - 1) / per : 0) + (p.v_by_page ? gk : 2 * gk);
-    p.parts = parts_of((int64_t)a->n_seqs * a->max_q_len, groups);
+    p.parts = parts_of((int64_t)a->n_seqs * a->max_q_len, groups, kAppendWaves);
     const int64_t row_blocks = ((int64_t)p.max_q_len * p.parts + kWaves - 1) / kWaves;
     const int64_t chunks = ((int64_t)p.max_q_len + GLA_PAGE_SIZE - 2) / GLA_PAGE_SIZE + 1;  // pages a sequence may touch
     const int64_t v_blocks = p.v_by_page ? (chunks * p.n_kv * (kv->head_dim / 64) + kWaves - 1) / kWaves : 0;

@@ -70,22 +70,26 @@ __device__ __forceinline__ int8_t quantize_one(float x, float inv_d) {
     return (r != r) ? (int8_t)0 : (int8_t)r;
 }
 
-// Quantise and store the 8 elements gi .. gi + 7 of a row's K (which = 0) or V
-// (1); the block's other 24 are in the three neighbouring lanes of an aligned
-// group of four, which run this together.
-__device__ __forceinline__ void store_q8(const RowOps &o, int64_t row, int gi, int which, const float (&x)[8]) {
+// Quantise and store the N (8 or 4) elements gi .. gi + N - 1 of a row's K
+// (which = 0) or V (1); the rest of the block of 32 is in the neighbouring lanes
+// of an aligned group of 32 / N, which run this together.
+template <int N>
+__device__ __forceinline__ void store_q8(const RowOps &o, int64_t row, int gi, int which, const float (&x)[N]) {
+    static_assert(N == 4 || N == 8, "blocks of 32 in 8 or 4 lanes");
     uint8_t *dst = const_cast<uint8_t *>(which ? o.L.v : o.L.k);
     float max_abs = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) max_abs = fmaxf(max_abs, fabsf(x[j]));
-    // quad_perm [1 0 3 2], then [2 3 0 1]
+    for (int j = 0; j < N; j++) max_abs = fmaxf(max_abs, fabsf(x[j]));
+    // quad_perm [1 0 3 2], then [2 3 0 1]; of eight lanes then the other quad
     max_abs = fmaxf(max_abs, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(max_abs), 0xB1, 0xf, 0xf, true)));
     max_abs = fmaxf(max_abs, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(max_abs), 0x4E, 0xf, 0xf, true)));
+    if (N == 4)
+        max_abs = fmaxf(max_abs, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(max_abs), 0x141, 0xf, 0xf, true)));
     const float dsc = max_abs > 0.0f ? max_abs / 127.0f : 1.0f;
     const float inv_d = 1.0f / dsc;
-    uint32_t w[2];
+    uint32_t w[N / 4];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < N / 4; j++) {
         const uint32_t b0 = (uint8_t)quantize_one(x[4 * j + 0], inv_d);
         const uint32_t b1 = (uint8_t)quantize_one(x[4 * j + 1], inv_d);
         const uint32_t b2 = (uint8_t)quantize_one(x[4 * j + 2], inv_d);
@@ -93,10 +97,14 @@ __device__ __forceinline__ void store_q8(const RowOps &o, int64_t row, int gi, i
         w[j] = (b0 | (b1 << 8) | (b2 << 16) | (b3 << 24)) ^ 0x80808080u;  // stored as x + 128
     }
     if (!which) {  // K: 8 dims of a slot are 8 consecutive bytes
-        *reinterpret_cast<uint2 *>(dst + q8_off(o, row, gi, 0)) = make_uint2(w[0], w[1]);
+        uint8_t *at = dst + q8_off(o, row, gi, 0);
+        if constexpr (N == 8)
+            *reinterpret_cast<uint2 *>(at) = make_uint2(w[0], w[1]);
+        else
+            *reinterpret_cast<uint32_t *>(at) = w[0];
     } else {  // V: one byte per element, 4-position columns
 #pragma unroll
-        for (int j = 0; j < 8; j++) dst[q8_off(o, row, gi + j, 1)] = (uint8_t)(w[j >> 2] >> ((j & 3) * 8));
+        for (int j = 0; j < N; j++) dst[q8_off(o, row, gi + j, 1)] = (uint8_t)(w[j >> 2] >> ((j & 3) * 8));
     }
     if ((gi & 31) == 0) {
         uint8_t *sb = const_cast<uint8_t *>(which ? o.L.vs : o.L.ks);

@@ -372,7 +372,7 @@ typedef enum gla_rope_scaling {
     GLA_ROPE_YARN = 3
 } gla_rope_scaling;
 typedef struct gla_rope_spec {
-    int head_dim; /* 1 .. 512 */
+    int head_dim; /* 1 .. 256 */
     int rot_dim;  /* rotated dimensions of a head, even, <= head_dim; 0: all (head_dim even) */
     int freq_dim; /* the exponent's denominator; 0: rot_dim (gla_rope's is head_dim) */
     gla_rope_layout layout;

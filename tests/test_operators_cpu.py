@@ -46,7 +46,7 @@ def test_bands_and_yarn_end_at_both_frequencies(hip_lib):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(head_dim=0), dict(head_dim=-2), dict(head_dim=513), dict(head_dim=7), dict(head_dim=64, rot_dim=66),
+    dict(head_dim=0), dict(head_dim=-2), dict(head_dim=257), dict(head_dim=7), dict(head_dim=64, rot_dim=66),
     dict(head_dim=64, rot_dim=31), dict(head_dim=64, rot_dim=-2), dict(head_dim=64, freq_dim=-1),
     dict(head_dim=64, freq_base=0.0), dict(head_dim=64, freq_base=-1.0), dict(head_dim=64, freq_base=float("nan")),
     dict(head_dim=64, freq_base=float("inf")), dict(head_dim=64, scaling="linear", factor=0.0),
