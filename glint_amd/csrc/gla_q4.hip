@@ -18,6 +18,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gla_internal.h"
 
@@ -113,63 +114,931 @@ __global__ __launch_bounds__(256) void q4_repack_kernel(const uint8_t *ggml, int
     }
 }
 
-// ---- the product --------------------------------------------------------------------
+// ---- operands ----------------------------------------------------------------------
 
-__device__ __forceinline__ float half_of(uint32_t w, int hi) {
-    return __half2float(__ushort_as_half((unsigned short)(hi ? w >> 16 : w & 0xffffu)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ half2v h2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
+__device__ __forceinline__ half2v both(float x) { return half2v{(_Float16)x, (_Float16)x}; }
+__device__ __forceinline__ float lo_of(uint32_t w) { return (float)h2(w)[0]; }
+__device__ __forceinline__ float hi_of(uint32_t w) { return (float)h2(w)[1]; }
+
+// The 8 nibbles of a dword as halves n * s + b, where lo = {s, b - 1024 s} and
+// hi = {s / 16, b - 64 s}: a nibble under the bits of 1024 is 1024 + n, four bits
+// further up 1024 + 16 n. Every result here is exact.
+struct Scale2 {
+    half2v s, b;
+};
+// (u & mask) | 0x64006400 in one instruction, which needs the constant in a register
+__device__ __forceinline__ half2v under_1024(uint32_t u, uint32_t mask) {
+    uint32_t o, k = 0x64006400u;
+    asm("" : "+v"(k));
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(o) : "v"(u), "s"(mask), "v"(k));
+    return h2(o);
+}
+__device__ __forceinline__ half8 nibbles(uint32_t w, const Scale2 &lo, const Scale2 &hi) {
+    half8 o;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t u = w >> (8 * i);
+        const half2v a = __builtin_elementwise_fma(under_1024(u, 0x000f000fu), lo.s, lo.b);
+        const half2v b = __builtin_elementwise_fma(under_1024(u, 0x00f000f0u), hi.s, hi.b);
+        o[4 * i] = a[0];
+        o[4 * i + 1] = a[1];
+        o[4 * i + 2] = b[0];
+        o[4 * i + 3] = b[1];
+    }
+    return o;
+}
+// Q4_0: n - 8
+__device__ __forceinline__ half8 nibbles_q4_0(uint32_t w) {
+    return nibbles(w, {both(1.0f), both(-1032.0f)}, {both(0.0625f), both(-72.0f)});
+}
+// byte j of w, as both halves of a pair
+__device__ __forceinline__ half2v byte_pair(uint32_t w, int j) {
+    return h2(__builtin_amdgcn_perm(0x64646464u, w, 0x07000700u | (uint32_t)j | (uint32_t)j << 16)) - both(1024.0f);
+}
+// Q4_K: n * (scale byte j of sc), at most 15 * 63
+__device__ __forceinline__ half8 nibbles_q4_k(uint32_t w, uint32_t sc, int j) {
+    const half2v s = byte_pair(sc, j);
+    return nibbles(w, {s, s * both(-1024.0f)}, {s * both(0.0625f), s * both(-64.0f)});
+}
+// Q4_K: 32 times the four minimum bytes
+__device__ __forceinline__ half4 minima(uint32_t mn) {
+    const half2v a = __builtin_elementwise_fma(h2(__builtin_amdgcn_perm(0x64646464u, mn, 0x07010700u)), both(32.0f), both(-32768.0f));
+    const half2v b = __builtin_elementwise_fma(h2(__builtin_amdgcn_perm(0x64646464u, mn, 0x07030702u)), both(32.0f), both(-32768.0f));
+    return half4{a[0], a[1], b[0], b[1]};
 }
 
-// y[v][row], one wave per row tile, up to 4 vectors a workgroup row: each lane
-// multiplies its row's elements in f32 and the four element groups are summed.
-template <bool K>
-__global__ __launch_bounds__(64) void matvec_q4_plain_kernel(const Weights w, const float *x, int n_vec, float *y) {
-    const int lane = threadIdx.x;
-    const int tile = blockIdx.x;
-    const int r = lane & 15, kg = lane >> 4;
-    const int v0 = blockIdx.y * 4;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int quad = 0; quad < w.n_quads; quad++) {
-        const int64_t tq = (int64_t)tile * w.n_quads + quad;
-        const uint4 q = *reinterpret_cast<const uint4 *>(w.quants + (tq * 64 + lane) * 16);
-        const uint2 a = *reinterpret_cast<const uint2 *>(w.aux + (tq * 16 + r) * 8);
-        const uint32_t sup = K ? w.super[((int64_t)tile * (w.n_quads / 2) + quad / 2) * 16 + r] : 0;
-        const uint32_t qs[4] = {q.x, q.y, q.z, q.w};
+// x enters the products as two halves, hi = f16(x 2^s) and lo = f16(x 2^s - hi),
+// s bringing the largest finite |x| of a range into [2^13, 2^14): 22 bits of every
+// value whose size matters. An infinity is its own hi piece (lo 0), a NaN both.
+// The range's largest |x| is kept as bits, which order as the values do.
+constexpr uint32_t kInf = 0x7f800000u;
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ int shift_of(uint32_t mx) { return min(140 - (int)(mx >> 23), 120); }
+__device__ __forceinline__ float exp2_of(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    // within a row of 16 lanes by rotation, then rows 0/1 and 2/3, then the halves
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max(b[0], b[1]);
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0xB1, 0xf, 0xf, true));
+    return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x4E, 0xf, 0xf, true));
+}
+// Pieces of x * mul (a power of two); `odd`: the range has an infinity or a NaN.
+__device__ __forceinline__ void pieces(float x, float mul, bool odd, _Float16 &hi, _Float16 &lo) {
+    hi = (_Float16)(x * mul);
+    lo = (_Float16)fmaf(x, mul, -(float)hi);
+    if (odd && abs_bits(x) == kInf) lo = (_Float16)0.0f;
+}
+// 8 floats from byte `at` of a row's `bytes` (wave-uniform), zeros past them: the
+// bounds check of the buffer loads, which also take rows at any 4-byte address.
+__device__ __forceinline__ void load_row(float (&e)[8], const float *row, int bytes, int at) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(row), 0, bytes, 0x00027000);
+    const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0), b = __builtin_amdgcn_raw_buffer_load_b128(r, at + 16, 0, 0);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int c = quad * 128 + j * 32 + kg * 8;
-            if (c >= w.cols) continue;
-            const float s = K ? half_of(sup, 0) * (float)((a.x >> (8 * j)) & 255u) : half_of(j < 2 ? a.x : a.y, j & 1);
-            const float m = K ? half_of(sup, 1) * (float)((a.y >> (8 * j)) & 255u) : 0.0f;
+    for (int j = 0; j < 4; j++) {
+        e[j] = __uint_as_float(a[j]);
+        e[4 + j] = __uint_as_float(b[j]);
+    }
+}
+
+// ---- up to 8 vectors ------------------------------------------------------------------
+
+// y[v][row] for up to NV vectors, RT row tiles a workgroup. The eight waves split
+// K; a wave takes its quads four at a time (a chunk of 512 columns): its lanes load
+// 8 elements of each vector, find the chunk's largest |x| of each vector, and put
+// the pieces into the wave's LDS in the order of the B operand, whose 16 columns
+// are the hi pieces of the vectors and then their lo pieces: one MFMA multiplies
+// 16 rows x 32 columns of weights with all of them. No wave waits for another
+// until the sums are merged.
+//   Q4_0: a group's product times its rows' scales goes into the sum (C = A B is
+//   16 rows x 16 columns, lane (column l % 16, rows l / 16 * 4 + r)).
+//   Q4_K: A holds nibble * scale, exact, so a quad's four groups add up in the
+//   MFMA; the rows' d multiplies once a quad. The minima are a product of their
+//   own: four minima of a row with the sums of x over the four groups (in pieces,
+//   scaled by 2^-5; the minima carry 2^5).
+constexpr int kChunk = 4;  // quads
+constexpr int kFewWaves = 8;
+template <bool K, int NV, int RT>
+__global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Weights w, const float *x, int n_vec, float *y) {
+    constexpr int COLS = 2 * NV;
+    constexpr int PITCH = 65;             // half8 from column to column: 64 of [group][kg], and one for the banks
+    constexpr int PIECES = COLS * PITCH;  // of a wave's chunk
+    constexpr int SUMS = K ? kChunk * COLS : 0;    // half4: [quad][column]
+    constexpr int WAVE = PIECES * 16 + SUMS * 8;
+    constexpr int RED = kFewWaves * RT * 64 * 16;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kFewWaves * WAVE > RED ? kFewWaves * WAVE : RED];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, kg = lane >> 4;
+    half8 *px = reinterpret_cast<half8 *>(lds + wave * WAVE);
+    half4 *ps = reinterpret_cast<half4 *>(lds + wave * WAVE + PIECES * 16);
+    constexpr int UNIT = K ? 2 : 1;  // whole superblocks a wave
+    const int per = (w.n_quads / UNIT + kFewWaves - 1) / kFewWaves * UNIT;
+    const int q0 = min(w.n_quads, wave * per), q1 = min(w.n_quads, q0 + per);
+    const int tile0 = blockIdx.x * RT;
+
+    floatx4 total[RT];
 #pragma unroll
-            for (int v = 0; v < 4; v++) {
-                if (v0 + v >= n_vec) continue;
-                const float *xv = x + (int64_t)(v0 + v) * w.cols + c;
-                float t = 0.0f, sum = 0.0f;
+    for (int t = 0; t < RT; t++) total[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    for (int c0 = q0; c0 < q1; c0 += kChunk) {
+        // x first: loads return in order, so the pieces do not wait for weights
+        float e[NV][8];
+        const int bytes = (min(w.cols, q1 * 128) - c0 * 128) * 4;  // of the wave's columns from here on
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float n = (float)((qs[j] >> (e / 2 * 4 + e % 2 * 16)) & 15u) - (K ? 0.0f : 8.0f);
-                    t = fmaf(n, xv[e], t);
-                    sum += xv[e];
+        for (int v = 0; v < NV; v++)
+            load_row(e[v], x + (int64_t)min(v, n_vec - 1) * w.cols + c0 * 128, v < n_vec ? bytes : 0, lane * 32);
+        u32x4 qw[RT][kChunk];
+        u32x4 sc[RT][kChunk][2];      // Q4_0: the 32 bytes of rows kg * 4 .. +3
+        u32x2 am[RT][kChunk];         // Q4_K: the lane's row's scales and minima
+        u32x4 sup[RT][kChunk / 2];  // Q4_K: d and dmin of rows kg * 4 .. +3
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int i = 0; i < kChunk; i++) {
+                const int64_t tq = (int64_t)min(tile0 + t, w.n_tiles - 1) * w.n_quads + min(c0 + i, w.n_quads - 1);
+                qw[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(w.quants + (tq * 64 + lane) * 16));
+                if constexpr (K) {
+                    am[t][i] = *reinterpret_cast<const u32x2 *>(w.aux + (tq * 16 + col) * 8);
+                } else {
+                    const u32x4 *s = reinterpret_cast<const u32x4 *>(w.aux + (tq * 16 + kg * 4) * 8);
+                    sc[t][i][0] = s[0];
+                    sc[t][i][1] = s[1];
                 }
-                acc[v] = fmaf(t, s, acc[v]);
-                if (K) acc[v] = fmaf(-sum, m, acc[v]);
+            }
+        if constexpr (K) {
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+#pragma unroll
+                for (int i = 0; i < kChunk / 2; i++) {
+                    const int sb = min((c0 >> 1) + i, w.n_quads / 2 - 1);
+                    sup[t][i] = *reinterpret_cast<const u32x4 *>(
+                        w.super + ((int64_t)min(tile0 + t, w.n_tiles - 1) * (w.n_quads / 2) + sb) * 16 + kg * 4);
+                }
+        }
+        float undo = 0.0f;  // 2^-s of the lane's column
+        uint32_t mx[NV];
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            mx[v] = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) mx[v] = max(mx[v], abs_bits(e[v][j]));
+            mx[v] = wave_max(mx[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            uint32_t top = __builtin_amdgcn_readfirstlane(mx[v]);
+            const bool odd = top >= kInf;
+            if (odd) {  // scaled by what is finite
+                mx[v] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) mx[v] = max(mx[v], abs_bits(e[v][j]) < kInf ? abs_bits(e[v][j]) : 0);
+                top = __builtin_amdgcn_readfirstlane(wave_max(mx[v]));
+            }
+            const int sh = shift_of(top);
+            const float mul = exp2_of(sh);
+            if (col == v || col == NV + v) undo = exp2_of(-sh);
+            half8 hi, lo;
+            float sum = 0.0f;
+            const auto split = [&](bool odd) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    _Float16 a, b;
+                    pieces(e[v][j], mul, odd, a, b);
+                    hi[j] = a;
+                    lo[j] = b;
+                    sum = fmaf(e[v][j], mul, sum);
+                }
+            };
+            if (odd)
+                split(true);
+            else
+                split(false);
+            px[v * PITCH + lane] = hi;  // lane = group * 4 + kg of the chunk
+            px[(NV + v) * PITCH + lane] = lo;
+            if constexpr (K) {
+                _Float16 a, b;
+                pieces(quad_sum(sum), 0.03125f, true, a, b);
+                if ((lane & 3) == 0) {
+                    _Float16 *to = reinterpret_cast<_Float16 *>(ps + (lane >> 4) * COLS) + ((lane >> 2) & 3);
+                    to[v * 4] = a;
+                    to[(NV + v) * 4] = b;
+                }
             }
         }
-    }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        floatx4 acc[RT];
 #pragma unroll
-    for (int v = 0; v < 4; v++) {
-        acc[v] += __shfl_xor(acc[v], 16);
-        acc[v] += __shfl_xor(acc[v], 32);
-        const int row = tile * 16 + r;
-        if (kg == 0 && row < w.rows && v0 + v < n_vec) y[(int64_t)(v0 + v) * w.rows + row] = acc[v];
+        for (int t = 0; t < RT; t++) acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kChunk; i++) {
+            if (c0 + i >= q1) break;
+            half8 bx[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                bx[j] = half8{};
+                if (col < COLS) bx[j] = px[col * PITCH + (i * 4 + j) * 4 + kg];
+            }
+            if constexpr (K) {
+                half4 bs = {};
+                if (col < COLS && kg == 0) bs = ps[i * COLS + col];
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    floatx4 c = zero;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nibbles_q4_k(qw[t][i][j], am[t][i][0], j), bx[j], c, 0, 0, 0);
+                    half4 mn = minima(am[t][i][1]);
+                    if (kg) mn = half4{};
+                    const floatx4 m = __builtin_amdgcn_mfma_f32_16x16x16f16(mn, bs, zero, 0, 0, 0);
+                    const u32x4 dd = sup[t][i >> 1];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        acc[t][r] = fmaf(c[r], lo_of(dd[r]), acc[t][r]);
+                        acc[t][r] = fmaf(-m[r], hi_of(dd[r]), acc[t][r]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const floatx4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nibbles_q4_0(qw[t][i][j]), bx[j], zero, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const uint32_t s = sc[t][i][r >> 1][(r & 1) * 2 + (j >> 1)];
+                            acc[t][r] = fmaf(c[r], (j & 1) ? hi_of(s) : lo_of(s), acc[t][r]);
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++) total[t] += acc[t] * undo;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the pieces are read before the next chunk's are written
+        __builtin_amdgcn_wave_barrier();
     }
+
+    // the waves in order, the hi and then the lo column of a vector
+    __syncthreads();
+    floatx4 *red = reinterpret_cast<floatx4 *>(lds);
+#pragma unroll
+    for (int t = 0; t < RT; t++) red[(wave * RT + t) * 64 + lane] = total[t];
+    __syncthreads();
+    for (int i = threadIdx.x; i < RT * 16 * NV; i += kFewWaves * 64) {
+        const int rr = i & 15, t = (i >> 4) % RT, v = (i >> 4) / RT;
+        const float *f = reinterpret_cast<const float *>(red) + (t * 64 + (rr >> 2) * 16) * 4 + (rr & 3);
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kFewWaves; k++) sum += f[k * RT * 256 + v * 4] + f[k * RT * 256 + (NV + v) * 4];
+        const int row = (tile0 + t) * 16 + rr;
+        if (v < n_vec && row < w.rows) y[(int64_t)v * w.rows + row] = sum;
+    }
+}
+
+// ---- more vectors: the pieces of x, once per call ----------------------------------
+
+// A workgroup per vector: its scale from the largest finite |x| of the row, then
+// the pieces in B-operand order, xp[v / 16][group][piece][lane = kg * 16 + v % 16]
+// = 8 halves, zeros past the columns, and undo[v] = 2^-s. Q4_K: the sums of each
+// group, times 2^-5 and in pieces, xm[v / 16][quad][v % 16] = {hi of the quad's four
+// groups, lo of them}. Vectors up to the next 16 are left as they are: a column of
+// the product is its vector's alone.
+constexpr int kSplitThreads = 512;
+constexpr int kSplitUnits = 4;  // units of 8 elements a thread keeps; a wider row is read twice
+template <bool K>
+__global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x, int cols, int n_quads, _Float16 *xp,
+                                                                 _Float16 *xm, float *undo) {
+    const int v = blockIdx.x, t = threadIdx.x;
+    const float *row = x + (int64_t)v * cols;
+    const int units = n_quads * 16, in = cols / 8;
+    float e[kSplitUnits][8];
+    const auto load = [&](float (&d)[8], int u) { load_row(d, row, in * 32, u * 32); };  // zeros past the row
+    const auto bits_of = [](const float (&d)[8], bool finite) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t a = abs_bits(d[j]);
+            m = max(m, finite && a >= kInf ? 0u : a);
+        }
+        return m;
+    };
+    __shared__ uint32_t red[2][kSplitThreads / 64];
+    const auto group_max = [&](bool finite, int at) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < kSplitUnits; i++) m = max(m, bits_of(e[i], finite));
+        for (int u = kSplitUnits * kSplitThreads + t; u < in; u += kSplitThreads) {
+            float d[8];
+            load(d, u);
+            m = max(m, bits_of(d, finite));
+        }
+        m = wave_max(m);
+        if ((t & 63) == 0) red[at][t >> 6] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSplitThreads / 64; i++) m = max(m, red[at][i]);
+        return m;
+    };
+#pragma unroll
+    for (int i = 0; i < kSplitUnits; i++) load(e[i], i * kSplitThreads + t);
+    uint32_t top = group_max(false, 0);
+    const bool odd = top >= kInf;
+    if (odd) top = group_max(true, 1);
+    const int sh = shift_of(top);
+    const float mul = exp2_of(sh);
+    if (t == 0) undo[v] = exp2_of(-sh);
+    const auto put = [&](const float (&d)[8], int u) {
+        half8 hi, lo;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            _Float16 a, b;
+            pieces(d[j], mul, odd, a, b);
+            hi[j] = a;
+            lo[j] = b;
+            sum = fmaf(d[j], mul, sum);
+        }
+        _Float16 *to = xp + (((int64_t)(v >> 4) * n_quads * 4 + (u >> 2)) * 128 + (u & 3) * 16 + (v & 15)) * 8;
+        *reinterpret_cast<half8 *>(to) = hi;
+        *reinterpret_cast<half8 *>(to + 512) = lo;
+        if constexpr (K) {
+            _Float16 a, b;
+            pieces(quad_sum(sum), 0.03125f, true, a, b);  // units of a group are four neighbouring threads
+            if ((u & 3) == 0) {
+                _Float16 *m = xm + (((int64_t)(v >> 4) * n_quads + (u >> 4)) * 16 + (v & 15)) * 8 + ((u >> 2) & 3);
+                m[0] = a;
+                m[4] = b;
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kSplitUnits; i++)
+        if (i * kSplitThreads + t < units) put(e[i], i * kSplitThreads + t);
+    for (int u = kSplitUnits * kSplitThreads + t; u < units; u += kSplitThreads) {
+        float d[8];
+        load(d, u);
+        put(d, u);
+    }
+}
+
+struct Pieces {
+    const _Float16 *xp;
+    const _Float16 *xm;
+    const float *undo;
+};
+
+// ---- up to 64 vectors --------------------------------------------------------------
+
+constexpr int kMidWaves = 8;
+constexpr int kMaxSlices = 8;
+
+__device__ __forceinline__ floatx4 load_agent4(const float *p) {
+    uint64_t *q = reinterpret_cast<uint64_t *>(const_cast<float *>(p));
+    const uint64_t a = __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint64_t b = __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return floatx4{__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)b),
+                   __uint_as_float((uint32_t)(b >> 32))};
+}
+
+// y[v][row] for RT row tiles x up to 16 NVT VH vectors a workgroup, and one of
+// gridDim.y slices of K: the eight waves are VH ranges of vectors x 8 / VH ranges of
+// the slice's quads. Every fragment of x that a wave reads serves RT row tiles, every
+// fragment of weights NVT vector tiles; x comes D groups ahead, the weights a quad
+// ahead. Bound: the pieces of x, which a workgroup reads whole but for its slice (64
+// vectors of 4,096: 1 MB, 256 MB through the L2s from 256 workgroups at ~24 TB/s), so
+// many vectors take more rows and a slice of K. The waves are merged in LDS in order;
+// with slices the sums go out as agent-scope stores, and the row group's last
+// workgroup to arrive adds the slices in order.
+template <bool K, int NVT, int RT, int VH>
+__global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Weights w, const Pieces px, int n_vec, float *y,
+                                                                      float *part, int64_t slice_stride,
+                                                                      int32_t *arrivals) {
+    constexpr int UNIT = K ? 2 : 1, D = NVT * RT <= 4 && NVT <= 2 ? 4 : 2, KW = kMidWaves / VH;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, kg = lane >> 4;
+    const int tile0 = blockIdx.x * RT;
+    const int vt0 = wave / KW * NVT, last_vt = (n_vec - 1) >> 4;
+    const int units = w.n_quads / UNIT;
+    const int ps = (units + gridDim.y - 1) / gridDim.y;
+    const int s0 = min(units, (int)blockIdx.y * ps), s1 = min(units, s0 + ps);
+    const int per = (s1 - s0 + KW - 1) / KW;
+    const int q0 = min(s1, s0 + wave % KW * per) * UNIT, q1 = min(s1, s0 + (wave % KW + 1) * per) * UNIT;
+    const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+
+    floatx4 acc[RT][NVT];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int v = 0; v < NVT; v++) acc[t][v] = zero;
+
+    half8 bh[D][NVT], bl[D][NVT];
+    const auto load_x = [&](half8 (&h)[NVT], half8 (&l)[NVT], int group) {
+#pragma unroll
+        for (int v = 0; v < NVT; v++) {
+            const _Float16 *src = px.xp + (((int64_t)min(vt0 + v, last_vt) * w.n_quads * 4 + group) * 128 + lane) * 8;
+            h[v] = *reinterpret_cast<const half8 *>(src);
+            l[v] = *reinterpret_cast<const half8 *>(src + 512);
+        }
+    };
+    // sc: Q4_0 the 32 bytes of the C rows' scales; Q4_K [0] the A row's scales and
+    // minima, [1] the C rows' d and dmin. bm: Q4_K the sums of x.
+    u32x4 qw[RT], sc[RT][2];
+    half8 bm[NVT];
+    const auto load_w = [&](u32x4 (&q)[RT], u32x4 (&s)[RT][2], half8 (&m)[NVT], int quad) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int64_t tile = min(tile0 + t, w.n_tiles - 1);
+            const int64_t tq = tile * w.n_quads + quad;
+            q[t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(w.quants + (tq * 64 + lane) * 16));
+            if constexpr (K) {
+                const u32x2 a = *reinterpret_cast<const u32x2 *>(w.aux + (tq * 16 + col) * 8);
+                s[t][0] = u32x4{a[0], a[1], 0, 0};
+                s[t][1] = *reinterpret_cast<const u32x4 *>(w.super + (tile * (w.n_quads / 2) + (quad >> 1)) * 16 + kg * 4);
+            } else {
+                const u32x4 *p = reinterpret_cast<const u32x4 *>(w.aux + (tq * 16 + kg * 4) * 8);
+                s[t][0] = p[0];
+                s[t][1] = p[1];
+            }
+        }
+        if constexpr (K)
+#pragma unroll
+            for (int v = 0; v < NVT; v++)
+                m[v] = *reinterpret_cast<const half8 *>(px.xm + (((int64_t)min(vt0 + v, last_vt) * w.n_quads + quad) * 16 + col) * 8);
+    };
+    if (q0 < q1) {
+        load_w(qw, sc, bm, q0);
+#pragma unroll
+        for (int i = 0; i < D; i++) load_x(bh[i], bl[i], q0 * 4 + i);
+        __builtin_amdgcn_sched_barrier(0);
+        for (int q = q0; q < q1; q++) {
+            u32x4 qn[RT], sn[RT][2];
+            half8 mn[NVT];
+            load_w(qn, sn, mn, min(q + 1, q1 - 1));
+            __builtin_amdgcn_sched_barrier(0);
+            floatx4 c[RT][NVT];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    const half8 a = K ? nibbles_q4_k(qw[t][j], sc[t][0][0], j) : nibbles_q4_0(qw[t][j]);
+#pragma unroll
+                    for (int v = 0; v < NVT; v++)
+                        c[t][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh[j % D][v], K && j ? c[t][v] : zero, 0, 0, 0);
+#pragma unroll
+                    for (int v = 0; v < NVT; v++)
+                        c[t][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl[j % D][v], c[t][v], 0, 0, 0);
+                    if constexpr (!K)
+#pragma unroll
+                        for (int v = 0; v < NVT; v++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const uint32_t s = sc[t][r >> 1][(r & 1) * 2 + (j >> 1)];
+                                acc[t][v][r] = fmaf(c[t][v][r], (j & 1) ? hi_of(s) : lo_of(s), acc[t][v][r]);
+                            }
+                }
+                load_x(bh[j % D], bl[j % D], min(q * 4 + j + D, q1 * 4 - 1));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (K)
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    // k = 0..3 the minima with the sums' hi pieces, 4..7 with their lo
+                    // ones; the other lanes' rows of A are zeros, their B is not
+                    const half4 m4 = minima(sc[t][0][1]);
+                    const half8 am = kg ? half8{} : half8{m4[0], m4[1], m4[2], m4[3], m4[0], m4[1], m4[2], m4[3]};
+#pragma unroll
+                    for (int v = 0; v < NVT; v++) {
+                        const floatx4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(am, kg ? half8{} : bm[v], zero, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            acc[t][v][r] = fmaf(c[t][v][r], lo_of(sc[t][1][r]), acc[t][v][r]);
+                            acc[t][v][r] = fmaf(-m[r], hi_of(sc[t][1][r]), acc[t][v][r]);
+                        }
+                    }
+                }
+#pragma unroll
+            for (int t = 0; t < RT; t++) qw[t] = qn[t], sc[t][0] = sn[t][0], sc[t][1] = sn[t][1];
+#pragma unroll
+            for (int v = 0; v < NVT; v++) bm[v] = mn[v];
+        }
+    }
+
+    // merge the waves through LDS, in order: 4 floats after every 16 lanes, so that
+    // a wave's reads of 16 rows x 4 vectors fall in distinct banks
+    constexpr int S = 272, VT = NVT * VH;
+    __shared__ __attribute__((aligned(16))) float red[KW * RT * VT * S];
+    const auto at = [&](int kw, int t, int v, int ln) { return ((kw * RT + t) * VT + v) * S + 4 * ln + 4 * (ln >> 4); };
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int v = 0; v < NVT; v++) *reinterpret_cast<floatx4 *>(&red[at(wave % KW, t, vt0 + v, lane)]) = acc[t][v];
+    __syncthreads();
+    const int n_slices = gridDim.y;
+    for (int i = threadIdx.x; i < RT * 16 * VT * 16; i += kMidWaves * 64) {
+        const int rl = i % (RT * 16), vv = i / (RT * 16);  // consecutive threads, consecutive rows
+        const int from = at(0, rl >> 4, vv >> 4, ((rl & 15) >> 2) * 16 + (vv & 15)) + (rl & 3);
+        float sum = red[from];
+#pragma unroll
+        for (int k = 1; k < KW; k++) sum += red[from + k * RT * VT * S];
+        const int row = tile0 * 16 + rl;
+        if (row < w.rows && vv < n_vec) {
+            const int64_t to = (int64_t)vv * w.rows + row;
+            if (n_slices > 1)
+                store_agent(part + blockIdx.y * slice_stride + to, sum);
+            else
+                y[to] = sum * px.undo[vv];
+        }
+    }
+    if (n_slices == 1) return;
+    __shared__ int lds_last;
+    if (!arrive_last(arrivals + blockIdx.x, n_slices, &lds_last)) return;
+    constexpr int NQ = RT * 16 * VT * 16 / 4;  // row quads
+    if (w.rows % 4 == 0 && ((uintptr_t)y & 15) == 0) {
+        for (int qd = threadIdx.x; qd < NQ; qd += kMidWaves * 64) {
+            const int vv = qd / (RT * 4), row = tile0 * 16 + 4 * (qd % (RT * 4));
+            if (row >= w.rows || vv >= n_vec) continue;
+            const int64_t to = (int64_t)vv * w.rows + row;
+            floatx4 t[kMaxSlices];
+#pragma unroll
+            for (int s = 0; s < kMaxSlices; s++)
+                if (s < n_slices) t[s] = load_agent4(part + s * slice_stride + to);
+            floatx4 sum = t[0];
+#pragma unroll
+            for (int s = 1; s < kMaxSlices; s++)
+                if (s < n_slices) sum += t[s];
+            *reinterpret_cast<floatx4 *>(y + to) = sum * px.undo[vv];
+        }
+    } else {
+        for (int i = threadIdx.x; i < NQ * 4; i += kMidWaves * 64) {
+            const int vv = i / (RT * 16), row = tile0 * 16 + i % (RT * 16);
+            if (row >= w.rows || vv >= n_vec) continue;
+            const int64_t to = (int64_t)vv * w.rows + row;
+            float sum = load_agent(part + to);
+            for (int s = 1; s < n_slices; s++) sum += load_agent(part + s * slice_stride + to);
+            y[to] = sum * px.undo[vv];
+        }
+    }
+}
+
+// ---- many vectors ----------------------------------------------------------------------
+
+__device__ __forceinline__ void store_agent2(float *p, float a, float b) {
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// y[v][row] for 128 rows x 32 VT vectors a workgroup, and one of gridDim.z slices of
+// K: four waves of 4 row tiles x VT vector tiles, 2 x 2 of them, which share weights
+// and pieces of x through LDS. A step is a group of 32 columns: the pieces come by
+// LDS copies two steps ahead into a ring of three, the weights of a quad of groups
+// (with scales, and for Q4_K the sums of x) during the quad before, each wave issuing
+// the same number of copies at the same step, so that the waits can count them. The
+// copies of steps past the end repeat the last ones.
+template <bool K, int VT>
+__global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w, const Pieces px, int n_vec, float *y,
+                                                             float *part, int64_t slice_stride, int32_t *arrivals) {
+    constexpr int RT = 4, UNIT = K ? 2 : 1;
+    constexpr int XS = 2 * VT * 2048;                    // a ring slot of x: the pieces of 2 VT tiles
+    constexpr int AUX = 2 * RT * 1024, SUP = AUX + 1024, XM = SUP + 1024, WS = K ? XM + 4096 : SUP;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[3 * XS + 2 * WS];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, kg = lane >> 4;
+    const int tile_wg = blockIdx.x * 2 * RT, vt_wg = blockIdx.y * 2 * VT;
+    const int rt0 = (wave & 1) * RT, vt0 = (wave >> 1) * VT;
+    const int last_tile = w.n_tiles - 1, last_vt = (n_vec - 1) >> 4;
+    const uint32_t base = __builtin_amdgcn_readfirstlane(
+        (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)&lds[0]);
+
+    const int units = w.n_quads / UNIT;
+    const int ps = (units + gridDim.z - 1) / gridDim.z;
+    const int q0 = min(units, (int)blockIdx.z * ps) * UNIT, q1 = min(units, (int)(blockIdx.z + 1) * ps) * UNIT;
+
+    // the wave's copies: VT of 2 VT x 2 pieces, two row tiles and their scales
+    const uint8_t *xsrc[VT];
+#pragma unroll
+    for (int c = 0; c < VT; c++) {
+        const int i = wave * VT + c;
+        xsrc[c] = reinterpret_cast<const uint8_t *>(px.xp) +
+                  (int64_t)min(vt_wg + (i >> 1), last_vt) * w.n_quads * 8192 + (i & 1) * 1024;
+    }
+    const int ta = min(tile_wg + 2 * wave, last_tile), tb = min(ta + 1, last_tile);
+    const uint8_t *qa = w.quants + (int64_t)ta * w.n_quads * 1024, *qb = w.quants + (int64_t)tb * w.n_quads * 1024;
+    const uint8_t *as = w.aux + (int64_t)ta * w.n_quads * 128;
+    const uint32_t aoff = (uint32_t)((lane >> 5) * (tb - ta)) * (uint32_t)w.n_quads * 128 + (lane & 31) * 4;
+    const uint8_t *ss = reinterpret_cast<const uint8_t *>(w.super) + (int64_t)ta * (w.n_quads / 2) * 64;
+    const uint32_t soff = (uint32_t)(((lane >> 4) & 1) * (tb - ta)) * (uint32_t)(w.n_quads / 2) * 64 + (lane & 15) * 4;
+    const int va = min(vt_wg + wave * (VT / 2), last_vt), vb = min(va + 1, last_vt);
+    const uint8_t *ms = reinterpret_cast<const uint8_t *>(px.xm) + (int64_t)va * w.n_quads * 256;
+    const uint32_t moff = (VT == 4 ? (uint32_t)(((lane >> 4) & 1) * (vb - va)) * (uint32_t)w.n_quads * 256 : 0u) + (lane & 15) * 16;
+    const auto copy_x = [&](int s, int slot) {
+#pragma unroll
+        for (int c = 0; c < VT; c++) lds_copy16(xsrc[c] + (int64_t)s * 2048, lane * 16, base + slot * XS + (wave * VT + c) * 1024);
+    };
+    const auto copy_w = [&](int as_quad, int q, int j) {  // part j of quad q's weights, where quad as_quad's go
+        const uint32_t to = base + 3 * XS + (as_quad & 1) * WS;
+        if (j == 0) {
+            lds_copy16(qa + (int64_t)q * 1024, lane * 16, to + 2 * wave * 1024);
+            if (K) lds_copy16(ms + (int64_t)q * 256, moff, to + XM + wave * 1024);
+        } else if (j == 1) {
+            lds_copy16(qb + (int64_t)q * 1024, lane * 16, to + (2 * wave + 1) * 1024);
+        } else if (j == 2) {
+            lds_copy4(as + (int64_t)q * 128, aoff, to + AUX + wave * 256);
+            if (K) lds_copy4(ss + (int64_t)(q >> 1) * 64, soff, to + SUP + wave * 256);
+        }
+    };
+
+    const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    floatx4 acc[RT][VT];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int v = 0; v < VT; v++) acc[t][v] = zero;
+
+    if (q0 < q1) {
+        const int s_last = q1 * 4 - 1;
+#pragma unroll
+        for (int j = 0; j < 3; j++) copy_w(q0, q0, j);
+        copy_x(q0 * 4, 0);
+        copy_x(q0 * 4 + 1, 1);  // a quad has four groups
+        int slot = 0;  // of step s
+        for (int q = q0; q < q1; q++) {
+            const uint8_t *ws = lds + 3 * XS + (q & 1) * WS;
+            u32x4 qw[RT], sc[RT][2];
+            u32x2 am[RT];
+            floatx4 c[RT][VT];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                // step s's x has landed once only the copies of the step before are in
+                // flight; every wave is past step s - 1, whose slot is free
+                constexpr int kBefore[4] = {VT, VT + 1 + K, VT + 1, VT + 1 + K};
+                if (j == 0)
+                    wait_vm<kBefore[0]>();
+                else if (j == 1)
+                    wait_vm<kBefore[1]>();
+                else if (j == 2)
+                    wait_vm<kBefore[2]>();
+                else
+                    wait_vm<kBefore[3]>();
+                __syncthreads();
+                copy_x(min(q * 4 + j + 2, s_last), slot == 0 ? 2 : slot - 1);
+                copy_w(q + 1, min(q + 1, q1 - 1), j);
+                const uint8_t *xl = lds + slot * XS + vt0 * 2048 + lane * 16;
+                slot = slot == 2 ? 0 : slot + 1;
+                if (j == 0) {
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        const int i = rt0 + t;
+                        qw[t] = *reinterpret_cast<const u32x4 *>(ws + i * 1024 + lane * 16);
+                        const uint8_t *a = ws + AUX + (i >> 1) * 256 + (i & 1) * 128;
+                        if constexpr (K) {
+                            am[t] = *reinterpret_cast<const u32x2 *>(a + col * 8);
+                            sc[t][0] = *reinterpret_cast<const u32x4 *>(ws + SUP + (i >> 1) * 256 + (i & 1) * 64 + kg * 16);
+                        } else {
+                            sc[t][0] = *reinterpret_cast<const u32x4 *>(a + kg * 32);
+                            sc[t][1] = *reinterpret_cast<const u32x4 *>(a + kg * 32 + 16);
+                        }
+                    }
+                }
+                half8 bh[VT], bl[VT];
+#pragma unroll
+                for (int v = 0; v < VT; v++) {
+                    bh[v] = *reinterpret_cast<const half8 *>(xl + v * 2048);
+                    bl[v] = *reinterpret_cast<const half8 *>(xl + v * 2048 + 1024);
+                }
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    const half8 a = K ? nibbles_q4_k(qw[t][j], am[t][0], j) : nibbles_q4_0(qw[t][j]);
+#pragma unroll
+                    for (int v = 0; v < VT; v++)
+                        c[t][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh[v], K && j ? c[t][v] : zero, 0, 0, 0);
+#pragma unroll
+                    for (int v = 0; v < VT; v++) c[t][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl[v], c[t][v], 0, 0, 0);
+                    if constexpr (!K)
+#pragma unroll
+                        for (int v = 0; v < VT; v++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const uint32_t f = sc[t][r >> 1][(r & 1) * 2 + (j >> 1)];
+                                acc[t][v][r] = fmaf(c[t][v][r], (j & 1) ? hi_of(f) : lo_of(f), acc[t][v][r]);
+                            }
+                }
+            }
+            if constexpr (K) {
+                half8 bm[VT];
+#pragma unroll
+                for (int v = 0; v < VT; v++) {
+                    const int i = vt0 + v;
+                    bm[v] = *reinterpret_cast<const half8 *>(ws + XM + i / (VT / 2) * 1024 + i % (VT / 2) * 256 + col * 16);
+                    if (kg) bm[v] = half8{};
+                }
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    const half4 m4 = minima(am[t][1]);
+                    const half8 a = kg ? half8{} : half8{m4[0], m4[1], m4[2], m4[3], m4[0], m4[1], m4[2], m4[3]};
+#pragma unroll
+                    for (int v = 0; v < VT; v++) {
+                        const floatx4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bm[v], zero, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            acc[t][v][r] = fmaf(c[t][v][r], lo_of(sc[t][0][r]), acc[t][v][r]);
+                            acc[t][v][r] = fmaf(-m[r], hi_of(sc[t][0][r]), acc[t][v][r]);
+                        }
+                    }
+                }
+            }
+        }
+        wait_vm<0>();  // no copy outlives the workgroup's LDS
+    }
+
+    // the lane's outputs: of vector (vt_wg + vt0 + v) * 16 + col the rows
+    // (tile_wg + rt0 + t) * 16 + 4 kg .. +3
+    const bool quads = w.rows % 4 == 0 && ((uintptr_t)y & 15) == 0;
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int v = 0; v < VT; v++) {
+            const int vec = (vt_wg + vt0 + v) * 16 + col;
+            if (vec >= n_vec) continue;
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const int row = (tile_wg + rt0 + t) * 16 + kg * 4;
+                if (row < w.rows) f((int64_t)vec * w.rows + row, w.rows - row, acc[t][v], vec);
+            }
+        }
+    };
+    if (gridDim.z > 1) {
+        float *o = part + blockIdx.z * slice_stride;
+        each([&](int64_t at, int left, const floatx4 &t, int) {
+            if (quads) {
+                store_agent2(o + at, t[0], t[1]);
+                store_agent2(o + at + 2, t[2], t[3]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (r < left) store_agent(o + at + r, t[r]);
+            }
+        });
+        __shared__ int last;
+        if (!arrive_last(arrivals + blockIdx.y * gridDim.x + blockIdx.x, gridDim.z, &last)) return;
+        const int n_slices = gridDim.z;
+        each([&](int64_t at, int left, floatx4 &t, int) {
+            floatx4 got[kMaxSlices];
+#pragma unroll
+            for (int s = 0; s < kMaxSlices; s++)
+                if (s < n_slices) {
+                    if (quads) {
+                        got[s] = load_agent4(part + s * slice_stride + at);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) got[s][r] = r < left ? load_agent(part + s * slice_stride + at + r) : 0.0f;
+                    }
+                }
+            t = got[0];
+#pragma unroll
+            for (int s = 1; s < kMaxSlices; s++)
+                if (s < n_slices) t += got[s];
+        });
+    }
+    each([&](int64_t at, int left, const floatx4 &t, int vec) {
+        const floatx4 o = t * px.undo[vec];
+        if (quads) {
+            *reinterpret_cast<floatx4 *>(y + at) = o;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (r < left) y[at + r] = o[r];
+        }
+    });
 }
 
 constexpr int kMaxVec = 262128;
+constexpr int kMaxCols = 1 << 26;  // a row of x is addressed by 32 bits of bytes
 
 int launched(const char *what) {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GLA_OK : set_error(GLA_ERR_KERNEL, "%s launch: %s", what, hipGetErrorString(e));
+}
+
+template <bool K, int NV>
+int launch_few(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
+    // Two row tiles a workgroup share the pieces of x where a tile each would be
+    // more than one workgroup per CU: 6144 x 4096 Q4_0, 4 vectors 7.5 us (one tile
+    // each: 10.3), 8 vectors 10.2 (14.4); below that one each is faster (4096 x
+    // 4096, 1 vector 4.5, two tiles 6.3). One vector, whose pieces are cheap, from
+    // three workgroups per CU on.
+    const auto go = [&](auto kernel, int tiles) {
+        hipLaunchKernelGGL(kernel, dim3((w->n_tiles + tiles - 1) / tiles), dim3(kFewWaves * 64), 0, ctx->stream, p, x, n, y);
+    };
+    if (w->n_tiles > (NV == 1 ? 2 : 1) * ctx->n_cu)
+        go(matvec_q4_few_kernel<K, NV, 2>, 2);
+    else
+        go(matvec_q4_few_kernel<K, NV, 1>, 1);
+    return launched("matvec_q4_few_kernel");
+}
+
+int few(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
+    const auto of = [&](auto k) {
+        constexpr bool K = decltype(k)::value;
+        return n == 1 ? launch_few<K, 1>(ctx, w, p, x, n, y) : n == 2 ? launch_few<K, 2>(ctx, w, p, x, n, y)
+             : n <= 4 ? launch_few<K, 4>(ctx, w, p, x, n, y) : launch_few<K, 8>(ctx, w, p, x, n, y);
+    };
+    return w->format == GLA_Q4_K ? of(std::true_type()) : of(std::false_type());
+}
+
+constexpr int kFewVec = 8;
+
+// Pieces, sums and scales of n vectors in the stream's scratch, with `part` bytes behind them.
+int make_pieces(gla_ctx *ctx, const gla_q4w *w, const float *x, int n, size_t part, Pieces *px, float **partials) {
+    const bool k = w->format == GLA_Q4_K;
+    const size_t tiles = (size_t)(n + 15) / 16;
+    const size_t xp = tiles * w->n_quads * 4 * 2048, xm = k ? tiles * w->n_quads * 256 : 0;
+    const size_t un = ((size_t)n * sizeof(float) + 255) / 256 * 256;
+    void *scr = nullptr;
+    if (int rc = ensure_scratch(ctx, xp + xm + un + part, &scr)) return rc;
+    uint8_t *base = (uint8_t *)scr;
+    px->xp = (const _Float16 *)base;
+    px->xm = (const _Float16 *)(base + xp);
+    px->undo = (const float *)(base + xp + xm);
+    if (partials) *partials = (float *)(base + xp + xm + un);
+    hipLaunchKernelGGL(k ? split_q4_kernel<true> : split_q4_kernel<false>, dim3(n), dim3(kSplitThreads), 0, ctx->stream, x,
+                       w->cols, w->n_quads, (_Float16 *)px->xp, (_Float16 *)px->xm, (float *)px->undo);
+    return launched("split_q4_kernel");
+}
+
+int mid(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
+    const bool k = w->format == GLA_Q4_K;
+    int rt = w->n_tiles <= ctx->n_cu ? 1 : 2;
+    if (n > 32) rt = 4;
+    if (n <= 16 && w->n_tiles > 2 * ctx->n_cu) rt = 4;
+    const int groups = (w->n_tiles + rt - 1) / rt;
+    const int units = k ? w->n_quads / 2 : w->n_quads;
+    const int waves = n > 32 ? 4 : 8;  // ranges of a slice's quads
+    int slices = n > 32 ? ctx->n_cu / groups : 1;
+    slices = std::max(1, std::min({kMaxSlices, slices, units / waves}));
+    const int64_t stride = (int64_t)n * w->rows;
+    Pieces px;
+    float *part = nullptr;
+    int32_t *arrivals = nullptr;
+    if (slices > 1)
+        if (int rc = ensure_arrivals(ctx, (size_t)groups, &arrivals)) return rc;
+    if (int rc = make_pieces(ctx, w, x, n, slices > 1 ? (size_t)slices * stride * sizeof(float) : 0, &px, &part)) return rc;
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(groups, slices), dim3(kMidWaves * 64), 0, ctx->stream, p, px, n, y, part, stride, arrivals);
+        return launched("matvec_q4_mid_kernel");
+    };
+    const auto of = [&](auto kk) {
+        constexpr bool K = decltype(kk)::value;
+        if (n > 32)
+            return rt == 4 ? go(matvec_q4_mid_kernel<K, 2, 4, 2>) : rt == 2 ? go(matvec_q4_mid_kernel<K, 2, 2, 2>) : go(matvec_q4_mid_kernel<K, 2, 1, 2>);
+        if (n > 16) return rt == 2 ? go(matvec_q4_mid_kernel<K, 2, 2, 1>) : rt == 4 ? go(matvec_q4_mid_kernel<K, 2, 4, 1>) : go(matvec_q4_mid_kernel<K, 2, 1, 1>);
+        return rt == 4   ? go(matvec_q4_mid_kernel<K, 1, 4, 1>)
+               : rt == 2 ? go(matvec_q4_mid_kernel<K, 1, 2, 1>)
+                         : go(matvec_q4_mid_kernel<K, 1, 1, 1>);
+    };
+    return k ? of(std::true_type()) : of(std::false_type());
+}
+
+int many(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
+    const bool k = w->format == GLA_Q4_K;
+    const int vec_tiles = (n + 15) / 16, row_blocks = (w->n_tiles + 7) / 8;
+    const int vt = row_blocks * ((vec_tiles + 7) / 8) >= ctx->n_cu ? 4 : 2;
+    const int vec_blocks = (vec_tiles + 2 * vt - 1) / (2 * vt);
+    const int units = k ? w->n_quads / 2 : w->n_quads;
+    const int64_t wgs = (int64_t)row_blocks * vec_blocks, stride = (int64_t)n * w->rows;
+    int slices = (int)std::max<int64_t>(1, ctx->n_cu / wgs);
+    slices = std::max(1, std::min({kMaxSlices, slices, units / 2}));
+    while (slices > 1 && (size_t)slices * stride * sizeof(float) > ((size_t)28 << 20)) slices--;
+    Pieces px;
+    float *part = nullptr;
+    int32_t *arrivals = nullptr;
+    if (slices > 1)
+        if (int rc = ensure_arrivals(ctx, (size_t)wgs, &arrivals)) return rc;
+    if (int rc = make_pieces(ctx, w, x, n, slices > 1 ? (size_t)slices * stride * sizeof(float) : 0, &px, &part)) return rc;
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(row_blocks, vec_blocks, slices), dim3(256), 0, ctx->stream, p, px, n, y, part, stride,
+                           arrivals);
+        return launched("matvec_q4_gemm_kernel");
+    };
+    if (vt == 4) return k ? go(matvec_q4_gemm_kernel<true, 4>) : go(matvec_q4_gemm_kernel<false, 4>);
+    return k ? go(matvec_q4_gemm_kernel<true, 2>) : go(matvec_q4_gemm_kernel<false, 2>);
 }
 
 }  // namespace
@@ -187,6 +1056,7 @@ int gla_q4w_create(gla_ctx *ctx, gla_q4_format format, const uint8_t *ggml_host,
     const bool k = format == GLA_Q4_K;
     GLA_REQUIRE(rows > 0 && cols > 0 && cols % (k ? 256 : 32) == 0,
                 "gla_q4w_create: rows %d, cols %d (cols must be a positive multiple of %d)", rows, cols, k ? 256 : 32);
+    GLA_REQUIRE(cols <= kMaxCols, "gla_q4w_create: %d columns (at most %d)", cols, kMaxCols);
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
     ctx->q4ws.reserve(ctx->q4ws.size() + 1);
     gla_q4w *w = new gla_q4w();
@@ -254,13 +1124,9 @@ int gla_matvec_q4(gla_ctx *ctx, const gla_q4w *w, const float *x, int n_vec, flo
     GLA_REQUIRE(x && y, "gla_matvec_q4: NULL buffer");
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
     const Weights p{w->quants, w->aux, w->super, w->rows, w->cols, w->n_tiles, w->n_quads};
-    for (int v0 = 0; v0 < n_vec; v0 += 4 * 65535) {
-        const int n = std::min(n_vec - v0, 4 * 65535);
-        auto kernel = w->format == GLA_Q4_K ? matvec_q4_plain_kernel<true> : matvec_q4_plain_kernel<false>;
-        hipLaunchKernelGGL(kernel, dim3(w->n_tiles, (n + 3) / 4), dim3(64), 0, ctx->stream, p, x + (int64_t)v0 * w->cols, n,
-                           y + (int64_t)v0 * w->rows);
-    }
-    return launched("matvec_q4_plain_kernel");
+    if (n_vec <= kFewVec) return few(ctx, w, p, x, n_vec, y);
+    if (n_vec <= 64) return mid(ctx, w, p, x, n_vec, y);
+    return many(ctx, w, p, x, n_vec, y);
     GLA_GUARD_END
 }
 
