@@ -194,9 +194,23 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
     const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
     return max(b[0], b[1]);
 }
+// ... of the lanes that are equal mod 4
+__device__ __forceinline__ uint32_t wave_max4(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max(b[0], b[1]);
+}
+// Sums of four neighbouring lanes; of the four lanes of a row that are equal mod 4.
 __device__ __forceinline__ float quad_sum(float x) {
     x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0xB1, 0xf, 0xf, true));
     return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x4E, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float apart_sum(float x) {
+    x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x124, 0xf, 0xf, true));
+    return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xf, 0xf, true));
 }
 // Pieces of x * mul (a power of two); `odd`: the range has an infinity or a NaN.
 __device__ __forceinline__ void pieces(float x, float mul, bool odd, _Float16 &hi, _Float16 &lo) {
@@ -414,22 +428,40 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
 
 // ---- more vectors: the pieces of x, once per call ----------------------------------
 
-// A workgroup per vector: its scale from the largest finite |x| of the row, then
-// the pieces in B-operand order, xp[v / 16][group][piece][lane = kg * 16 + v % 16]
-// = 8 halves, zeros past the columns, and undo[v] = 2^-s. Q4_K: the sums of each
-// group, times 2^-5 and in pieces, xm[v / 16][quad][v % 16] = {hi of the quad's four
-// groups, lo of them}. Vectors up to the next 16 are left as they are: a column of
-// the product is its vector's alone.
+// A workgroup per VQ vectors (thread t: vector t % VQ): their scales from the largest
+// finite |x| of a row, then the pieces in B-operand order, xp[v / 16][group][piece]
+// [lane = kg * 16 + v % 16] = 8 halves, zeros past the columns, and undo[v] = 2^-s.
+// Q4_K: the sums of each group, times 2^-5 and in pieces, xm[v / 16][superblock][piece]
+// [v % 16] = the eight groups' halves. Vectors up to the next 16 are left as they are:
+// a column of the product is its vector's alone. Many vectors go four a workgroup, so
+// that 64 bytes are written together (1,999 x 4,096: 29 us at one, whose 16-byte
+// pieces met in memory); up to 64 one, for the chip's sake.
 constexpr int kSplitThreads = 512;
 constexpr int kSplitUnits = 4;  // units of 8 elements a thread keeps; a wider row is read twice
-template <bool K>
-__global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x, int cols, int n_quads, _Float16 *xp,
-                                                                 _Float16 *xm, float *undo) {
-    const int v = blockIdx.x, t = threadIdx.x;
-    const float *row = x + (int64_t)v * cols;
+template <bool K, int VQ>
+__global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x, int n_vec, int cols, int n_quads,
+                                                                 _Float16 *xp, _Float16 *xm, float *undo) {
+    constexpr int PASS = kSplitThreads / VQ;  // units of a vector a pass
+    const int t = threadIdx.x, vq = t % VQ, ut = t / VQ;
+    const int v = blockIdx.x * VQ + vq;
     const int units = n_quads * 16, in = cols / 8;
     float e[kSplitUnits][8];
-    const auto load = [&](float (&d)[8], int u) { load_row(d, row, in * 32, u * 32); };  // zeros past the row
+    const float *row = x + (int64_t)min(v, n_vec - 1) * cols;
+    const bool aligned = ((uintptr_t)x & 15) == 0;  // rows are 128-byte multiples apart
+    const auto fetch = [&](float (&d)[8], int u) {
+        const float *p = row + (int64_t)min(u, in - 1) * 8;
+        if (aligned) {
+            const floatx4 a = reinterpret_cast<const floatx4 *>(p)[0], b = reinterpret_cast<const floatx4 *>(p)[1];
+#pragma unroll
+            for (int j = 0; j < 4; j++) d[j] = a[j], d[4 + j] = b[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) d[j] = p[j];
+        }
+        if (u >= in)
+#pragma unroll
+            for (int j = 0; j < 8; j++) d[j] = 0.0f;
+    };
     const auto bits_of = [](const float (&d)[8], bool finite) {
         uint32_t m = 0;
 #pragma unroll
@@ -439,31 +471,35 @@ __global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x,
         }
         return m;
     };
-    __shared__ uint32_t red[2][kSplitThreads / 64];
+    __shared__ uint32_t red[2][kSplitThreads / 64][VQ];
     const auto group_max = [&](bool finite, int at) {
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < kSplitUnits; i++) m = max(m, bits_of(e[i], finite));
-        for (int u = kSplitUnits * kSplitThreads + t; u < in; u += kSplitThreads) {
+        for (int u = kSplitUnits * PASS + ut; u < in; u += PASS) {
             float d[8];
-            load(d, u);
+            fetch(d, u);
             m = max(m, bits_of(d, finite));
         }
-        m = wave_max(m);
-        if ((t & 63) == 0) red[at][t >> 6] = m;
+        m = VQ == 1 ? wave_max(m) : wave_max4(m);
+        if ((t & 63) < VQ) red[at][t >> 6][vq] = m;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kSplitThreads / 64; i++) m = max(m, red[at][i]);
+        for (int i = 0; i < kSplitThreads / 64; i++) m = max(m, red[at][i][vq]);
         return m;
     };
 #pragma unroll
-    for (int i = 0; i < kSplitUnits; i++) load(e[i], i * kSplitThreads + t);
+    for (int i = 0; i < kSplitUnits; i++) fetch(e[i], i * PASS + ut);
     uint32_t top = group_max(false, 0);
     const bool odd = top >= kInf;
-    if (odd) top = group_max(true, 1);
+    if (__syncthreads_or(odd)) {
+        const uint32_t fin = group_max(true, 1);
+        if (odd) top = fin;
+    }
     const int sh = shift_of(top);
     const float mul = exp2_of(sh);
-    if (t == 0) undo[v] = exp2_of(-sh);
+    if (v >= n_vec) return;
+    if (ut == 0) undo[v] = exp2_of(-sh);
     const auto put = [&](const float (&d)[8], int u) {
         half8 hi, lo;
         float sum = 0.0f;
@@ -480,20 +516,21 @@ __global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x,
         *reinterpret_cast<half8 *>(to + 512) = lo;
         if constexpr (K) {
             _Float16 a, b;
-            pieces(quad_sum(sum), 0.03125f, true, a, b);  // units of a group are four neighbouring threads
+            // units of a group are four threads, neighbours or VQ apart
+            pieces(VQ == 1 ? quad_sum(sum) : apart_sum(sum), 0.03125f, true, a, b);
             if ((u & 3) == 0) {
-                _Float16 *m = xm + (((int64_t)(v >> 4) * n_quads + (u >> 4)) * 16 + (v & 15)) * 8 + ((u >> 2) & 3);
+                _Float16 *m = xm + (((int64_t)(v >> 4) * (n_quads / 2) + (u >> 5)) * 32 + (v & 15)) * 8 + ((u >> 2) & 7);
                 m[0] = a;
-                m[4] = b;
+                m[128] = b;
             }
         }
     };
 #pragma unroll
     for (int i = 0; i < kSplitUnits; i++)
-        if (i * kSplitThreads + t < units) put(e[i], i * kSplitThreads + t);
-    for (int u = kSplitUnits * kSplitThreads + t; u < units; u += kSplitThreads) {
+        if (i * PASS + ut < units) put(e[i], i * PASS + ut);
+    for (int u = kSplitUnits * PASS + ut; u < units; u += PASS) {
         float d[8];
-        load(d, u);
+        fetch(d, u);
         put(d, u);
     }
 }
@@ -504,7 +541,7 @@ struct Pieces {
     const float *undo;
 };
 
-// ---- up to 64 vectors --------------------------------------------------------------
+// ---- up to 128 vectors --------------------------------------------------------------
 
 constexpr int kMidWaves = 8;
 constexpr int kMaxSlices = 8;
@@ -581,7 +618,8 @@ __global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Wei
         if constexpr (K)
 #pragma unroll
             for (int v = 0; v < NVT; v++)
-                m[v] = *reinterpret_cast<const half8 *>(px.xm + (((int64_t)min(vt0 + v, last_vt) * w.n_quads + quad) * 16 + col) * 8);
+                m[v] = *reinterpret_cast<const half8 *>(
+                    px.xm + (((int64_t)min(vt0 + v, last_vt) * (w.n_quads / 2) + (quad >> 1)) * 32 + (kg & 1) * 16 + col) * 8);
     };
     if (q0 < q1) {
         load_w(qw, sc, bm, q0);
@@ -620,13 +658,15 @@ __global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Wei
             if constexpr (K)
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
-                    // k = 0..3 the minima with the sums' hi pieces, 4..7 with their lo
-                    // ones; the other lanes' rows of A are zeros, their B is not
+                    // k = 0..7 this quad's minima, zeros at the other's places, with the sums'
+                    // hi pieces, 8..15 with their lo ones; the other lanes zeros
                     const half4 m4 = minima(sc[t][0][1]);
-                    const half8 am = kg ? half8{} : half8{m4[0], m4[1], m4[2], m4[3], m4[0], m4[1], m4[2], m4[3]};
+                    const half8 am = kg > 1  ? half8{}
+                                     : q & 1 ? half8{0, 0, 0, 0, m4[0], m4[1], m4[2], m4[3]}
+                                             : half8{m4[0], m4[1], m4[2], m4[3], 0, 0, 0, 0};
 #pragma unroll
                     for (int v = 0; v < NVT; v++) {
-                        const floatx4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(am, kg ? half8{} : bm[v], zero, 0, 0, 0);
+                        const floatx4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(am, kg > 1 ? half8{} : bm[v], zero, 0, 0, 0);
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             acc[t][v][r] = fmaf(c[t][v][r], lo_of(sc[t][1][r]), acc[t][v][r]);
@@ -711,14 +751,17 @@ __device__ __forceinline__ void store_agent2(float *p, float a, float b) {
 // LDS copies two steps ahead into a ring of three, the weights of a quad of groups
 // (with scales, and for Q4_K the sums of x) during the quad before, each wave issuing
 // the same number of copies at the same step, so that the waits can count them. The
-// copies of steps past the end repeat the last ones.
+// copies of steps past the end repeat the last ones. Bound: matrix and vector issue;
+// the scales of a row tile's products are applied, and the next tile's nibbles
+// unpacked, between the MFMAs of this one.
 template <bool K, int VT>
 __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w, const Pieces px, int n_vec, float *y,
-                                                             float *part, int64_t slice_stride, int32_t *arrivals) {
+                                                                float *part, int64_t slice_stride, int32_t *arrivals) {
     constexpr int RT = 4, UNIT = K ? 2 : 1;
-    constexpr int XS = 2 * VT * 2048;                    // a ring slot of x: the pieces of 2 VT tiles
+    constexpr int XS = 2 * VT * 2048;  // a ring slot of x: the pieces of 2 VT tiles
     constexpr int AUX = 2 * RT * 1024, SUP = AUX + 1024, XM = SUP + 1024, WS = K ? XM + 4096 : SUP;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[3 * XS + 2 * WS];
+    constexpr int RING = VT == 2 && !K ? 4 : 3;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[RING * XS + 2 * WS];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, kg = lane >> 4;
@@ -732,7 +775,8 @@ __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w,
     const int ps = (units + gridDim.z - 1) / gridDim.z;
     const int q0 = min(units, (int)blockIdx.z * ps) * UNIT, q1 = min(units, (int)(blockIdx.z + 1) * ps) * UNIT;
 
-    // the wave's copies: VT of 2 VT x 2 pieces, two row tiles and their scales
+    // the wave's copies: VT of 2 VT x 2 pieces, two row tiles and their scales, and
+    // (Q4_K, a superblock at a time) the sums of VT / 2 vector tiles
     const uint8_t *xsrc[VT];
 #pragma unroll
     for (int c = 0; c < VT; c++) {
@@ -747,17 +791,17 @@ __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w,
     const uint8_t *ss = reinterpret_cast<const uint8_t *>(w.super) + (int64_t)ta * (w.n_quads / 2) * 64;
     const uint32_t soff = (uint32_t)(((lane >> 4) & 1) * (tb - ta)) * (uint32_t)(w.n_quads / 2) * 64 + (lane & 15) * 4;
     const int va = min(vt_wg + wave * (VT / 2), last_vt), vb = min(va + 1, last_vt);
-    const uint8_t *ms = reinterpret_cast<const uint8_t *>(px.xm) + (int64_t)va * w.n_quads * 256;
-    const uint32_t moff = (VT == 4 ? (uint32_t)(((lane >> 4) & 1) * (vb - va)) * (uint32_t)w.n_quads * 256 : 0u) + (lane & 15) * 16;
+    const uint8_t *ms = reinterpret_cast<const uint8_t *>(px.xm) + (int64_t)va * (w.n_quads / 2) * 512;
+    const uint32_t moff = (VT == 4 ? (uint32_t)((lane >> 5) * (vb - va)) * (uint32_t)(w.n_quads / 2) * 512 : 0u) + (lane & 31) * 16;
     const auto copy_x = [&](int s, int slot) {
 #pragma unroll
         for (int c = 0; c < VT; c++) lds_copy16(xsrc[c] + (int64_t)s * 2048, lane * 16, base + slot * XS + (wave * VT + c) * 1024);
     };
     const auto copy_w = [&](int as_quad, int q, int j) {  // part j of quad q's weights, where quad as_quad's go
-        const uint32_t to = base + 3 * XS + (as_quad & 1) * WS;
+        const uint32_t to = base + RING * XS + (as_quad & 1) * WS;
         if (j == 0) {
             lds_copy16(qa + (int64_t)q * 1024, lane * 16, to + 2 * wave * 1024);
-            if (K) lds_copy16(ms + (int64_t)q * 256, moff, to + XM + wave * 1024);
+            if (K) lds_copy16(ms + (int64_t)(q >> 1) * 512, moff, to + XM + wave * 1024);
         } else if (j == 1) {
             lds_copy16(qb + (int64_t)q * 1024, lane * 16, to + (2 * wave + 1) * 1024);
         } else if (j == 2) {
@@ -778,91 +822,119 @@ __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w,
 #pragma unroll
         for (int j = 0; j < 3; j++) copy_w(q0, q0, j);
         copy_x(q0 * 4, 0);
-        copy_x(q0 * 4 + 1, 1);  // a quad has four groups
-        int slot = 0;  // of step s
-        for (int q = q0; q < q1; q++) {
-            const uint8_t *ws = lds + 3 * XS + (q & 1) * WS;
-            u32x4 qw[RT], sc[RT][2];
-            u32x2 am[RT];
-            floatx4 c[RT][VT];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                // step s's x has landed once only the copies of the step before are in
-                // flight; every wave is past step s - 1, whose slot is free
-                constexpr int kBefore[4] = {VT, VT + 1 + K, VT + 1, VT + 1 + K};
-                if (j == 0)
-                    wait_vm<kBefore[0]>();
-                else if (j == 1)
-                    wait_vm<kBefore[1]>();
-                else if (j == 2)
-                    wait_vm<kBefore[2]>();
-                else
-                    wait_vm<kBefore[3]>();
-                __syncthreads();
-                copy_x(min(q * 4 + j + 2, s_last), slot == 0 ? 2 : slot - 1);
-                copy_w(q + 1, min(q + 1, q1 - 1), j);
-                const uint8_t *xl = lds + slot * XS + vt0 * 2048 + lane * 16;
-                slot = slot == 2 ? 0 : slot + 1;
-                if (j == 0) {
+        for (int i = 1; i < RING - 1; i++) copy_x(q0 * 4 + i, i);  // a quad has four groups
+        int slot = 0;           // of the step
+        for (int q = q0; q < q1; q += UNIT) {
+            floatx4 c[K ? RT : 2][VT];  // Q4_0: this tile's products and the last one's
+            uint32_t mins[RT];          // Q4_K: the first quad's minima
 #pragma unroll
-                    for (int t = 0; t < RT; t++) {
-                        const int i = rt0 + t;
-                        qw[t] = *reinterpret_cast<const u32x4 *>(ws + i * 1024 + lane * 16);
-                        const uint8_t *a = ws + AUX + (i >> 1) * 256 + (i & 1) * 128;
-                        if constexpr (K) {
-                            am[t] = *reinterpret_cast<const u32x2 *>(a + col * 8);
-                            sc[t][0] = *reinterpret_cast<const u32x4 *>(ws + SUP + (i >> 1) * 256 + (i & 1) * 64 + kg * 16);
-                        } else {
-                            sc[t][0] = *reinterpret_cast<const u32x4 *>(a + kg * 32);
-                            sc[t][1] = *reinterpret_cast<const u32x4 *>(a + kg * 32 + 16);
-                        }
-                    }
-                }
-                half8 bh[VT], bl[VT];
-#pragma unroll
-                for (int v = 0; v < VT; v++) {
-                    bh[v] = *reinterpret_cast<const half8 *>(xl + v * 2048);
-                    bl[v] = *reinterpret_cast<const half8 *>(xl + v * 2048 + 1024);
-                }
-#pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    const half8 a = K ? nibbles_q4_k(qw[t][j], am[t][0], j) : nibbles_q4_0(qw[t][j]);
+            for (int h = 0; h < UNIT; h++) {
+                const uint8_t *ws = lds + RING * XS + ((q + h) & 1) * WS;
+                u32x4 qw[RT], sc[RT][2];
+                u32x2 am[RT];
+                const auto unpack = [&](int t, int j) { return K ? nibbles_q4_k(qw[t][j], am[t][0], j) : nibbles_q4_0(qw[t][j]); };
+                const auto scale = [&](int t, int j) {  // Q4_0: the products of tile t, group j
 #pragma unroll
                     for (int v = 0; v < VT; v++)
-                        c[t][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh[v], K && j ? c[t][v] : zero, 0, 0, 0);
-#pragma unroll
-                    for (int v = 0; v < VT; v++) c[t][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl[v], c[t][v], 0, 0, 0);
-                    if constexpr (!K)
-#pragma unroll
-                        for (int v = 0; v < VT; v++)
-#pragma unroll
-                            for (int r = 0; r < 4; r++) {
-                                const uint32_t f = sc[t][r >> 1][(r & 1) * 2 + (j >> 1)];
-                                acc[t][v][r] = fmaf(c[t][v][r], (j & 1) ? hi_of(f) : lo_of(f), acc[t][v][r]);
-                            }
-                }
-            }
-            if constexpr (K) {
-                half8 bm[VT];
-#pragma unroll
-                for (int v = 0; v < VT; v++) {
-                    const int i = vt0 + v;
-                    bm[v] = *reinterpret_cast<const half8 *>(ws + XM + i / (VT / 2) * 1024 + i % (VT / 2) * 256 + col * 16);
-                    if (kg) bm[v] = half8{};
-                }
-#pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    const half4 m4 = minima(am[t][1]);
-                    const half8 a = kg ? half8{} : half8{m4[0], m4[1], m4[2], m4[3], m4[0], m4[1], m4[2], m4[3]};
-#pragma unroll
-                    for (int v = 0; v < VT; v++) {
-                        const floatx4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bm[v], zero, 0, 0, 0);
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            acc[t][v][r] = fmaf(c[t][v][r], lo_of(sc[t][0][r]), acc[t][v][r]);
-                            acc[t][v][r] = fmaf(-m[r], hi_of(sc[t][0][r]), acc[t][v][r]);
+                            const uint32_t f = sc[t][r >> 1][(r & 1) * 2 + (j >> 1)];
+                            acc[t][v][r] = fmaf(c[t & 1][v][r], (j & 1) ? hi_of(f) : lo_of(f), acc[t][v][r]);
+                        }
+                };
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    // step s's x has landed once only the copies of the step before are in
+                    // flight; every wave is past step s - 1, whose slot is free
+                    if (j == 0)
+                        wait_vm<VT>();
+                    else if (j == 1)
+                        wait_vm<(RING == 4 ? VT : 0) + VT + 1 + K>();
+                    else if (j == 2)
+                        wait_vm<(RING == 4 ? VT + 1 + K : 0) + VT + 1>();
+                    else
+                        wait_vm<(RING == 4 ? VT + 1 : 0) + VT + 1 + K>();
+                    __syncthreads();
+                    const int qn = min(q + h + 1, q1 - 1);
+                    copy_x(min((q + h) * 4 + j + RING - 1, s_last), slot == 0 ? RING - 1 : slot - 1);
+                    copy_w(q + h + 1, qn, j);
+                    const uint8_t *xl = lds + slot * XS + vt0 * 2048 + lane * 16;
+                    slot = slot == RING - 1 ? 0 : slot + 1;
+                    if (j == 0) {
+#pragma unroll
+                        for (int t = 0; t < RT; t++) {
+                            const int i = rt0 + t;
+                            qw[t] = *reinterpret_cast<const u32x4 *>(ws + i * 1024 + lane * 16);
+                            const uint8_t *a = ws + AUX + (i >> 1) * 256 + (i & 1) * 128;
+                            if constexpr (K) {
+                                am[t] = *reinterpret_cast<const u32x2 *>(a + col * 8);
+                            } else {
+                                sc[t][0] = *reinterpret_cast<const u32x4 *>(a + kg * 32);
+                                sc[t][1] = *reinterpret_cast<const u32x4 *>(a + kg * 32 + 16);
+                            }
                         }
                     }
+                    half8 bh[VT], bl[VT];
+#pragma unroll
+                    for (int v = 0; v < VT; v++) {
+                        bh[v] = *reinterpret_cast<const half8 *>(xl + v * 2048);
+                        bl[v] = *reinterpret_cast<const half8 *>(xl + v * 2048 + 1024);
+                    }
+                    half8 a = unpack(0, j);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        floatx4(&ct)[VT] = c[K ? t : t & 1];
+#pragma unroll
+                        for (int v = 0; v < VT; v++)
+                            ct[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh[v], K && (h || j) ? ct[v] : zero, 0, 0, 0);
+#pragma unroll
+                        for (int v = 0; v < VT; v++) ct[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl[v], ct[v], 0, 0, 0);
+                        if (!K && t) scale(t - 1, j);
+                        if (!K && !t && j) scale(RT - 1, j - 1);
+                        if (t + 1 < RT) a = unpack(t + 1, j);
+#pragma unroll
+                        for (int i = 0; i < 2 * VT; i++) {
+                            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                // MFMA
+                            __builtin_amdgcn_sched_group_barrier(0x2, K ? 16 / (2 * VT) : (11 + 4 * VT) / (2 * VT), 0);  // VALU
+                        }
+                    }
+                }
+                if constexpr (K) {
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        if (h == 0) mins[t] = am[t][1];
+                    }
+                    if (h) {
+                        // the superblock's minima with its sums of x: k = 0..7 their hi pieces,
+                        // 8..15 their lo ones, the other lanes zeros
+                        half8 bm[VT];
+#pragma unroll
+                        for (int v = 0; v < VT; v++) {
+                            const int i = vt0 + v;
+                            bm[v] = *reinterpret_cast<const half8 *>(ws + XM + i / (VT / 2) * 1024 + i % (VT / 2) * 512 +
+                                                                     ((kg & 1) * 16 + col) * 16);
+                            if (kg > 1) bm[v] = half8{};
+                        }
+#pragma unroll
+                        for (int t = 0; t < RT; t++) {
+                            const int i = rt0 + t;
+                            const u32x4 dd = *reinterpret_cast<const u32x4 *>(ws + SUP + (i >> 1) * 256 + (i & 1) * 64 + kg * 16);
+                            const half4 m0 = minima(mins[t]), m1 = minima(am[t][1]);
+                            const half8 a = kg > 1 ? half8{} : half8{m0[0], m0[1], m0[2], m0[3], m1[0], m1[1], m1[2], m1[3]};
+#pragma unroll
+                            for (int v = 0; v < VT; v++) {
+                                const floatx4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bm[v], zero, 0, 0, 0);
+#pragma unroll
+                                for (int r = 0; r < 4; r++) {
+                                    acc[t][v][r] = fmaf(c[t][v][r], lo_of(dd[r]), acc[t][v][r]);
+                                    acc[t][v][r] = fmaf(-m[r], hi_of(dd[r]), acc[t][v][r]);
+                                }
+                            }
+                        }
+                    }
+                } else {
+                    scale(RT - 1, 3);
                 }
             }
         }
@@ -969,7 +1041,7 @@ constexpr int kFewVec = 8;
 int make_pieces(gla_ctx *ctx, const gla_q4w *w, const float *x, int n, size_t part, Pieces *px, float **partials) {
     const bool k = w->format == GLA_Q4_K;
     const size_t tiles = (size_t)(n + 15) / 16;
-    const size_t xp = tiles * w->n_quads * 4 * 2048, xm = k ? tiles * w->n_quads * 256 : 0;
+    const size_t xp = tiles * w->n_quads * 4 * 2048, xm = k ? tiles * (w->n_quads / 2) * 512 : 0;
     const size_t un = ((size_t)n * sizeof(float) + 255) / 256 * 256;
     void *scr = nullptr;
     if (int rc = ensure_scratch(ctx, xp + xm + un + part, &scr)) return rc;
@@ -978,21 +1050,25 @@ int make_pieces(gla_ctx *ctx, const gla_q4w *w, const float *x, int n, size_t pa
     px->xm = (const _Float16 *)(base + xp);
     px->undo = (const float *)(base + xp + xm);
     if (partials) *partials = (float *)(base + xp + xm + un);
-    hipLaunchKernelGGL(k ? split_q4_kernel<true> : split_q4_kernel<false>, dim3(n), dim3(kSplitThreads), 0, ctx->stream, x,
-                       w->cols, w->n_quads, (_Float16 *)px->xp, (_Float16 *)px->xm, (float *)px->undo);
+    const bool four = n > 64;
+    auto kernel = k ? (four ? split_q4_kernel<true, 4> : split_q4_kernel<true, 1>)
+                    : (four ? split_q4_kernel<false, 4> : split_q4_kernel<false, 1>);
+    hipLaunchKernelGGL(kernel, dim3(four ? (n + 3) / 4 : n), dim3(kSplitThreads), 0, ctx->stream, x, n, w->cols, w->n_quads,
+                       (_Float16 *)px->xp, (_Float16 *)px->xm, (float *)px->undo);
     return launched("split_q4_kernel");
 }
 
 int mid(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
     const bool k = w->format == GLA_Q4_K;
-    int rt = w->n_tiles <= ctx->n_cu ? 1 : 2;
-    if (n > 32) rt = 4;
-    if (n <= 16 && w->n_tiles > 2 * ctx->n_cu) rt = 4;
+    // Up to 32 vectors as few row tiles a workgroup as give every CU one. More vectors
+    // take four and slices of K, about a workgroup per CU in all: the pieces that a
+    // workgroup reads are its slice's. us, Q4_0 4096 x 4096, 64 vectors: one tile, no
+    // slices 19.4; four tiles, 1 / 2 / 4 / 8 slices 29.3 / 22.0 / 18.7 / 24.1.
+    const int rt = n > 32 || (n <= 16 && w->n_tiles > 2 * ctx->n_cu) ? 4 : w->n_tiles > ctx->n_cu ? 2 : 1;
     const int groups = (w->n_tiles + rt - 1) / rt;
     const int units = k ? w->n_quads / 2 : w->n_quads;
-    const int waves = n > 32 ? 4 : 8;  // ranges of a slice's quads
-    int slices = n > 32 ? ctx->n_cu / groups : 1;
-    slices = std::max(1, std::min({kMaxSlices, slices, units / waves}));
+    const int ranges = n > 64 ? 2 : n > 32 ? 4 : 8;  // of a slice's quads
+    const int slices = n <= 32 ? 1 : std::max(1, std::min({kMaxSlices, ctx->n_cu / groups, units / ranges}));
     const int64_t stride = (int64_t)n * w->rows;
     Pieces px;
     float *part = nullptr;
@@ -1006,26 +1082,32 @@ int mid(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n,
     };
     const auto of = [&](auto kk) {
         constexpr bool K = decltype(kk)::value;
-        if (n > 32)
-            return rt == 4 ? go(matvec_q4_mid_kernel<K, 2, 4, 2>) : rt == 2 ? go(matvec_q4_mid_kernel<K, 2, 2, 2>) : go(matvec_q4_mid_kernel<K, 2, 1, 2>);
-        if (n > 16) return rt == 2 ? go(matvec_q4_mid_kernel<K, 2, 2, 1>) : rt == 4 ? go(matvec_q4_mid_kernel<K, 2, 4, 1>) : go(matvec_q4_mid_kernel<K, 2, 1, 1>);
-        return rt == 4   ? go(matvec_q4_mid_kernel<K, 1, 4, 1>)
+        if (n > 64) return go(matvec_q4_mid_kernel<K, 2, 4, 4>);
+        if (n > 32) return go(matvec_q4_mid_kernel<K, 2, 4, 2>);
+        if (n > 16) return rt == 1 ? go(matvec_q4_mid_kernel<K, 2, 1, 1>) : go(matvec_q4_mid_kernel<K, 2, 2, 1>);
+        return rt == 1   ? go(matvec_q4_mid_kernel<K, 1, 1, 1>)
                : rt == 2 ? go(matvec_q4_mid_kernel<K, 1, 2, 1>)
-                         : go(matvec_q4_mid_kernel<K, 1, 1, 1>);
+                         : go(matvec_q4_mid_kernel<K, 1, 4, 1>);
     };
     return k ? of(std::true_type()) : of(std::false_type());
 }
 
 int many(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
     const bool k = w->format == GLA_Q4_K;
+    // Workgroups of 128 vectors where they fill two on every CU, else of 64. Fewer than
+    // 768 of these take slices of K (each of eight quads or more) as long as their
+    // partial sums stay within 28 MB. us, 64 wide with 1 / 2 / 4 slices: Q4_0 6144 x
+    // 4096, 200 vectors 62.9 / 54.5 / 50.6, 400 79.5 / 71.2 / 71.3; 1024 x 4096, 400
+    // 65.3 / 45.5 / 36.2; 576 x 576, 200 16.9 / 20.3. 64 wide / 128: 6144 x 4096,
+    // 1,024 vectors 118 / 126, 1,999 221 / 210; Q4_K 1,999 234 / 204.
     const int vec_tiles = (n + 15) / 16, row_blocks = (w->n_tiles + 7) / 8;
-    const int vt = row_blocks * ((vec_tiles + 7) / 8) >= ctx->n_cu ? 4 : 2;
+    const int vt = (int64_t)row_blocks * ((vec_tiles + 7) / 8) >= 2 * ctx->n_cu ? 4 : 2;
     const int vec_blocks = (vec_tiles + 2 * vt - 1) / (2 * vt);
-    const int units = k ? w->n_quads / 2 : w->n_quads;
     const int64_t wgs = (int64_t)row_blocks * vec_blocks, stride = (int64_t)n * w->rows;
-    int slices = (int)std::max<int64_t>(1, ctx->n_cu / wgs);
-    slices = std::max(1, std::min({kMaxSlices, slices, units / 2}));
-    while (slices > 1 && (size_t)slices * stride * sizeof(float) > ((size_t)28 << 20)) slices--;
+    int slices = 1;
+    while (vt == 2 && 2 * slices <= kMaxSlices && 2 * slices * wgs <= 3 * ctx->n_cu && 2 * slices * 8 <= w->n_quads &&
+           (size_t)(2 * slices) * stride * sizeof(float) <= ((size_t)28 << 20))
+        slices *= 2;
     Pieces px;
     float *part = nullptr;
     int32_t *arrivals = nullptr;
@@ -1125,7 +1207,10 @@ int gla_matvec_q4(gla_ctx *ctx, const gla_q4w *w, const float *x, int n_vec, flo
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
     const Weights p{w->quants, w->aux, w->super, w->rows, w->cols, w->n_tiles, w->n_quads};
     if (n_vec <= kFewVec) return few(ctx, w, p, x, n_vec, y);
-    if (n_vec <= 64) return mid(ctx, w, p, x, n_vec, y);
+    // The mid kernel up to 128 vectors, but for tall matrices, whose rows fill the chip
+    // by themselves (us, mid / gemm: 6144 x 4096, 100 vectors 34.3 / 42.6; 1024 x 4096
+    // 24.8 / 34.9; 16384 x 4096 63.7 / 57.9).
+    if (n_vec <= 64 || (n_vec <= 128 && w->n_tiles <= 2 * ctx->n_cu)) return mid(ctx, w, p, x, n_vec, y);
     return many(ctx, w, p, x, n_vec, y);
     GLA_GUARD_END
 }
