@@ -183,12 +183,16 @@ constexpr uint32_t kInf = 0x7f800000u;
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ int shift_of(uint32_t mx) { return min(140 - (int)(mx >> 23), 120); }
 __device__ __forceinline__ float exp2_of(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-    // within a row of 16 lanes by rotation, then rows 0/1 and 2/3, then the halves
+// the largest of a row of 16 lanes, by rotation
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));
+}
+// ... of the wave: then rows 0/1 and 2/3, then the halves
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    x = row_max(x);
     const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
     x = max(a[0], a[1]);
     const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
@@ -233,8 +237,8 @@ __device__ __forceinline__ void load_row(float (&e)[8], const float *row, int by
 // ---- up to 8 vectors ------------------------------------------------------------------
 
 // y[v][row] for up to NV vectors, RT row tiles a workgroup. The eight waves split
-// K; a wave takes its quads four at a time (a chunk of 512 columns): its lanes load
-// 8 elements of each vector, find the chunk's largest |x| of each vector, and put
+// K; a wave takes its quads CH at a time (a chunk; four, or one where that is all
+// there is, four vectors side by side then): its lanes load 8 elements of each vector, find the chunk's largest |x| of each vector, and put
 // the pieces into the wave's LDS in the order of the B operand, whose 16 columns
 // are the hi pieces of the vectors and then their lo pieces: one MFMA multiplies
 // 16 rows x 32 columns of weights with all of them. No wave waits for another
@@ -245,22 +249,26 @@ __device__ __forceinline__ void load_row(float (&e)[8], const float *row, int by
 //   MFMA; the rows' d multiplies once a quad. The minima are a product of their
 //   own: four minima of a row with the sums of x over the four groups (in pieces,
 //   scaled by 2^-5; the minima carry 2^5).
-constexpr int kChunk = 4;  // quads
 constexpr int kFewWaves = 8;
-template <bool K, int NV, int RT>
+template <bool K, int NV, int RT, int CH>
 __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Weights w, const float *x, int n_vec, float *y) {
     constexpr int COLS = 2 * NV;
-    constexpr int PITCH = 65;             // half8 from column to column: 64 of [group][kg], and one for the banks
-    constexpr int PIECES = COLS * PITCH;  // of a wave's chunk
-    constexpr int SUMS = K ? kChunk * COLS : 0;    // half4: [quad][column]
-    constexpr int WAVE = PIECES * 16 + SUMS * 8;
+    constexpr int LANES = 16 * CH;                // of a vector's chunk, 8 elements each
+    constexpr int VP = 64 / LANES;                // vectors at a time
+    constexpr int NI = (NV + VP - 1) / VP;
+    constexpr int PITCH = LANES + 1;              // half8 from column to column: [group][kg], and one for the banks
+    constexpr int PIECES = COLS * PITCH;          // of a wave's chunk
+    constexpr int SUMS = K ? CH * COLS : 0;       // half4: [quad][column]
+    constexpr int WAVE = (PIECES * 16 + SUMS * 8 + NV * 4 + 15) / 16 * 16;
     constexpr int RED = kFewWaves * RT * 64 * 16;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kFewWaves * WAVE > RED ? kFewWaves * WAVE : RED];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, kg = lane >> 4;
+    const int vg = lane / LANES, vl = lane % LANES;  // the vector of a pass, and the lane's eight of its chunk
     half8 *px = reinterpret_cast<half8 *>(lds + wave * WAVE);
     half4 *ps = reinterpret_cast<half4 *>(lds + wave * WAVE + PIECES * 16);
+    float *pu = reinterpret_cast<float *>(lds + wave * WAVE + PIECES * 16 + SUMS * 8);
     constexpr int UNIT = K ? 2 : 1;  // whole superblocks a wave
     const int per = (w.n_quads / UNIT + kFewWaves - 1) / kFewWaves * UNIT;
     const int q0 = min(w.n_quads, wave * per), q1 = min(w.n_quads, q0 + per);
@@ -270,21 +278,28 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
 #pragma unroll
     for (int t = 0; t < RT; t++) total[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    for (int c0 = q0; c0 < q1; c0 += kChunk) {
+    for (int c0 = q0; c0 < q1; c0 += CH) {
         // x first: loads return in order, so the pieces do not wait for weights
-        float e[NV][8];
+        float e[NI][8];
         const int bytes = (min(w.cols, q1 * 128) - c0 * 128) * 4;  // of the wave's columns from here on
 #pragma unroll
-        for (int v = 0; v < NV; v++)
-            load_row(e[v], x + (int64_t)min(v, n_vec - 1) * w.cols + c0 * 128, v < n_vec ? bytes : 0, lane * 32);
-        u32x4 qw[RT][kChunk];
-        u32x4 sc[RT][kChunk][2];      // Q4_0: the 32 bytes of rows kg * 4 .. +3
-        u32x2 am[RT][kChunk];         // Q4_K: the lane's row's scales and minima
-        u32x4 sup[RT][kChunk / 2];  // Q4_K: d and dmin of rows kg * 4 .. +3
+        for (int i = 0; i < NI; i++) {
+            if constexpr (VP == 1) {
+                load_row(e[i], x + (int64_t)min(i, n_vec - 1) * w.cols + c0 * 128, i < n_vec ? bytes : 0, lane * 32);
+            } else {
+                const int v = i * VP + vg;
+                const bool in = v < n_vec && vl * 32 < bytes;
+                load_row(e[i], x + c0 * 128, ((n_vec - 1) * w.cols + w.cols - c0 * 128) * 4, in ? v * w.cols * 4 + vl * 32 : -32);
+            }
+        }
+        u32x4 qw[RT][CH];
+        u32x4 sc[RT][CH][2];            // Q4_0: the 32 bytes of rows kg * 4 .. +3
+        u32x2 am[RT][CH];               // Q4_K: the lane's row's scales and minima
+        u32x4 sup[RT][(CH + 1) / 2];    // Q4_K: d and dmin of rows kg * 4 .. +3
 #pragma unroll
         for (int t = 0; t < RT; t++)
 #pragma unroll
-            for (int i = 0; i < kChunk; i++) {
+            for (int i = 0; i < CH; i++) {
                 const int64_t tq = (int64_t)min(tile0 + t, w.n_tiles - 1) * w.n_quads + min(c0 + i, w.n_quads - 1);
                 qw[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(w.quants + (tq * 64 + lane) * 16));
                 if constexpr (K) {
@@ -299,57 +314,58 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
 #pragma unroll
             for (int t = 0; t < RT; t++)
 #pragma unroll
-                for (int i = 0; i < kChunk / 2; i++) {
+                for (int i = 0; i < (CH + 1) / 2; i++) {
                     const int sb = min((c0 >> 1) + i, w.n_quads / 2 - 1);
                     sup[t][i] = *reinterpret_cast<const u32x4 *>(
                         w.super + ((int64_t)min(tile0 + t, w.n_tiles - 1) * (w.n_quads / 2) + sb) * 16 + kg * 4);
                 }
         }
-        float undo = 0.0f;  // 2^-s of the lane's column
-        uint32_t mx[NV];
+        uint32_t mx[NI];
 #pragma unroll
-        for (int v = 0; v < NV; v++) {
-            mx[v] = 0;
+        for (int i = 0; i < NI; i++) {
+            mx[i] = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++) mx[v] = max(mx[v], abs_bits(e[v][j]));
-            mx[v] = wave_max(mx[v]);
+            for (int j = 0; j < 8; j++) mx[i] = max(mx[i], abs_bits(e[i][j]));
+            mx[i] = VP == 1 ? wave_max(mx[i]) : row_max(mx[i]);
         }
 #pragma unroll
-        for (int v = 0; v < NV; v++) {
-            uint32_t top = __builtin_amdgcn_readfirstlane(mx[v]);
-            const bool odd = top >= kInf;
+        for (int i = 0; i < NI; i++) {
+            uint32_t top = VP == 1 ? __builtin_amdgcn_readfirstlane(mx[i]) : mx[i];
+            const bool odd = VP == 1 ? top >= kInf : __any(top >= kInf);
             if (odd) {  // scaled by what is finite
-                mx[v] = 0;
+                mx[i] = 0;
 #pragma unroll
-                for (int j = 0; j < 8; j++) mx[v] = max(mx[v], abs_bits(e[v][j]) < kInf ? abs_bits(e[v][j]) : 0);
-                top = __builtin_amdgcn_readfirstlane(wave_max(mx[v]));
+                for (int j = 0; j < 8; j++) mx[i] = max(mx[i], abs_bits(e[i][j]) < kInf ? abs_bits(e[i][j]) : 0);
+                top = VP == 1 ? __builtin_amdgcn_readfirstlane(wave_max(mx[i])) : row_max(mx[i]);
             }
             const int sh = shift_of(top);
             const float mul = exp2_of(sh);
-            if (col == v || col == NV + v) undo = exp2_of(-sh);
             half8 hi, lo;
             float sum = 0.0f;
             const auto split = [&](bool odd) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     _Float16 a, b;
-                    pieces(e[v][j], mul, odd, a, b);
+                    pieces(e[i][j], mul, odd, a, b);
                     hi[j] = a;
                     lo[j] = b;
-                    sum = fmaf(e[v][j], mul, sum);
+                    sum = fmaf(e[i][j], mul, sum);
                 }
             };
             if (odd)
                 split(true);
             else
                 split(false);
-            px[v * PITCH + lane] = hi;  // lane = group * 4 + kg of the chunk
-            px[(NV + v) * PITCH + lane] = lo;
+            const int v = i * VP + vg;
+            if (v >= NV) continue;  // (more lanes than vectors)
+            if (vl == 0) pu[v] = exp2_of(-sh);
+            px[v * PITCH + vl] = hi;  // vl = group * 4 + kg of the chunk
+            px[(NV + v) * PITCH + vl] = lo;
             if constexpr (K) {
                 _Float16 a, b;
                 pieces(quad_sum(sum), 0.03125f, true, a, b);
-                if ((lane & 3) == 0) {
-                    _Float16 *to = reinterpret_cast<_Float16 *>(ps + (lane >> 4) * COLS) + ((lane >> 2) & 3);
+                if ((vl & 3) == 0) {
+                    _Float16 *to = reinterpret_cast<_Float16 *>(ps + (vl >> 4) * COLS) + ((vl >> 2) & 3);
                     to[v * 4] = a;
                     to[(NV + v) * 4] = b;
                 }
@@ -357,12 +373,13 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        const float undo = pu[col % NV];  // 2^-s of the lane's column (of the first 2 NV)
         floatx4 acc[RT];
 #pragma unroll
         for (int t = 0; t < RT; t++) acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < kChunk; i++) {
+        for (int i = 0; i < CH; i++) {
             if (c0 + i >= q1) break;
             half8 bx[4];
 #pragma unroll
@@ -1020,9 +1037,11 @@ int launch_few(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x,
         hipLaunchKernelGGL(kernel, dim3((w->n_tiles + tiles - 1) / tiles), dim3(kFewWaves * 64), 0, ctx->stream, p, x, n, y);
     };
     if (w->n_tiles > (NV == 1 ? 2 : 1) * ctx->n_cu)
-        go(matvec_q4_few_kernel<K, NV, 2>, 2);
+        go(matvec_q4_few_kernel<K, NV, 2, 4>, 2);
+    else if (w->n_quads > kFewWaves)
+        go(matvec_q4_few_kernel<K, NV, 1, 4>, 1);
     else
-        go(matvec_q4_few_kernel<K, NV, 1>, 1);
+        go(matvec_q4_few_kernel<K, NV, 1, 1>, 1);
     return launched("matvec_q4_few_kernel");
 }
 
