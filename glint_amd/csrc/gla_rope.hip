@@ -581,11 +581,12 @@ int gla_rope_rows(gla_ctx *ctx, const gla_rope_plan *plan, const float *x, int64
     const int d = plan->head_dim;
     const int lanes = (d + 3) / 4, per = 64 / lanes;
     const int parts = parts_of(n_rows, (n_heads + per - 1) / per, kRopeWaves);
-    const unsigned blocks = (unsigned)(((int64_t)n_rows * parts + kWaves - 1) / kWaves);
+    const int64_t blocks = ((int64_t)n_rows * parts + kWaves - 1) / kWaves;
+    GLA_REQUIRE(blocks <= INT32_MAX / (kWaves * 64), "gla_rope_rows: %d rows are too many for one call", n_rows);
     const bool vec = d % 4 == 0 && aligned16(x, x_stride) && aligned16(out, out_stride);
     auto kernel = plan->half ? (vec ? rope_rows_kernel<kHalf, true> : rope_rows_kernel<kHalf, false>)
                              : (vec ? rope_rows_kernel<kAdjacent, true> : rope_rows_kernel<kAdjacent, false>);
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kWaves * 64), kWaves * wave_lds(plan->half ? kHalf : kAdjacent, plan->pairs),
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kWaves * 64), kWaves * wave_lds(plan->half ? kHalf : kAdjacent, plan->pairs),
                        ctx->stream, rope_of(plan), x, x_stride, out, out_stride, n_rows, n_heads, d, lanes, parts, pos);
     return launched("rope_rows_kernel");
     GLA_GUARD_END

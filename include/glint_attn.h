@@ -79,10 +79,11 @@ const char *gla_last_error(void);
  * the condition GpuBackend::new reports as GpuAdapterNotFound
  * (src/backend/gpu.rs:44-56); the caller then stays on its CPU path. */
 int gla_create(int device, gla_ctx **out);
-/* Frees the context and the device memory of every cache, pool and weight
- * set created on it; their handles must still be released
- * (gla_kv_destroy, gla_q8w_destroy), which then frees only the handle, and
- * any other use of them fails with GLA_ERR_INVALID. */
+/* Frees the context and the device memory of every cache, pool, weight set
+ * and rotary plan created on it; their handles must still be released
+ * (gla_kv_destroy, gla_q8w_destroy, gla_q4w_destroy, gla_rope_plan_destroy),
+ * which then frees only the handle, and any other use of them fails with
+ * GLA_ERR_INVALID. */
 int gla_destroy(gla_ctx *ctx);
 
 /* Run subsequent work on `hip_stream` (a hipStream_t); NULL restores the
@@ -397,7 +398,8 @@ int gla_rope_plan_destroy(gla_rope_plan *plan);
 /* Rotate device rows: x [n_rows] rows of [n_heads][head_dim] floats, x_stride
  * floats apart (0: n_heads * head_dim), into out likewise; row r at position
  * pos[r] (device int32). out may be x with the same stride (in place); other
- * overlaps are not allowed. Asynchronous; allocates nothing. */
+ * overlaps are not allowed. At most 33,554,428 rows a call (else
+ * GLA_ERR_INVALID: split it). Asynchronous; allocates nothing. */
 int gla_rope_rows(gla_ctx *ctx, const gla_rope_plan *plan, const float *x, int64_t x_stride, float *out,
                   int64_t out_stride, int n_rows, int n_heads, const int32_t *pos);
 
@@ -473,7 +475,10 @@ int gla_q4w_cols(const gla_q4w *w);
 
 /* y[v][r] = sum_c W[r][c] * x[v][c] for n_vec vectors, as gla_matvec_q8_0:
  * x device [n_vec][cols], y device [n_vec][rows], f32, y apart from x.
- * Asynchronous. n_vec above 262,128 is refused (split the call). */
+ * Asynchronous; up to 8 vectors allocate nothing, more take scratch of the
+ * stream, which the first call of a size allocates: make that call before
+ * capturing it into a graph (a capture that would allocate is refused,
+ * GLA_ERR_INVALID). n_vec above 262,128 is refused (split the call). */
 int gla_matvec_q4(gla_ctx *ctx, const gla_q4w *w, const float *x, int n_vec, float *y);
 
 #ifdef __cplusplus
