@@ -392,6 +392,13 @@ Status PagedKvCache::make_writable(size_t layer, size_t first_page, size_t last_
     return {};
 }
 
+// Pages for positions pos0 .. pos0 + n - 1 of `layer`, present and private.
+Status PagedKvCache::own_pages(size_t layer, size_t pos0, size_t n) {
+    if (n == 0) return {};
+    std::lock_guard<std::mutex> g(pool_.inner_->mu);
+    return make_writable(layer, pos0 / PAGE_SIZE, (pos0 + n - 1) / PAGE_SIZE);
+}
+
 void PagedKvCache::write(size_t layer, size_t pos, const float *k, const float *v) { write_chunk(layer, pos, 1, k, v); }
 
 void PagedKvCache::write_chunk(size_t layer, size_t pos0, size_t n, const float *k, const float *v) {
@@ -625,7 +632,7 @@ struct GpuBackend::Staging {
         void *ptr = nullptr;
         size_t bytes = 0;
     };
-    enum { Q, OUT, TABLE, START, LEN, SLOT, QSTART, POSOFF, POS, N_BUFS };
+    enum { Q, OUT, TABLE, START, LEN, SLOT, QSTART, POSOFF, POS, K, V, N_BUFS };
     std::shared_ptr<Device> dev;
     Buf bufs[N_BUFS];
 
@@ -1005,6 +1012,191 @@ Status GpuBackend::rope(float *x, size_t n_rows, size_t n_heads, size_t head_dim
                      "gla_rope");
     if (!s) return s;
     return check(gla_memcpy_dtoh(dev_->ctx(), x, px.value(), bytes), "gla_memcpy_dtoh");
+}
+
+GpuQ4Weights::GpuQ4Weights(std::shared_ptr<Device> dev, gla_q4w *w, size_t rows, size_t cols)
+    : dev_(std::move(dev)), w_(w), rows_(rows), cols_(cols) {}
+GpuQ4Weights::GpuQ4Weights(GpuQ4Weights &&o) noexcept
+    : dev_(std::move(o.dev_)), w_(o.w_), rows_(o.rows_), cols_(o.cols_) {
+    o.w_ = nullptr;
+}
+GpuQ4Weights &GpuQ4Weights::operator=(GpuQ4Weights &&o) noexcept {
+    if (this != &o) {
+        if (w_) gla_q4w_destroy(w_);
+        dev_ = std::move(o.dev_);
+        w_ = o.w_;
+        rows_ = o.rows_;
+        cols_ = o.cols_;
+        o.w_ = nullptr;
+    }
+    return *this;
+}
+GpuQ4Weights::~GpuQ4Weights() {
+    if (w_) gla_q4w_destroy(w_);
+}
+
+Result<GpuQ4Weights> GpuBackend::upload_q4(gla_q4_format format, const uint8_t *ggml, size_t n_bytes, size_t rows,
+                                           size_t cols) {
+    const size_t group = format == GLA_Q4_K ? 256 : 32, size = format == GLA_Q4_K ? 144 : 18;
+    if (cols % group != 0 || rows == 0 || cols == 0 || rows > INT32_MAX || cols > INT32_MAX)
+        return GlintError::gpu_buffer_error(fmt("upload_q4: %zu x %zu is no matrix of this format", rows, cols));
+    if (n_bytes != rows * (cols / group) * size)
+        return GlintError::gpu_buffer_error(fmt("upload_q4: %zu bytes for %zu x %zu (expected %zu)", n_bytes, rows, cols,
+                                                rows * (cols / group) * size));
+    gla_q4w *w = nullptr;
+    Status s = check(gla_q4w_create(dev_->ctx(), format, ggml, (int)rows, (int)cols, &w), "gla_q4w_create");
+    if (!s) return s.error();
+    return GpuQ4Weights(dev_, w, rows, cols);
+}
+
+Result<std::vector<float>> GpuBackend::matvec_q4(const GpuQ4Weights &w, const float *x, size_t n_vec) {
+    if (!w.handle()) return GlintError::gpu_shader_error("matvec_q4: weights not uploaded");
+    if (n_vec == 0) return std::vector<float>();
+    if (n_vec > INT32_MAX) return GlintError::gpu_shader_error("matvec_q4: too many vectors");
+    Staging &st = *stage_;
+    Result<void *> px = st.put(Staging::Q, x, n_vec * w.cols() * sizeof(float));
+    if (!px) return px.error();
+    Result<void *> py = st.get(Staging::OUT, n_vec * w.rows() * sizeof(float));
+    if (!py) return py.error();
+    Status s = check(gla_matvec_q4(dev_->ctx(), w.handle(), (const float *)px.value(), (int)n_vec, (float *)py.value()),
+                     "gla_matvec_q4");
+    if (!s) return s.error();
+    std::vector<float> y(n_vec * w.rows());
+    s = check(gla_memcpy_dtoh(dev_->ctx(), y.data(), py.value(), y.size() * sizeof(float)), "gla_memcpy_dtoh");
+    if (!s) return s.error();
+    return y;
+}
+
+GpuRopePlan::GpuRopePlan(std::shared_ptr<Device> dev, gla_rope_plan *p, size_t head_dim)
+    : dev_(std::move(dev)), p_(p), head_dim_(head_dim) {}
+GpuRopePlan::GpuRopePlan(GpuRopePlan &&o) noexcept : dev_(std::move(o.dev_)), p_(o.p_), head_dim_(o.head_dim_) {
+    o.p_ = nullptr;
+}
+GpuRopePlan &GpuRopePlan::operator=(GpuRopePlan &&o) noexcept {
+    if (this != &o) {
+        if (p_) gla_rope_plan_destroy(p_);
+        dev_ = std::move(o.dev_);
+        p_ = o.p_;
+        head_dim_ = o.head_dim_;
+        o.p_ = nullptr;
+    }
+    return *this;
+}
+GpuRopePlan::~GpuRopePlan() {
+    if (p_) gla_rope_plan_destroy(p_);
+}
+
+Result<GpuRopePlan> GpuBackend::create_rope_plan(const gla_rope_spec &spec) {
+    gla_rope_plan *p = nullptr;
+    Status s = check(gla_rope_plan_create(dev_->ctx(), &spec, &p), "gla_rope_plan_create");
+    if (!s) return s.error();
+    return GpuRopePlan(dev_, p, (size_t)spec.head_dim);
+}
+
+Status GpuBackend::rope_rows(const GpuRopePlan &plan, float *x, size_t n_rows, size_t n_heads, const int32_t *pos) {
+    if (!plan.handle()) return GlintError::gpu_shader_error("rope_rows: no plan");
+    if (n_rows == 0) return {};
+    if (n_rows > INT32_MAX || n_heads > INT32_MAX) return GlintError::gpu_shader_error("rope_rows: shape out of range");
+    const size_t bytes = n_rows * n_heads * plan.head_dim() * sizeof(float);
+    Staging &st = *stage_;
+    Result<void *> px = st.put(Staging::Q, x, bytes);
+    if (!px) return px.error();
+    Result<void *> pp = st.put(Staging::POS, pos, n_rows * sizeof(int32_t));
+    if (!pp) return pp.error();
+    Status s = check(gla_rope_rows(dev_->ctx(), plan.handle(), (const float *)px.value(), 0, (float *)px.value(), 0,
+                                   (int)n_rows, (int)n_heads, (const int32_t *)pp.value()),
+                     "gla_rope_rows");
+    if (!s) return s;
+    return check(gla_memcpy_dtoh(dev_->ctx(), x, px.value(), bytes), "gla_memcpy_dtoh");
+}
+
+Result<std::vector<float>> GpuBackend::append_batch(const std::vector<AppendSeq> &seqs, const float *q, const float *k,
+                                                    const float *v, size_t layer, const AttnShape &shape,
+                                                    const GpuRopePlan *plan) {
+    const size_t B = seqs.size();
+    const size_t row = (size_t)shape.n_heads * shape.head_dim;
+    if (B == 0) return std::vector<float>();
+    if (plan && !plan->handle()) return GlintError::gpu_shader_error("append_batch: no plan");
+    std::vector<const KvStore *> stores(B);
+    for (size_t b = 0; b < B; b++) stores[b] = seqs[b].kv;
+    std::vector<const KvStore *> sorted = stores;
+    std::sort(sorted.begin(), sorted.end(), std::less<>());
+    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+        return GlintError::gpu_shader_error("append_batch: a cache given twice");
+    Result<Source> src = source_of(stores, "append_batch");
+    if (!src) return src.error();
+    const Source &S = src.value();
+    if (S.kv_dim != (size_t)shape.n_kv_heads * shape.head_dim)
+        return GlintError::gpu_shader_error("append_batch: n_kv_heads * head_dim does not match the cache");
+    std::vector<int32_t> q_start(B + 1, 0), pos_off(B), slot, table;
+    int max_q = 0, stride = 1;
+    for (size_t b = 0; b < B; b++) {
+        const size_t end = seqs[b].pos_offset + seqs[b].n_rows;
+        if (end > INT32_MAX || (size_t)q_start[b] + seqs[b].n_rows > INT32_MAX)
+            return GlintError::gpu_shader_error("append_batch: positions out of range");
+        if (S.paged) {
+            if (layer >= seqs[b].kv->as_paged()->n_layers())
+                return GlintError::gpu_shader_error("append_batch: layer out of range");
+        } else {
+            const GpuKvBuffer *g = seqs[b].kv->gpu_buffer();
+            if (layer >= g->n_layers) return GlintError::gpu_shader_error("append_batch: layer out of range");
+            if (end > g->max_seq_len)
+                return GlintError::gpu_shader_error(fmt("append_batch: positions to %zu > max_seq_len %zu", end,
+                                                        g->max_seq_len));
+            slot.push_back(g->seq);
+        }
+        q_start[b + 1] = q_start[b] + (int32_t)seqs[b].n_rows;
+        pos_off[b] = (int32_t)seqs[b].pos_offset;
+        max_q = std::max(max_q, (int)seqs[b].n_rows);
+    }
+    const size_t rows = (size_t)q_start[B];
+    if (rows == 0) return std::vector<float>();
+    if (S.paged) {
+        for (size_t b = 0; b < B; b++) {
+            Status s = seqs[b].kv->as_paged()->own_pages(layer, seqs[b].pos_offset, seqs[b].n_rows);
+            if (!s) return s.error();
+            stride = std::max(stride, (int)seqs[b].kv->as_paged()->page_table(layer).size());
+        }
+        table.assign(B * (size_t)stride, -1);
+        for (size_t b = 0; b < B; b++) {
+            const auto &t = seqs[b].kv->as_paged()->page_table(layer);
+            std::copy(t.begin(), t.end(), table.begin() + (ptrdiff_t)(b * stride));
+        }
+    }
+    gla_append_args a{};
+    a.kv = const_cast<gla_kv *>(S.kv);
+    a.layer = (int)layer;
+    a.n_seqs = (int)B;
+    Staging &st = *stage_;
+    Result<void *> p = st.put(Staging::Q, q, rows * row * sizeof(float));
+    if (!p) return p.error();
+    a.q = (const float *)p.value();
+    a.q_out = (float *)p.value();
+    if (!(p = st.put(Staging::K, k, rows * S.kv_dim * sizeof(float)))) return p.error();
+    a.k = (const float *)p.value();
+    if (!(p = st.put(Staging::V, v, rows * S.kv_dim * sizeof(float)))) return p.error();
+    a.v = (const float *)p.value();
+    if (!(p = st.put(Staging::QSTART, q_start.data(), (B + 1) * 4))) return p.error();
+    a.q_start = (const int32_t *)p.value();
+    if (!(p = st.put(Staging::POSOFF, pos_off.data(), B * 4))) return p.error();
+    a.pos_offset = (const int32_t *)p.value();
+    if (S.paged) {
+        if (!(p = st.put(Staging::TABLE, table.data(), table.size() * 4))) return p.error();
+        a.page_table = (const int32_t *)p.value();
+        a.page_table_stride = stride;
+    } else {
+        if (!(p = st.put(Staging::SLOT, slot.data(), B * 4))) return p.error();
+        a.seq_slot = (const int32_t *)p.value();
+    }
+    a.max_q_len = max_q;
+    a.rope = plan ? plan->handle() : nullptr;
+    a.n_heads = (int)shape.n_heads;
+    Status s = check(gla_kv_append(dev_->ctx(), &a), "gla_kv_append");
+    if (!s) return s.error();
+    std::vector<float> out(rows * row);
+    s = check(gla_memcpy_dtoh(dev_->ctx(), out.data(), a.q_out, out.size() * sizeof(float)), "gla_memcpy_dtoh");
+    if (!s) return s.error();
+    return out;
 }
 
 size_t window_start(size_t pos, size_t sliding_window, bool alternating, size_t layer) {

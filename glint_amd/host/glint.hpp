@@ -204,6 +204,7 @@ class KvStore {
                               const std::vector<std::vector<uint8_t>> &v_layers, size_t token_count) = 0;
     virtual const GpuKvBuffer *gpu_buffer() const { return nullptr; }
     virtual const PagedKvCache *as_paged() const { return nullptr; }
+    virtual PagedKvCache *as_paged() { return nullptr; }
 };
 
 // ---- page storage --------------------------------------------------------------
@@ -348,9 +349,12 @@ class PagedKvCache final : public KvStore {
     Status import_raw(const std::vector<std::vector<uint8_t>> &k_layers,
                       const std::vector<std::vector<uint8_t>> &v_layers, size_t token_count) override;
     const PagedKvCache *as_paged() const override { return this; }
+    PagedKvCache *as_paged() override { return this; }
 
   private:
+    friend class GpuBackend;  // append_batch makes pages writable
     PagedKvCache(const PagePool &pool, std::vector<std::vector<int32_t>> table, size_t len);
+    Status own_pages(size_t layer, size_t pos0, size_t n);
     Status ensure_capacity(size_t total_positions);
     Status make_writable(size_t layer, size_t first_page, size_t last_page);
     std::vector<float> row_at(size_t layer, size_t pos, bool v) const;
@@ -416,6 +420,14 @@ struct PrefillSeq {
     size_t pos_offset = 0;
 };
 
+// One sequence of a batched append: its cache, its n_rows new rows and the
+// absolute position of the first.
+struct AppendSeq {
+    KvStore *kv = nullptr;
+    size_t n_rows = 0;
+    size_t pos_offset = 0;
+};
+
 // Attention shape and numerics shared by a call.
 struct AttnShape {
     uint32_t n_heads = 0;
@@ -446,6 +458,45 @@ class GpuQ8Weights {
     std::shared_ptr<Device> dev_;
     gla_q8w *w_ = nullptr;
     size_t rows_ = 0, cols_ = 0;
+};
+
+// GGML Q4_0 or Q4_K weights on the device, like GpuQ8Weights.
+class GpuQ4Weights {
+  public:
+    GpuQ4Weights(GpuQ4Weights &&o) noexcept;
+    GpuQ4Weights &operator=(GpuQ4Weights &&o) noexcept;
+    GpuQ4Weights(const GpuQ4Weights &) = delete;
+    GpuQ4Weights &operator=(const GpuQ4Weights &) = delete;
+    ~GpuQ4Weights();
+    size_t rows() const { return rows_; }
+    size_t cols() const { return cols_; }
+    const gla_q4w *handle() const { return w_; }
+
+  private:
+    friend class GpuBackend;
+    GpuQ4Weights(std::shared_ptr<Device> dev, gla_q4w *w, size_t rows, size_t cols);
+    std::shared_ptr<Device> dev_;
+    gla_q4w *w_ = nullptr;
+    size_t rows_ = 0, cols_ = 0;
+};
+
+// Rotary frequencies on the device (gla_rope_plan). Move-only.
+class GpuRopePlan {
+  public:
+    GpuRopePlan(GpuRopePlan &&o) noexcept;
+    GpuRopePlan &operator=(GpuRopePlan &&o) noexcept;
+    GpuRopePlan(const GpuRopePlan &) = delete;
+    GpuRopePlan &operator=(const GpuRopePlan &) = delete;
+    ~GpuRopePlan();
+    size_t head_dim() const { return head_dim_; }
+    const gla_rope_plan *handle() const { return p_; }
+
+  private:
+    friend class GpuBackend;
+    GpuRopePlan(std::shared_ptr<Device> dev, gla_rope_plan *p, size_t head_dim);
+    std::shared_ptr<Device> dev_;
+    gla_rope_plan *p_ = nullptr;
+    size_t head_dim_ = 0;
 };
 
 class GpuBackend {
@@ -510,6 +561,25 @@ class GpuBackend {
     // heads, row r at position pos[r], in place on host data.
     Status rope(float *x, size_t n_rows, size_t n_heads, size_t head_dim, const int32_t *pos, float freq_base,
                 float scaling_factor, size_t rot_dim);
+
+    // A Q4_0 (rows * cols / 32 * 18 bytes) or Q4_K (rows * cols / 256 * 144)
+    // tensor, and its product with n_vec host vectors, like the Q8_0 ones above.
+    Result<GpuQ4Weights> upload_q4(gla_q4_format format, const uint8_t *ggml, size_t n_bytes, size_t rows, size_t cols);
+    Result<std::vector<float>> matvec_q4(const GpuQ4Weights &w, const float *x, size_t n_vec);
+    // A rotary specification (include/glint_attn.h), and rows rotated by it in
+    // place on host data, row r at position pos[r].
+    Result<GpuRopePlan> create_rope_plan(const gla_rope_spec &spec);
+    Status rope_rows(const GpuRopePlan &plan, float *x, size_t n_rows, size_t n_heads, const int32_t *pos);
+    // The K and V of a batch's new positions in one layer, K rotated by `plan`
+    // (nullptr: as it is) on the way into the caches, and the rotated queries:
+    // k, v [sum n_rows][n_kv_heads*head_dim], q [sum n_rows][n_heads*head_dim]
+    // host -> q's shape. The storages are those decode_batch takes; pages a
+    // sequence lacks or shares are made its own first, as KvStore::write does,
+    // but an exhausted pool is an error here, not a panic. A cache comes at most
+    // once in a call. advance() stays with the caller.
+    Result<std::vector<float>> append_batch(const std::vector<AppendSeq> &seqs, const float *q, const float *k,
+                                            const float *v, size_t layer, const AttnShape &shape,
+                                            const GpuRopePlan *plan);
 
   private:
     explicit GpuBackend(std::shared_ptr<Device> dev);

@@ -991,6 +991,167 @@ DEVICE_TEST(test_rope_through_host_layer) {
     }
 }
 
+// Q4_0 and Q4_K through the host layer against the f64 product of the
+// dequantised rows, and sizes that are no matrix of the format.
+DEVICE_TEST(test_matvec_q4_matches_f64) {
+    struct Shape {
+        gla_q4_format format;
+        size_t rows, cols, n_vec;
+    };
+    const Shape shapes[] = {{GLA_Q4_0, 50, 96, 3}, {GLA_Q4_0, 33, 576, 20}, {GLA_Q4_K, 40, 512, 1}, {GLA_Q4_K, 17, 256, 140}};
+    Rng rng(0x0404);
+    for (const Shape &sh : shapes) {
+        const bool kq = sh.format == GLA_Q4_K;
+        const size_t group = kq ? 256 : 32, size = kq ? 144 : 18, nb = sh.cols / group;
+        std::vector<uint8_t> raw(sh.rows * nb * size);
+        std::vector<double> wd(sh.rows * sh.cols), wm(sh.rows * sh.cols, 0.0);
+        for (uint8_t &b : raw) b = (uint8_t)(rng.uniform() * 256.0);
+        for (size_t i = 0; i < sh.rows * nb; i++) {
+            uint8_t *b = raw.data() + i * size;
+            double *d = wd.data() + i * group, *m = wm.data() + i * group;
+            for (int h = 0; h < (kq ? 2 : 1); h++) {  // normal f16s in [2^-12, 2^-2)
+                const uint16_t bits = (uint16_t)(((3 + (int)(rng.uniform() * 10.0)) << 10) | (int)(rng.uniform() * 1024.0));
+                b[2 * h] = (uint8_t)bits, b[2 * h + 1] = (uint8_t)(bits >> 8);
+            }
+            const double s0 = f16_to_f32((uint16_t)(b[0] | b[1] << 8));
+            if (!kq) {
+                for (int j = 0; j < 16; j++) d[j] = s0 * ((b[2 + j] & 15) - 8), d[16 + j] = s0 * ((b[2 + j] >> 4) - 8);
+                continue;
+            }
+            const double s1 = f16_to_f32((uint16_t)(b[2] | b[3] << 8));
+            for (int g = 0; g < 8; g++) {
+                const uint8_t *c = b + 4;
+                const int sc = g < 4 ? c[g] & 63 : (c[g + 4] & 15) | (c[g - 4] >> 6) << 4;
+                const int mn = g < 4 ? c[g + 4] & 63 : (c[g + 4] >> 4) | (c[g] >> 6) << 4;
+                for (int j = 0; j < 32; j++) {
+                    const int n = b[16 + g / 2 * 32 + j] >> (g % 2 * 4) & 15;
+                    d[g * 32 + j] = s0 * sc * n;
+                    m[g * 32 + j] = s1 * mn;
+                }
+            }
+        }
+        auto w = backend().upload_q4(sh.format, raw.data(), raw.size(), sh.rows, sh.cols).expect("upload");
+        CHECK_EQ(w.rows(), sh.rows);
+        CHECK_EQ(w.cols(), sh.cols);
+        const auto x = rng.normal(sh.n_vec * sh.cols);
+        const auto y = backend().matvec_q4(w, x.data(), sh.n_vec).expect("matvec");
+        CHECK_EQ(y.size(), sh.n_vec * sh.rows);
+        for (size_t v = 0; v < sh.n_vec; v++)
+            for (size_t r = 0; r < sh.rows; r++) {
+                double exact = 0.0, mag = 0.0;
+                for (size_t c = 0; c < sh.cols; c++) {
+                    const double xv = x[v * sh.cols + c], dd = wd[r * sh.cols + c], mm = wm[r * sh.cols + c];
+                    exact += xv * (dd - mm);
+                    mag += std::fabs(xv) * (std::fabs(dd) + mm);
+                }
+                CHECK_MSG(std::fabs(y[v * sh.rows + r] - exact) <= 4e-6 * mag,
+                          sh.rows << "x" << sh.cols << " vec " << v << " row " << r << ": " << y[v * sh.rows + r] << " vs "
+                                  << exact);
+            }
+        CHECK(!backend().upload_q4(sh.format, raw.data(), raw.size() - 1, sh.rows, sh.cols).ok());
+        CHECK(!backend().upload_q4(sh.format, raw.data(), raw.size(), sh.rows, sh.cols + 16).ok());
+        auto moved = std::move(w);
+        CHECK(moved.handle() != nullptr && w.handle() == nullptr);
+        CHECK(!backend().matvec_q4(w, x.data(), 1).ok());
+    }
+}
+
+// append_batch over forked sequences of a page pool and over contiguous caches:
+// rotated K and V land where write() would put them, queries come back rotated, a
+// shared page is copied first, and rows_of a full pool are refused.
+DEVICE_TEST(test_append_batch) {
+    gla_rope_spec spec{};
+    spec.head_dim = (int)HEAD_DIM;
+    spec.layout = GLA_ROPE_HALF;
+    spec.freq_base = 10000.0;
+    auto plan = backend().create_rope_plan(spec).expect("plan");
+    const AttnShape shape{4, (uint32_t)N_KV_HEADS, (uint32_t)HEAD_DIM, 0.125f, 0.0f};
+    const size_t q_dim = 4 * HEAD_DIM, half = HEAD_DIM / 2;
+    Rng rng(0xa99e);
+    const auto rotated = [&](const float *x, size_t heads, size_t pos) {
+        std::vector<float> y(x, x + heads * HEAD_DIM);
+        for (size_t h = 0; h < heads; h++)
+            for (size_t i = 0; i < half; i++) {
+                const double ang = (double)pos * std::pow(10000.0, -2.0 * (double)i / (double)HEAD_DIM);
+                const double a = x[h * HEAD_DIM + i], b = x[h * HEAD_DIM + half + i];
+                y[h * HEAD_DIM + i] = (float)(a * std::cos(ang) - b * std::sin(ang));
+                y[h * HEAD_DIM + half + i] = (float)(a * std::sin(ang) + b * std::cos(ang));
+            }
+        return y;
+    };
+    const auto near = [](const std::vector<float> &a, const std::vector<float> &b) {
+        if (a.size() != b.size()) return false;
+        for (size_t i = 0; i < a.size(); i++)
+            if (std::fabs(a[i] - b[i]) > 2e-7f * (1.0f + std::fabs(b[i]))) return false;
+        return true;
+    };
+    PagePool pool = backend().create_page_pool(8, N_KV_HEADS, HEAD_DIM).expect("pool");
+    PagedKvCache first(pool, 1);
+    first.reserve(20).expect("reserve");
+    const auto k0 = rng.normal(20 * KV_DIM), v0 = rng.normal(20 * KV_DIM);
+    first.write_chunk(0, 0, 20, k0.data(), v0.data());
+    for (int i = 0; i < 20; i++) first.advance();
+    PagedKvCache second = first.fork_from(20);  // shares both pages, the second half filled
+    CHECK(second.is_page_shared(0, 1));
+    const size_t n[2] = {3, 14};
+    const auto q = rng.normal(17 * q_dim), k = rng.normal(17 * KV_DIM), v = rng.normal(17 * KV_DIM);
+    const auto out = backend().append_batch({{&first, n[0], 20}, {&second, n[1], 20}}, q.data(), k.data(), v.data(), 0, shape,
+                                            &plan).expect("append");
+    CHECK_EQ(out.size(), q.size());
+    CHECK(!second.is_page_shared(0, 1) && second.is_page_shared(0, 0));
+    size_t r = 0;
+    for (int b = 0; b < 2; b++) {
+        PagedKvCache &c = b ? second : first;
+        for (size_t pos = 0; pos < 20; pos++) {
+            CHECK(c.k_at(0, pos) == std::vector<float>(k0.begin() + (ptrdiff_t)(pos * KV_DIM), k0.begin() + (ptrdiff_t)((pos + 1) * KV_DIM)));
+        }
+        for (size_t i = 0; i < n[b]; i++, r++) {
+            CHECK(near(c.k_at(0, 20 + i), rotated(k.data() + r * KV_DIM, N_KV_HEADS, 20 + i)));
+            CHECK(c.v_at(0, 20 + i) == std::vector<float>(v.begin() + (ptrdiff_t)(r * KV_DIM), v.begin() + (ptrdiff_t)((r + 1) * KV_DIM)));
+            CHECK(near(std::vector<float>(out.begin() + (ptrdiff_t)(r * q_dim), out.begin() + (ptrdiff_t)((r + 1) * q_dim)),
+                       rotated(q.data() + r * q_dim, 4, 20 + i)));
+        }
+    }
+    // a full pool: an error, and nothing panics
+    const std::vector<float> many(100 * KV_DIM, 1.0f), many_q(100 * q_dim, 1.0f);
+    CHECK(!backend().append_batch({{&first, 100, 23}}, many_q.data(), many.data(), many.data(), 0, shape, &plan).ok());
+    // contiguous caches, without a plan: the rows as they are
+    auto caches = backend().create_kv_caches(2, 1, 16, N_KV_HEADS, HEAD_DIM).expect("caches");
+    const auto same = backend().append_batch({{&caches[1], 2, 5}}, q.data(), k.data(), v.data(), 0, shape, nullptr).expect("append");
+    CHECK(same == std::vector<float>(q.begin(), q.begin() + (ptrdiff_t)(2 * q_dim)));
+    std::vector<float> head(HEAD_DIM);
+    caches[1].read_k_head(0, 6, 1, HEAD_DIM, head.data());
+    CHECK(head == std::vector<float>(k.begin() + (ptrdiff_t)(KV_DIM + HEAD_DIM), k.begin() + (ptrdiff_t)(KV_DIM + 2 * HEAD_DIM)));
+    CHECK(!backend().append_batch({{&caches[0], 2, 15}}, q.data(), k.data(), v.data(), 0, shape, nullptr).ok());
+    CHECK(!backend().append_batch({{&caches[0], 1, 0}, {&caches[0], 1, 1}}, q.data(), k.data(), v.data(), 0, shape, nullptr).ok());
+    CHECK(!backend().append_batch({{&caches[0], 1, 0}, {&first, 1, 0}}, q.data(), k.data(), v.data(), 0, shape, nullptr).ok());
+}
+
+DEVICE_TEST(test_rope_rows_through_host_layer) {
+    gla_rope_spec spec{};
+    spec.head_dim = 6;
+    spec.rot_dim = 4;
+    spec.freq_base = 100.0;
+    spec.scaling = GLA_ROPE_LINEAR;
+    spec.factor = 2.0;
+    auto plan = backend().create_rope_plan(spec).expect("plan");
+    Rng rng(0x7a7e);
+    const auto x = rng.normal(3 * 2 * 6);
+    auto y = x;
+    const int32_t pos[] = {0, 7, -3};
+    backend().rope_rows(plan, y.data(), 3, 2, pos).expect("rope");
+    for (size_t r = 0; r < 3; r++)
+        for (size_t h = 0; h < 2; h++)
+            for (size_t i = 0; i < 6; i += 2) {
+                const size_t o = (r * 2 + h) * 6 + i;
+                const double ang = i < 4 ? pos[r] / 2.0 * std::pow(100.0, -(double)i / 4.0) : 0.0;
+                CHECK(std::fabs(y[o] - (x[o] * std::cos(ang) - x[o + 1] * std::sin(ang))) <= 2e-7 * (1.0 + std::fabs(x[o]) + std::fabs(x[o + 1])));
+                CHECK(std::fabs(y[o + 1] - (x[o] * std::sin(ang) + x[o + 1] * std::cos(ang))) <= 2e-7 * (1.0 + std::fabs(x[o]) + std::fabs(x[o + 1])));
+            }
+    spec.factor = 0.0;
+    CHECK(!backend().create_rope_plan(spec).ok());
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
