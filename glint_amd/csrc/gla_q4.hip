@@ -297,29 +297,24 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
         u32x2 am[RT][CH];               // Q4_K: the lane's row's scales and minima
         u32x4 sup[RT][(CH + 1) / 2];    // Q4_K: d and dmin of rows kg * 4 .. +3
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int i = 0; i < CH; i++)
 #pragma unroll
-            for (int i = 0; i < CH; i++) {
-                const int64_t tq = (int64_t)min(tile0 + t, w.n_tiles - 1) * w.n_quads + min(c0 + i, w.n_quads - 1);
+            for (int t = 0; t < RT; t++) {
+                const int64_t tile = min(tile0 + t, w.n_tiles - 1);
+                const int64_t tq = tile * w.n_quads + min(c0 + i, w.n_quads - 1);
                 qw[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(w.quants + (tq * 64 + lane) * 16));
                 if constexpr (K) {
                     am[t][i] = *reinterpret_cast<const u32x2 *>(w.aux + (tq * 16 + col) * 8);
+                    if (i % 2 == 0) {
+                        const int sb = min((c0 >> 1) + i / 2, w.n_quads / 2 - 1);
+                        sup[t][i >> 1] = *reinterpret_cast<const u32x4 *>(w.super + (tile * (w.n_quads / 2) + sb) * 16 + kg * 4);
+                    }
                 } else {
                     const u32x4 *s = reinterpret_cast<const u32x4 *>(w.aux + (tq * 16 + kg * 4) * 8);
                     sc[t][i][0] = s[0];
                     sc[t][i][1] = s[1];
                 }
             }
-        if constexpr (K) {
-#pragma unroll
-            for (int t = 0; t < RT; t++)
-#pragma unroll
-                for (int i = 0; i < (CH + 1) / 2; i++) {
-                    const int sb = min((c0 >> 1) + i, w.n_quads / 2 - 1);
-                    sup[t][i] = *reinterpret_cast<const u32x4 *>(
-                        w.super + ((int64_t)min(tile0 + t, w.n_tiles - 1) * (w.n_quads / 2) + sb) * 16 + kg * 4);
-                }
-        }
         uint32_t mx[NI];
 #pragma unroll
         for (int i = 0; i < NI; i++) {
@@ -452,7 +447,9 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
 // [v % 16] = the eight groups' halves. Vectors up to the next 16 are left as they are:
 // a column of the product is its vector's alone. Many vectors go four a workgroup, so
 // that 64 bytes are written together (1,999 x 4,096: 29 us at one, whose 16-byte
-// pieces met in memory); up to 64 one, for the chip's sake.
+// pieces met in memory). Up to 64 take a workgroup each, for the chip's sake, twice:
+// both find the scale, each writes every other of the thread's units (4,096 columns, 16
+// vectors with their product 12.1 -> 11.4 us; 576 8.1 -> 6.5).
 constexpr int kSplitThreads = 512;
 constexpr int kSplitUnits = 4;  // units of 8 elements a thread keeps; a wider row is read twice
 template <bool K, int VQ>
@@ -542,10 +539,12 @@ __global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x,
             }
         }
     };
+    const int seg = blockIdx.y, segs = gridDim.y;
 #pragma unroll
     for (int i = 0; i < kSplitUnits; i++)
-        if (i * PASS + ut < units) put(e[i], i * PASS + ut);
-    for (int u = kSplitUnits * PASS + ut; u < units; u += PASS) {
+        if (i % segs == seg && i * PASS + ut < units) put(e[i], i * PASS + ut);
+    for (int i = kSplitUnits + seg; i * PASS + ut < units; i += segs) {
+        const int u = i * PASS + ut;
         float d[8];
         fetch(d, u);
         put(d, u);
@@ -558,43 +557,31 @@ struct Pieces {
     const float *undo;
 };
 
-// ---- up to 128 vectors --------------------------------------------------------------
+// ---- some vectors -------------------------------------------------------------------
 
 constexpr int kMidWaves = 8;
-constexpr int kMaxSlices = 8;
 
-__device__ __forceinline__ floatx4 load_agent4(const float *p) {
-    uint64_t *q = reinterpret_cast<uint64_t *>(const_cast<float *>(p));
-    const uint64_t a = __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const uint64_t b = __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return floatx4{__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)b),
-                   __uint_as_float((uint32_t)(b >> 32))};
-}
-
-// y[v][row] for RT row tiles x up to 16 NVT VH vectors a workgroup, and one of
-// gridDim.y slices of K: the eight waves are VH ranges of vectors x 8 / VH ranges of
-// the slice's quads. Every fragment of x that a wave reads serves RT row tiles, every
-// fragment of weights NVT vector tiles; x comes D groups ahead, the weights a quad
-// ahead. Bound: the pieces of x, which a workgroup reads whole but for its slice (64
-// vectors of 4,096: 1 MB, 256 MB through the L2s from 256 workgroups at ~24 TB/s), so
-// many vectors take more rows and a slice of K. The waves are merged in LDS in order;
-// with slices the sums go out as agent-scope stores, and the row group's last
-// workgroup to arrive adds the slices in order.
+// y[v][row] for RT row tiles x up to 16 NVT VH vectors a workgroup: the eight waves
+// are VH ranges of vectors x 8 / VH ranges of K. Every fragment of x that a wave reads
+// serves RT row tiles, every fragment of weights NVT vector tiles; x comes D groups
+// ahead, the weights a quad ahead, and the waves are merged in LDS in order. Bound: a
+// short wave's latencies (launch, the first weights, the merge: 10 of 16.7 us at 4096 x
+// 4096 and 64 vectors), then the vector unit, whose 11 instructions to unpack a dword
+// of nibbles serve NVT tiles. Workgroups for other vectors read the same weights again
+// from L2, which costs less than slices of K that have to be joined through memory
+// (64 vectors, Q4_0 4096 x 4096 19.4 -> 16.7 us, 1024 x 4096 17.4 -> 11.9, Q4_K 6144 x
+// 4096 25.5 -> 20.8).
 template <bool K, int NVT, int RT, int VH>
-__global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Weights w, const Pieces px, int n_vec, float *y,
-                                                                      float *part, int64_t slice_stride,
-                                                                      int32_t *arrivals) {
+__global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Weights w, const Pieces px, int n_vec, float *y) {
     constexpr int UNIT = K ? 2 : 1, D = NVT * RT <= 4 && NVT <= 2 ? 4 : 2, KW = kMidWaves / VH;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, kg = lane >> 4;
     const int tile0 = blockIdx.x * RT;
-    const int vt0 = wave / KW * NVT, last_vt = (n_vec - 1) >> 4;
+    const int vb = blockIdx.y * (NVT * VH), vt0 = wave / KW * NVT, last_vt = (n_vec - 1) >> 4;
     const int units = w.n_quads / UNIT;
-    const int ps = (units + gridDim.y - 1) / gridDim.y;
-    const int s0 = min(units, (int)blockIdx.y * ps), s1 = min(units, s0 + ps);
-    const int per = (s1 - s0 + KW - 1) / KW;
-    const int q0 = min(s1, s0 + wave % KW * per) * UNIT, q1 = min(s1, s0 + (wave % KW + 1) * per) * UNIT;
+    const int per = (units + KW - 1) / KW;
+    const int q0 = min(units, wave % KW * per) * UNIT, q1 = min(units, (wave % KW + 1) * per) * UNIT;
     const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 
     floatx4 acc[RT][NVT];
@@ -607,7 +594,7 @@ __global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Wei
     const auto load_x = [&](half8 (&h)[NVT], half8 (&l)[NVT], int group) {
 #pragma unroll
         for (int v = 0; v < NVT; v++) {
-            const _Float16 *src = px.xp + (((int64_t)min(vt0 + v, last_vt) * w.n_quads * 4 + group) * 128 + lane) * 8;
+            const _Float16 *src = px.xp + (((int64_t)min(vb + vt0 + v, last_vt) * w.n_quads * 4 + group) * 128 + lane) * 8;
             h[v] = *reinterpret_cast<const half8 *>(src);
             l[v] = *reinterpret_cast<const half8 *>(src + 512);
         }
@@ -636,7 +623,7 @@ __global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Wei
 #pragma unroll
             for (int v = 0; v < NVT; v++)
                 m[v] = *reinterpret_cast<const half8 *>(
-                    px.xm + (((int64_t)min(vt0 + v, last_vt) * (w.n_quads / 2) + (quad >> 1)) * 32 + (kg & 1) * 16 + col) * 8);
+                    px.xm + (((int64_t)min(vb + vt0 + v, last_vt) * (w.n_quads / 2) + (quad >> 1)) * 32 + (kg & 1) * 16 + col) * 8);
     };
     if (q0 < q1) {
         load_w(qw, sc, bm, q0);
@@ -708,62 +695,34 @@ __global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Wei
 #pragma unroll
         for (int v = 0; v < NVT; v++) *reinterpret_cast<floatx4 *>(&red[at(wave % KW, t, vt0 + v, lane)]) = acc[t][v];
     __syncthreads();
-    const int n_slices = gridDim.y;
     for (int i = threadIdx.x; i < RT * 16 * VT * 16; i += kMidWaves * 64) {
-        const int rl = i % (RT * 16), vv = i / (RT * 16);  // consecutive threads, consecutive rows
-        const int from = at(0, rl >> 4, vv >> 4, ((rl & 15) >> 2) * 16 + (vv & 15)) + (rl & 3);
+        const int rl = i % (RT * 16), vl = i / (RT * 16);  // consecutive threads, consecutive rows
+        const int from = at(0, rl >> 4, vl >> 4, ((rl & 15) >> 2) * 16 + (vl & 15)) + (rl & 3);
         float sum = red[from];
 #pragma unroll
         for (int k = 1; k < KW; k++) sum += red[from + k * RT * VT * S];
-        const int row = tile0 * 16 + rl;
-        if (row < w.rows && vv < n_vec) {
-            const int64_t to = (int64_t)vv * w.rows + row;
-            if (n_slices > 1)
-                store_agent(part + blockIdx.y * slice_stride + to, sum);
-            else
-                y[to] = sum * px.undo[vv];
-        }
-    }
-    if (n_slices == 1) return;
-    __shared__ int lds_last;
-    if (!arrive_last(arrivals + blockIdx.x, n_slices, &lds_last)) return;
-    constexpr int NQ = RT * 16 * VT * 16 / 4;  // row quads
-    if (w.rows % 4 == 0 && ((uintptr_t)y & 15) == 0) {
-        for (int qd = threadIdx.x; qd < NQ; qd += kMidWaves * 64) {
-            const int vv = qd / (RT * 4), row = tile0 * 16 + 4 * (qd % (RT * 4));
-            if (row >= w.rows || vv >= n_vec) continue;
-            const int64_t to = (int64_t)vv * w.rows + row;
-            floatx4 t[kMaxSlices];
-#pragma unroll
-            for (int s = 0; s < kMaxSlices; s++)
-                if (s < n_slices) t[s] = load_agent4(part + s * slice_stride + to);
-            floatx4 sum = t[0];
-#pragma unroll
-            for (int s = 1; s < kMaxSlices; s++)
-                if (s < n_slices) sum += t[s];
-            *reinterpret_cast<floatx4 *>(y + to) = sum * px.undo[vv];
-        }
-    } else {
-        for (int i = threadIdx.x; i < NQ * 4; i += kMidWaves * 64) {
-            const int vv = i / (RT * 16), row = tile0 * 16 + i % (RT * 16);
-            if (row >= w.rows || vv >= n_vec) continue;
-            const int64_t to = (int64_t)vv * w.rows + row;
-            float sum = load_agent(part + to);
-            for (int s = 1; s < n_slices; s++) sum += load_agent(part + s * slice_stride + to);
-            y[to] = sum * px.undo[vv];
-        }
+        const int row = tile0 * 16 + rl, v = vb * 16 + vl;
+        if (row < w.rows && v < n_vec) y[(int64_t)v * w.rows + row] = sum * px.undo[v];
     }
 }
 
 // ---- many vectors ----------------------------------------------------------------------
+
+__device__ __forceinline__ floatx4 load_agent4(const float *p) {
+    uint64_t *q = reinterpret_cast<uint64_t *>(const_cast<float *>(p));
+    const uint64_t a = __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint64_t b = __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return floatx4{__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)b),
+                   __uint_as_float((uint32_t)(b >> 32))};
+}
 
 __device__ __forceinline__ void store_agent2(float *p, float a, float b) {
     __hip_atomic_store(reinterpret_cast<uint64_t *>(p), (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a),
                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// y[v][row] for 128 rows x 32 VT vectors a workgroup, and one of gridDim.z slices of
-// K: four waves of 4 row tiles x VT vector tiles, 2 x 2 of them, which share weights
+// y[v][row] for 128 rows x 32 VT vectors a workgroup, and one of gridDim.z (one or two)
+// slices of K: four waves of 4 row tiles x VT vector tiles, 2 x 2 of them, which share weights
 // and pieces of x through LDS. A step is a group of 32 columns: the pieces come by
 // LDS copies two steps ahead into a ring of three, the weights of a quad of groups
 // (with scales, and for Q4_K the sums of x) during the quad before, each wave issuing
@@ -987,23 +946,15 @@ __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w,
         });
         __shared__ int last;
         if (!arrive_last(arrivals + blockIdx.y * gridDim.x + blockIdx.x, gridDim.z, &last)) return;
-        const int n_slices = gridDim.z;
+        o = part + (1 - (int)blockIdx.z) * slice_stride;
         each([&](int64_t at, int left, floatx4 &t, int) {
-            floatx4 got[kMaxSlices];
+            if (quads) {
+                t += load_agent4(o + at);
+            } else {
 #pragma unroll
-            for (int s = 0; s < kMaxSlices; s++)
-                if (s < n_slices) {
-                    if (quads) {
-                        got[s] = load_agent4(part + s * slice_stride + at);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; r++) got[s][r] = r < left ? load_agent(part + s * slice_stride + at + r) : 0.0f;
-                    }
-                }
-            t = got[0];
-#pragma unroll
-            for (int s = 1; s < kMaxSlices; s++)
-                if (s < n_slices) t += got[s];
+                for (int r = 0; r < 4; r++)
+                    if (r < left) t[r] += load_agent(o + at + r);
+            }
         });
     }
     each([&](int64_t at, int left, const floatx4 &t, int vec) {
@@ -1072,67 +1023,72 @@ int make_pieces(gla_ctx *ctx, const gla_q4w *w, const float *x, int n, size_t pa
     const bool four = n > 64;
     auto kernel = k ? (four ? split_q4_kernel<true, 4> : split_q4_kernel<true, 1>)
                     : (four ? split_q4_kernel<false, 4> : split_q4_kernel<false, 1>);
-    hipLaunchKernelGGL(kernel, dim3(four ? (n + 3) / 4 : n), dim3(kSplitThreads), 0, ctx->stream, x, n, w->cols, w->n_quads,
+    hipLaunchKernelGGL(kernel, dim3(four ? (n + 3) / 4 : n, four ? 1 : 2), dim3(kSplitThreads), 0, ctx->stream, x, n, w->cols, w->n_quads,
                        (_Float16 *)px->xp, (_Float16 *)px->xm, (float *)px->undo);
     return launched("split_q4_kernel");
 }
 
-int mid(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
-    const bool k = w->format == GLA_Q4_K;
-    // Up to 32 vectors as few row tiles a workgroup as give every CU one. More vectors
-    // take four and slices of K, about a workgroup per CU in all: the pieces that a
-    // workgroup reads are its slice's. us, Q4_0 4096 x 4096, 64 vectors: one tile, no
-    // slices 19.4; four tiles, 1 / 2 / 4 / 8 slices 29.3 / 22.0 / 18.7 / 24.1.
-    const int rt = n > 32 || (n <= 16 && w->n_tiles > 2 * ctx->n_cu) ? 4 : w->n_tiles > ctx->n_cu ? 2 : 1;
-    const int groups = (w->n_tiles + rt - 1) / rt;
-    const int units = k ? w->n_quads / 2 : w->n_quads;
-    const int ranges = n > 64 ? 2 : n > 32 ? 4 : 8;  // of a slice's quads
-    const int slices = n <= 32 ? 1 : std::max(1, std::min({kMaxSlices, ctx->n_cu / groups, units / ranges}));
-    const int64_t stride = (int64_t)n * w->rows;
+struct Tile {
+    int nv, rt;  // of 16 vectors, of 16 rows
+};
+// The mid kernel's tiles, and its cost: rounds of a workgroup per CU, each the tile's
+// products and two for what comes before and after them. (A call of 4,096 columns
+// takes about 8 us + 1.33 a unit of cost, Q4_K 8 + 1.5.)
+constexpr int kMidCost = 34;
+constexpr Tile kMidTiles[] = {{1, 1}, {1, 2}, {1, 3}, {1, 4}, {2, 3}, {2, 4}, {4, 4}, {8, 4}};
+Tile mid_tile(const gla_ctx *ctx, const gla_q4w *w, int n, int64_t *cost) {
+    Tile best = kMidTiles[0];
+    *cost = INT64_MAX;
+    for (const Tile &t : kMidTiles) {
+        const int64_t wgs = (int64_t)((w->n_tiles + t.rt - 1) / t.rt) * (((n + 15) / 16 + t.nv - 1) / t.nv);
+        const int64_t c = (wgs + ctx->n_cu - 1) / ctx->n_cu * (t.nv * t.rt + 2);
+        if (c < *cost) best = t, *cost = c;
+    }
+    return best;
+}
+
+int mid(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y, Tile t) {
     Pieces px;
-    float *part = nullptr;
-    int32_t *arrivals = nullptr;
-    if (slices > 1)
-        if (int rc = ensure_arrivals(ctx, (size_t)groups, &arrivals)) return rc;
-    if (int rc = make_pieces(ctx, w, x, n, slices > 1 ? (size_t)slices * stride * sizeof(float) : 0, &px, &part)) return rc;
+    if (int rc = make_pieces(ctx, w, x, n, 0, &px, nullptr)) return rc;
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(groups, slices), dim3(kMidWaves * 64), 0, ctx->stream, p, px, n, y, part, stride, arrivals);
+        hipLaunchKernelGGL(kernel, dim3((w->n_tiles + t.rt - 1) / t.rt, ((n + 15) / 16 + t.nv - 1) / t.nv), dim3(kMidWaves * 64),
+                           0, ctx->stream, p, px, n, y);
         return launched("matvec_q4_mid_kernel");
     };
     const auto of = [&](auto kk) {
         constexpr bool K = decltype(kk)::value;
-        if (n > 64) return go(matvec_q4_mid_kernel<K, 2, 4, 4>);
-        if (n > 32) return go(matvec_q4_mid_kernel<K, 2, 4, 2>);
-        if (n > 16) return rt == 1 ? go(matvec_q4_mid_kernel<K, 2, 1, 1>) : go(matvec_q4_mid_kernel<K, 2, 2, 1>);
-        return rt == 1   ? go(matvec_q4_mid_kernel<K, 1, 1, 1>)
-               : rt == 2 ? go(matvec_q4_mid_kernel<K, 1, 2, 1>)
-                         : go(matvec_q4_mid_kernel<K, 1, 4, 1>);
+        switch (t.nv * 8 + t.rt) {
+        case 1 * 8 + 1: return go(matvec_q4_mid_kernel<K, 1, 1, 1>);
+        case 1 * 8 + 2: return go(matvec_q4_mid_kernel<K, 1, 2, 1>);
+        case 1 * 8 + 3: return go(matvec_q4_mid_kernel<K, 1, 3, 1>);
+        case 1 * 8 + 4: return go(matvec_q4_mid_kernel<K, 1, 4, 1>);
+        case 2 * 8 + 3: return go(matvec_q4_mid_kernel<K, 2, 3, 1>);
+        case 2 * 8 + 4: return go(matvec_q4_mid_kernel<K, 2, 4, 1>);
+        case 4 * 8 + 4: return go(matvec_q4_mid_kernel<K, 2, 4, 2>);
+        default: return go(matvec_q4_mid_kernel<K, 2, 4, 4>);
+        }
     };
-    return k ? of(std::true_type()) : of(std::false_type());
+    return w->format == GLA_Q4_K ? of(std::true_type()) : of(std::false_type());
 }
 
 int many(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
     const bool k = w->format == GLA_Q4_K;
-    // Workgroups of 128 vectors where they fill two on every CU, else of 64. Fewer than
-    // 768 of these take slices of K (each of eight quads or more) as long as their
-    // partial sums stay within 28 MB. us, 64 wide with 1 / 2 / 4 slices: Q4_0 6144 x
-    // 4096, 200 vectors 62.9 / 54.5 / 50.6, 400 79.5 / 71.2 / 71.3; 1024 x 4096, 400
-    // 65.3 / 45.5 / 36.2; 576 x 576, 200 16.9 / 20.3. 64 wide / 128: 6144 x 4096,
-    // 1,024 vectors 118 / 126, 1,999 221 / 210; Q4_K 1,999 234 / 204.
+    // Workgroups of 128 vectors where they fill two on every CU, else of 64. us, 64 wide
+    // / 128: 6144 x 4096, 1,024 vectors 118 / 126, 1,999 221 / 210; Q4_K 1,999 234 / 204.
+    // Fewer than 384 of 64 are two slices of K (of eight quads or more), as long as
+    // their partial sums stay within 28 MB: 6144 x 4096, 400 vectors 79.5 -> 71.2.
     const int vec_tiles = (n + 15) / 16, row_blocks = (w->n_tiles + 7) / 8;
     const int vt = (int64_t)row_blocks * ((vec_tiles + 7) / 8) >= 2 * ctx->n_cu ? 4 : 2;
     const int vec_blocks = (vec_tiles + 2 * vt - 1) / (2 * vt);
     const int64_t wgs = (int64_t)row_blocks * vec_blocks, stride = (int64_t)n * w->rows;
-    int slices = 1;
-    while (vt == 2 && 2 * slices <= kMaxSlices && 2 * slices * wgs <= 3 * ctx->n_cu && 2 * slices * 8 <= w->n_quads &&
-           (size_t)(2 * slices) * stride * sizeof(float) <= ((size_t)28 << 20))
-        slices *= 2;
+    const size_t partials = (size_t)(2 * stride) * sizeof(float);
+    const int slices = vt == 2 && 2 * wgs <= 3 * ctx->n_cu && w->n_quads >= 16 && partials <= ((size_t)28 << 20) ? 2 : 1;
     Pieces px;
     float *part = nullptr;
     int32_t *arrivals = nullptr;
     if (slices > 1)
         if (int rc = ensure_arrivals(ctx, (size_t)wgs, &arrivals)) return rc;
-    if (int rc = make_pieces(ctx, w, x, n, slices > 1 ? (size_t)slices * stride * sizeof(float) : 0, &px, &part)) return rc;
+    if (int rc = make_pieces(ctx, w, x, n, slices > 1 ? partials : 0, &px, &part)) return rc;
     const auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(row_blocks, vec_blocks, slices), dim3(256), 0, ctx->stream, p, px, n, y, part, stride,
                            arrivals);
@@ -1226,10 +1182,13 @@ int gla_matvec_q4(gla_ctx *ctx, const gla_q4w *w, const float *x, int n_vec, flo
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
     const Weights p{w->quants, w->aux, w->super, w->rows, w->cols, w->n_tiles, w->n_quads};
     if (n_vec <= kFewVec) return few(ctx, w, p, x, n_vec, y);
-    // The mid kernel up to 128 vectors, but for tall matrices, whose rows fill the chip
-    // by themselves (us, mid / gemm: 6144 x 4096, 100 vectors 34.3 / 42.6; 1024 x 4096
-    // 24.8 / 34.9; 16384 x 4096 63.7 / 57.9).
-    if (n_vec <= 64 || (n_vec <= 128 && w->n_tiles <= 2 * ctx->n_cu)) return mid(ctx, w, p, x, n_vec, y);
+    // The mid kernel's small tiles while their products are few, then the other's large
+    // ones (us, mid / many: Q4_0 4096 x 4096, 128 vectors 22.4 / 37.3, 512 53.1 / 58.2;
+    // 1024 x 4096, 1,500 54.2 / 61.9; Q4_K 6144 x 4096, 192 49.3 / 58.0, 320 64.5 / 57.1;
+    // 14336 x 4096, 64 35.1 / 45.6, 160 91.7 / 78.2).
+    int64_t cost;
+    const Tile t = mid_tile(ctx, w, n_vec, &cost);
+    if (cost <= kMidCost) return mid(ctx, w, p, x, n_vec, y, t);
     return many(ctx, w, p, x, n_vec, y);
     GLA_GUARD_END
 }

@@ -289,3 +289,27 @@ def test_too_many_rows_are_refused(backend):
     plan, buf = be.create_rope_plan(4), be.buffer(np.zeros(64, np.float32))
     with pytest.raises(GlaError, match="too many"):
         be.rope_rows(plan, buf, 33554429, 1, buf)
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("rows, cols, n", [(1027, 2048, 2500), (1028, 2048, 2500), (1027, 512, 8100), (48, 1024, 2000), (1027, 256, 4000)])
+def test_products_of_many_vectors_and_odd_rows(backend, fmt, rows, cols, n):
+    """Large tiles with K in two slices (rows that a vector store fits and not), in one, and 128 vectors wide; y 4 bytes off."""
+    rng = np.random.default_rng(rows + n)
+    raw = q4.ggml(rng, fmt, rows, cols)
+    w = backend.create_q4_weights(raw, rows, cols, fmt)
+    x = rng.standard_normal((n, cols)).astype(np.float32)
+    parts = q4.parts(raw, fmt)
+    for shift in (0, 1):
+        q4.check(q4.run(backend, w, x, shift=shift), x, *parts)
+
+
+def test_products_of_every_tile(backend):
+    """Rows and vectors that take each of the middle kernel's tiles, cut short on both sides."""
+    rng = np.random.default_rng(16)
+    for fmt, cols in (("q4_0", 96), ("q4_k", 512)):
+        for rows, n in ((1000, 33), (6001, 17), (6100, 30), (8100, 32), (6100, 63), (8100, 60), (14000, 61), (14300, 120)):
+            raw = q4.ggml(rng, fmt, rows, cols)
+            w = backend.create_q4_weights(raw, rows, cols, fmt)
+            x = rng.standard_normal((n, cols)).astype(np.float32)
+            q4.check(q4.run(backend, w, x, shift=rows // 100 % 2), x, *q4.parts(raw, fmt))
