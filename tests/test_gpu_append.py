@@ -297,3 +297,25 @@ def test_refusals(backend):
                  (ints.ptr, buf.ptr, buf.ptr, -1), (ints.ptr, C.c_void_p(buf.ptr.value + 4), buf.ptr, 1)):
         assert lib.gla_kv_read_rows(be.ctx, cache.handle, *args) == _lib.GLA_ERR_INVALID
     be.sync()
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_quants_of_every_magnitude(backend, n):
+    """Blocks whose quotients fall on halves, blocks from the smallest subnormals to the largest floats, with zeros, infinities
+    and NaN: the storage's bytes are the oracle's, row by row and page by page."""
+    be = backend
+    rng = np.random.default_rng(n)
+    k = rng.integers(-254, 255, (n, 8, 32)).astype(np.float64) / 2 * 2.0 ** rng.integers(-149, 120, (n, 8, 1))
+    k[..., 0] = np.where(rng.random((n, 8)) < 0.8, 127.0, 1.0) * np.abs(k).max(-1) / 127.0
+    k[rng.random(k.shape) < 0.03] = 0.0
+    odd = rng.random(k.shape) < 0.002
+    k[odd] = rng.choice([np.inf, -np.inf, np.nan], odd.sum())
+    k[0, 0] = 0.0
+    k[1, 1] = 2.0 ** -149
+    k = np.clip(k, -3.4e38, 3.4e38, where=np.isfinite(k), out=k).astype(np.float32).reshape(n, 256)
+    v = k[:, ::-1].copy()
+    cache = be.create_kv_cache(1, 48, 2, 128, "q8", 1)
+    be.append(cache, be.buffer(k), be.buffer(v), be.buffer(np.array([0, n], np.int32)), be.buffer(np.array([5], np.int32)), 1, n)
+    be.sync()
+    for got, x in zip(cache.export_rows(np.arange(5, 5 + n)), (k, v)):
+        assert np.array_equal(np.asarray(got, np.uint8).reshape(n, -1), q8_values(x)[0])
