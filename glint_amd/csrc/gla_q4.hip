@@ -975,6 +975,9 @@ __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w,
 
 constexpr int kMaxVec = 262128;
 constexpr int kMaxCols = 1 << 26;  // a row of x is addressed by 32 bits of bytes
+// A launch has fewer than 2^32 threads: 512 a row tile, and 64 a piece to repack.
+constexpr int kMaxRows = 1 << 26;
+constexpr int64_t kMaxPieces = (1 << 26) - 4;
 
 int launched(const char *what) {
     const hipError_t e = hipGetLastError();
@@ -1118,6 +1121,8 @@ int gla_q4w_create(gla_ctx *ctx, gla_q4_format format, const uint8_t *ggml_host,
     GLA_REQUIRE(rows > 0 && cols > 0 && cols % (k ? 256 : 32) == 0,
                 "gla_q4w_create: rows %d, cols %d (cols must be a positive multiple of %d)", rows, cols, k ? 256 : 32);
     GLA_REQUIRE(cols <= kMaxCols, "gla_q4w_create: %d columns (at most %d)", cols, kMaxCols);
+    GLA_REQUIRE(rows <= kMaxRows && ((int64_t)rows + 15) / 16 * ((cols + 127) / 128) <= kMaxPieces,
+                "gla_q4w_create: %d x %d is too large for one launch", rows, cols);
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
     ctx->q4ws.reserve(ctx->q4ws.size() + 1);
     gla_q4w *w = new gla_q4w();

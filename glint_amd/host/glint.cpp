@@ -1132,7 +1132,8 @@ Result<std::vector<float>> GpuBackend::append_batch(const std::vector<AppendSeq>
     int max_q = 0, stride = 1;
     for (size_t b = 0; b < B; b++) {
         const size_t end = seqs[b].pos_offset + seqs[b].n_rows;
-        if (end > INT32_MAX || (size_t)q_start[b] + seqs[b].n_rows > INT32_MAX)
+        if (std::max(seqs[b].pos_offset, seqs[b].n_rows) > INT32_MAX || end > INT32_MAX ||
+            (size_t)q_start[b] + seqs[b].n_rows > INT32_MAX)
             return GlintError::gpu_shader_error("append_batch: positions out of range");
         if (S.paged) {
             if (layer >= seqs[b].kv->as_paged()->n_layers())

@@ -91,6 +91,8 @@ int gla_destroy(gla_ctx *ctx);
  * its own device scratch (decode split partials, prefill tile images,
  * matvec activation pieces), so calls queued on different streams at once
  * never share it and may overlap; calls on one stream run in order as usual.
+ * A graph uses the scratch of the stream it was captured on: graphs of one
+ * stream are replayed one after another, wherever they are launched.
  * That scratch is held until gla_destroy or gla_release_stream. The stream
  * must outlive its use by the context: switch away from it (or release it)
  * before destroying it. The context itself is not thread-safe: switch
@@ -464,7 +466,8 @@ int gla_matvec_q8_0(gla_ctx *ctx, const gla_q8w *w, const float *x, int n_vec, f
  *   Q4_K  rows x (cols / 256) blocks of 144 bytes, [f16 d][f16 dmin][12 bytes:
  *         eight 6-bit scales and eight 6-bit minima][128 bytes of nibbles],
  *         value (d * scale) * nibble - dmin * minimum in groups of 32
- * cols a multiple of 32 (Q4_0) or 256 (Q4_K), at most 2^26. Returns when the weights are on
+ * cols a multiple of 32 (Q4_0) or 256 (Q4_K); rows and cols at most 2^26, and
+ * rows * cols about 2^37 (GLA_ERR_INVALID above). Returns when the weights are on
  * the device; handles behave as gla_q8w's do. */
 typedef enum gla_q4_format { GLA_Q4_0 = 0, GLA_Q4_K = 1 } gla_q4_format;
 typedef struct gla_q4w gla_q4w;

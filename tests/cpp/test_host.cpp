@@ -1123,6 +1123,8 @@ DEVICE_TEST(test_append_batch) {
     caches[1].read_k_head(0, 6, 1, HEAD_DIM, head.data());
     CHECK(head == std::vector<float>(k.begin() + (ptrdiff_t)(KV_DIM + HEAD_DIM), k.begin() + (ptrdiff_t)(KV_DIM + 2 * HEAD_DIM)));
     CHECK(!backend().append_batch({{&caches[0], 2, 15}}, q.data(), k.data(), v.data(), 0, shape, nullptr).ok());
+    CHECK(!backend().append_batch({{&caches[0], 2, SIZE_MAX}}, q.data(), k.data(), v.data(), 0, shape, nullptr).ok());
+    CHECK(!backend().append_batch({{&caches[0], SIZE_MAX, 2}}, q.data(), k.data(), v.data(), 0, shape, nullptr).ok());
     CHECK(!backend().append_batch({{&caches[0], 1, 0}, {&caches[0], 1, 1}}, q.data(), k.data(), v.data(), 0, shape, nullptr).ok());
     CHECK(!backend().append_batch({{&caches[0], 1, 0}, {&first, 1, 0}}, q.data(), k.data(), v.data(), 0, shape, nullptr).ok());
 }

@@ -1,11 +1,14 @@
 """The operators as a layer uses them: a fused 4-bit Q/K/V projection, the append that rotates and stores, attention and the
 4-bit output projection, on a paged or contiguous cache; every stage against 64 bits from the stage's own input on the device.
 Then the same steps captured into a graph, and on two streams."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import rope_ref
 import test_gpu_matvec_q4 as q4
+from glint_amd import _lib
 from glint_amd._lib import GlaError
 from glint_amd.attn import HipStream
 from helpers import assert_close, attention_f64
@@ -286,6 +289,10 @@ def test_v_by_row_and_by_page_alike(backend, lo):
 
 def test_too_many_rows_are_refused(backend):
     be = backend
+    few, out = np.zeros(18, np.uint8), C.c_void_p()
+    for fmt, rows, cols in ((0, (1 << 26) + 1, 32), (0, 1 << 24, 1 << 14), (1, 1 << 14, 1 << 24), (0, 1, (1 << 26) + 32)):
+        assert _lib.lib().gla_q4w_create(be.ctx, fmt, few.ctypes.data, rows, cols, C.byref(out)) == _lib.GLA_ERR_INVALID
+        assert not out.value
     plan, buf = be.create_rope_plan(4), be.buffer(np.zeros(64, np.float32))
     with pytest.raises(GlaError, match="too many"):
         be.rope_rows(plan, buf, 33554429, 1, buf)
