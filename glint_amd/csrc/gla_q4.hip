@@ -249,10 +249,12 @@ __device__ __forceinline__ void load_row(float (&e)[8], const float *row, int by
 //   MFMA; the rows' d multiplies once a quad. The minima are a product of their
 //   own: four minima of a row with the sums of x over the four groups (in pieces,
 //   scaled by 2^-5; the minima carry 2^5).
+// Columns past the vectors multiply what the first ones do, and their sums are not used:
+// zeros there cost 16 instructions a quad.
 // Bound: one chain of launch (2.7 us), loads from HBM, unpacking and the merge; the
-// vector unit is busy 38% of it (99 instructions for 16 rows x 128 columns of Q4_0, 132
-// of Q4_K). us: Q4_0 4096 x 4096, 1 / 2 / 4 / 8 vectors 4.4 / 4.8 / 5.7 / 7.2; 14336 x
-// 4096, 1 vector 11.8 (33 MB, 2.8 TB/s).
+// vector unit is busy a third of it (85 instructions for 16 rows x 128 columns of Q4_0,
+// 115 of Q4_K). us: Q4_0 4096 x 4096, 1 / 2 / 4 / 8 vectors 4.3 / 4.6 / 5.5 / 7.2; 14336
+// x 4096, 1 vector 10.9 (33 MB, 3.0 TB/s).
 constexpr int kFewWaves = 8;
 template <bool K, int NV, int RT, int CH>
 __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Weights w, const float *x, int n_vec, float *y) {
@@ -382,13 +384,9 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
             if (c0 + i >= q1) break;
             half8 bx[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                bx[j] = half8{};
-                if (col < COLS) bx[j] = px[col * PITCH + (i * 4 + j) * 4 + kg];
-            }
+            for (int j = 0; j < 4; j++) bx[j] = px[col % COLS * PITCH + (i * 4 + j) * 4 + kg];
             if constexpr (K) {
-                half4 bs = {};
-                if (col < COLS && kg == 0) bs = ps[i * COLS + col];
+                const half4 bs = ps[i * COLS + col % COLS];
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
                     floatx4 c = zero;
@@ -407,16 +405,19 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
                 }
             } else {
 #pragma unroll
-                for (int t = 0; t < RT; t++)
+                for (int t = 0; t < RT; t++) {
+                    floatx4 c[4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const floatx4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nibbles_q4_0(qw[t][i][j]), bx[j], zero, 0, 0, 0);
+                    for (int j = 0; j < 4; j++)
+                        c[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(nibbles_q4_0(qw[t][i][j]), bx[j], zero, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const uint32_t s = sc[t][i][r >> 1][(r & 1) * 2 + (j >> 1)];
-                            acc[t][r] = fmaf(c[r], (j & 1) ? hi_of(s) : lo_of(s), acc[t][r]);
+                            acc[t][r] = fmaf(c[j][r], (j & 1) ? hi_of(s) : lo_of(s), acc[t][r]);
                         }
-                    }
+                }
             }
         }
 #pragma unroll
