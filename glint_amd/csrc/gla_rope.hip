@@ -91,10 +91,19 @@ __host__ __device__ constexpr size_t wave_lds(int mode, int pairs) {
     return mode == kCopy ? 0 : (size_t)pairs * sizeof(double2) + (mode == kHalf ? kMaxHeadDim * sizeof(float) : 0);
 }
 
+// cos and sin of pairs p0, p0 + step, ... at position pos: a lane evaluates one each
+// and reads those that it needs from LDS (evaluations of a lane's own eight elements
+// cost a call of one row 1.1 us of its 4.4).
+__device__ __forceinline__ void turn_table(const Rope &r, double pos, double2 *table, int p0, int step) {
+    for (int p = p0; p < r.pairs; p += step) {
+        double2 t;
+        cos_sin(pos * r.turns[p], r.amplitude, t.x, t.y);
+        table[p] = t;
+    }
+}
+
 // The factors of a lane's elements e0 .. e0 + 3 of a head; elements from
-// 2 * pairs on are left alone. The wave's lanes evaluate one pair each and read
-// the factors they need from LDS: evaluations of a lane's own eight elements cost
-// a call of one row 1.1 us of its 4.4.
+// 2 * pairs on are left alone.
 template <int MODE, bool V>
 struct Turn {
     static constexpr int N = MODE == kAdjacent ? 2 : 4;
@@ -102,22 +111,15 @@ struct Turn {
     const int pairs, e0, head_dim;
     float *stage;  // kHalf: the head's place in LDS, filled by the wave's lanes of this head
 
-    __device__ __forceinline__ Turn(const Rope &r, int lane, int e0, int h, int head_dim, double pos, double2 *lds)
+    __device__ __forceinline__ Turn(const Rope &r, int e0, int h, int head_dim, const double2 *table, float *wave_stage)
         : pairs(r.pairs), e0(e0), head_dim(head_dim) {
         if constexpr (MODE != kCopy) {
-            stage = reinterpret_cast<float *>(lds + r.pairs) + h * head_dim;
-            for (int p = lane; p < r.pairs; p += 64) {
-                double2 t;
-                cos_sin(pos * r.turns[p], r.amplitude, t.x, t.y);
-                lds[p] = t;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            stage = wave_stage + h * head_dim;
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 const int e = MODE == kAdjacent ? e0 / 2 + j : e0 + j;
                 const bool second = MODE == kHalf && e >= r.pairs;
-                const double2 t = lds[min(second ? e - r.pairs : e, r.pairs - 1)];
+                const double2 t = table[min(second ? e - r.pairs : e, r.pairs - 1)];
                 c[j] = t.x;
                 s[j] = MODE == kHalf && !second ? -t.y : t.y;
             }
@@ -234,7 +236,11 @@ __global__ __launch_bounds__(kWaves * 64) void rope_rows_kernel(const Rope r, co
 #pragma unroll
     for (int i = 0; i < kAhead; i++)
         if (g0 + i < g1) load(ring[i], g0 + i);
-    const Turn<MODE, V> t(r, lane, e0, h, head_dim, (double)pos[row], lds + wave * (wave_lds(MODE, r.pairs) / sizeof(double2)));
+    double2 *table = lds + wave * (wave_lds(MODE, r.pairs) / sizeof(double2));
+    turn_table(r, (double)pos[row], table, lane, 64);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const Turn<MODE, V> t(r, e0, h, head_dim, table, reinterpret_cast<float *>(table + r.pairs));
     stream_groups(ring, g0, g1, load, [&](float (&e)[4], int g) {
         t.apply(e);
         const int head = g * per + h;
@@ -250,7 +256,7 @@ struct Append {
     Rope rope;
     const int32_t *q_start, *pos_offset;
     int n_seqs, max_q_len, parts;
-    int row_blocks;   // blocks of a sequence that take rows; the others take pages of V
+    int row_blocks;  // blocks of a sequence that take rows; the others take pages of V
     int v_by_page;
     const float *k, *v, *q;
     float *q_out;
@@ -349,7 +355,7 @@ __device__ __forceinline__ void append_v_page(const Append &a, int b, int idx, i
 // of q, of K and (unless V goes page by page) of V in turn, head_dim / 4 lanes a
 // head. Bound: memory for f32 prompts (6,144 rows of 48 x 128, 314 MB, 59.8 us, 5.2
 // TB/s); the instructions that rotate in 64 bits and quantise, and K's stores of 8
-// bytes a piece, for Q8_0 ones (264 MB, 60.1 us); launch and one chain of position,
+// bytes a piece, for Q8_0 ones (264 MB, 56.6 us); launch and one chain of position,
 // sine, quantise and store for single tokens (64 rows 5.0 us, a launch being 2.7).
 template <int MODE, bool V>
 __global__ __launch_bounds__(kWaves * 64) void kv_append_kernel(const Append a) {
@@ -361,7 +367,15 @@ __global__ __launch_bounds__(kWaves * 64) void kv_append_kernel(const Append a) 
         append_v_page(a, b, (blockIdx.x - a.row_blocks) * kWaves + wave, lane);
         return;
     }
-    const uint32_t item = blockIdx.x * kWaves + wave;
+    // Workgroups go round the eight XCDs; of a Q8_0 storage 16 rows at a time go to one,
+    // whose L2 then puts the 8-byte pieces of their K together (6,570 ragged rows 63.4 ->
+    // 61.4 us).
+    uint32_t block = blockIdx.x;
+    if (a.o.q8) {
+        const uint32_t page = GLA_PAGE_SIZE / kWaves * a.parts, at = block / (8 * page) * (8 * page), o = block - at;
+        if (at + 8 * page <= (uint32_t)a.row_blocks) block = at + o % 8 * page + o / 8;
+    }
+    const uint32_t item = block * kWaves + wave;
     const int i = (int)(item / (uint32_t)a.parts);
     const int part = (int)(item - (uint32_t)i * a.parts);
     const int first = a.q_start[b], last = a.q_start[b + 1];
@@ -415,10 +429,22 @@ __global__ __launch_bounds__(kWaves * 64) void kv_append_kernel(const Append a) 
                                                        elem_off(a.o, row, gi, 4)), e, 4);
         });
     };
+    double2 *own = lds + wave * (wave_lds(MODE, a.rope.pairs) / sizeof(double2)), *table = own;
+    if constexpr (MODE != kCopy) {
+        if (a.parts % kWaves == 0) {  // the workgroup's waves have one row
+            table = lds;
+            turn_table(a.rope, (double)pos, table, threadIdx.x, kWaves * 64);
+            __syncthreads();
+        } else if (g0 < gq + gk) {
+            turn_table(a.rope, (double)pos, table, lane, 64);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
     if (MODE == kCopy || g0 >= gq + gk)
-        rest(Turn<kCopy, V>(a.rope, lane, e0, h, head_dim, 0.0, nullptr));
+        rest(Turn<kCopy, V>(a.rope, e0, h, head_dim, nullptr, nullptr));
     else
-        rest(Turn<MODE, V>(a.rope, lane, e0, h, head_dim, (double)pos, lds + wave * (wave_lds(MODE, a.rope.pairs) / sizeof(double2))));
+        rest(Turn<MODE, V>(a.rope, e0, h, head_dim, table, reinterpret_cast<float *>(own + a.rope.pairs)));
 }
 
 bool aligned16(const void *p, int64_t stride) { return ((uintptr_t)p & 15) == 0 && stride % 4 == 0; }

@@ -319,3 +319,36 @@ def test_quants_of_every_magnitude(backend, n):
     be.sync()
     for got, x in zip(cache.export_rows(np.arange(5, 5 + n)), (k, v)):
         assert np.array_equal(np.asarray(got, np.uint8).reshape(n, -1), q8_values(x)[0])
+
+
+@pytest.mark.parametrize("n_heads, n_kv, d", [(4, 2, 64), (16, 8, 128), (2, 1, 256)])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_long_prompts_into_a_quantised_pool(backend, n_heads, n_kv, d, layout):
+    """Prompts of several hundred rows beside short ones: the pool holds what write_rows stores of the rotated rows, every
+    query is rotated, and rows outside the prompts stay as they were."""
+    be = backend
+    rng = np.random.default_rng(d)
+    lens, past = [300, 5, 0, 131, 517], [3, 16, 9, 21, 0]
+    q, k, v, row = batch(rng, n_heads, n_kv, d, lens, True)
+    pages = sum(-(-(n + p) // PAGE) for n, p in zip(lens, past))
+    order, table, at = rng.permutation(pages).astype(np.int32), np.full((5, 40), -1, np.int32), 0
+    for b, (n, p) in enumerate(zip(lens, past)):
+        m = -(-(n + p) // PAGE)
+        table[b, :m] = order[at:at + m]
+        at += m
+    spec = dict(layout=layout, freq_base=500000.0)
+    pools = [be.create_page_pool(pages, n_kv, d, "q8") for _ in range(2)]
+    plan = be.create_rope_plan(d, **spec)
+    got = append(be, pools[0], q, k, v, row, lens, past, plan, tail=2, page_table=be.buffer(table), page_table_stride=40)
+    pos = np.concatenate([np.arange(p, p + n) for n, p in zip(lens, past)])
+    check_f32(got[:len(pos)], q, pos, spec)
+    assert np.all(got[len(pos):] == -9.0)
+    # K as the library rotates it alone (one rounding, so the same f32), written row by row
+    turned = be.buffer(k)
+    be.rope_rows(plan, turned, len(pos), n_kv, be.buffer(pos.astype(np.int32)))
+    be.sync()
+    check_f32(turned.download(k.shape), k, pos, spec)
+    pools[1].write_rows(rows_of(lens, past, table=table), turned.download((len(pos), n_kv * d)), v.reshape(len(pos), -1))
+    every = np.arange(pages * PAGE)
+    for a, b in zip(pools[0].export_rows(every), pools[1].export_rows(every)):
+        assert np.array_equal(a, b)
