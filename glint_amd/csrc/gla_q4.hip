@@ -128,12 +128,6 @@ __device__ __forceinline__ half2v both(float x) { return half2v{(_Float16)x, (_F
 __device__ __forceinline__ float lo_of(uint32_t w) { return (float)h2(w)[0]; }
 __device__ __forceinline__ float hi_of(uint32_t w) { return (float)h2(w)[1]; }
 
-// The 8 nibbles of a dword as halves n * s + b, where lo = {s, b - 1024 s} and
-// hi = {s / 16, b - 64 s}: a nibble under the bits of 1024 is 1024 + n, four bits
-// further up 1024 + 16 n. Every result here is exact.
-struct Scale2 {
-    half2v s, b;
-};
 // (u & mask) | 0x64006400 in one instruction, which needs the constant in a register
 __device__ __forceinline__ half2v under_1024(uint32_t u, uint32_t mask) {
     uint32_t o, k = 0x64006400u;
@@ -141,23 +135,21 @@ __device__ __forceinline__ half2v under_1024(uint32_t u, uint32_t mask) {
     asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(o) : "v"(u), "s"(mask), "v"(k));
     return h2(o);
 }
-__device__ __forceinline__ half8 nibbles(uint32_t w, const Scale2 &lo, const Scale2 &hi) {
+// Q4_0: n - 8 of the 8 nibbles of a dword. A nibble under the bits of 1024 is 1024 + n,
+// four bits further up 1024 + 16 n; every result is exact.
+__device__ __forceinline__ half8 nibbles_q4_0(uint32_t w) {
     half8 o;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const uint32_t u = w >> (8 * i);
-        const half2v a = __builtin_elementwise_fma(under_1024(u, 0x000f000fu), lo.s, lo.b);
-        const half2v b = __builtin_elementwise_fma(under_1024(u, 0x00f000f0u), hi.s, hi.b);
+        const half2v a = under_1024(u, 0x000f000fu) - both(1032.0f);
+        const half2v b = __builtin_elementwise_fma(under_1024(u, 0x00f000f0u), both(0.0625f), both(-72.0f));
         o[4 * i] = a[0];
         o[4 * i + 1] = a[1];
         o[4 * i + 2] = b[0];
         o[4 * i + 3] = b[1];
     }
     return o;
-}
-// Q4_0: n - 8
-__device__ __forceinline__ half8 nibbles_q4_0(uint32_t w) {
-    return nibbles(w, {both(1.0f), both(-1032.0f)}, {both(0.0625f), both(-72.0f)});
 }
 // An integer up to 2047 as the bits of a half is that many times 2^-24 (subnormals and
 // the binade above them), and the MFMA takes it so: Q4_K's A operands are integers, its
@@ -258,9 +250,9 @@ __device__ __forceinline__ void load_row(float (&e)[8], const float *row, int by
 // Columns past the vectors multiply what the first ones do, and their sums are not used:
 // zeros there cost 16 instructions a quad.
 // Bound: one chain of launch (2.7 us), loads from HBM, unpacking and the merge; the
-// vector unit is busy a third of it (85 instructions for 16 rows x 128 columns of Q4_0,
-// 115 of Q4_K). us: Q4_0 4096 x 4096, 1 / 2 / 4 / 8 vectors 4.3 / 4.6 / 5.5 / 7.2; 14336
-// x 4096, 1 vector 10.9 (33 MB, 3.0 TB/s).
+// vector unit is busy a third of it (about 85 instructions for 16 rows x 128 columns of
+// Q4_0, 100 of Q4_K). us: Q4_0 4096 x 4096, 1 / 2 / 4 / 8 vectors 4.3 / 4.5 / 5.5 / 7.2;
+// 14336 x 4096, 1 vector 10.8, Q4_K 10.2 (33 MB, 3.2 TB/s).
 constexpr int kFewWaves = 8;
 template <bool K, int NV, int RT, int CH>
 __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Weights w, const float *x, int n_vec, float *y) {
@@ -1088,7 +1080,7 @@ int mid(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n,
 int many(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
     const bool k = w->format == GLA_Q4_K;
     // Workgroups of 128 vectors where they fill two on every CU, else of 64. us, 64 wide
-    // / 128: 6144 x 4096, 1,024 vectors 118 / 126, 1,999 221 / 210; Q4_K 1,999 234 / 204.
+    // / 128: 6144 x 4096, 1,024 vectors 117 / 118, 1,999 216 / 210; Q4_K 1,999 222 / 193.
     // Fewer than 384 of 64 are two slices of K (of eight quads or more), as long as
     // their partial sums stay within 28 MB: 6144 x 4096, 400 vectors 79.5 -> 71.2.
     const int vec_tiles = (n + 15) / 16, row_blocks = (w->n_tiles + 7) / 8;
@@ -1199,9 +1191,9 @@ int gla_matvec_q4(gla_ctx *ctx, const gla_q4w *w, const float *x, int n_vec, flo
     const Weights p{w->quants, w->aux, w->super, w->rows, w->cols, w->n_tiles, w->n_quads};
     if (n_vec <= kFewVec) return few(ctx, w, p, x, n_vec, y);
     // The mid kernel's small tiles while their products are few, then the other's large
-    // ones (us, mid / many: Q4_0 4096 x 4096, 128 vectors 22.4 / 37.3, 512 53.1 / 58.2;
-    // 1024 x 4096, 1,500 54.2 / 61.9; Q4_K 6144 x 4096, 192 49.3 / 58.0, 320 64.5 / 57.1;
-    // 14336 x 4096, 64 35.1 / 45.6, 160 91.7 / 78.2).
+    // ones (us, mid / many: Q4_0 4096 x 4096, 128 vectors 23.0 / 41.3, 512 53.8 / 57.1;
+    // 1024 x 4096, 1,500 54.4 / 56.7; Q4_K 6144 x 4096, 192 48.7 / 50.6, 320 62.0 / 55.1;
+    // 14336 x 4096, 64 34.6 / 38.8, 160 91.1 / 74.9).
     int64_t cost;
     const Tile t = mid_tile(ctx, w, n_vec, &cost);
     if (cost <= kMidCost) return mid(ctx, w, p, x, n_vec, y, t);
