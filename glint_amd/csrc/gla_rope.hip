@@ -460,10 +460,11 @@ Rope rope_of(const gla_rope_plan *p) { return Rope{p->turns, p->pairs, p->amplit
 
 // Parts of a row's `groups` that waves take: about `waves` of them in all, at
 // most one group each. Short waves keep the last round of a long call short;
-// waves of rows that ragged sequences do not have cost an append a little. us
-// for 4,096 / 16,384 / 32,768 / 65,536 / 131,072: 7,993 query rows 55.3 / 51.6 /
-// 50.3 / 49.5 / 48.9, ragged prompts into a Q8_0 pool (append and read) 96 / 90 /
-// 92 / 96 / 107, into f32 caches 68.7 / 60.9 / 58.8 / 64.2 / 70.5.
+// waves of rows that ragged sequences do not have cost an append a little. us:
+// 7,993 query rows, 4,096 / 16,384 / 32,768 / 65,536 / 131,072 waves 55.3 / 51.6 /
+// 50.3 / 49.5 / 48.9; appends, 6,000 / 16,384 / 24,576: 6,570 ragged rows into a Q8_0
+// pool 65.5 / 61.5 / 61.4, 6,144 of one length 60.4 / 56.4 / 56.9, 7,968 ragged f32
+// ones 82.9 / 79.9 / 79.6.
 constexpr int kRopeWaves = 65536, kAppendWaves = 24576;
 int parts_of(int64_t rows, int groups, int waves) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(groups, (waves + rows - 1) / rows));
