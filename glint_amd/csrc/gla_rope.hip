@@ -39,7 +39,7 @@ void detach_rope(gla_rope_plan *r) {
 namespace {
 
 constexpr int kMaxHeadDim = 256;
-constexpr int kWaves = 4;   // waves of a workgroup, each on its own
+constexpr int kWaves = 4;   // waves of a workgroup, each on its own but for the sines of a shared row
 constexpr int kAhead = 4;   // groups whose loads a wave has in flight
 constexpr int kVByPage = 16;
 

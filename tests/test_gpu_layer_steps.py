@@ -320,3 +320,52 @@ def test_products_of_every_tile(backend):
             w = backend.create_q4_weights(raw, rows, cols, fmt)
             x = rng.standard_normal((n, cols)).astype(np.float32)
             q4.check(q4.run(backend, w, x, shift=rows // 100 % 2), x, *q4.parts(raw, fmt))
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k"])
+def test_slices_of_k_captured_and_on_two_streams(backend, fmt):
+    """A product whose workgroups are two slices of K (the last to arrive adds them): a graph replayed between eager calls, and
+    two streams at once; every result has the bits of a call by itself, and those are the product's."""
+    be = backend
+    rows, cols, n = 6144, 2048, 400
+    rng = np.random.default_rng(17)
+    raw = q4.ggml(rng, fmt, rows, cols)
+    w = be.create_q4_weights(raw, rows, cols, fmt)
+    xs = [rng.standard_normal((n, cols)).astype(np.float32) for _ in range(3)]
+    x = [be.buffer(a) for a in xs]
+    y = [be.empty(n * rows * 4) for _ in range(3)]
+    want = []
+    for i in range(3):
+        be.matvec_q4(w, x[i], n, y[i])
+        be.sync()
+        want.append(y[i].download((n, rows)))
+    q4.check(want[0], xs[0], *q4.parts(raw, fmt))
+    s = [HipStream(), HipStream()]
+    try:
+        be.set_stream(s[0])
+        inp, out = be.buffer(xs[0]), be.empty(n * rows * 4)
+        be.matvec_q4(w, inp, n, y[0])
+        be.sync()
+        g = be.capture(lambda: be.matvec_q4(w, inp, n, out))
+        for rep in range(4):
+            inp.upload(xs[rep % 3])
+            be.matvec_q4(w, x[2], n, y[2])
+            g.replay()
+            be.matvec_q4(w, x[1], n, y[1])
+            be.sync()
+            assert np.array_equal(out.download((n, rows)), want[rep % 3])
+            assert np.array_equal(y[1].download((n, rows)), want[1]) and np.array_equal(y[2].download((n, rows)), want[2])
+        g.destroy()
+        for rep in range(3):
+            for i in range(3):
+                be.set_stream(s[i % 2])
+                be.matvec_q4(w, x[i], n, y[i])
+            for t in s:
+                t.synchronize()
+            be.set_stream(None)
+            for i in range(3):
+                assert np.array_equal(y[i].download((n, rows)), want[i]), (rep, i)
+    finally:
+        be.set_stream(None)
+        for t in s:
+            t.destroy()
