@@ -175,7 +175,9 @@ __device__ __forceinline__ half4 minima(uint32_t mn) {
 
 // x enters the products as two halves, hi = f16(x 2^s) and lo = f16(x 2^s - hi),
 // s bringing the largest finite |x| of a range into [2^13, 2^14): 22 bits of every
-// value whose size matters. An infinity is its own hi piece (lo 0), a NaN both.
+// value whose size matters. A NaN is both its pieces. An infinity is its own hi piece (lo 0)
+// in Q4_0; in Q4_K, where a weight's nibble and minimum multiply x in sums of their own and
+// an infinity would end as inf - inf, it is 0 and infinite_terms adds its products.
 // The range's largest |x| is kept as bits, which order as the values do.
 constexpr uint32_t kInf = 0x7f800000u;
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -220,6 +222,11 @@ __device__ __forceinline__ void pieces(float x, float mul, bool odd, _Float16 &h
     lo = (_Float16)fmaf(x, mul, -(float)hi);
     if (odd && abs_bits(x) == kInf) lo = (_Float16)0.0f;
 }
+// Q4_K: x as it enters the pieces and the sums
+template <bool K>
+__device__ __forceinline__ float without_inf(float x, bool odd) {
+    return K && odd && abs_bits(x) == kInf ? 0.0f : x;
+}
 // 8 floats from byte `at` of a row's `bytes` (wave-uniform), zeros past them: the
 // bounds check of the buffer loads, which also take rows at any 4-byte address.
 __device__ __forceinline__ void load_row(float (&e)[8], const float *row, int bytes, int at) {
@@ -230,6 +237,31 @@ __device__ __forceinline__ void load_row(float (&e)[8], const float *row, int by
         e[j] = __uint_as_float(a[j]);
         e[4 + j] = __uint_as_float(b[j]);
     }
+}
+
+// Q4_K: the products of row `row` with the infinite elements of x, each with the whole
+// weight, as the definition has it: an infinity by the weight's sign, NaN for a weight of
+// 0 and for infinities of both signs. Only outputs of vectors that hold an infinity come
+// here. d * scale * nibble and dmin * minimum are exact in f32, so their difference is 0
+// where the weight is.
+__device__ float infinite_terms(const Weights &w, const float *x, int row) {
+    const int64_t tile = row >> 4, r = row & 15;
+    float sum = 0.0f;
+    for (int c0 = 0; c0 < w.cols; c0 += 8) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) any |= abs_bits(x[c0 + k]) == kInf ? 1u << k : 0u;
+        if (!any) continue;
+        const int64_t tq = tile * w.n_quads + (c0 >> 7);
+        const int j = (c0 >> 5) & 3;
+        const uint32_t q = reinterpret_cast<const uint32_t *>(w.quants)[(tq * 64 + ((c0 >> 3) & 3) * 16 + r) * 4 + j];
+        const uint8_t *a = w.aux + (tq * 16 + r) * 8;
+        const uint32_t d = w.super[(tile * (w.n_quads / 2) + (c0 >> 8)) * 16 + r];
+        const float scale = lo_of(d) * (float)a[j], low = hi_of(d) * (float)a[4 + j];
+        for (int k = 0; k < 8; k++)
+            if (any >> k & 1) sum += fmaf(scale, (float)((q >> (k / 2 * 4 + k % 2 * 16)) & 15u), -low) * x[c0 + k];
+    }
+    return sum;
 }
 
 // ---- up to 8 vectors ------------------------------------------------------------------
@@ -266,6 +298,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
     constexpr int WAVE = (PIECES * 16 + SUMS * 8 + NV * 4 + 15) / 16 * 16;
     constexpr int RED = kFewWaves * RT * 64 * 16;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kFewWaves * WAVE > RED ? kFewWaves * WAVE : RED];
+    __shared__ uint32_t inf_of[K ? kFewWaves : 1];  // Q4_K: bit v, the wave's columns of vector v may hold an infinity
+    uint32_t inf = 0;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, kg = lane >> 4;
@@ -332,6 +366,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
             uint32_t top = VP == 1 ? __builtin_amdgcn_readfirstlane(mx[i]) : mx[i];
             const bool odd = VP == 1 ? top >= kInf : __any(top >= kInf);
             if (odd) {  // scaled by what is finite
+                inf |= ((1u << VP) - 1) << (i * VP);
                 mx[i] = 0;
 #pragma unroll
                 for (int j = 0; j < 8; j++) mx[i] = max(mx[i], abs_bits(e[i][j]) < kInf ? abs_bits(e[i][j]) : 0);
@@ -344,11 +379,12 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
             const auto split = [&](bool odd) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
+                    const float t = without_inf<K>(e[i][j], odd);
                     _Float16 a, b;
-                    pieces(e[i][j], mul, odd, a, b);
+                    pieces(t, mul, odd, a, b);
                     hi[j] = a;
                     lo[j] = b;
-                    sum = fmaf(e[i][j], mul, sum);
+                    sum = fmaf(t, mul, sum);
                 }
             };
             if (odd)
@@ -362,7 +398,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
             px[(NV + v) * PITCH + vl] = lo;
             if constexpr (K) {
                 _Float16 a, b;
-                pieces(quad_sum(sum), 0.03125f, true, a, b);
+                pieces(quad_sum(sum), 0.03125f, false, a, b);
                 if ((vl & 3) == 0) {
                     _Float16 *to = reinterpret_cast<_Float16 *>(ps + (vl >> 4) * COLS) + ((vl >> 2) & 3);
                     to[v * 4] = a;
@@ -429,6 +465,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
     floatx4 *red = reinterpret_cast<floatx4 *>(lds);
 #pragma unroll
     for (int t = 0; t < RT; t++) red[(wave * RT + t) * 64 + lane] = total[t];
+    if (K && lane == 0) inf_of[wave] = inf;
     __syncthreads();
     for (int i = threadIdx.x; i < RT * 16 * NV; i += kFewWaves * 64) {
         const int rr = i & 15, t = (i >> 4) % RT, v = (i >> 4) / RT;
@@ -439,6 +476,15 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
         const int row = (tile0 + t) * 16 + rr;
         if (v < n_vec && row < w.rows) y[(int64_t)v * w.rows + row] = sum;
     }
+    if constexpr (K) {
+        for (int k = 0; k < kFewWaves; k++) inf |= inf_of[k];
+        if (inf)  // the thread's own outputs again
+            for (int i = threadIdx.x; i < RT * 16 * NV; i += kFewWaves * 64) {
+                const int row = (tile0 + (i >> 4) % RT) * 16 + (i & 15), v = (i >> 4) / RT;
+                if (v < n_vec && row < w.rows && (inf >> v & 1))
+                    y[(int64_t)v * w.rows + row] += infinite_terms(w, x + (int64_t)v * w.cols, row);
+            }
+    }
 }
 
 // ---- more vectors: the pieces of x, once per call ----------------------------------
@@ -447,7 +493,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Wei
 // finite |x| of a row, then the pieces in B-operand order, xp[v / 16][group][piece]
 // [lane = kg * 16 + v % 16] = 8 halves, zeros past the columns, and undo[v] = 2^-s.
 // Q4_K: the sums of each group, times 2^-5 and in pieces, xm[v / 16][superblock][piece]
-// [v % 16] = the eight groups' halves. Vectors up to the next 16 are left as they are:
+// [v % 16] = the eight groups' halves, and undo[v] < 0 of a vector that holds an infinity
+// and no NaN. Vectors up to the next 16 are left as they are:
 // a column of the product is its vector's alone. Many vectors go four a workgroup, so
 // that 64 bytes are written together (1,999 x 4,096: 29 us at one, whose 16-byte
 // pieces met in memory). Up to 64 take a workgroup each, for the chip's sake, twice:
@@ -508,7 +555,7 @@ __global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x,
 #pragma unroll
     for (int i = 0; i < kSplitUnits; i++) fetch(e[i], i * PASS + ut);
     uint32_t top = group_max(false, 0);
-    const bool odd = top >= kInf;
+    const bool odd = top >= kInf, inf = top == kInf;
     if (__syncthreads_or(odd)) {
         const uint32_t fin = group_max(true, 1);
         if (odd) top = fin;
@@ -516,17 +563,18 @@ __global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x,
     const int sh = shift_of(top);
     const float mul = exp2_of(sh);
     if (v >= n_vec) return;
-    if (ut == 0) undo[v] = exp2_of(-sh);
+    if (ut == 0) undo[v] = K && inf ? -exp2_of(-sh) : exp2_of(-sh);
     const auto put = [&](const float (&d)[8], int u) {
         half8 hi, lo;
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
+            const float t = without_inf<K>(d[j], odd);
             _Float16 a, b;
-            pieces(d[j], mul, odd, a, b);
+            pieces(t, mul, odd, a, b);
             hi[j] = a;
             lo[j] = b;
-            sum = fmaf(d[j], mul, sum);
+            sum = fmaf(t, mul, sum);
         }
         _Float16 *to = xp + (((int64_t)(v >> 4) * n_quads * 4 + (u >> 2)) * 128 + (u & 3) * 16 + (v & 15)) * 8;
         *reinterpret_cast<half8 *>(to) = hi;
@@ -534,7 +582,7 @@ __global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x,
         if constexpr (K) {
             _Float16 a, b;
             // units of a group are four threads, neighbours or VQ apart
-            pieces(VQ == 1 ? quad_sum(sum) : apart_sum(sum), 0.03125f, true, a, b);
+            pieces(VQ == 1 ? quad_sum(sum) : apart_sum(sum), 0.03125f, false, a, b);
             if ((u & 3) == 0) {
                 _Float16 *m = xm + (((int64_t)(v >> 4) * (n_quads / 2) + (u >> 5)) * 32 + (v & 15)) * 8 + ((u >> 2) & 7);
                 m[0] = a;
@@ -558,6 +606,7 @@ struct Pieces {
     const _Float16 *xp;
     const _Float16 *xm;
     const float *undo;
+    const float *x;  // the vectors themselves, for the infinities among them
 };
 
 // ---- some vectors -------------------------------------------------------------------
@@ -698,6 +747,7 @@ __global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Wei
 #pragma unroll
         for (int v = 0; v < NVT; v++) *reinterpret_cast<floatx4 *>(&red[at(wave % KW, t, vt0 + v, lane)]) = acc[t][v];
     __syncthreads();
+    bool inf = false;  // Q4_K: of a vector with an infinity
     for (int i = threadIdx.x; i < RT * 16 * VT * 16; i += kMidWaves * 64) {
         const int rl = i % (RT * 16), vl = i / (RT * 16);  // consecutive threads, consecutive rows
         const int from = at(0, rl >> 4, vl >> 4, ((rl & 15) >> 2) * 16 + (vl & 15)) + (rl & 3);
@@ -705,8 +755,18 @@ __global__ __launch_bounds__(kMidWaves * 64) void matvec_q4_mid_kernel(const Wei
 #pragma unroll
         for (int k = 1; k < KW; k++) sum += red[from + k * RT * VT * S];
         const int row = tile0 * 16 + rl, v = vb * 16 + vl;
-        if (row < w.rows && v < n_vec) y[(int64_t)v * w.rows + row] = (K ? sum * kUnscale : sum) * px.undo[v];
+        if (row < w.rows && v < n_vec) {
+            const float undo = px.undo[v];
+            y[(int64_t)v * w.rows + row] = K ? sum * kUnscale * fabsf(undo) : sum * undo;
+            inf |= K && undo < 0;
+        }
     }
+    if (inf)  // the thread's own outputs again
+        for (int i = threadIdx.x; i < RT * 16 * VT * 16; i += kMidWaves * 64) {
+            const int row = tile0 * 16 + i % (RT * 16), v = vb * 16 + i / (RT * 16);
+            if (row < w.rows && v < n_vec && px.undo[v] < 0)
+                y[(int64_t)v * w.rows + row] += infinite_terms(w, px.x + (int64_t)v * w.cols, row);
+        }
 }
 
 // ---- many vectors ----------------------------------------------------------------------
@@ -960,8 +1020,11 @@ __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w,
             }
         });
     }
+    bool inf = false;  // Q4_K: of a vector with an infinity
     each([&](int64_t at, int left, const floatx4 &t, int vec) {
-        const floatx4 o = (K ? t * kUnscale : t) * px.undo[vec];
+        const float undo = px.undo[vec];
+        const floatx4 o = K ? t * kUnscale * fabsf(undo) : t * undo;
+        inf |= K && undo < 0;
         if (quads) {
             *reinterpret_cast<floatx4 *>(y + at) = o;
         } else {
@@ -970,6 +1033,15 @@ __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w,
                 if (r < left) y[at + r] = o[r];
         }
     });
+    if (inf)  // the lane's own outputs again
+        for (int v = 0; v < VT; v++) {
+            const int vec = (vt_wg + vt0 + v) * 16 + col;
+            if (vec >= n_vec || !(px.undo[vec] < 0)) continue;
+            for (int t = 0; t < RT * 4; t++) {
+                const int row = (tile_wg + rt0 + t / 4) * 16 + kg * 4 + t % 4;
+                if (row < w.rows) y[(int64_t)vec * w.rows + row] += infinite_terms(w, px.x + (int64_t)vec * w.cols, row);
+            }
+        }
 }
 
 constexpr int kMaxVec = 262128;
@@ -1025,6 +1097,7 @@ int make_pieces(gla_ctx *ctx, const gla_q4w *w, const float *x, int n, size_t pa
     px->xp = (const _Float16 *)base;
     px->xm = (const _Float16 *)(base + xp);
     px->undo = (const float *)(base + xp + xm);
+    px->x = x;
     if (partials) *partials = (float *)(base + xp + xm + un);
     const bool four = n > 64;
     auto kernel = k ? (four ? split_q4_kernel<true, 4> : split_q4_kernel<true, 1>)

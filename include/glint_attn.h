@@ -477,7 +477,9 @@ int gla_q4w_rows(const gla_q4w *w);
 int gla_q4w_cols(const gla_q4w *w);
 
 /* y[v][r] = sum_c W[r][c] * x[v][c] for n_vec vectors, as gla_matvec_q8_0:
- * x device [n_vec][cols], y device [n_vec][rows], f32, y apart from x.
+ * x device [n_vec][cols], y device [n_vec][rows], f32, y apart from x. Infinite
+ * and NaN elements of x act as in that sum (infinity times a weight of 0 is NaN)
+ * and stay in their vector's outputs.
  * Asynchronous; up to 8 vectors allocate nothing, more take scratch of the
  * stream, which the first call of a size allocates: make that call before
  * capturing it into a graph (a capture that would allocate is refused,

@@ -1,0 +1,87 @@
+"""gla_matvec_q4 where it can go wrong beside its sizes."""
+import numpy as np
+import pytest
+
+from test_gpu_matvec_q4 import ggml, parts, run
+
+pytestmark = pytest.mark.gpu
+
+
+def with_zero_weights(rng, fmt, rows, cols):
+    """Random blocks, some of whose weights are 0: nibbles of 8 are (Q4_0); nibbles of 0 in blocks without minima (Q4_K)."""
+    raw = ggml(rng, fmt, rows, cols)
+    if fmt == "q4_k":
+        raw[rng.random(raw.shape[:2]) < 0.3, 2:4] = 0
+    return raw
+
+
+def odd_vectors(rng, n, cols):
+    """Ordinary vectors, and among them some with infinities: one, two of one sign, two that differ, beside a NaN, nothing but."""
+    x = rng.standard_normal((n, cols)).astype(np.float32)
+    for i in range(n):
+        at = rng.permutation(cols)
+        kind = i % 8 if n > 1 else 1
+        if kind == 1:
+            x[i, at[0]] = np.inf
+        elif kind == 2:
+            x[i, cols - 1] = -np.inf
+        elif kind == 3:
+            x[i, at[:2]] = np.inf
+        elif kind == 4:
+            c = at[0] // 32 * 32  # in one group
+            x[i, [c + 3, c + 17]] = np.inf, -np.inf
+        elif kind == 5:
+            x[i, 0], x[i, at[0]] = np.inf, np.nan
+        elif kind == 6:
+            x[i] = -np.inf
+    return x
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("rows, cols, ns", [(40, 1024, (1, 2, 3, 5, 8, 9, 20, 70)), (300, 4096, (1, 2, 4, 7, 33)), (4113, 512, (2, 4, 8, 30)),
+                                            (8209, 512, (1,)), (14000, 512, (61, 120)), (1027, 2048, (2500,)), (1028, 512, (8100,))])
+def test_infinities_meet_the_whole_weight(backend, fmt, rows, cols, ns):
+    """An infinite element times a weight is an infinity of the weight's sign, and NaN where the weight is 0; sums of them, and
+    with finite products, are IEEE's. Both formats, every kernel: 64 bits say which outputs are NaN, +inf, -inf and finite."""
+    rng = np.random.default_rng(rows + cols)
+    raw = with_zero_weights(rng, fmt, rows, cols)
+    w = backend.create_q4_weights(raw, rows, cols, fmt)
+    wd, wm = parts(raw, fmt)
+    whole = wd - wm  # exact: 21 bits against 17, within a few binades
+    assert (whole == 0).any()
+    sign = np.sign(whole)
+    alike = (sign == sign[:, :1]).all(1) & (sign[:, 0] != 0)
+    every = np.where(alike, np.copysign(np.inf, -sign[:, 0]), np.nan)  # all of x is -inf
+    for n in ns:
+        x = odd_vectors(rng, n, cols)
+        got = run(backend, w, x, shift=n % 2)
+        odd = ~np.isfinite(x).all(1)
+        assert odd.any() and np.isfinite(got[~odd]).all()
+        want = np.zeros((int(odd.sum()), rows))
+        for i, v in enumerate(x[odd].astype(np.float64)):
+            at = ~np.isfinite(v)
+            if at.all():
+                want[i] = every
+            else:
+                with np.errstate(invalid="ignore"):
+                    want[i] = (whole[:, at] * v[at]).sum(1)
+        assert not np.isfinite(want).any()
+        assert np.array_equal(got[odd].astype(np.float64), want, equal_nan=True), n
+
+
+@pytest.mark.parametrize("n", [1, 6, 20, 2500])
+def test_infinities_leave_the_other_vectors_their_bits(backend, n):
+    """An infinity in one vector of a call changes no bit of the others'."""
+    rows, cols = (1027, 2048) if n > 70 else (40, 1024)
+    rng = np.random.default_rng(n)
+    raw = ggml(rng, "q4_k", rows, cols)
+    w = backend.create_q4_weights(raw, rows, cols, "q4_k")
+    x = rng.standard_normal((n, cols)).astype(np.float32)
+    clean = run(backend, w, x)
+    x[n // 2, 5] = np.inf
+    got = run(backend, w, x)
+    rest = np.arange(n) != n // 2
+    assert np.array_equal(got[rest], clean[rest])
+    wd, wm = parts(raw, "q4_k")
+    with np.errstate(invalid="ignore"):
+        assert np.array_equal(got[n // 2].astype(np.float64), (wd - wm)[:, 5] * np.inf, equal_nan=True)
