@@ -265,6 +265,7 @@ struct Append {
 };
 
 constexpr int kMaxGridY = 32768;  // sequences along y, the rest along z
+constexpr int kMaxSeqs = kMaxGridY * 65535;  // a launch's limit along z
 
 // The storage page of (b, page lp of the sequence), or -1 where there is none.
 __device__ __forceinline__ int64_t storage_page(const PageMap &pm, int b, int64_t lp) {
@@ -634,7 +635,8 @@ int gla_kv_append(gla_ctx *ctx, const gla_append_args *a) {
         GLA_REQUIRE(a->rope->head_dim == kv->head_dim, "gla_kv_append: the rotary plan is for heads of %d, the storage's are %d",
                     a->rope->head_dim, kv->head_dim);
     }
-    GLA_REQUIRE(a->n_seqs >= 0 && a->max_q_len >= 0, "gla_kv_append: n_seqs %d, max_q_len %d", a->n_seqs, a->max_q_len);
+    GLA_REQUIRE(a->n_seqs >= 0 && a->n_seqs <= kMaxSeqs && a->max_q_len >= 0,
+                "gla_kv_append: n_seqs %d (0 to %d), max_q_len %d", a->n_seqs, kMaxSeqs, a->max_q_len);
     Append p;
     memset(&p, 0, sizeof(p));
     p.k_stride = a->k_stride ? a->k_stride : kv->kv_dim;

@@ -422,7 +422,7 @@ int gla_rope_rows(gla_ctx *ctx, const gla_rope_plan *plan, const float *x, int64
 typedef struct gla_append_args {
     gla_kv *kv;
     int layer;                 /* caches */
-    int n_seqs;
+    int n_seqs;                /* B, at most 2,147,450,880 */
     const int32_t *seq_slot;   /* caches: device int32[B] or NULL */
     const int32_t *page_table; /* pools: device int32[B][page_table_stride] */
     int page_table_stride;
