@@ -567,15 +567,21 @@ __global__ __launch_bounds__(kSplitThreads) void split_q4_kernel(const float *x,
     const auto put = [&](const float (&d)[8], int u) {
         half8 hi, lo;
         float sum = 0.0f;
+        const auto split = [&](bool odd) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float t = without_inf<K>(d[j], odd);
-            _Float16 a, b;
-            pieces(t, mul, odd, a, b);
-            hi[j] = a;
-            lo[j] = b;
-            sum = fmaf(t, mul, sum);
-        }
+            for (int j = 0; j < 8; j++) {
+                const float t = without_inf<K>(d[j], odd);
+                _Float16 a, b;
+                pieces(t, mul, odd, a, b);
+                hi[j] = a;
+                lo[j] = b;
+                sum = fmaf(t, mul, sum);
+            }
+        };
+        if (odd)
+            split(true);
+        else
+            split(false);
         _Float16 *to = xp + (((int64_t)(v >> 4) * n_quads * 4 + (u >> 2)) * 128 + (u & 3) * 16 + (v & 15)) * 8;
         *reinterpret_cast<half8 *>(to) = hi;
         *reinterpret_cast<half8 *>(to + 512) = lo;
