@@ -790,8 +790,10 @@ __device__ __forceinline__ void store_agent2(float *p, float a, float b) {
                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// y[v][row] for 128 rows x 32 VT vectors a workgroup, and one of gridDim.z (one or two)
-// slices of K: four waves of 4 row tiles x VT vector tiles, 2 x 2 of them, which share weights
+// y[v][row] for 128 rows x 32 VT vectors a workgroup, and one of `slices` (one or two) slices
+// of K, slice0 + blockIdx.z: two workgroups of one launch, whose last to arrive adds the
+// slices, or two launches, whose second adds to y (undo and kUnscale are powers of two: the
+// same bits). Four waves of 4 row tiles x VT vector tiles, 2 x 2 of them, which share weights
 // and pieces of x through LDS. A step is a group of 32 columns: the pieces come by
 // LDS copies two steps ahead into a ring of three, the weights of a quad of groups
 // (with scales, and for Q4_K the sums of x) during the quad before, each wave issuing
@@ -801,7 +803,8 @@ __device__ __forceinline__ void store_agent2(float *p, float a, float b) {
 // unpacked, between the MFMAs of this one.
 template <bool K, int VT>
 __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w, const Pieces px, int n_vec, float *y,
-                                                                float *part, int64_t slice_stride, int32_t *arrivals) {
+                                                                int slices, int slice0, float *part, int64_t slice_stride,
+                                                                int32_t *arrivals) {
     constexpr int RT = 4, UNIT = K ? 2 : 1;
     constexpr int XS = 2 * VT * 2048;  // a ring slot of x: the pieces of 2 VT tiles
     constexpr int AUX = 2 * RT * 1024, SUP = AUX + 1024, XM = SUP + 1024, WS = K ? XM + 4096 : SUP;
@@ -817,8 +820,8 @@ __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w,
         (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)&lds[0]);
 
     const int units = w.n_quads / UNIT;
-    const int ps = (units + gridDim.z - 1) / gridDim.z;
-    const int q0 = min(units, (int)blockIdx.z * ps) * UNIT, q1 = min(units, (int)(blockIdx.z + 1) * ps) * UNIT;
+    const int ps = (units + slices - 1) / slices, slice = slice0 + (int)blockIdx.z;
+    const int q0 = min(units, slice * ps) * UNIT, q1 = min(units, (slice + 1) * ps) * UNIT;
 
     // the wave's copies: VT of 2 VT x 2 pieces, two row tiles and their scales, and
     // (Q4_K, a superblock at a time) the sums of VT / 2 vector tiles
@@ -1027,19 +1030,21 @@ __global__ __launch_bounds__(256, 2) void matvec_q4_gemm_kernel(const Weights w,
         });
     }
     bool inf = false;  // Q4_K: of a vector with an infinity
+    const bool add = gridDim.z < (unsigned)slices && slice > 0;
     each([&](int64_t at, int left, const floatx4 &t, int vec) {
         const float undo = px.undo[vec];
-        const floatx4 o = K ? t * kUnscale * fabsf(undo) : t * undo;
+        floatx4 o = K ? t * kUnscale * fabsf(undo) : t * undo;
         inf |= K && undo < 0;
         if (quads) {
+            if (add) o += *reinterpret_cast<const floatx4 *>(y + at);
             *reinterpret_cast<floatx4 *>(y + at) = o;
         } else {
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                if (r < left) y[at + r] = o[r];
+                if (r < left) y[at + r] = add ? o[r] + y[at + r] : o[r];
         }
     });
-    if (inf)  // the lane's own outputs again
+    if (inf && slice0 + (int)gridDim.z == slices)  // the lane's own outputs again
         for (int v = 0; v < VT; v++) {
             const int vec = (vt_wg + vt0 + v) * 16 + col;
             if (vec >= n_vec || !(px.undo[vec] < 0)) continue;
@@ -1091,20 +1096,28 @@ int few(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n,
 
 constexpr int kFewVec = 8;
 
-// Pieces, sums and scales of n vectors in the stream's scratch, with `part` bytes behind them.
-int make_pieces(gla_ctx *ctx, const gla_q4w *w, const float *x, int n, size_t part, Pieces *px, float **partials) {
-    const bool k = w->format == GLA_Q4_K;
+// Bytes of the pieces, the sums and the scales of n vectors.
+struct PieceBytes {
+    size_t xp, xm, undo;
+    size_t all() const { return xp + xm + undo; }
+};
+PieceBytes piece_bytes(const gla_q4w *w, int n) {
     const size_t tiles = (size_t)(n + 15) / 16;
-    const size_t xp = tiles * w->n_quads * 4 * 2048, xm = k ? tiles * (w->n_quads / 2) * 512 : 0;
-    const size_t un = ((size_t)n * sizeof(float) + 255) / 256 * 256;
+    return {tiles * w->n_quads * 4 * 2048, w->format == GLA_Q4_K ? tiles * (w->n_quads / 2) * 512 : 0,
+            ((size_t)n * sizeof(float) + 255) / 256 * 256};
+}
+
+// Makes them in the stream's scratch.
+int make_pieces(gla_ctx *ctx, const gla_q4w *w, const float *x, int n, Pieces *px) {
+    const bool k = w->format == GLA_Q4_K;
+    const PieceBytes b = piece_bytes(w, n);
     void *scr = nullptr;
-    if (int rc = ensure_scratch(ctx, xp + xm + un + part, &scr)) return rc;
+    if (int rc = ensure_scratch(ctx, b.all(), &scr)) return rc;
     uint8_t *base = (uint8_t *)scr;
     px->xp = (const _Float16 *)base;
-    px->xm = (const _Float16 *)(base + xp);
-    px->undo = (const float *)(base + xp + xm);
+    px->xm = (const _Float16 *)(base + b.xp);
+    px->undo = (const float *)(base + b.xp + b.xm);
     px->x = x;
-    if (partials) *partials = (float *)(base + xp + xm + un);
     const bool four = n > 64;
     auto kernel = k ? (four ? split_q4_kernel<true, 4> : split_q4_kernel<true, 1>)
                     : (four ? split_q4_kernel<false, 4> : split_q4_kernel<false, 1>);
@@ -1134,7 +1147,7 @@ Tile mid_tile(const gla_ctx *ctx, const gla_q4w *w, int n, int64_t *cost) {
 
 int mid(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y, Tile t) {
     Pieces px;
-    if (int rc = make_pieces(ctx, w, x, n, 0, &px, nullptr)) return rc;
+    if (int rc = make_pieces(ctx, w, x, n, &px)) return rc;
     const auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((w->n_tiles + t.rt - 1) / t.rt, ((n + 15) / 16 + t.nv - 1) / t.nv), dim3(kMidWaves * 64),
                            0, ctx->stream, p, px, n, y);
@@ -1168,16 +1181,27 @@ int many(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n
     const int64_t wgs = (int64_t)row_blocks * vec_blocks, stride = (int64_t)n * w->rows;
     const size_t partials = (size_t)(2 * stride) * sizeof(float);
     const int slices = vt == 2 && 2 * wgs <= 3 * ctx->n_cu && w->n_quads >= 16 && partials <= ((size_t)28 << 20) ? 2 : 1;
-    Pieces px;
-    float *part = nullptr;
+    const size_t behind = piece_bytes(w, n).all();
+    void *scr = nullptr;
     int32_t *arrivals = nullptr;
-    if (slices > 1)
-        if (int rc = ensure_arrivals(ctx, (size_t)wgs, &arrivals)) return rc;
-    if (int rc = make_pieces(ctx, w, x, n, slices > 1 ? partials : 0, &px, &part)) return rc;
+    bool at_once = true;
+    if (slices > 1 && (ensure_scratch(ctx, behind + partials, &scr) != GLA_OK || ensure_arrivals(ctx, (size_t)wgs, &arrivals) != GLA_OK)) {
+        // the partial sums or their counters cannot be had (a capture in which they would
+        // have to grow, a full device): a slice after the other
+        clear_error();
+        (void)hipGetLastError();
+        at_once = false;
+    }
+    Pieces px;
+    if (int rc = make_pieces(ctx, w, x, n, &px)) return rc;
+    float *part = at_once && slices > 1 ? (float *)((uint8_t *)scr + behind) : nullptr;
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(row_blocks, vec_blocks, slices), dim3(256), 0, ctx->stream, p, px, n, y, part, stride,
-                           arrivals);
-        return launched("matvec_q4_gemm_kernel");
+        for (int slice = 0; slice < (at_once ? 1 : slices); slice++) {
+            hipLaunchKernelGGL(kernel, dim3(row_blocks, vec_blocks, at_once ? slices : 1), dim3(256), 0, ctx->stream, p, px, n, y,
+                               slices, slice, part, stride, arrivals);
+            if (int rc = launched("matvec_q4_gemm_kernel")) return rc;
+        }
+        return (int)GLA_OK;
     };
     if (vt == 4) return k ? go(matvec_q4_gemm_kernel<true, 4>) : go(matvec_q4_gemm_kernel<false, 4>);
     return k ? go(matvec_q4_gemm_kernel<true, 2>) : go(matvec_q4_gemm_kernel<false, 2>);

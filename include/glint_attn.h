@@ -483,7 +483,8 @@ int gla_q4w_cols(const gla_q4w *w);
  * Asynchronous; up to 8 vectors allocate nothing, more take scratch of the
  * stream, which the first call of a size allocates: make that call before
  * capturing it into a graph (a capture that would allocate is refused,
- * GLA_ERR_INVALID). n_vec above 262,128 is refused (split the call). */
+ * GLA_ERR_INVALID; partial sums that alone would not fit are done without, the
+ * same bits in two launches). n_vec above 262,128 is refused (split the call). */
 int gla_matvec_q4(gla_ctx *ctx, const gla_q4w *w, const float *x, int n_vec, float *y);
 
 #ifdef __cplusplus

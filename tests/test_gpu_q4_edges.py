@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from glint_amd.attn import HipStream
 from test_gpu_matvec_q4 import ggml, parts, run
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +86,37 @@ def test_infinities_leave_the_other_vectors_their_bits(backend, n):
     wd, wm = parts(raw, "q4_k")
     with np.errstate(invalid="ignore"):
         assert np.array_equal(got[n // 2].astype(np.float64), (wd - wm)[:, 5] * np.inf, equal_nan=True)
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("rows, n, larger", [(6144, 400, 2000), (1027, 2500, 4000)])
+def test_slices_without_their_own_scratch(backend, fmt, rows, n, larger):
+    """A product in two slices of K whose partial sums and counters would have to grow during a capture takes the slices one
+    after the other: an earlier call of more vectors, which needs neither, is enough before the capture. The bits are those of
+    two slices at once, replay by replay."""
+    be, cols = backend, 2048
+    rng = np.random.default_rng(rows)
+    raw = ggml(rng, fmt, rows, cols)
+    w = be.create_q4_weights(raw, rows, cols, fmt)
+    xs = [rng.standard_normal((n, cols)).astype(np.float32) for _ in range(2)]
+    xs[1][3, 100] = np.inf
+    want = [run(be, w, x) for x in xs]
+    assert np.isfinite(want[0]).all()
+    s = HipStream()
+    try:
+        be.set_stream(s)
+        inp, out = be.buffer(xs[0]), be.empty(n * rows * 4)
+        big, y = be.buffer(rng.standard_normal((larger, cols)).astype(np.float32)), be.empty(larger * rows * 4)
+        be.matvec_q4(w, big, larger, y)
+        be.sync()
+        g = be.capture(lambda: be.matvec_q4(w, inp, n, out))
+        for rep in range(4):
+            inp.upload(xs[rep % 2])
+            be.matvec_q4(w, big, larger, y)
+            g.replay()
+            be.sync()
+            assert np.array_equal(out.download((n, rows)), want[rep % 2], equal_nan=True), rep
+        g.destroy()
+    finally:
+        be.set_stream(None)
+        s.destroy()
