@@ -59,8 +59,10 @@ static int grow(gla_ctx *ctx, void **ptr, size_t *cur, size_t need, bool pinned)
     size_t want = std::max(need, *cur * 2);
     void *fresh = nullptr;
     hipError_t e = pinned ? hipHostMalloc(&fresh, want, hipHostMallocDefault) : hipMalloc(&fresh, want);
-    if (e != hipSuccess)
+    if (e != hipSuccess) {
+        (void)hipGetLastError();  // not the next launch's
         return set_error(GLA_ERR_BUFFER, "allocation of %zu bytes failed: %s", want, hipGetErrorString(e));
+    }
     if (*ptr) ctx->retired.emplace_back(*ptr, pinned);
     *ptr = fresh;
     *cur = want;
@@ -129,8 +131,10 @@ int ensure_arrivals(gla_ctx *ctx, size_t n, int32_t **out) {
     const size_t want = std::max<size_t>(n, std::max<size_t>(1024, 2 * ss->n_arrivals));
     void *fresh = nullptr;
     hipError_t e = hipMalloc(&fresh, want * sizeof(int32_t));
-    if (e != hipSuccess)
+    if (e != hipSuccess) {
+        (void)hipGetLastError();  // not the next launch's
         return set_error(GLA_ERR_BUFFER, "allocation of %zu arrival counters failed: %s", want, hipGetErrorString(e));
+    }
     // (queued on the stream: ordered before every launch that uses them)
     e = hipMemsetAsync(fresh, 0, want * sizeof(int32_t), ctx->stream);
     if (e != hipSuccess) {
@@ -403,8 +407,10 @@ static int kv_alloc(gla_ctx *ctx, gla_kv *kv) {
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
     void *p = nullptr;
     hipError_t e = hipMalloc(&p, bytes ? bytes : 256);
-    if (e != hipSuccess)
+    if (e != hipSuccess) {
+        (void)hipGetLastError();  // not the next launch's
         return set_error(GLA_ERR_BUFFER, "KV storage of %zu bytes: %s", bytes, hipGetErrorString(e));
+    }
     kv->base = (uint8_t *)p;
     kv->ctx = ctx;
     if (bytes) {

@@ -43,10 +43,14 @@
 
 #include "../../include/glint_attn.h"
 
-#define GLA_CHECK_HIP(expr, code)                                                                   \
-    do {                                                                                            \
-        hipError_t _e = (expr);                                                                     \
-        if (_e != hipSuccess) return gla::set_error((code), "%s: %s", #expr, hipGetErrorString(_e)); \
+// (a reported error is taken from the runtime, or the next launch's check would report it again)
+#define GLA_CHECK_HIP(expr, code)                                                     \
+    do {                                                                              \
+        hipError_t _e = (expr);                                                       \
+        if (_e != hipSuccess) {                                                       \
+            (void)hipGetLastError();                                                  \
+            return gla::set_error((code), "%s: %s", #expr, hipGetErrorString(_e));    \
+        }                                                                             \
     } while (0)
 
 #define GLA_GUARD_BEGIN try {

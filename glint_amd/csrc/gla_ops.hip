@@ -1034,6 +1034,7 @@ int gla_q8w_create(gla_ctx *ctx, const uint8_t *ggml_host, int rows, int cols, g
     if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     if (raw) (void)hipFree(raw);
     if (e != hipSuccess) {
+        (void)hipGetLastError();  // not the next launch's
         (void)hipFree(w->quants);
         (void)hipFree(w->scales);
         delete w;
