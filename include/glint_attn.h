@@ -476,7 +476,12 @@ int gla_q4w_destroy(gla_q4w *w);
 int gla_q4w_rows(const gla_q4w *w);
 int gla_q4w_cols(const gla_q4w *w);
 
-/* y[v][r] = sum_c W[r][c] * x[v][c] for n_vec vectors, as gla_matvec_q8_0:
+/* y[v][r] = sum_c W[r][c] * x[v][c] for n_vec vectors. A vector's outputs do not
+ * depend on the others' values, but their rounding depends on n_vec (unlike
+ * gla_matvec_q8_0's from 5 vectors on): calls of different n_vec agree to f32
+ * rounding of the sum of |W[r][c] * x[v][c]| (for Q4_K of its nibbles' and its
+ * minima's parts), not bit for bit. x counts with 22 bits, and with an absolute
+ * error of 2^-38 of the largest |x| of its vector where that is more.
  * x device [n_vec][cols], y device [n_vec][rows], f32, y apart from x. Infinite
  * and NaN elements of x act as in that sum (infinity times a weight of 0 is NaN)
  * and stay in their vector's outputs.

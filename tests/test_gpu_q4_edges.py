@@ -120,3 +120,27 @@ def test_slices_without_their_own_scratch(backend, fmt, rows, n, larger):
     finally:
         be.set_stream(None)
         s.destroy()
+
+
+@pytest.mark.parametrize("fmt, rows, cols", [("q4_0", 96, 4096), ("q4_k", 96, 4096), ("q4_0", 4113, 576), ("q4_k", 1027, 2048)])
+def test_batches_agree_within_their_roundings(backend, fmt, rows, cols):
+    """The first vectors in batches that take other kernels, tiles and slices. Each call is off by at most 2^-22 of |x| and
+    2^-38 of the largest |x| for the pieces, and half a step of f32 for each of cols / 32 + 64 additions (the longest chain);
+    two calls by twice that. The same call twice, and with other vectors behind, has the same bits."""
+    rng = np.random.default_rng(rows)
+    raw = ggml(rng, fmt, rows, cols)
+    w = backend.create_q4_weights(raw, rows, cols, fmt)
+    wd, wm = parts(raw, fmt)
+    x = rng.standard_normal((2500, cols)).astype(np.float32)
+    x[0, 7] = 3e4  # an outlier: the scale of its own vector alone
+    a = np.abs(x[:2].astype(np.float64))
+    size = a @ (np.abs(wd) + wm).T
+    largest = a.max(1, keepdims=True) * (np.abs(wd) + wm).sum(1)[None]
+    bound = 2 * (size * (2.0 ** -22 + (cols / 32 + 64) * 2.0 ** -24) + largest * 2.0 ** -38)
+    base = run(backend, w, x[:2])
+    for n in (4, 8, 9, 33, 64, 100, 130, 400, 2500):
+        got = run(backend, w, x[:n])[:2]
+        assert np.all(np.abs(got.astype(np.float64) - base) <= bound), n
+        other = x[:n].copy()
+        other[2:] = -other[2:] * 1e3
+        assert np.array_equal(run(backend, w, other)[:2], got), n
