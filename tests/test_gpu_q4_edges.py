@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import q4_structured as st
 from glint_amd.attn import HipStream
 from test_gpu_matvec_q4 import ggml, parts, run
 
@@ -144,3 +145,55 @@ def test_batches_agree_within_their_roundings(backend, fmt, rows, cols):
         other = x[:n].copy()
         other[2:] = -other[2:] * 1e3
         assert np.array_equal(run(backend, w, other)[:2], got), n
+
+
+# (format, rows, columns): short rows, rows that leave waves without a quad or end inside one, the widest that is kept in
+# registers when x is split (16,384 columns) and wider ones, tall matrices (two row tiles a workgroup)
+STRUCTURED = [("q4_0", 33, 96), ("q4_0", 40, 576), ("q4_0", 47, 2080), ("q4_0", 20, 4128), ("q4_0", 33, 16384), ("q4_0", 33, 16416),
+              ("q4_0", 17, 20480), ("q4_0", 4113, 5152), ("q4_k", 33, 256), ("q4_k", 47, 768), ("q4_k", 300, 4096), ("q4_k", 17, 16384),
+              ("q4_k", 17, 16640), ("q4_k", 20, 20480), ("q4_k", 4113, 5120)]
+
+
+@pytest.mark.parametrize("fmt, rows, cols", STRUCTURED)
+def test_low_pieces_count_at_every_width(backend, fmt, rows, cols):
+    """Vectors of four elements that need both pieces, each column in turn: a low piece that is lost, or of another column, is far
+    outside the bound (shown on the CPU with the mistakes planted)."""
+    rng = np.random.default_rng(cols + rows)
+    raw = ggml(rng, fmt, rows, cols)
+    w = backend.create_q4_weights(raw, rows, cols, fmt)
+    wd, wm = parts(raw, fmt)
+    first = 0
+    for n in (1, 2, 4, 7, 8, 9, 16, 40, 64, 65, 130, 400, 1100):
+        x = st.vectors(rng, n, cols, first if n < 400 else 0)
+        assert st.holds(run(backend, w, x, shift=n % 2), x, wd, wm), n
+        if cols > 16384 and n > 8:
+            x = st.vectors(rng, n, cols, 16384)
+            assert st.holds(run(backend, w, x, shift=n % 2), x, wd, wm), (n, "tail")
+        first += n
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("outlier", [1e3, 1e6, 1e9])
+def test_an_outlier_on_zero_weights(backend, fmt, outlier):
+    """The largest |x| sets the scale of its vector's pieces. Where all its weights are 0 (nibbles of 8; a superblock without
+    scale and minimum), what is left of the others shows: an element is off by 2^-22 of itself (two halves, half a step of 11
+    bits each) or by 2^-38 of the largest (half a step of the smallest half, 2^-25, against 2^13), whichever is more."""
+    rows, cols, at = 48, 4096, 1030
+    rng = np.random.default_rng(23)
+    raw = ggml(rng, fmt, rows, cols)
+    if fmt == "q4_0":
+        raw[:, at // 32, 2 + at % 16] = raw[:, at // 32, 2 + at % 16] & 0xF0 | 8  # column 1030 is value 6 of its block
+    else:
+        raw[:, at // 256, :4] = 0
+    w = backend.create_q4_weights(raw, rows, cols, fmt)
+    wd, wm = parts(raw, fmt)
+    assert not wd[:, at].any() and not wm[:, at].any()
+    for n in (1, 3, 8, 9, 70, 300):
+        x = rng.standard_normal((n, cols)).astype(np.float32)
+        x[:, at] = outlier
+        rest = np.abs(x.astype(np.float64))
+        rest[:, at] = 0
+        mag = np.abs(wd) + wm
+        bound = rest @ mag.T * (2.0 ** -22 + (cols / 32 + 64) * 2.0 ** -24) + outlier * mag.sum(1) * 2.0 ** -38
+        got = run(backend, w, x).astype(np.float64)
+        assert np.all(np.abs(got - x.astype(np.float64) @ (wd - wm).T) <= bound), n
