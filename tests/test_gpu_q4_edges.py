@@ -4,7 +4,7 @@ import pytest
 
 import q4_structured as st
 from glint_amd.attn import HipStream
-from test_gpu_matvec_q4 import ggml, parts, run
+from test_gpu_matvec_q4 import check, ggml, parts, run
 
 pytestmark = pytest.mark.gpu
 
@@ -197,3 +197,36 @@ def test_an_outlier_on_zero_weights(backend, fmt, outlier):
         bound = rest @ mag.T * (2.0 ** -22 + (cols / 32 + 64) * 2.0 ** -24) + outlier * mag.sum(1) * 2.0 ** -38
         got = run(backend, w, x).astype(np.float64)
         assert np.all(np.abs(got - x.astype(np.float64) @ (wd - wm).T) <= bound), n
+
+
+@pytest.mark.parametrize("fmt, cols", [("q4_0", 576), ("q4_0", 2048), ("q4_0", 2080), ("q4_0", 5152), ("q4_k", 512), ("q4_k", 2048),
+                                       ("q4_k", 2304), ("q4_k", 5120)])
+@pytest.mark.parametrize("rows, ns", [(4113, (2, 3, 4, 5, 8)), (4129, (2, 4, 7)), (8209, (1, 6)), (8225, (1,))])
+def test_tall_matrices_and_few_vectors(backend, fmt, cols, rows, ns):
+    """More row tiles than compute units (258 and 259; for one vector 514 and 515): two tiles a workgroup, the second one missing
+    at the end of an odd number. Rows shorter than a wave's chunk, rows that end inside one, and longer ones."""
+    rng = np.random.default_rng(rows + cols)
+    raw = ggml(rng, fmt, rows, cols)
+    w = backend.create_q4_weights(raw, rows, cols, fmt)
+    wd, wm = parts(raw, fmt)
+    for n in ns:
+        x = rng.standard_normal((n, cols)).astype(np.float32)
+        check(run(backend, w, x, shift=n % 2), x, wd, wm)
+        x = st.vectors(rng, n, cols, int(rng.integers(0, cols)))
+        assert st.holds(run(backend, w, x), x, wd, wm), n
+
+
+@pytest.mark.parametrize("fmt, cols", [("q4_0", 2080), ("q4_k", 2304)])
+@pytest.mark.parametrize("rows, n", [(1000, 33), (6133, 16), (6001, 17), (8100, 32), (6100, 63), (8100, 60), (14000, 61), (14300, 120)],
+                         ids=["1x1", "1x2", "1x3", "1x4", "2x3", "2x4", "4x4", "8x4"])
+def test_tiles_with_quads_for_every_wave(backend, fmt, cols, rows, n):
+    """The middle kernel's tiles (of 16 vectors x of 16 rows, as 256 compute units choose them) over rows long enough that the
+    ranges of K that its waves merge have work, the last of them less."""
+    rng = np.random.default_rng(rows + n)
+    raw = ggml(rng, fmt, rows, cols)
+    w = backend.create_q4_weights(raw, rows, cols, fmt)
+    wd, wm = parts(raw, fmt)
+    x = rng.standard_normal((n, cols)).astype(np.float32)
+    check(run(backend, w, x, shift=n % 2), x, wd, wm)
+    x = st.vectors(rng, n, cols, int(rng.integers(0, cols)))
+    assert st.holds(run(backend, w, x), x, wd, wm)
