@@ -153,9 +153,10 @@ int64_t gla_kv_row_id(const gla_kv *kv, int seq, int layer, int pos);
  * src/cache/paged.rs:467-490). Q8_0 storage quantises on write with the
  * rules of KvCacheQ8::quantize_into (src/cache/mod.rs:296-315), bit-exactly.
  * Device pointers; asynchronous. rows: int64[n_rows]; k, v: [n_rows][kv_dim].
- * The rows are written in parallel: ids repeated within one call leave one
- * of their rows (which one is unspecified), and ids outside the storage are
- * skipped on the device. */
+ * The rows are written in parallel: where ids are repeated within one call
+ * every stored value is one of theirs, which one is unspecified and may differ
+ * from value to value (a Q8_0 quant may lie beside another row's scale): repeat
+ * none that is read later. Ids outside the storage are skipped on the device. */
 int gla_kv_write_rows(gla_ctx *ctx, gla_kv *kv, const int64_t *rows_dev, const float *k_dev,
                       const float *v_dev, int n_rows);
 /* The same with host pointers; returns when the rows are written. */
@@ -415,10 +416,12 @@ int gla_rope_rows(gla_ctx *ctx, const gla_rope_plan *plan, const float *x, int64
  * K and V of a row whose position is outside the storage (a cache's max_seq, a
  * pool's page_table_stride * 16 positions), whose seq_slot is no sequence or
  * whose page id is no page are not stored (the reference panics; a clamped
- * write would overwrite another row); its query is rotated all the same. Rows
- * of one call that meet at one place of the storage (a page in two tables) leave
- * one of them, which one is unspecified. Rows past max_q_len of a sequence and
- * rows outside every sequence are left alone. Asynchronous; allocates nothing. */
+ * write would overwrite another row); its query is rotated all the same. Where
+ * rows of one call meet at one place of the storage (a page in two tables), every
+ * stored value is one of theirs, which one is unspecified and may differ from value
+ * to value (a Q8_0 quant may lie beside another row's scale): give each sequence
+ * pages of its own first. Rows past max_q_len of a sequence and rows outside every
+ * sequence are left alone. Asynchronous; allocates nothing. */
 typedef struct gla_append_args {
     gla_kv *kv;
     int layer;                 /* caches */

@@ -8,6 +8,8 @@ from glint_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
+PAGE = 16
+
 
 def test_more_sequences_than_a_launch_has_are_refused(backend):
     """The count of workgroups along z is made of n_seqs: neither its sum nor the launch may overflow. (No array of that length
@@ -25,3 +27,40 @@ def test_more_sequences_than_a_launch_has_are_refused(backend):
     a.n_seqs = 1
     assert lib.gla_kv_append(be.ctx, C.byref(a)) == _lib.GLA_OK
     be.sync()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "q8"])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_rows_that_meet_at_one_place(backend, dtype, n):
+    """Three sequences whose tables share their pages: every stored byte is one of the three rows' at its place (which one, the
+    call does not say), and the rest of the pool stays. The same for row ids that are repeated."""
+    be, n_kv, d, pages = backend, 2, 128, 8
+    rng = np.random.default_rng(n)
+    k, v = (rng.standard_normal((3 * n, n_kv * d)).astype(np.float32) for _ in "kv")
+    shared = np.array([5, 2, 7], np.int32)
+    rows = np.array([shared[(3 + i) // PAGE] * PAGE + (3 + i) % PAGE for i in range(n)])
+    every = np.arange(pages * PAGE)
+    rest = np.setdiff1d(every, rows)
+    old = rng.standard_normal((len(every), n_kv * d)).astype(np.float32)
+
+    def pool():
+        p = be.create_page_pool(pages, n_kv, d, dtype)
+        p.write_rows(every, old, -old)
+        return p
+
+    want = []
+    for i in range(3):
+        p = pool()
+        p.write_rows(rows, k[i * n:(i + 1) * n], v[i * n:(i + 1) * n])
+        want.append(p.export_rows(every))
+    by_append, by_ids = pool(), pool()
+    be.append(by_append, be.buffer(k), be.buffer(v), be.buffer(np.arange(0, 3 * n + 1, n, dtype=np.int32)),
+              be.buffer(np.full(3, 3, np.int32)), 3, n, page_table=be.buffer(np.tile(shared, (3, 1))), page_table_stride=3)
+    by_ids.write_rows(np.tile(rows, 3), k, v)
+    be.sync()
+    for p in (by_append, by_ids):
+        for which, got in enumerate(p.export_rows(every)):
+            got = np.asarray(got).view(np.uint8).reshape(len(every), -1)
+            each = [np.asarray(t[which]).view(np.uint8).reshape(len(every), -1) for t in want]
+            assert np.array_equal(got[rest], each[0][rest])
+            assert np.all((got == each[0]) | (got == each[1]) | (got == each[2]))
