@@ -92,7 +92,9 @@ int gla_destroy(gla_ctx *ctx);
  * matvec activation pieces), so calls queued on different streams at once
  * never share it and may overlap; calls on one stream run in order as usual.
  * A graph uses the scratch of the stream it was captured on: graphs of one
- * stream are replayed one after another, wherever they are launched.
+ * stream are replayed one after another, wherever they are launched, and one
+ * that is launched on another stream never beside the first one's own calls
+ * (they would share partial sums, pieces and counters): wait in between.
  * That scratch is held until gla_destroy or gla_release_stream. The stream
  * must outlive its use by the context: switch away from it (or release it)
  * before destroying it. The context itself is not thread-safe: switch

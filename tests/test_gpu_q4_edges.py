@@ -230,3 +230,43 @@ def test_tiles_with_quads_for_every_wave(backend, fmt, cols, rows, n):
     check(run(backend, w, x, shift=n % 2), x, wd, wm)
     x = st.vectors(rng, n, cols, int(rng.integers(0, cols)))
     assert st.holds(run(backend, w, x), x, wd, wm)
+
+
+def test_a_graph_launched_on_another_stream(backend):
+    """Products captured on one stream and replayed on another, between that one's own calls and without a wait: the graph has the
+    scratch and counters of the first stream, the calls those of the second."""
+    be, rows, cols = backend, 6144, 2048
+    rng = np.random.default_rng(31)
+    raw = ggml(rng, "q4_k", rows, cols)
+    w = be.create_q4_weights(raw, rows, cols, "q4_k")
+    sizes = (40, 400)  # pieces; pieces, partial sums and counters
+    xs = [[rng.standard_normal((n, cols)).astype(np.float32) for n in sizes] for _ in range(2)]
+    want = [[run(be, w, x) for x in pair] for pair in xs]
+    x = [[be.buffer(a) for a in pair] for pair in xs]
+    y = [[be.empty(n * rows * 4) for n in sizes] for _ in range(2)]
+
+    def step(i):
+        for a, b, n in zip(x[i], y[i], sizes):
+            be.matvec_q4(w, a, n, b)
+
+    streams = [HipStream(), HipStream()]
+    try:
+        be.set_stream(streams[0])
+        step(0)
+        be.sync()
+        g = be.capture(lambda: step(0))
+        be.set_stream(streams[1])
+        for rep in range(4):
+            step(1)
+            g.replay()
+            step(1)
+            be.sync()
+            for i in range(2):
+                for b, n, right in zip(y[i], sizes, want[i]):
+                    assert np.array_equal(b.download((n, rows)), right), (rep, i, n)
+                    b.upload(np.zeros((n, rows), np.float32))
+        g.destroy()
+    finally:
+        be.set_stream(None)
+        for s in streams:
+            s.destroy()
