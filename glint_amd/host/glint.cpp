@@ -747,7 +747,10 @@ namespace {
 struct Source {
     const gla_kv *kv = nullptr;
     bool paged = false;
-    size_t kv_dim = 0;
+    size_t n_kv_heads = 0, head_dim = 0, kv_dim = 0;
+    // The device reads rows of n_heads * head_dim as the storage has them, so a shape
+    // that only multiplies to its kv_dim would be staged in rows of another length.
+    bool fits(const AttnShape &s) const { return s.n_kv_heads == n_kv_heads && s.head_dim == head_dim; }
 };
 
 Result<Source> source_of(const std::vector<const KvStore *> &stores, const char *what) {
@@ -757,23 +760,25 @@ Result<Source> source_of(const std::vector<const KvStore *> &stores, const char 
         if (!s) return GlintError::gpu_shader_error(fmt("%s: cache %zu is null", what, i));
         const gla_kv *kv;
         bool paged;
-        size_t kv_dim;
+        size_t n_kv_heads, head_dim;
         if (const PagedKvCache *p = s->as_paged()) {
             kv = p->pool().store().device_kv();
             paged = true;
-            kv_dim = p->pool().kv_dim();
+            n_kv_heads = p->pool().store().n_kv_heads();
+            head_dim = p->pool().store().head_dim();
         } else if (const GpuKvBuffer *b = s->gpu_buffer()) {
             kv = b->kv;
             paged = false;
-            kv_dim = b->n_kv_heads * b->head_dim;
+            n_kv_heads = b->n_kv_heads;
+            head_dim = b->head_dim;
         } else {
             kv = nullptr;
             paged = false;
-            kv_dim = 0;
+            n_kv_heads = head_dim = 0;
         }
         if (!kv) return GlintError::gpu_shader_error(fmt("%s: cache %zu is not device-resident", what, i));
         if (i == 0) {
-            src = Source{kv, paged, kv_dim};
+            src = Source{kv, paged, n_kv_heads, head_dim, n_kv_heads * head_dim};
         } else if (kv != src.kv) {
             return GlintError::gpu_shader_error(fmt("%s: caches must share one device storage or page pool", what));
         }
@@ -793,8 +798,8 @@ Result<std::vector<float>> GpuBackend::decode_batch(const std::vector<DecodeSeq>
     Result<Source> src = source_of(stores, "decode_batch");
     if (!src) return src.error();
     const Source &S = src.value();
-    if (S.kv_dim != (size_t)shape.n_kv_heads * shape.head_dim)
-        return GlintError::gpu_shader_error("decode_batch: n_kv_heads * head_dim does not match the cache");
+    if (!S.fits(shape))
+        return GlintError::gpu_shader_error("decode_batch: n_kv_heads or head_dim does not match the cache");
     std::vector<int32_t> start(B), len(B), slot;
     std::vector<int32_t> table;
     int stride = 0;
@@ -873,8 +878,8 @@ Result<std::vector<float>> GpuBackend::prefill_batch(const std::vector<PrefillSe
     Result<Source> src = source_of(stores, "prefill_batch");
     if (!src) return src.error();
     const Source &S = src.value();
-    if (S.kv_dim != (size_t)shape.n_kv_heads * shape.head_dim)
-        return GlintError::gpu_shader_error("prefill_batch: n_kv_heads * head_dim does not match the cache");
+    if (!S.fits(shape))
+        return GlintError::gpu_shader_error("prefill_batch: n_kv_heads or head_dim does not match the cache");
     std::vector<int32_t> q_start(B + 1, 0), pos_off(B), slot, table;
     int stride = 0, max_q = 0;
     for (size_t b = 0; b < B; b++) {
@@ -1126,8 +1131,8 @@ Result<std::vector<float>> GpuBackend::append_batch(const std::vector<AppendSeq>
     Result<Source> src = source_of(stores, "append_batch");
     if (!src) return src.error();
     const Source &S = src.value();
-    if (S.kv_dim != (size_t)shape.n_kv_heads * shape.head_dim)
-        return GlintError::gpu_shader_error("append_batch: n_kv_heads * head_dim does not match the cache");
+    if (!S.fits(shape))
+        return GlintError::gpu_shader_error("append_batch: n_kv_heads or head_dim does not match the cache");
     std::vector<int32_t> q_start(B + 1, 0), pos_off(B), slot, table;
     int max_q = 0, stride = 1;
     for (size_t b = 0; b < B; b++) {

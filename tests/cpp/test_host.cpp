@@ -1129,6 +1129,33 @@ DEVICE_TEST(test_append_batch) {
     CHECK(!backend().append_batch({{&caches[0], 1, 0}, {&first, 1, 0}}, q.data(), k.data(), v.data(), 0, shape, nullptr).ok());
 }
 
+// Shapes that multiply to the cache's kv_dim but are not its heads: rows of another
+// length than the device reads. All three calls over a batch refuse them.
+DEVICE_TEST(test_shapes_that_only_multiply_to_the_caches) {
+    PagePool pool = backend().create_page_pool(4, N_KV_HEADS, HEAD_DIM).expect("pool");
+    PagedKvCache paged(pool, 1);
+    paged.reserve(4).expect("reserve");
+    auto caches = backend().create_kv_caches(1, 1, 16, N_KV_HEADS, HEAD_DIM).expect("caches");
+    Rng rng(0x5a9e);
+    const auto x = rng.normal(4 * 16 * HEAD_DIM);
+    for (KvStore *c : {static_cast<KvStore *>(&paged), static_cast<KvStore *>(&caches[0])}) {
+        for (const uint32_t by : {2u, 4u}) {
+            for (const bool narrow : {true, false}) {
+                const uint32_t n_kv = narrow ? (uint32_t)N_KV_HEADS * by : (uint32_t)N_KV_HEADS / 2;
+                const uint32_t d = narrow ? (uint32_t)HEAD_DIM / by : (uint32_t)HEAD_DIM * 2;
+                const AttnShape shape{n_kv, n_kv, d, 0.125f, 0.0f};
+                CHECK(!backend().append_batch({{c, 2, 0}}, x.data(), x.data(), x.data(), 0, shape, nullptr).ok());
+                CHECK(!backend().decode_batch({{c, 0, 2}}, x.data(), 0, shape).ok());
+                CHECK(!backend().prefill_batch({{c, 2, 0}}, x.data(), 0, shape).ok());
+            }
+        }
+        const AttnShape own{2 * (uint32_t)N_KV_HEADS, (uint32_t)N_KV_HEADS, (uint32_t)HEAD_DIM, 0.125f, 0.0f};
+        CHECK(backend().append_batch({{c, 2, 0}}, x.data(), x.data(), x.data(), 0, own, nullptr).ok());
+        CHECK(backend().decode_batch({{c, 0, 2}}, x.data(), 0, own).ok());
+        CHECK(backend().prefill_batch({{c, 2, 0}}, x.data(), 0, own).ok());
+    }
+}
+
 DEVICE_TEST(test_rope_rows_through_host_layer) {
     gla_rope_spec spec{};
     spec.head_dim = 6;
