@@ -646,7 +646,8 @@ class GpuBackend:
         """Upload GGML Q4_0 ("q4_0") or Q4_K ("q4_k") bytes (gla_q4w_create)."""
         code, group, size = _Q4_FORMATS[fmt]
         raw = np.ascontiguousarray(ggml, dtype=np.uint8).reshape(-1)
-        assert raw.size == rows * (cols // group) * size
+        if raw.size != rows * (cols // group) * size:
+            raise ValueError(f"{raw.size} bytes are no {rows} x {cols} matrix of {fmt}")
         h = C.c_void_p()
         check(_lib.lib().gla_q4w_create(self.ctx, code, _ptr(raw), rows, cols, C.byref(h)))
         return Q4Weights(self, h, rows, cols, fmt)
