@@ -5,6 +5,8 @@ import numpy as np
 import pytest
 
 from glint_amd import _lib
+from glint_amd.attn import HipStream
+from test_gpu_append import View
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +66,55 @@ def test_rows_that_meet_at_one_place(backend, dtype, n):
             each = [np.asarray(t[which]).view(np.uint8).reshape(len(every), -1) for t in want]
             assert np.array_equal(got[rest], each[0][rest])
             assert np.all((got == each[0]) | (got == each[1]) | (got == each[2]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "q8"])
+@pytest.mark.parametrize("lens", [[1, 1, 1, 1], [40, 0, 17, 1]])
+def test_captured_rotation_append_and_reading(backend, dtype, lens):
+    """gla_rope_rows, gla_kv_append into a page pool and gla_kv_read_rows in one graph, replayed on another stream than the plan
+    was made on, with new rows, positions and pages in between and eager calls beside: every replay has the eager bits."""
+    be, heads, n_kv, d, n = backend, 4, 2, 128, sum(lens)
+    rng = np.random.default_rng(n)
+    plan = be.create_rope_plan(d, layout="half", rot_dim=96)
+    s = HipStream()
+    try:
+        be.set_stream(s)
+        pages, stride, width = 40, 8, (heads + 2 * n_kv) * d
+        pools = [be.create_page_pool(pages, n_kv, d, dtype) for _ in range(2)]
+        starts = be.buffer(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+        row, table, past, pos, rows = (be.empty(4 * k) for k in (n * width, 4 * stride, 4, n, 2 * n))
+        outs = [[be.empty(4 * n * w) for w in (heads * d, heads * d, n_kv * d, n_kv * d)] for _ in range(2)]
+
+        def step(i):
+            turned, q, k, v = outs[i]
+            be.rope_rows(plan, row, n, heads, pos, out=turned, x_stride=width)
+            be.append(pools[i], View(row, heads * d), View(row, (heads + n_kv) * d), starts, past, 4, max(lens), rope=plan, q=row,
+                      q_out=q, n_heads=heads, k_stride=width, v_stride=width, q_stride=width, page_table=table, page_table_stride=stride)
+            pools[i].read_rows_device(rows, k, v, n)
+
+        def inputs():
+            t = rng.permutation(pages)[:4 * stride].astype(np.int32).reshape(4, stride)
+            p = rng.integers(0, stride * PAGE - max(lens) + 1, 4)
+            at = np.concatenate([np.arange(a, a + m) for a, m in zip(p, lens)])
+            owner = np.repeat(np.arange(4), lens)
+            row.upload(rng.standard_normal((n, width)).astype(np.float32))
+            table.upload(t), past.upload(p.astype(np.int32)), pos.upload(at.astype(np.int32))
+            rows.upload(t[owner, at // PAGE].astype(np.int64) * PAGE + at % PAGE)
+
+        inputs()
+        g = be.capture(lambda: step(1))
+        for rep in range(5):
+            inputs()
+            step(0)
+            g.replay()
+            be.sync()
+            for a, b, w in zip(*outs, (heads * d, heads * d, n_kv * d, n_kv * d)):
+                a, b = a.download((n, w)), b.download((n, w))
+                assert np.isfinite(a).all() and np.array_equal(a.view(np.uint32), b.view(np.uint32)), rep
+            assert np.array_equal(outs[0][0].download((n, heads * d)), outs[0][1].download((n, heads * d)))
+            for a, b in zip(*(p.export_rows(np.arange(pages * PAGE)) for p in pools)):
+                assert np.array_equal(a, b), rep
+        g.destroy()
+    finally:
+        be.set_stream(None)
+        s.destroy()
