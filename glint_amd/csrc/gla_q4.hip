@@ -155,7 +155,7 @@ __device__ __forceinline__ half8 nibbles_q4_0(uint32_t w) {
 // the binade above them), and the MFMA takes it so: Q4_K's A operands are integers, its
 // products 2^-24 of their value, which kUnscale takes back. A mask and a product a pair
 // of nibbles instead of a mask, a conversion and its constants: 14336 x 4096, 1 vector
-// 12.2 -> 10.2 us; 6144 x 4096, 1 vector 6.5 -> 6.1, 1,999 203 -> 198.
+// 12.2 -> 10.2 us; 6144 x 4096, 1 vector 6.5 -> 6.1, 1,999 vectors 2% less (194).
 constexpr float kUnscale = 0x1p24f;
 // Q4_K: n * (scale byte j of sc), at most 15 * 63; one 24-bit product for a pair
 __device__ __forceinline__ half8 nibbles_q4_k(uint32_t w, uint32_t sc, int j) {
@@ -174,8 +174,9 @@ __device__ __forceinline__ half4 minima(uint32_t mn) {
 }
 
 // x enters the products as two halves, hi = f16(x 2^s) and lo = f16(x 2^s - hi),
-// s bringing the largest finite |x| of a range into [2^13, 2^14): 22 bits of every
-// value whose size matters. A NaN is both its pieces. An infinity is its own hi piece (lo 0)
+// s bringing the largest finite |x| of a range into [2^13, 2^14): off by 2^-22 of x
+// (half a step of 11 bits, twice) or, where lo is subnormal, by 2^-25 and so 2^-38 of the
+// largest. A NaN is both its pieces. An infinity is its own hi piece (lo 0)
 // in Q4_0; in Q4_K, where a weight's nibble and minimum multiply x in sums of their own and
 // an infinity would end as inf - inf, it is 0 and infinite_terms adds its products.
 // The range's largest |x| is kept as bits, which order as the values do.
@@ -280,11 +281,14 @@ __device__ float infinite_terms(const Weights &w, const float *x, int row) {
 //   own: four minima of a row with the sums of x over the four groups (in pieces,
 //   scaled by 2^-5; the minima carry 2^5).
 // Columns past the vectors multiply what the first ones do, and their sums are not used:
-// zeros there cost 16 instructions a quad.
+// zeros there cost 16 instructions a quad. A chunk's weights are loaded for CH quads
+// whether or not the wave has so many: where columns are no multiple of 4,096 a wave
+// loads some of the next one's as well.
 // Bound: one chain of launch (2.7 us), loads from HBM, unpacking and the merge; the
 // vector unit is busy a third of it (about 85 instructions for 16 rows x 128 columns of
-// Q4_0, 100 of Q4_K). us: Q4_0 4096 x 4096, 1 / 2 / 4 / 8 vectors 4.3 / 4.5 / 5.5 / 7.2;
-// 14336 x 4096, 1 vector 10.8, Q4_K 10.2 (33 MB, 3.2 TB/s).
+// Q4_0, 100 of Q4_K). us: Q4_0 4096 x 4096, 1 / 2 / 4 / 8 vectors 4.3 / 4.6 / 5.5 / 7.2;
+// 4096 x 2048, 1 / 4 3.9 / 4.8; 5120 x 5120 8.0 / 9.9; 49152 x 576 15.8 / 23.8;
+// 14336 x 4096, 1 vector 10.9, Q4_K 10.3 (33 MB, 3.2 TB/s).
 constexpr int kFewWaves = 8;
 template <bool K, int NV, int RT, int CH>
 __global__ __launch_bounds__(kFewWaves * 64) void matvec_q4_few_kernel(const Weights w, const float *x, int n_vec, float *y) {
@@ -1068,11 +1072,12 @@ int launched(const char *what) {
 
 template <bool K, int NV>
 int launch_few(gla_ctx *ctx, const gla_q4w *w, const Weights &p, const float *x, int n, float *y) {
-    // Two row tiles a workgroup share the pieces of x where a tile each would be
-    // more than one workgroup per CU: 6144 x 4096 Q4_0, 4 vectors 7.5 us (one tile
-    // each: 10.3), 8 vectors 10.2 (14.4); below that one each is faster (4096 x
-    // 4096, 1 vector 4.5, two tiles 6.3). One vector, whose pieces are cheap, from
-    // three workgroups per CU on.
+    // Two row tiles a workgroup share the pieces of x where a tile each would be more
+    // than one workgroup per CU. us, two tiles / one: 6144 x 4096 Q4_0, 2 vectors
+    // 6.5 / 6.2, 4 7.4 / 9.1, 8 10.8 / 12.9; Q4_K 6.5 / 6.7, 7.8 / 10.1, 10.4 / 14.3.
+    // Below that one each is faster (4096 x 4096 Q4_0, 2 vectors 6.2 / 4.6). One vector,
+    // whose pieces are cheap, from three workgroups per CU on (6144 x 4096 6.0 / 5.7, Q4_K
+    // 6.5 / 6.2; 14336 x 4096 10.8 / 9.6, Q4_K 10.2 / 10.4).
     const auto go = [&](auto kernel, int tiles) {
         hipLaunchKernelGGL(kernel, dim3((w->n_tiles + tiles - 1) / tiles), dim3(kFewWaves * 64), 0, ctx->stream, p, x, n, y);
     };
@@ -1131,7 +1136,8 @@ struct Tile {
 };
 // The mid kernel's tiles, and its cost: rounds of a workgroup per CU, each the tile's
 // products and two for what comes before and after them. (A call of 4,096 columns
-// takes about 8 us + 1.33 a unit of cost, Q4_K 8 + 1.5.)
+// takes about 8 us + 1.33 a unit of cost, Q4_K 8 + 1.5. The two are fitted there: of
+// 16,384 columns they are half a unit, of 576 some fourteen.)
 constexpr int kMidCost = 34;
 constexpr Tile kMidTiles[] = {{1, 1}, {1, 2}, {1, 3}, {1, 4}, {2, 3}, {2, 4}, {4, 4}, {8, 4}};
 Tile mid_tile(const gla_ctx *ctx, const gla_q4w *w, int n, int64_t *cost) {
@@ -1294,9 +1300,12 @@ int gla_matvec_q4(gla_ctx *ctx, const gla_q4w *w, const float *x, int n_vec, flo
     const Weights p{w->quants, w->aux, w->super, w->rows, w->cols, w->n_tiles, w->n_quads};
     if (n_vec <= kFewVec) return few(ctx, w, p, x, n_vec, y);
     // The mid kernel's small tiles while their products are few, then the other's large
-    // ones (us, mid / many: Q4_0 4096 x 4096, 128 vectors 23.0 / 41.3, 512 53.8 / 57.1;
-    // 1024 x 4096, 1,500 54.4 / 56.7; Q4_K 6144 x 4096, 192 48.7 / 50.6, 320 62.0 / 55.1;
-    // 14336 x 4096, 64 34.6 / 38.8, 160 91.1 / 74.9).
+    // ones (us, mid / many: Q4_0 4096 x 4096, 128 vectors 22.6 / 41.6, 400 52.7 / 52.8, 512
+    // 53.5 / 57.7; 1024 x 4096, 1,500 54.4 / 56.7; Q4_K 6144 x 4096, 128 34.4 / 39.2, 192
+    // 48.1 / 51.1, 256 56.4 / 51.7, 320 61.8 / 55.1; 14336 x 4096, 64 34.6 / 38.8, 160 91.1 /
+    // 74.9; other widths: Q4_0 4096 x 16384, 64 40.4 / 113, 256 108 / 128, 512 194 / 175; 960
+    // x 576, 256 11.3 / 17.5, 1,024 17.1 / 19.9; 49152 x 576, 32 19.4 / 19.6, 64 28.1 / 20.5).
+    // The rule takes the slower one of Q4_K 6144 x 4096, 256, and 4096 x 16384, 512 vectors.
     int64_t cost;
     const Tile t = mid_tile(ctx, w, n_vec, &cost);
     if (cost <= kMidCost) return mid(ctx, w, p, x, n_vec, y, t);

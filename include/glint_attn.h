@@ -441,7 +441,7 @@ typedef struct gla_append_args {
     int64_t v_stride;
     const float *q;            /* device rows of [n_heads][head_dim], q_stride floats apart (0: dense), or NULL */
     int64_t q_stride;
-    float *q_out;              /* device [rows][n_heads][head_dim]; may be q where that is dense */
+    float *q_out;              /* device [rows][n_heads][head_dim]; q itself where that is dense, else apart from q, k and v */
     int n_heads;               /* of q */
 } gla_append_args;
 int gla_kv_append(gla_ctx *ctx, const gla_append_args *args);
