@@ -244,11 +244,12 @@ __device__ __forceinline__ void load_row(float (&e)[8], const float *row, int by
 // weight, as the definition has it: an infinity by the weight's sign, NaN for a weight of
 // 0 and for infinities of both signs. Only outputs of vectors that hold an infinity come
 // here. d * scale * nibble and dmin * minimum are exact in f32, so their difference is 0
-// where the weight is.
+// where the weight is. A walk through x by each output's thread: 6144 x 4096, 1 vector 6 ->
+// 105 us, 1,999 vectors with an infinity each 0.2 -> 21 ms.
 __device__ float infinite_terms(const Weights &w, const float *x, int row) {
     const int64_t tile = row >> 4, r = row & 15;
     float sum = 0.0f;
-    for (int c0 = 0; c0 < w.cols; c0 += 8) {
+    for (int c0 = 0; c0 < w.cols && sum == sum; c0 += 8) {  // a NaN stays one
         uint32_t any = 0;
 #pragma unroll
         for (int k = 0; k < 8; k++) any |= abs_bits(x[c0 + k]) == kInf ? 1u << k : 0u;
