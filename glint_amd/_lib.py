@@ -22,6 +22,7 @@ GLA_ERR_POOL_EXHAUSTED = -6
 
 GLA_PAGE_SIZE = 16
 GLA_DECODE_NOALLOC_SCRATCH_BYTES = 16 << 20
+GLA_BLOCK_NORM_MAX_DIM = 16384
 GLA_KV_F32 = 0
 GLA_KV_Q8_0 = 1
 GLA_PREC_F32 = 0
@@ -94,6 +95,41 @@ class PrefillArgs(C.Structure):
         ("precision", C.c_int),
         ("q", C.c_void_p),
         ("out", C.c_void_p),
+    ]
+
+
+class DecodeSharedArgs(C.Structure):
+    _fields_ = [
+        ("decode", DecodeArgs),
+        ("n_groups", C.c_int),
+        ("group_start", C.c_void_p),
+        ("prefix_len", C.c_void_p),
+        ("max_group", C.c_int),
+        ("max_prefix_len", C.c_int),
+        ("max_own_len", C.c_int),
+        ("group_start_host", C.c_void_p),
+        ("prefix_len_host", C.c_void_p),
+    ]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = [
+        ("n_rows", C.c_int),
+        ("dim", C.c_int),
+        ("eps", C.c_float),
+        ("scale", C.c_float),
+        ("x", C.c_void_p),
+        ("x_stride", C.c_int64),
+        ("y", C.c_void_p),
+        ("y_stride", C.c_int64),
+        ("post", C.c_void_p),
+        ("gate", C.c_void_p),
+        ("gate_stride", C.c_int64),
+        ("pre", C.c_void_p),
+        ("x_out", C.c_void_p),
+        ("x_out_stride", C.c_int64),
+        ("norm_out", C.c_void_p),
+        ("norm_out_stride", C.c_int64),
     ]
 
 
@@ -172,6 +208,10 @@ SIGNATURES = {
     "gla_window_start": (_L, [_L, _L, _I, _I]),
     "gla_decode": (_I, [_P, C.POINTER(DecodeArgs)]),
     "gla_decode_noalloc": (_I, [_P, C.POINTER(DecodeArgs)]),
+    "gla_decode_sinks": (_I, [_P, C.POINTER(DecodeArgs), _I]),
+    "gla_decode_shared": (_I, [_P, C.POINTER(DecodeSharedArgs)]),
+    "gla_prefill_sinks": (_I, [_P, C.POINTER(PrefillArgs), _I]),
+    "gla_block_norm": (_I, [_P, C.POINTER(BlockNormArgs)]),
     "gla_prefill": (_I, [_P, C.POINTER(PrefillArgs)]),
     "gla_attention": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _F, _F, _P]),
     "gla_attention_resident": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P]),

@@ -532,11 +532,26 @@ class GpuBackend:
                softcap: Optional[float] = None, layer: int = 0, seq_slot: Optional[DeviceBuffer] = None,
                page_table: Optional[DeviceBuffer] = None, page_table_stride: int = 0,
                kv_start_host: Optional[np.ndarray] = None, kv_len_host: Optional[np.ndarray] = None,
-               noalloc: bool = False) -> None:
+               noalloc: bool = False, n_sinks: int = 0) -> None:
         """gla_decode on device buffers (asynchronous on the backend's stream). kv_start_host /
         kv_len_host: optional host copies of the device arrays (int32[B]); they let the library
         size the launch to the real lengths. noalloc: call gla_decode_noalloc (partials in the
-        library's static per-GPU scratch; nothing is allocated)."""
+        library's static per-GPU scratch; nothing is allocated). n_sinks: call gla_decode_sinks
+        (the first n_sinks positions stay visible beside the window; not with noalloc)."""
+        if noalloc and n_sinks:
+            raise ValueError("noalloc takes no sinks")
+        a, _hosts = self._decode_args(kv, q, out, kv_start, kv_len, n_seqs, max_kv_len, n_heads, scale, softcap, layer,
+                                      seq_slot, page_table, page_table_stride, kv_start_host, kv_len_host)
+        if n_sinks:
+            check(_lib.lib().gla_decode_sinks(self.ctx, C.byref(a), n_sinks))
+            return
+        fn = _lib.lib().gla_decode_noalloc if noalloc else _lib.lib().gla_decode
+        check(fn(self.ctx, C.byref(a)))
+
+    @staticmethod
+    def _decode_args(kv, q, out, kv_start, kv_len, n_seqs, max_kv_len, n_heads, scale, softcap, layer, seq_slot, page_table,
+                     page_table_stride, kv_start_host, kv_len_host):
+        """gla_decode_args, and the host arrays that have to outlive the call."""
         a = _lib.DecodeArgs()
         a.kv = kv.handle
         a.layer = layer
@@ -554,6 +569,7 @@ class GpuBackend:
         a.out = out.ptr
         if (kv_start_host is None) != (kv_len_host is None):
             raise ValueError("pass both kv_start_host and kv_len_host, or neither")
+        hosts = ()
         if kv_start_host is not None:
             hs = np.ascontiguousarray(kv_start_host, dtype=np.int32)
             hl = np.ascontiguousarray(kv_len_host, dtype=np.int32)
@@ -561,15 +577,58 @@ class GpuBackend:
                 raise ValueError("kv_start_host / kv_len_host must be int32[n_seqs]")
             a.kv_start_host = hs.ctypes.data
             a.kv_len_host = hl.ctypes.data
-        fn = _lib.lib().gla_decode_noalloc if noalloc else _lib.lib().gla_decode
-        check(fn(self.ctx, C.byref(a)))
+            hosts = (hs, hl)
+        return a, hosts
+
+    def decode_shared(self, kv: _KvBase, q: DeviceBuffer, out: DeviceBuffer, kv_start: DeviceBuffer,
+                      kv_len: DeviceBuffer, n_seqs: int, max_kv_len: int, n_heads: int, scale: float,
+                      group_start: DeviceBuffer, prefix_len: DeviceBuffer, n_groups: int, max_group: int,
+                      max_prefix_len: int, max_own_len: int, softcap: Optional[float] = None, layer: int = 0,
+                      seq_slot: Optional[DeviceBuffer] = None, page_table: Optional[DeviceBuffer] = None,
+                      page_table_stride: int = 0, kv_start_host: Optional[np.ndarray] = None,
+                      kv_len_host: Optional[np.ndarray] = None, group_start_host: Optional[np.ndarray] = None,
+                      prefix_len_host: Optional[np.ndarray] = None) -> None:
+        """gla_decode_shared on device buffers (asynchronous on the backend's stream): decode's arguments, then the
+        groups of rows that begin with the same positions, and their bounds."""
+        if (group_start_host is None) != (prefix_len_host is None):
+            raise ValueError("pass both group_start_host and prefix_len_host, or neither")
+        s = _lib.DecodeSharedArgs()
+        s.decode, _hosts = self._decode_args(kv, q, out, kv_start, kv_len, n_seqs, max_kv_len, n_heads, scale, softcap,
+                                             layer, seq_slot, page_table, page_table_stride, kv_start_host, kv_len_host)
+        s.n_groups = n_groups
+        s.group_start, s.prefix_len = group_start.ptr, prefix_len.ptr
+        s.max_group, s.max_prefix_len, s.max_own_len = max_group, max_prefix_len, max_own_len
+        if group_start_host is not None:
+            hg = np.ascontiguousarray(group_start_host, dtype=np.int32)
+            hp = np.ascontiguousarray(prefix_len_host, dtype=np.int32)
+            if hg.shape != (n_groups + 1,) or hp.shape != (n_groups,):
+                raise ValueError("group_start_host / prefix_len_host must be int32[n_groups + 1] / int32[n_groups]")
+            s.group_start_host, s.prefix_len_host = hg.ctypes.data, hp.ctypes.data
+        check(_lib.lib().gla_decode_shared(self.ctx, C.byref(s)))
+
+    def block_norm(self, x: DeviceBuffer, n_rows: int, dim: int, eps: float, y: Optional[DeviceBuffer] = None,
+                   post: Optional[DeviceBuffer] = None, gate: Optional[DeviceBuffer] = None, scale: float = 1.0,
+                   x_out: Optional[DeviceBuffer] = None, pre: Optional[DeviceBuffer] = None,
+                   norm_out: Optional[DeviceBuffer] = None, x_stride: int = 0, y_stride: int = 0, gate_stride: int = 0,
+                   x_out_stride: int = 0, norm_out_stride: int = 0) -> None:
+        """gla_block_norm on device rows: x_out = x + scale * gate * (y normed by post), norm_out = x_out normed by pre
+        (asynchronous on the backend's stream)."""
+        a = _lib.BlockNormArgs()
+        a.n_rows, a.dim, a.eps, a.scale = n_rows, dim, float(eps), float(scale)
+        for name, buf in (("x", x), ("y", y), ("post", post), ("gate", gate), ("pre", pre), ("x_out", x_out),
+                          ("norm_out", norm_out)):
+            setattr(a, name, buf.ptr if buf is not None else None)
+        a.x_stride, a.y_stride, a.gate_stride = x_stride, y_stride, gate_stride
+        a.x_out_stride, a.norm_out_stride = x_out_stride, norm_out_stride
+        check(_lib.lib().gla_block_norm(self.ctx, C.byref(a)))
 
     def prefill(self, kv: _KvBase, q: DeviceBuffer, out: DeviceBuffer, q_start: DeviceBuffer,
                 pos_offset: DeviceBuffer, n_seqs: int, max_q_len: int, n_heads: int, scale: float,
                 softcap: Optional[float] = None, sliding_window: Optional[int] = None, layer: int = 0,
                 seq_slot: Optional[DeviceBuffer] = None, page_table: Optional[DeviceBuffer] = None,
-                page_table_stride: int = 0, precision: str = "f32") -> None:
-        """gla_prefill on device buffers (asynchronous on the backend's stream)."""
+                page_table_stride: int = 0, precision: str = "f32", n_sinks: int = 0) -> None:
+        """gla_prefill on device buffers (asynchronous on the backend's stream); with n_sinks gla_prefill_sinks (the
+        first n_sinks positions stay visible beside the window)."""
         a = _lib.PrefillArgs()
         a.kv = kv.handle
         a.layer = layer
@@ -587,7 +646,10 @@ class GpuBackend:
         a.precision = {"f32": _lib.GLA_PREC_F32, "bf16": _lib.GLA_PREC_BF16}[precision]
         a.q = q.ptr
         a.out = out.ptr
-        check(_lib.lib().gla_prefill(self.ctx, C.byref(a)))
+        if n_sinks:
+            check(_lib.lib().gla_prefill_sinks(self.ctx, C.byref(a), n_sinks))
+        else:
+            check(_lib.lib().gla_prefill(self.ctx, C.byref(a)))
 
     def rope(self, x: DeviceBuffer, n_rows: int, n_heads: int, head_dim: int, pos: DeviceBuffer, freq_base: float,
              scaling_factor: float = 1.0, rot_dim: Optional[int] = None) -> None:

@@ -9,6 +9,7 @@ Outputs (in-tree, git-ignored, shipped with the tree to the GPU box):
     glint_amd/libglint_probe.so   achievable-peak probes for bench.py (stream read, MFMA loops)
     glint_amd/libglint_host.so    C++ host layer over the C ABI (glint_amd/host/glint.hpp)
     glint_amd/_build/test_host    its test program (tests/cpp/test_host.cpp; run by tests/test_host_cpp.py)
+    glint_amd/_build/test_pages   the page rules of windows, on the host (tests/cpp/test_pages.hip)
     oracle/liboracle.so           CPU oracle, built by oracle/Makefile (tests only)
 """
 from __future__ import annotations
@@ -28,6 +29,7 @@ SYNTH_LIB = PKG / "libglint_synth.so"
 PROBE_LIB = PKG / "libglint_probe.so"
 HOST_LIB = PKG / "libglint_host.so"
 HOST_TEST = BUILD / "test_host"
+PAGES_TEST = BUILD / "test_pages"
 ORACLE_DIR = ROOT / "oracle"
 ORACLE_LIB = ORACLE_DIR / "liboracle.so"
 
@@ -48,7 +50,7 @@ HIP_FLAGS = [
     f"-I{ROOT / 'include'}",
 ]
 HIP_SOURCES = ["gla_capi.hip", "gla_kvstore.hip", "gla_decode.hip", "gla_decode_q8.hip", "gla_prefill.hip",
-               "gla_ops.hip", "gla_rope.hip", "gla_q4.hip"]
+               "gla_prefill_sinks.hip", "gla_norm.hip", "gla_ops.hip", "gla_rope.hip", "gla_q4.hip"]
 
 
 def _run(cmd: list[str], cwd: Path | None = None) -> None:
@@ -101,6 +103,14 @@ def build_host_tests() -> Path:
     return HOST_TEST
 
 
+def build_pages_test() -> Path:
+    BUILD.mkdir(exist_ok=True)
+    tmp = PAGES_TEST.with_suffix(".tmp")
+    _run([HIPCC, *HIP_FLAGS, "--cuda-host-only", str(ROOT / "tests" / "cpp" / "test_pages.hip"), "-o", str(tmp)])
+    os.replace(tmp, PAGES_TEST)
+    return PAGES_TEST
+
+
 def build_synth() -> Path:
     tmp = SYNTH_LIB.with_suffix(".so.tmp")
     _run(["gcc", "-O2", "-fPIC", "-shared", "-std=c11", "-Wall", "-o", str(tmp), str(CSRC / "synth.c"),
@@ -121,6 +131,7 @@ def build_all(jobs: int = 4) -> None:
     build_probe()
     build_host()
     build_host_tests()
+    build_pages_test()
 
 
 if __name__ == "__main__":

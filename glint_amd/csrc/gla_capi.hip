@@ -759,18 +759,64 @@ int gla_decode_noalloc(gla_ctx *ctx, const gla_decode_args *a) {
     GLA_GUARD_END
 }
 
-int gla_prefill(gla_ctx *ctx, const gla_prefill_args *a) {
+int gla_decode_sinks(gla_ctx *ctx, const gla_decode_args *a, int n_sinks) {
     GLA_GUARD_BEGIN
-    GLA_REQUIRE(ctx && a && a->kv, "gla_prefill: NULL argument");
+    DecodeLaunch d;
+    bool nothing = false;
+    GLA_REQUIRE(n_sinks >= 0, "gla_decode_sinks: n_sinks < 0");
+    int rc = decode_launch_of(ctx, a, "gla_decode_sinks", &d, &nothing);
+    if (rc != GLA_OK || nothing) return rc;
+    d.n_sinks = n_sinks;
+    return launch_decode(ctx, d);
+    GLA_GUARD_END
+}
+
+int gla_decode_shared(gla_ctx *ctx, const gla_decode_shared_args *a) {
+    GLA_GUARD_BEGIN
+    const char *fn = "gla_decode_shared";
+    GLA_REQUIRE(ctx && a, "%s: NULL argument", fn);
+    DecodeLaunch d;
+    bool nothing = false;
+    int rc = decode_launch_of(ctx, &a->decode, fn, &d, &nothing);
+    if (rc != GLA_OK || nothing) return rc;
+    GLA_REQUIRE(a->n_groups >= 0 && a->n_groups <= d.n_seqs, "%s: n_groups %d is not in 0 .. n_seqs", fn, a->n_groups);
+    GLA_REQUIRE(a->n_groups == 0 || (a->group_start && a->prefix_len), "%s: NULL buffer", fn);
+    GLA_REQUIRE(a->max_group >= 0 && a->max_prefix_len >= 0 && a->max_own_len >= 0, "%s: a bound is negative", fn);
+    GLA_REQUIRE((a->group_start_host == nullptr) == (a->prefix_len_host == nullptr) &&
+                    (!a->group_start_host || d.kv_len_host),
+                "%s: pass group_start_host and prefix_len_host together, beside the windows' host copies", fn);
+    if (a->group_start_host) {
+        const int32_t *at = a->group_start_host, *len = a->prefix_len_host;
+        for (int g = 0; g < a->n_groups; g++) {
+            GLA_REQUIRE(at[g] >= 0 && at[g] <= at[g + 1] && at[g + 1] <= d.n_seqs && at[g + 1] - at[g] <= a->max_group,
+                        "%s: group %d has rows %d .. %d of %d, at most %d", fn, g, at[g], at[g + 1], d.n_seqs,
+                        a->max_group);
+            GLA_REQUIRE(len[g] >= 0 && len[g] <= a->max_prefix_len, "%s: group %d shares %d positions, not 0 .. %d", fn,
+                        g, len[g], a->max_prefix_len);
+        }
+        for (int b = 0, g = 0; b < d.n_seqs; b++) {
+            while (g < a->n_groups && at[g + 1] <= b) g++;
+            const int prefix = g < a->n_groups && at[g] <= b ? len[g] : 0;
+            const int64_t mine = (int64_t)d.kv_start_host[b] + d.kv_len_host[b] - prefix;
+            GLA_REQUIRE(mine <= a->max_own_len, "%s: row %d has %lld positions of its own, more than max_own_len %d", fn,
+                        b, (long long)mine, a->max_own_len);
+        }
+    }
+    return launch_decode(ctx, d);
+    GLA_GUARD_END
+}
+
+static int prefill_of(gla_ctx *ctx, const gla_prefill_args *a, const char *fn, int n_sinks) {
+    GLA_REQUIRE(ctx && a && a->kv, "%s: NULL argument", fn);
     const gla_kv *kv = a->kv;
-    if (int rc = check_owner(ctx, kv, "gla_prefill")) return rc;
-    GLA_REQUIRE(a->n_seqs >= 0, "gla_prefill: n_seqs < 0");
+    if (int rc = check_owner(ctx, kv, fn)) return rc;
+    GLA_REQUIRE(a->n_seqs >= 0, "%s: n_seqs < 0", fn);
     if (a->n_seqs == 0 || a->max_q_len == 0) return GLA_OK;
-    GLA_REQUIRE(a->q && a->out && a->q_start && a->pos_offset, "gla_prefill: NULL buffer");
-    GLA_REQUIRE(a->max_q_len > 0, "gla_prefill: max_q_len < 0");
+    GLA_REQUIRE(a->q && a->out && a->q_start && a->pos_offset, "%s: NULL buffer", fn);
+    GLA_REQUIRE(a->max_q_len > 0, "%s: max_q_len < 0", fn);
     GLA_REQUIRE(a->n_heads > 0 && a->n_heads % kv->n_kv_heads == 0,
-                "gla_prefill: n_heads %d is not a multiple of n_kv_heads %d", a->n_heads, kv->n_kv_heads);
-    GLA_REQUIRE(a->precision == GLA_PREC_F32 || a->precision == GLA_PREC_BF16, "gla_prefill: bad precision");
+                "%s: n_heads %d is not a multiple of n_kv_heads %d", fn, a->n_heads, kv->n_kv_heads);
+    GLA_REQUIRE(a->precision == GLA_PREC_F32 || a->precision == GLA_PREC_BF16, "%s: bad precision", fn);
     PrefillLaunch p;
     int rc = page_map_of(kv, a->layer, a->seq_slot, a->page_table, a->page_table_stride, &p.pm);
     if (rc != GLA_OK) return rc;
@@ -789,8 +835,22 @@ int gla_prefill(gla_ctx *ctx, const gla_prefill_args *a) {
     p.precision = a->precision;
     p.q = a->q;
     p.out = a->out;
+    // (without a window every row sees them already)
+    p.n_sinks = a->sliding_window > 0 ? n_sinks : 0;
     GLA_CHECK_HIP(hipSetDevice(ctx->device), GLA_ERR_DEVICE);
-    return launch_prefill(ctx, p);
+    return p.n_sinks > 0 ? launch_prefill_sinks(ctx, p) : launch_prefill(ctx, p);
+}
+
+int gla_prefill(gla_ctx *ctx, const gla_prefill_args *a) {
+    GLA_GUARD_BEGIN
+    return prefill_of(ctx, a, "gla_prefill", 0);
+    GLA_GUARD_END
+}
+
+int gla_prefill_sinks(gla_ctx *ctx, const gla_prefill_args *a, int n_sinks) {
+    GLA_GUARD_BEGIN
+    GLA_REQUIRE(n_sinks >= 0, "gla_prefill_sinks: n_sinks < 0");
+    return prefill_of(ctx, a, "gla_prefill_sinks", n_sinks);
     GLA_GUARD_END
 }
 

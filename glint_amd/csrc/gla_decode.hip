@@ -71,6 +71,7 @@ struct DecodeParams {
     // decode_combine_kernel.
     int merge_pages;
     int32_t *arrivals;
+    int n_sinks;  // SINKS kernels: first positions seen beside the window
 };
 
 // Sum over the 8 lanes of an aligned lane group (DPP: quad xor1, quad xor2,
@@ -150,11 +151,23 @@ struct SeqRange {
     int n_pages;
     int pps;         // pages per split
     int n_splits;
+    Visible v;       // SINKS kernels (fp is 0: pages are numbered as Visible does)
 };
 
+template <bool SINKS>
 __device__ __forceinline__ SeqRange seq_range(const DecodeParams &p, int b) {
     SeqRange r;
     int s = p.kv_start[b];
+    if constexpr (SINKS) {
+        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, p.n_sinks, 0);
+        r.start = r.v.start;
+        r.end = r.v.end;
+        r.fp = 0;
+        r.n_pages = r.v.n_pages;
+        r.pps = p.pps_fixed > 0 ? p.pps_fixed : split_pages(r.n_pages);
+        r.n_splits = min((r.n_pages + r.pps - 1) / r.pps, p.max_splits);
+        return r;
+    }
     int len = p.kv_len[b];
     s = s < 0 ? 0 : s;
     len = len < 0 ? 0 : (len > p.max_len ? p.max_len : len);
@@ -250,7 +263,7 @@ __device__ __forceinline__ void merge_splits_agent(const DecodeParams &p, int64_
     }
 }
 
-template <int D, int GT, int NSTEP, bool CAP>
+template <int D, int GT, int NSTEP, bool CAP, bool SINKS>
 __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodeParams p) {
     constexpr int EPL = D / 8;       // elements per lane
     constexpr int EPC = 4;           // floats per 16-byte chunk
@@ -271,7 +284,7 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
     const int gcount = min(GT, p.group - g0);
     const int h_base = kvh * p.group + g0;
 
-    const SeqRange r = seq_range(p, b);
+    const SeqRange r = seq_range<SINKS>(p, b);
     const int tid = threadIdx.x;
     if (r.n_pages == 0) {  // empty window: zero output (the reference's pre-zeroed buffer)
         if (split == 0)
@@ -320,13 +333,16 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
         bool valid[NSTEP];
         int64_t pid[PPW];
 #pragma unroll
-        for (int j = 0; j < PPW; j++) pid[j] = map_page(p.pm, b, (pb + j < pg1) ? pb + j : pb);
+        for (int j = 0; j < PPW; j++) {
+            const int pg = (pb + j < pg1) ? pb + j : pb;
+            pid[j] = map_page(p.pm, b, SINKS ? r.v.page(pg) : pg);
+        }
 #pragma unroll
         for (int s = 0; s < NSTEP; s++) {
             const int page = pb + s / 2;
             const int slot = (s & 1) * 8 + tg;
-            const int pos = page * 16 + slot;
-            valid[s] = page < pg1 && pos >= r.start && pos < r.end;
+            const int pos = (SINKS ? r.v.page(page) : page) * 16 + slot;
+            valid[s] = page < pg1 && (SINKS ? r.v.sees(pos) : pos >= r.start && pos < r.end);
             const int64_t base = pid[s / 2] * p.kv.page_stride + head_off + (int64_t)slot * p.kv.row_stride;
             const uint8_t *kp = p.kv.k + base;
             const uint8_t *vp = p.kv.v + base;
@@ -516,7 +532,7 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
 // group, q-head g = blockIdx.x). A row of D floats is read by D/4 lanes as
 // float4; the 256 threads form 256/(D/4) split groups that take every
 // NSG-th split, four splits in flight at a time, and are merged through LDS.
-template <int D, int GT>
+template <int D, int GT, bool SINKS>
 __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const DecodeParams p) {
     constexpr int RL = D / 4;             // lanes per row
     constexpr int NSG = kThreads / RL;    // split groups
@@ -530,7 +546,7 @@ __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const DecodePa
     const int g = blockIdx.x;
     const int gcount = min(GT, p.group - hg * GT);
     if (g >= gcount) return;
-    const SeqRange r = seq_range(p, b);
+    const SeqRange r = seq_range<SINKS>(p, b);
     if (r.n_splits <= 1 || r.n_pages <= p.merge_pages) return;  // (one split, or merged in the split kernel)
     const int sg = threadIdx.x / RL;
     const int e4 = threadIdx.x - sg * RL;
@@ -607,24 +623,30 @@ __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const DecodePa
         make_float4(AA.x * inv, AA.y * inv, AA.z * inv, AA.w * inv);
 }
 
-template <int D, int GT>
-int launch_typed(gla_ctx *ctx, const DecodeParams &prm, dim3 grid, bool combine) {
+template <int D, int GT, bool SINKS>
+int launch_as(gla_ctx *ctx, const DecodeParams &prm, dim3 grid, bool combine) {
     if (prm.softcap > 0.0f)
-        hipLaunchKernelGGL((decode_split_kernel<D, GT, kStepsPerIter, true>), grid, dim3(kThreads), 0, ctx->stream,
-                           prm);
+        hipLaunchKernelGGL((decode_split_kernel<D, GT, kStepsPerIter, true, SINKS>), grid, dim3(kThreads), 0,
+                           ctx->stream, prm);
     else
-        hipLaunchKernelGGL((decode_split_kernel<D, GT, kStepsPerIter, false>), grid, dim3(kThreads), 0, ctx->stream,
-                           prm);
+        hipLaunchKernelGGL((decode_split_kernel<D, GT, kStepsPerIter, false, SINKS>), grid, dim3(kThreads), 0,
+                           ctx->stream, prm);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "decode_split_kernel launch: %s", hipGetErrorString(e));
     if (combine) {
-        hipLaunchKernelGGL((decode_combine_kernel<D, GT>), dim3(GT, grid.x, grid.z), dim3(kThreads), 0, ctx->stream,
-                           prm);
+        hipLaunchKernelGGL((decode_combine_kernel<D, GT, SINKS>), dim3(GT, grid.x, grid.z), dim3(kThreads), 0,
+                           ctx->stream, prm);
         e = hipGetLastError();
         if (e != hipSuccess)
             return set_error(GLA_ERR_KERNEL, "decode_combine_kernel launch: %s", hipGetErrorString(e));
     }
     return GLA_OK;
+}
+
+template <int D, int GT>
+int launch_typed(gla_ctx *ctx, const DecodeParams &prm, dim3 grid, bool combine) {
+    return prm.n_sinks > 0 ? launch_as<D, GT, true>(ctx, prm, grid, combine)
+                           : launch_as<D, GT, false>(ctx, prm, grid, combine);
 }
 
 // Head-group width: the registers of a lane hold GT*(D/8) q values and as
@@ -666,8 +688,8 @@ int launch_decode(gla_ctx *ctx, const DecodeLaunch &d) {
     const int gt = pick_gt(D, group);
     const int n_hg = (group + gt - 1) / gt;
 
-    // pages a window can span (a start inside a page adds one)
-    const int max_pages = d.max_kv_len > 0 ? (d.max_kv_len + GLA_PAGE_SIZE - 1) / GLA_PAGE_SIZE + 1 : 1;
+    // pages a window can span (a start inside a page adds one), and its sinks'
+    const int max_pages = max_window_pages(d);
     const int64_t units = (int64_t)d.n_seqs * d.n_kv_heads * n_hg;
     // Split sizes come from each window alone (split_pages); GLA_DECODE_PPS
     // forces one size for every window (tuning only).
@@ -702,12 +724,13 @@ int launch_decode(gla_ctx *ctx, const DecodeLaunch &d) {
     if (const char *env = getenv("GLA_DECODE_MERGE_PAGES")) merge_pages = std::max(0, atoi(env));
     prm.merge_pages = merge_pages;
     prm.arrivals = nullptr;
+    prm.n_sinks = d.n_sinks;
     // Which merges the launch needs: exact from the host lengths, else from
     // the max_kv_len bound.
     bool any_short = false, any_long = false;
     if (d.kv_len_host) {
         for (int b = 0; b < d.n_seqs; b++) {
-            const int n = host_seq_pages(d.kv_start_host[b], d.kv_len_host[b], d.max_kv_len, d.pm.pos_limit);
+            const int n = host_pages(d, b);
             const int pps = pps_fixed > 0 ? pps_fixed : split_pages(n);
             if (std::min((n + pps - 1) / pps, max_splits) <= 1) continue;
             if (n <= merge_pages)

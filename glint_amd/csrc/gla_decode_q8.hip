@@ -100,6 +100,7 @@ struct Q8Params {
     // past a sequence's end (n_rows > 0; grid (units, n_rows, 1)). Else
     // n_rows = 0 and the grid is (units, max_wg, n_seqs).
     int n_rows;
+    int n_sinks;  // SINKS kernels: first positions seen beside the window
     uint16_t rows[kMaxRows];
 };
 
@@ -107,11 +108,21 @@ struct Range {
     int start, end;  // positions [start, end)
     int fp;          // first logical page
     int n_pages;
+    Visible v;       // SINKS kernels (fp is 0: pages are numbered as Visible does)
 };
 
+template <bool SINKS>
 __device__ __forceinline__ Range seq_range(const Q8Params &p, int b) {
     Range r;
     int s = p.kv_start[b];
+    if constexpr (SINKS) {
+        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, p.n_sinks, 0);
+        r.start = r.v.start;
+        r.end = r.v.end;
+        r.fp = 0;
+        r.n_pages = r.v.n_pages;
+        return r;
+    }
     int len = p.kv_len[b];
     s = s < 0 ? 0 : s;
     len = len < 0 ? 0 : (len > p.max_len ? p.max_len : len);
@@ -444,6 +455,7 @@ struct StepConst {
     float sm, kvs, softcap, qcap;
     bool cap;
     int pg0, npg, start, end;
+    Visible v;  // SINKS kernels
     int kg, ph;
     float pf;  // this lane's piece (0: hi, 1: lo) as a float
 };
@@ -459,7 +471,7 @@ struct StepState {
 // head): S = K.Q, the soft-cap, the window mask and the online softmax.
 // Leaves in pr the probabilities of the lane's four P' positions and in
 // vbad the positions whose V scale must be ignored (bit i).
-template <int D>
+template <int D, bool SINKS>
 __device__ __forceinline__ void step_qk(const RawK<D> &cur, int step, const StepConst<D> &c, StepState<D> &st,
                                         float (&pr)[4], int &vbad) {
     constexpr int NB = D / 32;
@@ -505,18 +517,34 @@ __device__ __forceinline__ void step_qk(const RawK<D> &cur, int step, const Step
     // on the lane's own page, are flagged so that their V scale is zeroed and
     // a non-finite scale of an unused position cannot reach the output.
     vbad = 0;
-    const int sp = (c.pg0 + 2 * step) * 16;             // first position of the step
-    const int lim1 = min(c.end, (c.pg0 + c.npg) * 16);  // page 1 of the step may be past the chunk
-    if (sp < c.start || sp + 32 > lim1) {
-        const int pos0 = sp + c.kg * 4;
+    if constexpr (SINKS) {
+        const int pa = c.v.page(c.pg0 + 2 * step), pb = c.v.page(c.pg0 + 2 * step + 1);
+        const bool two = 2 * step + 1 < c.npg;  // (else page 1 repeats page 0's data)
+        if (!(c.v.whole(pa) && two && c.v.whole(pb))) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const bool ok0 = pos0 + i >= c.start && pos0 + i < c.end;
-            const bool ok1 = pos0 + 16 + i >= c.start && pos0 + 16 + i < lim1;
-            s0[i] = ok0 ? s0[i] : -INFINITY;
-            s1[i] = ok1 ? s1[i] : -INFINITY;
-            const bool ok = c.ph ? ok1 : ok0;
-            vbad |= ok ? 0 : (1 << i);
+            for (int i = 0; i < 4; i++) {
+                const bool ok0 = c.v.sees(pa * 16 + c.kg * 4 + i);
+                const bool ok1 = two && c.v.sees(pb * 16 + c.kg * 4 + i);
+                s0[i] = ok0 ? s0[i] : -INFINITY;
+                s1[i] = ok1 ? s1[i] : -INFINITY;
+                const bool ok = c.ph ? ok1 : ok0;
+                vbad |= ok ? 0 : (1 << i);
+            }
+        }
+    } else {
+        const int sp = (c.pg0 + 2 * step) * 16;             // first position of the step
+        const int lim1 = min(c.end, (c.pg0 + c.npg) * 16);  // page 1 of the step may be past the chunk
+        if (sp < c.start || sp + 32 > lim1) {
+            const int pos0 = sp + c.kg * 4;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool ok0 = pos0 + i >= c.start && pos0 + i < c.end;
+                const bool ok1 = pos0 + 16 + i >= c.start && pos0 + 16 + i < lim1;
+                s0[i] = ok0 ? s0[i] : -INFINITY;
+                s1[i] = ok1 ? s1[i] : -INFINITY;
+                const bool ok = c.ph ? ok1 : ok0;
+                vbad |= ok ? 0 : (1 << i);
+            }
         }
     }
     const float tmax = max_rows(fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])),
@@ -584,7 +612,7 @@ __device__ __forceinline__ void step_pv(RawV<D> &cur, const StepConst<D> &c, Ste
 // One wave's chunk: flash attention of the group's q-heads over `ch` pages;
 // leaves O (unnormalised, true scale), m and l of each head at the start of
 // the wave's LDS slot ([kGT][D + 2] floats).
-template <int D>
+template <int D, bool SINKS>
 __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, int b, int kvh, int h_base,
                                            int gcount, int pg0, int npg, int lane, uint8_t *slot) {
     constexpr int NB = D / 32;  // Q8_0 blocks per head row
@@ -609,9 +637,17 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
         }
     }
     // physical page of chunk page `lane` (clamped into the pool by map_page)
-    const int pid_l = p.pm.page_table && p.pm.pt_stride >= 16
-                          ? chunk_ids_scalar(p.pm, b, pg0, npg, lane)
-                          : (int)map_page(p.pm, b, pg0 + min(lane, npg - 1));
+    int pid_l;
+    if constexpr (SINKS) {
+        // (a chunk on one side of the gap is as one without sinks)
+        const bool astride = pg0 < r.v.head && pg0 + npg > r.v.head;
+        pid_l = p.pm.page_table && p.pm.pt_stride >= 16 && !astride
+                    ? chunk_ids_scalar(p.pm, b, r.v.page(pg0), npg, lane)
+                    : (int)map_page(p.pm, b, r.v.page(pg0 + min(lane, npg - 1)));
+    } else {
+        pid_l = p.pm.page_table && p.pm.pt_stride >= 16 ? chunk_ids_scalar(p.pm, b, pg0, npg, lane)
+                                                        : (int)map_page(p.pm, b, pg0 + min(lane, npg - 1));
+    }
     const uint8_t *head_base = p.base + (int64_t)kvh * p.head_stride;
 
     // Start streaming the first step and request the chunk's V scales now,
@@ -722,6 +758,7 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
     c.npg = npg;
     c.start = r.start;
     c.end = r.end;
+    if constexpr (SINKS) c.v = r.v;
     c.kg = kg;
     c.ph = ph;
     c.pf = (float)piece;
@@ -744,7 +781,7 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
         }
         float pr[4];
         int vbad;
-        step_qk<D>(kr, step, c, st, pr, vbad);
+        step_qk<D, SINKS>(kr, step, c, st, pr, vbad);
         // the V half of `step` has landed; only the next K half may be in flight
         if (next)
             wait_vmem<NL>();
@@ -810,7 +847,7 @@ __host__ __device__ __forceinline__ int wg_span(int n, int full, int D) {
 // One workgroup item: (sequence b, its workgroup wg, KV head x head group hx).
 // The 4 waves take 4 consecutive chunks of the unit and merge them in LDS; a
 // unit longer than one workgroup writes one partial per workgroup.
-template <int D>
+template <int D, bool SINKS>
 __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlotBytesPerD * D], int b, int wg,
                                         int hx) {
     constexpr int kThreads = kWaves * 64;
@@ -824,7 +861,7 @@ __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlo
     const int h_base = kvh * p.group + g0;
     float *out = p.out + ((int64_t)b * p.n_heads + h_base) * D;
 
-    const Range r = seq_range(p, b);
+    const Range r = seq_range<SINKS>(p, b);
     if (r.n_pages == 0) {  // empty window: zero output (the reference's pre-zeroed buffer)
         if (wg == 0)
             for (int idx = tid; idx < gcount * D; idx += kThreads) out[idx] = 0.0f;
@@ -844,7 +881,7 @@ __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlo
     const int per_wave = ((wg_pages + 2 * kWaves - 1) / (2 * kWaves)) * 2;  // even: a step is two pages
     const int my0 = wave * per_wave;
     if (my0 < wg_pages) {
-        wave_chunk<D>(p, r, b, kvh, h_base, gcount, r.fp + wg * span + my0, min(per_wave, wg_pages - my0), lane,
+        wave_chunk<D, SINKS>(p, r, b, kvh, h_base, gcount, r.fp + wg * span + my0, min(per_wave, wg_pages - my0), lane,
                       slots[wave]);
     } else if (lane < kGT) {
         float *res = reinterpret_cast<float *>(slots[wave]);
@@ -926,7 +963,7 @@ __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlo
 // The head index runs fastest, so the workgroups reading the 8 head spans of
 // the same pages are dispatched together and the DRAM rows those pages open
 // are read out while open (measured ~25% over chunk-fastest order).
-template <int D>
+template <int D, bool SINKS>
 __global__ __launch_bounds__(kWaves * 64) void decode_q8_mfma_kernel(const Q8Params p) {
     // per wave: the streaming slot, later the wave's [kGT][D + 2] result
     __shared__ __attribute__((aligned(16))) uint8_t slots[kWaves][kSlotBytesPerD * D];
@@ -940,7 +977,7 @@ __global__ __launch_bounds__(kWaves * 64) void decode_q8_mfma_kernel(const Q8Par
         b = blockIdx.z;
         wg = blockIdx.y;
     }
-    q8_item<D>(p, slots, b, wg, blockIdx.x);
+    q8_item<D, SINKS>(p, slots, b, wg, blockIdx.x);
 }
 
 // Merge of the workgroup partials of every unit with more than one
@@ -949,7 +986,7 @@ __global__ __launch_bounds__(kWaves * 64) void decode_q8_mfma_kernel(const Q8Par
 // partials; the per-element arithmetic is that of a scalar merge: eight
 // partials at a time, all loads of a batch in flight together, (M, L, A)
 // absorbing the batch with one rescale).
-template <int D>
+template <int D, bool SINKS>
 __global__ __launch_bounds__(kGT * D / 4) void decode_q8_combine_kernel(const Q8Params p) {
     const int b = blockIdx.y;
     const int kvh = blockIdx.x / p.n_hg;
@@ -957,7 +994,7 @@ __global__ __launch_bounds__(kGT * D / 4) void decode_q8_combine_kernel(const Q8
     const int g0 = hg * p.hpw;
     const int gcount = min(p.hpw, p.group - g0);
     const int h_base = kvh * p.group + g0;
-    const Range r = seq_range(p, b);
+    const Range r = seq_range<SINKS>(p, b);
     const int span = wg_span(r.n_pages, kWaves * p.ch, D);  // pages per workgroup
     const int n_wg = min((r.n_pages + span - 1) / span, p.max_wg);
     if (n_wg <= 1) return;
@@ -1013,19 +1050,24 @@ __global__ __launch_bounds__(kGT * D / 4) void decode_q8_combine_kernel(const Q8
         make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
 }
 
-template <int D>
-int launch_d(gla_ctx *ctx, const Q8Params &prm, dim3 grid, int n_seqs) {
-    hipLaunchKernelGGL((decode_q8_mfma_kernel<D>), grid, dim3(kWaves * 64), 0, ctx->stream, prm);
+template <int D, bool SINKS>
+int launch_as(gla_ctx *ctx, const Q8Params &prm, dim3 grid, int n_seqs) {
+    hipLaunchKernelGGL((decode_q8_mfma_kernel<D, SINKS>), grid, dim3(kWaves * 64), 0, ctx->stream, prm);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "decode_q8_mfma_kernel launch: %s", hipGetErrorString(e));
     if (prm.max_wg > 1) {
-        hipLaunchKernelGGL((decode_q8_combine_kernel<D>), dim3(prm.n_kv_heads * prm.n_hg, n_seqs), dim3(kGT * D / 4),
-                           0, ctx->stream, prm);
+        hipLaunchKernelGGL((decode_q8_combine_kernel<D, SINKS>), dim3(prm.n_kv_heads * prm.n_hg, n_seqs),
+                           dim3(kGT * D / 4), 0, ctx->stream, prm);
         e = hipGetLastError();
         if (e != hipSuccess)
             return set_error(GLA_ERR_KERNEL, "decode_q8_combine_kernel launch: %s", hipGetErrorString(e));
     }
     return GLA_OK;
+}
+
+template <int D>
+int launch_d(gla_ctx *ctx, const Q8Params &prm, dim3 grid, int n_seqs) {
+    return prm.n_sinks > 0 ? launch_as<D, true>(ctx, prm, grid, n_seqs) : launch_as<D, false>(ctx, prm, grid, n_seqs);
 }
 
 // Workgroups of decode_q8_mfma_kernel<D> one CU holds at once (0 on error).
@@ -1034,7 +1076,7 @@ int resident_wgs() {
     static int cached = -1;
     if (cached < 0) {
         int n = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_q8_mfma_kernel<D>, kWaves * 64, 0) != hipSuccess)
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_q8_mfma_kernel<D, false>, kWaves * 64, 0) != hipSuccess)
             n = 0;
         cached = n;
     }
@@ -1081,12 +1123,11 @@ int choose_hpw(int group, int64_t wg_per_hg, int n_kv_heads, int64_t slots) {
 int launch_decode_q8(gla_ctx *ctx, const DecodeLaunch &d) {
     const int D = d.head_dim;
     const int group = d.n_heads / d.n_kv_heads;
-    // pages a window can span (a start inside a page adds one)
-    const int64_t max_pages = d.max_kv_len > 0 ? (d.max_kv_len + GLA_PAGE_SIZE - 1) / GLA_PAGE_SIZE + 1 : 1;
+    // pages a window can span (a start inside a page adds one), and its sinks'
+    const int64_t max_pages = max_window_pages(d);
     const bool host = d.kv_len_host != nullptr;
     auto pages_of = [&](int b) -> int {
-        return host ? host_seq_pages(d.kv_start_host[b], d.kv_len_host[b], d.max_kv_len, d.pm.pos_limit)
-                    : (int)max_pages;
+        return host ? host_pages(d, b) : (int)max_pages;
     };
     // Chunk size (pages per wave; even, at most 64). GLA_Q8_CHUNK_PAGES
     // forces another size (tuning and tests).
@@ -1130,6 +1171,7 @@ int launch_decode_q8(gla_ctx *ctx, const DecodeLaunch &d) {
     prm.ch = ch;
     prm.max_wg = (int)std::min<int64_t>(max_wg, 1 << 30);
     prm.max_len = d.max_kv_len;
+    prm.n_sinks = d.n_sinks;
     const bool cap = d.softcap > 0.0f;
     prm.q_mul = cap ? d.scale : d.scale * kLog2e;
     prm.softcap = cap ? d.softcap : 0.0f;

@@ -35,6 +35,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <exception>
 #include <new>
 #include <string>
@@ -202,6 +203,47 @@ __device__ __forceinline__ int64_t map_page(const PageMap &pm, int b, int lp) {
     return id < 0 ? 0 : (id >= pm.n_pages ? pm.n_pages - 1 : id);
 }
 
+// The pages that a window with sinks touches: of the positions j < end, those with
+// j >= start or j < sinks are seen. Page v of n_pages is the storage's logical
+// page v + (v >= head ? gap : 0): the pages of the sinks, then the window's; every
+// one holds a position that is seen. From `from` on only (a prefix that is read
+// apart; sinks are then 0).
+struct Visible {
+    int start, end, sinks;
+    int head, gap, n_pages;
+    __host__ __device__ __forceinline__ int page(int v) const { return v + (v >= head ? gap : 0); }
+    __host__ __device__ __forceinline__ bool sees(int pos) const { return pos < end && (pos >= start || pos < sinks); }
+    // every position of a logical page is seen, by the window or by the sinks alone
+    __host__ __device__ __forceinline__ bool whole(int page) const {
+        return page * 16 + 16 <= end && (page * 16 >= start || page * 16 + 16 <= sinks);
+    }
+};
+// With the decode kernels' clamping of start and length (their seq_range).
+__host__ __device__ __forceinline__ Visible visible_of(int start, int len, int max_len, int pos_limit, int n_sinks,
+                                                       int from) {
+    Visible r;
+    const int s0 = start < 0 ? 0 : start;
+    len = len < 0 ? 0 : (len > max_len ? max_len : len);
+    const int64_t e64 = (int64_t)s0 + len;
+    const int e = e64 > pos_limit ? pos_limit : (int)e64;
+    const int s = s0 > from ? s0 : from;
+    r.start = s;
+    r.end = e;
+    r.sinks = n_sinks;
+    r.head = r.gap = r.n_pages = 0;
+    if (s0 >= e || s >= e) return r;
+    const int before = ((n_sinks < s ? n_sinks : s) + 15) >> 4;  // pages of the sinks in front of the window
+    const int first = s >> 4, last = (e - 1) >> 4;
+    if (before >= first) {  // they meet the window's
+        r.n_pages = last + 1;
+    } else {
+        r.head = before;
+        r.gap = first - before;
+        r.n_pages = before + last - first + 1;
+    }
+    return r;
+}
+
 }  // namespace gla
 
 struct gla_ctx {
@@ -320,7 +362,20 @@ struct DecodeLaunch {
     // between calls), else the context's counters for its current stream
     int32_t *arrivals = nullptr;
     size_t arrivals_cap = 0;
+    // > 0: the first positions of a sequence that stay visible beside its window
+    int n_sinks = 0;
 };
+// Pages a sequence of the launch can have to read, from the bounds alone and from its host lengths.
+inline int max_window_pages(const DecodeLaunch &d) {
+    const int window = d.max_kv_len > 0 ? (d.max_kv_len + GLA_PAGE_SIZE - 1) / GLA_PAGE_SIZE + 1 : 1;
+    const int sinks = (std::min(d.n_sinks, d.pm.pos_limit) + GLA_PAGE_SIZE - 1) / GLA_PAGE_SIZE;
+    return d.n_sinks > 0 ? window + sinks : window;
+}
+inline int host_pages(const DecodeLaunch &d, int b) {
+    if (d.n_sinks > 0)
+        return visible_of(d.kv_start_host[b], d.kv_len_host[b], d.max_kv_len, d.pm.pos_limit, d.n_sinks, 0).n_pages;
+    return host_seq_pages(d.kv_start_host[b], d.kv_len_host[b], d.max_kv_len, d.pm.pos_limit);
+}
 // Device scratch of a decode launch: d.scratch (no allocation) or the
 // context's buffer for its current stream.
 int decode_scratch(gla_ctx *ctx, const DecodeLaunch &d, size_t bytes, void **out);
@@ -351,8 +406,10 @@ struct PrefillLaunch {
     gla_precision precision;
     const float *q;
     float *out;
+    int n_sinks = 0;  // launch_prefill_sinks: > 0
 };
 int launch_prefill(gla_ctx *ctx, const PrefillLaunch &p);
+int launch_prefill_sinks(gla_ctx *ctx, const PrefillLaunch &p);
 
 int launch_write_rows(gla_ctx *ctx, gla_kv *kv, const int64_t *rows, const float *k, const float *v, int n);
 int launch_read_rows(gla_ctx *ctx, const gla_kv *kv, const int64_t *rows, float *k, float *v, int n);

@@ -12,6 +12,10 @@
 //   O^T[d][query]  += V^T . P^T    P^T is packed from the lane's S^T
 //                                  accumulators: V's pieces hold the keys in
 //                                  that order, so no value changes its lane.
+// Sinks. The same code once more, with GLA_PREFILL_SINKS 1 (gla_prefill_sinks.hip),
+// is the prefill whose rows see the first n_sinks positions beside their window: the
+// tiles of the sinks come before the window's in every list of tiles (TileList). A
+// compile-time switch, so that a call without sinks runs what it ran before.
 #include <math.h>
 
 #include <algorithm>
@@ -19,9 +23,15 @@
 
 #include "gla_internal.h"
 
+#ifndef GLA_PREFILL_SINKS
+#define GLA_PREFILL_SINKS 0
+#endif
+
 namespace gla {
 
 namespace {
+
+constexpr bool kSinks = GLA_PREFILL_SINKS;
 
 constexpr int KT = 32;  // keys per tile
 constexpr float kLog2e = 1.4426950408889634f;
@@ -44,6 +54,7 @@ struct PrefillParams {
     float q_mul;       // scale*log2(e), or scale with a soft-cap
     float softcap;     // > 0: cap * tanh(s / cap)
     int sliding_window;
+    int n_sinks;  // kSinks: first positions seen beside the window
 };
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -109,6 +120,11 @@ struct SoftCap {
     }
 };
 
+// Whether key kp is in [lo, hi], or is a sink not past hi.
+__device__ __forceinline__ bool in_keys(int kp, int lo, int hi, int n_sinks) {
+    return (kp >= lo || (kSinks && kp < n_sinks)) && kp <= hi;
+}
+
 // Soft-cap and causal/window mask of one query column of a 32-key score tile
 // (sacc[mt][i]: key kbase + 16*mt + i), in place, log2 domain. The
 // soft-cap is a template argument and the mask one wave-uniform branch per
@@ -116,7 +132,7 @@ struct SoftCap {
 // branch around every score.
 template <bool CAP>
 __device__ __forceinline__ void cap_and_mask(floatx4 (&s)[2], float softcap, bool interior, int kbase, int qpos,
-                                             int qlo, int klo, int khi) {
+                                             int qlo, int klo, int khi, int n_sinks) {
     if constexpr (CAP) {
         const SoftCap f(softcap);
 #pragma unroll
@@ -131,7 +147,7 @@ __device__ __forceinline__ void cap_and_mask(floatx4 (&s)[2], float softcap, boo
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int kp = kbase + mt * 16 + i;
-                s[mt][i] = (kp >= lo && kp <= hi) ? s[mt][i] : -INFINITY;
+                s[mt][i] = (in_keys(kp, lo, hi, n_sinks)) ? s[mt][i] : -INFINITY;
             }
     }
 }
@@ -141,6 +157,31 @@ __device__ __forceinline__ int window_lo(int pos, int w) {
     int s = pos - w + 1;
     return s > 0 ? s : 0;
 }
+
+// The tiles of the keys [klo, khi] and of the sinks in front of them: tile i of `count`
+// is the KT keys from key0(i) on.
+struct TileList {
+    int first, count;
+    int head, gap;  // kSinks: the sinks' tiles that do not meet the others, and the tiles left out after them
+    __device__ __forceinline__ TileList(int klo, int khi, int n_sinks) {
+        first = klo / KT;
+        count = khi >= klo ? khi / KT - first + 1 : 0;
+        head = gap = 0;
+        if constexpr (kSinks) {
+            const int before = (min(min(n_sinks, klo), khi + 1) + KT - 1) / KT;
+            if (count > 0 && before >= first) {
+                first = 0;
+                count = khi / KT + 1;
+            } else if (before > 0) {
+                head = before;
+                gap = first - before;
+                first = 0;
+                count += before;
+            }
+        }
+    }
+    __device__ __forceinline__ int key0(int i) const { return (first + i + (kSinks && i >= head ? gap : 0)) * KT; }
+};
 
 // ---------------------------------------------------------------------------
 // bf16-input variant: Q, K, V and the probabilities are rounded to bf16 and
@@ -161,6 +202,13 @@ template <int D>
 constexpr int kKRowH = D + 8;  // K row in LDS (bf16): 16 bytes of padding
 constexpr int kVtRowH = KT + 8;  // Vt row in LDS (bf16): 32 keys + 16 bytes
 
+// Whether every row of a wave sees the whole tile at k0: the keys up to `hi` are behind
+// its first row, pos_last is its last row's position.
+__device__ __forceinline__ bool inside(const PrefillParams &p, int k0, int klo, int hi, int pos_last) {
+    if (kSinks && k0 + KT <= p.n_sinks) return k0 + KT - 1 <= hi;
+    return k0 >= klo && k0 + KT - 1 <= hi && (p.sliding_window <= 0 || k0 >= window_lo(pos_last, p.sliding_window));
+}
+
 // The 4 keys x 4 dims block of K and of V that one thread stages, as f32.
 struct Block44 {
     float4 k[4];  // k[i] = K[key 4*kq + i][4*dq .. 4*dq+3]
@@ -170,6 +218,7 @@ struct Block44 {
 template <int D, bool Q8>
 __device__ __forceinline__ void fetch_block44(const PrefillParams &p, int b, int kvh, int key0, int d0, int klo,
                                               int khi, Block44 &o) {
+    const int sinks = p.n_sinks;
     const int64_t head_off = (int64_t)kvh * p.kv.head_stride;
     // key0 is a multiple of 4, so the 4 keys share one page; a block past
     // khi (zeroed below) looks up khi's page, so the page-table read stays
@@ -192,7 +241,7 @@ __device__ __forceinline__ void fetch_block44(const PrefillParams &p, int b, int
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int kp = key0 + i;
-            const bool ok = kp >= klo && kp <= khi;
+            const bool ok = in_keys(kp, klo, khi, sinks);
             // K: 4 consecutive d of one slot are 4 consecutive bytes (q8k_off)
             const uint32_t w = *reinterpret_cast<const uint32_t *>(p.kv.k + hb + q8k_off(slot0 + i, d0, D));
             const float ksc = ok ? __half2float(__ushort_as_half(ksp[q8ks_off(slot0 + i, blk, D)])) : 0.0f;
@@ -206,7 +255,7 @@ __device__ __forceinline__ void fetch_block44(const PrefillParams &p, int b, int
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int kp = key0 + i;
-            if (kp >= klo && kp <= khi) {
+            if (in_keys(kp, klo, khi, sinks)) {
                 const int64_t base =
                     pid * p.kv.page_stride + head_off + (int64_t)((kp & 15)) * p.kv.row_stride + (int64_t)d0 * 4;
                 o.k[i] = *reinterpret_cast<const float4 *>(p.kv.k + base);
@@ -315,11 +364,11 @@ __device__ __forceinline__ float max3f(float a, float b, float c) { return max2f
 template <int NT, bool CAP, bool MASK>
 __device__ __forceinline__ void bf16_softmax_p(const floatx4 (&sacc)[2][NT], float (&m)[NT], float (&rs)[NT],
                                                bf16x8 (&pb)[NT], float softcap, int kbase, const int (&qpos)[NT],
-                                               const int (&qlo)[NT], int klo, int khi) {
+                                               const int (&qlo)[NT], int klo, int khi, int n_sinks) {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         floatx4 col[2] = {sacc[0][nt], sacc[1][nt]};
-        cap_and_mask<CAP>(col, softcap, !MASK, kbase, qpos[nt], qlo[nt], klo, khi);
+        cap_and_mask<CAP>(col, softcap, !MASK, kbase, qpos[nt], qlo[nt], klo, khi, n_sinks);
         float mx = max3f(max3f(col[0][0], col[0][1], col[0][2]), max3f(col[0][3], col[1][0], col[1][1]),
                          max2f(col[1][2], col[1][3]));
         const float m_old = m[nt];
@@ -370,7 +419,7 @@ __device__ __forceinline__ void bf16_softmax_interior(floatx4 (&sacc)[2][NT], fl
     for (int nt = 0; nt < NT; nt++) {
         if constexpr (CAP) {
             floatx4 col[2] = {sacc[0][nt], sacc[1][nt]};
-            cap_and_mask<CAP>(col, softcap, true, 0, 0, 0, 0, 0);
+            cap_and_mask<CAP>(col, softcap, true, 0, 0, 0, 0, 0, 0);
             sacc[0][nt] = col[0];
             sacc[1][nt] = col[1];
         }
@@ -411,12 +460,12 @@ template <int NT, int DT, bool CAP>
 __device__ __forceinline__ void bf16_softmax(floatx4 (&sacc)[2][NT], float (&m)[NT],
                                              floatx4 (&lacc)[NT], floatx4 (&o)[DT][NT], bf16x8 (&pb)[NT],
                                              float softcap, bool interior, int kbase, const int (&qpos)[NT],
-                                             const int (&qlo)[NT], int klo, int khi) {
+                                             const int (&qlo)[NT], int klo, int khi, int n_sinks) {
     float rs[NT];
     if (interior)
-        bf16_softmax_p<NT, CAP, false>(sacc, m, rs, pb, softcap, kbase, qpos, qlo, klo, khi);
+        bf16_softmax_p<NT, CAP, false>(sacc, m, rs, pb, softcap, kbase, qpos, qlo, klo, khi, n_sinks);
     else
-        bf16_softmax_p<NT, CAP, true>(sacc, m, rs, pb, softcap, kbase, qpos, qlo, klo, khi);
+        bf16_softmax_p<NT, CAP, true>(sacc, m, rs, pb, softcap, kbase, qpos, qlo, klo, khi, n_sinks);
     bf16_rescale<NT, DT>(rs, lacc, o);
 }
 
@@ -504,20 +553,21 @@ __global__ __launch_bounds__(kBf16Waves<D> * 64) void prefill_bf16_kernel(const 
     const int whi = min(khi, pos0 + wq0 + QW - 1);
     const int wlo = max(klo, window_lo(pos0 + wq0, p.sliding_window));
 
-    if (khi >= klo) {
-        const int kfirst = (klo / KT) * KT;
+    const TileList tiles(klo, khi, p.n_sinks);
+    if (tiles.count > 0) {
         TileBlocks<D, NTHR> tb;
-        fetch_tile_bf16<D, NTHR, Q8>(p, b, kvh, kfirst, klo, khi, tb);
+        fetch_tile_bf16<D, NTHR, Q8>(p, b, kvh, tiles.key0(0), klo, khi, tb);
         store_tile_bf16<D, NTHR>(tb, Kh[0], Vt[0]);
         __syncthreads();
         int buf = 0;
-        for (int k0 = kfirst; k0 <= khi; k0 += KT, buf ^= 1) {
-            const bool more = k0 + KT <= khi;
-            if (more) fetch_tile_bf16<D, NTHR, Q8>(p, b, kvh, k0 + KT, klo, khi, tb);
+        for (int i = 0; i < tiles.count; i++, buf ^= 1) {
+            const int k0 = tiles.key0(i);
+            const bool more = i + 1 < tiles.count;
+            if (more) fetch_tile_bf16<D, NTHR, Q8>(p, b, kvh, tiles.key0(i + 1), klo, khi, tb);
             const __bf16 *kh = Kh[buf];
             const __bf16 *vt = Vt[buf];
             // a tile wholly past this wave's last query or before its window adds nothing
-            if (k0 <= whi && k0 + KT - 1 >= wlo) {
+            if (k0 <= whi && (k0 + KT - 1 >= wlo || (kSinks && k0 < p.n_sinks))) {
             // S^T = K . Q^T
             floatx4 sacc[2][NT];
             bf16_score_init<NT>(sacc);
@@ -534,11 +584,10 @@ __global__ __launch_bounds__(kBf16Waves<D> * 64) void prefill_bf16_kernel(const 
                         sacc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mt], qb[nt][ks], sacc[mt][nt], 0, 0, 0);
             }
 
-            const bool interior = k0 >= klo && k0 + KT - 1 <= min(khi, pos0 + wq0) &&
-                                  (p.sliding_window <= 0 || k0 >= window_lo(pos0 + wq0 + QW - 1, p.sliding_window));
+            const bool interior = inside(p, k0, klo, min(khi, pos0 + wq0), pos0 + wq0 + QW - 1);
             bf16x8 pb[NT];
             bf16_softmax<NT, DT, CAP>(sacc, m, lacc, o, pb, p.softcap, interior, k0 + 4 * lgrp, qpos, qlo, klo,
-                                      khi);
+                                      khi, p.n_sinks);
 
             // O^T += V^T . P^T, and the row sums
             bf16_row_sums<NT>(lacc, pb);
@@ -688,9 +737,10 @@ __global__ __launch_bounds__(kBf16sWaves<D> * 64, kBf16sOccupancy<D>) void prefi
     const int whi = min(khi, pos0 + (wq0 | 31));
     const int wlo = max(klo, window_lo(pos0 + (wq0 & ~31), p.sliding_window));
 
-    if (khi >= klo) {
-        const int tfirst = klo / KT;
-        const int n = khi / KT - tfirst + 1;
+    const TileList tiles(klo, khi, p.n_sinks);
+    if (tiles.count > 0) {
+        const int tfirst = tiles.first;
+        const int n = tiles.count;
         const uint8_t *unit_img = img + ((int64_t)b * p.n_kv_heads + kvh) * n_tiles * kTileImage<D>;
         const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(
             (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)&ring[0][0]);
@@ -701,7 +751,7 @@ __global__ __launch_bounds__(kBf16sWaves<D> * 64, kBf16sOccupancy<D>) void prefi
         static_assert(NC % CPW == 0 && NC / CPW <= NW, "copies cover the tile");
         auto issue = [&](int i) {
             if (wave < NC / CPW) {
-                const uint8_t *src = unit_img + (int64_t)(tfirst + i) * kTileImage<D>;
+                const uint8_t *src = unit_img + (int64_t)(tiles.key0(i) / KT) * kTileImage<D>;
                 const uint32_t dst = ring_lds + (uint32_t)((i % RT) * kTileImage<D>);
 #pragma unroll
                 for (int c = 0; c < CPW; c++) {
@@ -759,7 +809,7 @@ __global__ __launch_bounds__(kBf16sWaves<D> * 64, kBf16sOccupancy<D>) void prefi
         // of the workgroup, when its waves share one query block (one q-head
         // each): no mask, no skip test and one lazy-maximum branch per tile.
         int n_int = 0;
-        if (p.hpw == NW) {
+        if (!kSinks && p.hpw == NW) {
             const int k_first = tfirst * KT;
             const bool lead = k_first >= klo &&
                               (p.sliding_window <= 0 || k_first >= window_lo(pos0 + wq0 + QW - 1, p.sliding_window));
@@ -777,18 +827,17 @@ __global__ __launch_bounds__(kBf16sWaves<D> * 64, kBf16sOccupancy<D>) void prefi
         }
         for (; i < n; i++) {
             arrive(i);
-            const int k0 = (tfirst + i) * KT;
+            const int k0 = tiles.key0(i);
             // a tile wholly past this wave's last query (the causal diagonal of
             // the workgroup's later waves) or before its window adds nothing
-            if (k0 > whi || k0 + KT - 1 < wlo) continue;
+            if (k0 > whi || (k0 + KT - 1 < wlo && !(kSinks && k0 < p.n_sinks))) continue;
             const uint8_t *kimg = ring[i % RT];
             floatx4 sacc[2][NT];
             scores(kimg, sacc);
-            const bool interior = k0 >= klo && k0 + KT - 1 <= min(khi, pos0 + wq0) &&
-                                  (p.sliding_window <= 0 || k0 >= window_lo(pos0 + wq0 + QW - 1, p.sliding_window));
+            const bool interior = inside(p, k0, klo, min(khi, pos0 + wq0), pos0 + wq0 + QW - 1);
             bf16x8 pb[NT];
             bf16_softmax<NT, DT, CAP>(sacc, m, lacc, o, pb, p.softcap, interior, k0 + 4 * lgrp, qpos, qlo, klo,
-                                      khi);
+                                      khi, p.n_sinks);
             accumulate(kimg + 64 * D, pb);
         }
     }
@@ -1023,6 +1072,7 @@ template <int D, bool Q8>
 struct SplitTile {
     static constexpr int NK = 4 * D / 256;  // 16-byte pieces of K (and of V) per thread
     static constexpr int KPW = 512 / D;     // f32: whole K rows per wave and round, the low bits of the lane
+    int sinks;  // kSinks: first keys in range beside [klo, khi]
     // f32: the rows' own 16-byte loads; Q8_0: quants and scales
     floatx4 ka[Q8 ? 1 : NK][2], va[Q8 ? 1 : NK][2];
     uint2 kw[Q8 ? NK : 1];
@@ -1037,6 +1087,7 @@ struct SplitTile {
 
     // keys outside [klo, khi] are zero (khi >= 0, and the tile meets the range)
     __device__ __forceinline__ void fetch(const PrefillParams &p, int b, int kvh, int k0, int klo, int khi) {
+        if constexpr (kSinks) sinks = p.n_sinks;
         const int64_t head_off = (int64_t)kvh * p.kv.head_stride;
         const int64_t hb0 = map_page(p.pm, b, min(k0, khi) >> 4) * p.kv.page_stride + head_off;
         const int64_t hb1 = map_page(p.pm, b, min(k0 + 16, khi) >> 4) * p.kv.page_stride + head_off;
@@ -1075,7 +1126,7 @@ struct SplitTile {
                 const int key = u / (D / 8);
                 const int kp = k0 + key;
                 va[r][0] = va[r][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (kp >= klo && kp <= khi) {
+                if (in_keys(kp, klo, khi, sinks)) {
                     const float *vr = reinterpret_cast<const float *>(p.kv.v + (key < 16 ? hb0 : hb1) +
                                                                       (int64_t)(kp & 15) * p.kv.row_stride) +
                                       8 * (u - key * (D / 8));
@@ -1088,7 +1139,7 @@ struct SplitTile {
                 const int key = k_row(r);
                 const int kp = k0 + key;
                 ka[r][0] = ka[r][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (kp >= klo && kp <= khi) {
+                if (in_keys(kp, klo, khi, sinks)) {
                     const float *kr = reinterpret_cast<const float *>(p.kv.k + (key < 16 ? hb0 : hb1) +
                                                                       (int64_t)(kp & 15) * p.kv.row_stride) +
                                       8 * k_col(r);
@@ -1105,7 +1156,7 @@ struct SplitTile {
         for (int r = 0; r < NK; r++) {
             const int i = threadIdx.x + 256 * r;
             const int kp = k0 + k_piece_key<D>(i);
-            const bool ok = kp >= klo && kp <= khi;
+            const bool ok = in_keys(kp, klo, khi, sinks);
             const float ksc = __half2float(__ushort_as_half(ks[r]));
 #pragma unroll
             for (int j = 0; j < 8; j++) {  // stored quants are x + 128
@@ -1113,7 +1164,7 @@ struct SplitTile {
                 kf[r][j] = ok ? (float)((int)((w >> (8 * (j & 3))) & 0xff) - 128) * ksc : 0.0f;
                 const int vp = k0 + v_piece_key(i, j);
                 const float vsc = __half2float(__ushort_as_half(vs[r][j]));
-                vf[r][j] = vp >= klo && vp <= khi
+                vf[r][j] = in_keys(vp, klo, khi, sinks)
                                ? (float)((int)((vw[r][j >> 2] >> (8 * (j & 3))) & 0xff) - 128) * vsc
                                : 0.0f;
             }
@@ -1144,7 +1195,7 @@ struct SplitTile {
                         low = min(low, bits);
                     }
                 }
-                const bool in = kp >= klo && kp <= khi;
+                const bool in = in_keys(kp, klo, khi, sinks);
                 const int e = class_of(in && top ? top + (7u << 23) : 0);
                 const bool small = top && (threadIdx.x < 32 ? low + (13u << 23) < top
                                                             : __uint_as_float(low) * pow2f(kTop - e) < kSmall);
@@ -1244,7 +1295,7 @@ struct SplitTile {
             const int32_t exps = key_exps(aux.k_exp[key], aux.v_exp[key]);
             const uint32_t odd_k = aux.odd[0], bad_v = aux.odd[1], small_v = aux.odd[2];
             const int kp = k0 + key;
-            const bool in = kp >= klo && kp <= khi;
+            const bool in = in_keys(kp, klo, khi, sinks);
             const uint32_t keys = (uint32_t)__ballot(in);
             const int32_t first = __builtin_amdgcn_readlane(exps, __builtin_ctz(keys));  // (a tile has a key in range)
             const bool same = !__ballot(in && exps != first);
@@ -1258,17 +1309,17 @@ struct SplitTile {
 };
 
 // The tiles that some query of sequence b attends.
-struct SeqTiles {
-    int lo, hi;        // the keys: [lo, hi], hi < 0 if there are none
-    int first, count;  // their tiles
-    __device__ __forceinline__ SeqTiles(const PrefillParams &p, int b) {
+struct SeqKeys {
+    int lo, hi;  // the keys: [lo, hi], hi < 0 if there are none
+    __device__ __forceinline__ SeqKeys(const PrefillParams &p, int b) {
         const int q_len = min(max(p.q_start[b + 1] - p.q_start[b], 0), p.max_q_len);
         const int pos0 = p.pos_offset[b];
         lo = window_lo(pos0, p.sliding_window);
         hi = q_len > 0 ? min(pos0 + q_len - 1, p.pm.pos_limit - 1) : -1;
-        first = lo / KT;
-        count = hi >= lo ? hi / KT - first + 1 : 0;
     }
+};
+struct SeqTiles : SeqKeys, TileList {
+    __device__ __forceinline__ SeqTiles(const PrefillParams &p, int b) : SeqKeys(p, b), TileList(lo, hi, p.n_sinks) {}
 };
 
 // Where the tile images of a (sequence, KV head) pair are. `start` null: every
@@ -1330,7 +1381,7 @@ __global__ __launch_bounds__(256) void stage_split_kernel(const PrefillParams p,
         const int kvh = item / seq.count;
         const int t = item - kvh * seq.count;
         if (!im.here(b, kvh, seq.count)) continue;
-        const int k0 = (seq.first + t) * KT;
+        const int k0 = seq.key0(t);
         SplitTile<D, Q8> tile;
         tile.fetch(p, b, kvh, k0, seq.lo, seq.hi);
         __syncthreads();  // aux is free
@@ -1363,7 +1414,8 @@ __global__ __launch_bounds__(256) void stage_bf16_kernel(const PrefillParams p, 
     const int khi = min(pos0 + q_len - 1, p.pm.pos_limit - 1);
     const int klo = window_lo(pos0, p.sliding_window);
     const int k0 = t * KT;
-    if (khi < klo || k0 > khi || k0 + KT - 1 < klo) return;  // a tile no query of the sequence reads
+    // a tile no query of the sequence reads
+    if (kSinks ? k0 > khi || (k0 + KT - 1 < klo && k0 >= p.n_sinks) : khi < klo || k0 > khi || k0 + KT - 1 < klo) return;
 
     uint8_t *dst = img + (((int64_t)b * p.n_kv_heads + kvh) * n_tiles + t) * kTileImage<D>;
     constexpr int NP = 4 * D;  // pieces of K (and of V) per tile
@@ -1386,7 +1438,7 @@ __global__ __launch_bounds__(256) void stage_bf16_kernel(const PrefillParams p, 
             const int key = u / (D / 8);
             const int kp = k0 + key;
             va[r][0] = va[r][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (kp >= klo && kp <= khi) {
+            if (in_keys(kp, klo, khi, p.n_sinks)) {
                 const float *vr = reinterpret_cast<const float *>(
                     p.kv.v + (key < 16 ? pid0 : pid1) * p.kv.page_stride + head_off +
                     (int64_t)(kp & 15) * p.kv.row_stride) + 8 * (u - key * (D / 8));
@@ -1402,7 +1454,7 @@ __global__ __launch_bounds__(256) void stage_bf16_kernel(const PrefillParams p, 
             const int key = mt * 16 + (rem & 15);
             const int kp = k0 + key;
             ka[r][0] = ka[r][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (kp >= klo && kp <= khi) {
+            if (in_keys(kp, klo, khi, p.n_sinks)) {
                 const float *kr = reinterpret_cast<const float *>(
                     p.kv.k + (key < 16 ? pid0 : pid1) * p.kv.page_stride + head_off +
                     (int64_t)(kp & 15) * p.kv.row_stride) + 8 * (rem >> 4);
@@ -1509,17 +1561,21 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
     const int q_last = min(q_len, qb0 + qwg) - 1;
     const int khi = min(pos0 + q_last, p.pm.pos_limit - 1);
     const int klo = window_lo(pos0 + qb0, p.sliding_window);
-    const int tfirst = klo / KT;
-    const int n = khi >= klo ? khi / KT - tfirst + 1 : 0;
+    const TileList tiles(klo, khi, p.n_sinks);
+    const int tfirst = tiles.first;
+    const int n = tiles.count;
     // the keys that some query of the sequence attends; others are zero in the images
     const int ulo = seq.lo, uhi = seq.hi;
     const int64_t first = STAGED ? im.first(b, kvh, p.n_kv_heads, seq.count) + tfirst - seq.first : 0;
     const TileMeta *unit_meta = im.meta + first;
     const uint8_t *unit_img = im.img + first * IMG;
+    // from a tile of the workgroup to its place among the pair's (the sinks' own come first in both)
+    const int skip = tiles.gap - seq.gap;
+    const auto place = [&](int i) __attribute__((always_inline)) { return kSinks && i >= tiles.head ? i + skip : i; };
     const uint32_t ring = __builtin_amdgcn_readfirstlane(
         (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)&lds[0]);
     auto issue = [&](int i) {
-        const uint8_t *src = unit_img + (int64_t)i * IMG;
+        const uint8_t *src = unit_img + (int64_t)place(i) * IMG;
         const uint32_t dst = ring + (uint32_t)((i & 1) * IMG);
 #pragma unroll
         for (int c = 0; c < CPW; c++) {
@@ -1530,7 +1586,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
 
     const auto issue_meta = [&](int i) __attribute__((always_inline)) {
         if (wave == 0)
-            lds_copy4(reinterpret_cast<const uint8_t *>(unit_meta + i), (uint32_t)(lane * 4),
+            lds_copy4(reinterpret_cast<const uint8_t *>(unit_meta + place(i)), (uint32_t)(lane * 4),
                       ring + METAS + (uint32_t)((i & 1) * sizeof(TileMeta)));
     };
 
@@ -1539,7 +1595,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
     // often differ from the rest)
     int32_t exps = kMixed;
     for (int i = 0; STAGED && i < n && exps == kMixed; i += 64) {
-        const int32_t mine = unit_meta[min(i + lane, n - 1)].head.exps;
+        const int32_t mine = unit_meta[place(min(i + lane, n - 1))].head.exps;
         const uint64_t found = __ballot(mine != kMixed);
         if (found) exps = __builtin_amdgcn_readlane(mine, __builtin_ctzll(found));
     }
@@ -1633,7 +1689,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
             for (int mt = 0; mt < 2; mt++) {
                 const int kp = k0 + 16 * mt + lrow;
                 kd[mt] = k_values4<D, Q8>(*a, hb[mt], lrow, lgrp * (D / 4) + d);
-                if (kp < ulo || kp > uhi) kd[mt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (!in_keys(kp, ulo, uhi, a->n_sinks)) kd[mt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) qd[nt] = *reinterpret_cast<const floatx4 *>(qp[nt] + d) * a->q_mul;
@@ -1700,7 +1756,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
 #pragma unroll
                 for (int j = 1; j < 8; j++) mine = reg == j ? pv[nt][j] : mine;
                 const float pk = __shfl(mine, ((key >> 2) & 3) * 16 + lrow);
-                const bool attends = kp >= qlo[nt] && kp <= qpos[nt];
+                const bool attends = in_keys(kp, qlo[nt], qpos[nt], p.n_sinks);
 #pragma unroll
                 for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -1713,8 +1769,8 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
     // Tile i. `same`: its keys' exponents are those of `exps`, and nothing is odd;
     // otherwise they are in `meta`.
     const auto attend = [&](auto same, int i, const uint8_t *kimg, const TileMeta *meta) __attribute__((always_inline)) {
-        const int k0 = (tfirst + i) * KT;
-        if (k0 > whi || k0 + KT - 1 < wlo) return;  // no query of this wave attends it
+        const int k0 = tiles.key0(i);
+        if (k0 > whi || (k0 + KT - 1 < wlo && !(kSinks && k0 < p.n_sinks))) return;  // no query of this wave attends it
 
         // S^T = K . Q^T: the hi products and the cross terms apart, added at
         // the end (the small terms are not rounded at the large ones' unit)
@@ -1761,8 +1817,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
         }
 
         // softmax: as the bf16 kernels' (a lazy maximum), in f32; c undoes the scales
-        const bool interior = k0 >= klo && k0 + KT - 1 <= min(khi, pos0 + wq0) &&
-                              (p.sliding_window <= 0 || k0 >= window_lo(pos0 + wq0 + QW - 1, p.sliding_window));
+        const bool interior = inside(p, k0, klo, min(khi, pos0 + wq0), pos0 + wq0 + QW - 1);
 #pragma unroll
         for (int mt = 0; mt < 2; mt++)
 #pragma unroll
@@ -1794,7 +1849,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
                 col[1] *= c[nt];
                 c[nt] = 1.0f;
             }
-            cap_and_mask<CAP>(col, p.softcap, interior, k0 + 4 * lgrp, qpos[nt], qlo[nt], klo, khi);
+            cap_and_mask<CAP>(col, p.softcap, interior, k0 + 4 * lgrp, qpos[nt], qlo[nt], klo, khi, p.n_sinks);
             float mx = max3f(max3f(col[0][0], col[0][1], col[0][2]), max3f(col[0][3], col[1][0], col[1][1]),
                              max2f(col[1][2], col[1][3])) * c[nt];
             if (__ballot(mx - m[nt] > kLazyF32)) {
@@ -1829,7 +1884,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int kp = k0 + (j >> 2) * 16 + 4 * lgrp + (j & 3);
-                    top = kp >= lo && kp <= hi ? max(top, v_exp_of(key[j])) : top;
+                    top = in_keys(kp, lo, hi, p.n_sinks) ? max(top, v_exp_of(key[j])) : top;
                 }
                 top = (int)umax_rows4((uint32_t)(top - kNoExp)) + kNoExp;
                 if (__ballot(top > rexp[nt] + kLazyExp)) {
@@ -1902,7 +1957,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
         const auto next_special = [&](int i) __attribute__((always_inline)) {
             if (!plain) return i;
             for (; i < n; i += 64) {
-                const TileHead h = unit_meta[min(i + lane, n - 1)].head;
+                const TileHead h = unit_meta[place(min(i + lane, n - 1))].head;
                 const uint64_t found = __ballot(h.exps != exps || (h.odd_k | h.bad_v | h.small_v));
                 if (found) return min(n, i + __builtin_ctzll(found));
             }
@@ -1926,8 +1981,11 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     const int e = v_exp_of(exps);
-                    const bool up = e > rexp[nt] + kLazyExp &&
-                                    (rexp[nt] == kNoExp || qpos[nt] >= (tfirst + i) * KT);
+                    bool up = e > rexp[nt] + kLazyExp && (rexp[nt] == kNoExp || qpos[nt] >= tiles.key0(i));
+                    // (a row that has attended sinks need not attend the first of the window's tiles)
+                    if constexpr (kSinks)
+                        up = up && (rexp[nt] == kNoExp || qlo[nt] < tiles.key0(stop - 1) + KT ||
+                                    tiles.key0(i) < p.n_sinks);
                     if (__ballot(up && rexp[nt] != kNoExp)) {
                         const float f = up && rexp[nt] != kNoExp ? ldexpf(1.0f, rexp[nt] - e) : 1.0f;
 #pragma unroll
@@ -1955,7 +2013,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
         SplitAux<D, Q8> &aux = *reinterpret_cast<SplitAux<D, Q8> *>(lds + IMG);
         constexpr bool AHEAD = D < 256;
         SplitTile<D, Q8> tile;
-        tile.fetch(p, b, kvh, tfirst * KT, ulo, uhi);
+        tile.fetch(p, b, kvh, tiles.key0(0), ulo, uhi);
         if (tid < 3) aux.odd[tid] = 0;
         __syncthreads();
         const auto put = [&](int base) {
@@ -1967,12 +2025,12 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
         };
         // tile i, ready for every wave
         const auto arrive = [&](int i) __attribute__((always_inline)) {
-            const int k0 = (tfirst + i) * KT;
+            const int k0 = tiles.key0(i);
             if (i > 0) __syncthreads();  // its place is free
             if (!AHEAD && i > 0) tile.fetch(p, b, kvh, k0, ulo, uhi);
             tile.convert(aux, k0, ulo, uhi, put(0), put(128 * D));
             __syncthreads();
-            if (AHEAD && i + 1 < n) tile.fetch(p, b, kvh, k0 + KT, ulo, uhi);
+            if (AHEAD && i + 1 < n) tile.fetch(p, b, kvh, tiles.key0(i + 1), ulo, uhi);
         };
         int i = 0;
         bool here = false;  // tile i is ready
@@ -2117,7 +2175,8 @@ int launch_split(gla_ctx *ctx, const PrefillParams &prm, int n_seqs, int n_hgrp,
     const int n_pairs = n_seqs * prm.n_kv_heads, n_units = n_pairs * n_hgrp;
     // tiles that one sequence can attend
     if (prm.sliding_window > 0)
-        n_tiles = (int)std::min<int64_t>(n_tiles, ((int64_t)prm.max_q_len + prm.sliding_window - 2) / KT + 2);
+        n_tiles = (int)std::min<int64_t>(n_tiles, ((int64_t)prm.max_q_len + prm.sliding_window - 2) / KT + 2 +
+                                                      (kSinks ? ((int64_t)prm.n_sinks + KT - 1) / KT : 0));
     constexpr size_t per = kSplitImage<D> + sizeof(TileMeta);
     const bool few = prm.max_q_len <= kUnstagedRows<D> && n_tiles <= kUnstagedTiles;
     Images im{};
@@ -2178,7 +2237,11 @@ int launch_f32(gla_ctx *ctx, bool q8, const PrefillParams &prm, int n_seqs, int 
 
 }  // namespace
 
+#if GLA_PREFILL_SINKS
+int launch_prefill_sinks(gla_ctx *ctx, const PrefillLaunch &a) {
+#else
 int launch_prefill(gla_ctx *ctx, const PrefillLaunch &a) {
+#endif
     const int D = a.head_dim;
     const int group = a.n_heads / a.n_kv_heads;
     const int hpw = (group % 4 == 0) ? 4 : ((group % 2 == 0) ? 2 : 1);
@@ -2217,6 +2280,7 @@ int launch_prefill(gla_ctx *ctx, const PrefillLaunch &a) {
     prm.q_mul = cap ? a.scale : a.scale * kLog2e;
     prm.softcap = cap ? a.softcap : 0.0f;
     prm.sliding_window = a.sliding_window;
+    prm.n_sinks = a.n_sinks;
     if (prm.n_qblocks > 65535) return set_error(GLA_ERR_INVALID, "prefill: %d query blocks > 65535", prm.n_qblocks);
     dim3 grid(a.n_seqs * a.n_kv_heads * (group / hpw), prm.n_qblocks, 1);
     if (a.precision == GLA_PREC_BF16) {

@@ -11,7 +11,7 @@
  *   - prefill attention loop                        src/transformer/forward.rs:927-958
  * and, beside it on a decode step, RoPE (src/tensor/ops.rs:212-245), the
  * Q8_0 weight matvec (src/tensor/quantized.rs:247-346, :587-610), the 4-bit
- * one and the append of rotated rows to a storage.
+ * one, the append of rotated rows to a storage and the norms between blocks.
  * The numerics follow flash_attn_1d_ext (src/tensor/flash.rs:46-124).
  *
  * Conventions (the same as Glint's outbound C API, include/glint.h:21-35):
@@ -320,6 +320,52 @@ typedef struct gla_prefill_args {
 
 int gla_prefill(gla_ctx *ctx, const gla_prefill_args *args);
 
+/* ---- contexts that keep, or share, their beginning ----------------------- */
+
+/* gla_decode whose rows also see the first n_sinks positions of their sequence,
+ * where a window has left them behind: row b attends the positions
+ * j < kv_start[b] + kv_len[b] with j >= kv_start[b] or j < n_sinks. kv_len,
+ * max_kv_len and the host copies are the window's alone, as in gla_decode; a row
+ * with kv_len 0 attends nothing (a zero output). n_sinks 0 is gla_decode; below 0
+ * is refused. What gla_decode says of indices, non-finite data, host copies and
+ * captures holds here. A row's bits follow from its own window and n_sinks. */
+int gla_decode_sinks(gla_ctx *ctx, const gla_decode_args *args, int n_sinks);
+
+/* gla_prefill whose rows also see the first n_sinks positions: the row at position
+ * p attends the positions j <= p with j > p - sliding_window or j < n_sinks (all
+ * of them without a window). n_sinks 0 is gla_prefill; below 0 is refused. */
+int gla_prefill_sinks(gla_ctx *ctx, const gla_prefill_args *args, int n_sinks);
+
+/* gla_decode of a batch whose neighbouring rows begin with the same positions: the
+ * sequences that a prefix cache gave the same pages. Rows group_start[g] ..
+ * group_start[g+1]-1 hold the same K and V at the positions before prefix_len[g];
+ * those of the pages that lie wholly before it are read once for the group, through
+ * its first row's pages (the table's row, or the cache's sequence), and multiplied
+ * with the queries of all its rows as one matrix product. Rows in no group share
+ * nothing. The results are gla_decode's but for rounding, which depends on the
+ * groups and the bounds: not bit-identical to it, nor from one grouping to another.
+ *
+ * Values that the host does not see are clamped into the batch and the storage as
+ * gla_decode's are: group starts that fall, or pages that differ where they are said
+ * to be the same, give wrong rows and GLA_OK, never an access outside the buffers.
+ * With the host copies they are checked before anything is launched
+ * (GLA_ERR_INVALID). Allocates scratch of the stream as gla_decode does: call it once
+ * before capturing it, without the host copies and with the bounds of every replay. */
+typedef struct gla_decode_shared_args {
+    gla_decode_args decode;     /* the batch, as gla_decode takes it; its windows count from the sequence's start */
+    int n_groups;
+    const int32_t *group_start; /* device int32[n_groups + 1], rising, within 0 .. n_seqs */
+    const int32_t *prefix_len;  /* device int32[n_groups]: positions that a group's rows share */
+    int max_group;              /* host: >= the rows of every group */
+    int max_prefix_len;         /* host: >= every prefix_len */
+    int max_own_len;            /* host: >= kv_start + kv_len - prefix_len of every row (0 for one that ends sooner;
+                                   prefix_len 0 for rows in no group) */
+    const int32_t *group_start_host; /* optional host copies, both or neither, */
+    const int32_t *prefix_len_host;  /* beside decode's: read during the call */
+} gla_decode_shared_args;
+
+int gla_decode_shared(gla_ctx *ctx, const gla_decode_shared_args *args);
+
 /* Host-buffer mirror of GpuBackend::attention (src/backend/gpu.rs:266-397):
  * q [n_heads][head_dim]; k, v [seq_len][n_kv_heads][head_dim]; out
  * [n_heads][head_dim]. Adds the soft-cap the wgpu shader lacks and has no
@@ -496,6 +542,39 @@ int gla_q4w_cols(const gla_q4w *w);
  * GLA_ERR_INVALID; partial sums that alone would not fit are done without, the
  * same bits in two launches). n_vec above 262,128 is refused (split the call). */
 int gla_matvec_q4(gla_ctx *ctx, const gla_q4w *w, const float *x, int n_vec, float *y);
+
+/* Norms around a transformer block in one pass over device rows of `dim` floats:
+ *     z        = post ? y / sqrt(mean(y^2) + eps) * post : y     (the block's output, normed)
+ *     x_out    = x + scale * gate * z                            (the residual stream)
+ *     norm_out = x_out / sqrt(mean(x_out^2) + eps) * pre         (the next block's input)
+ * the rms_norm and add shaders' job (src/backend/shaders) with what models put
+ * between them. y NULL: the stream stays x (post and gate NULL too). x_out or
+ * norm_out may be NULL; pre and norm_out come together. Strides are floats from row
+ * to row, 0: dim; gate_stride 0: one gate for all rows. An output may be x, y or a
+ * gate of rows, row for row (the same address and stride), or apart from all inputs
+ * and the other output; other overlaps are refused. Sums of squares are in 32 bits;
+ * a NaN or an infinity stays in its row. dim at most GLA_BLOCK_NORM_MAX_DIM;
+ * 16-byte aligned rows and strides are faster. Asynchronous; allocates nothing. */
+#define GLA_BLOCK_NORM_MAX_DIM 16384
+typedef struct gla_block_norm_args {
+    int n_rows;
+    int dim;
+    float eps;
+    float scale;
+    const float *x; /* device rows */
+    int64_t x_stride;
+    const float *y; /* device rows or NULL */
+    int64_t y_stride;
+    const float *post; /* device [dim] or NULL */
+    const float *gate; /* device rows, or [dim] with gate_stride 0, or NULL */
+    int64_t gate_stride;
+    const float *pre; /* device [dim] or NULL */
+    float *x_out;     /* device rows or NULL */
+    int64_t x_out_stride;
+    float *norm_out; /* device rows or NULL */
+    int64_t norm_out_stride;
+} gla_block_norm_args;
+int gla_block_norm(gla_ctx *ctx, const gla_block_norm_args *args);
 
 #ifdef __cplusplus
 }
