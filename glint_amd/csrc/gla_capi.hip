@@ -802,6 +802,18 @@ int gla_decode_shared(gla_ctx *ctx, const gla_decode_shared_args *a) {
                         b, (long long)mine, a->max_own_len);
         }
     }
+    d.pre.group_start = a->group_start;
+    d.pre.prefix_len = a->prefix_len;
+    d.pre.max_group = std::min(a->max_group, d.n_seqs);
+    d.pre.max_prefix = std::min(a->max_prefix_len, d.pm.pos_limit) & ~15;
+    d.pre.max_own = a->max_own_len;
+    d.pre.group_start_host = a->group_start_host;
+    d.pre.prefix_len_host = a->prefix_len_host;
+    // rows that share nothing are read one by one
+    if (a->n_groups > 0 && d.pre.max_group > 1 && d.pre.max_prefix > 0) {
+        d.pre.n_groups = a->n_groups;
+        plan_prefix(ctx, &d);
+    }
     return launch_decode(ctx, d);
     GLA_GUARD_END
 }

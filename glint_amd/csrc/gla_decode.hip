@@ -71,7 +71,8 @@ struct DecodeParams {
     // decode_combine_kernel.
     int merge_pages;
     int32_t *arrivals;
-    int n_sinks;  // SINKS kernels: first positions seen beside the window
+    int n_sinks;        // kWindowSinks
+    PrefixLaunch pre;   // kBehindPrefix: every split leaves a partial, merged with the prefix's by decode_combine_kernel
 };
 
 // Sum over the 8 lanes of an aligned lane group (DPP: quad xor1, quad xor2,
@@ -151,15 +152,17 @@ struct SeqRange {
     int n_pages;
     int pps;         // pages per split
     int n_splits;
-    Visible v;       // SINKS kernels (fp is 0: pages are numbered as Visible does)
+    Visible v;       // but for kWindow (fp is 0: pages are numbered as Visible does)
+    int prefix;      // kBehindPrefix: positions that the prefix's partials hold
 };
 
-template <bool SINKS>
+template <DecodeMode MODE>
 __device__ __forceinline__ SeqRange seq_range(const DecodeParams &p, int b) {
     SeqRange r;
     int s = p.kv_start[b];
-    if constexpr (SINKS) {
-        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, p.n_sinks, 0);
+    if constexpr (MODE != kWindow) {
+        r.prefix = MODE == kBehindPrefix ? row_prefix(p.pre, b) : 0;
+        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, MODE == kWindowSinks ? p.n_sinks : 0, r.prefix);
         r.start = r.v.start;
         r.end = r.v.end;
         r.fp = 0;
@@ -263,7 +266,7 @@ __device__ __forceinline__ void merge_splits_agent(const DecodeParams &p, int64_
     }
 }
 
-template <int D, int GT, int NSTEP, bool CAP, bool SINKS>
+template <int D, int GT, int NSTEP, bool CAP, DecodeMode MODE>
 __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodeParams p) {
     constexpr int EPL = D / 8;       // elements per lane
     constexpr int EPC = 4;           // floats per 16-byte chunk
@@ -284,10 +287,10 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
     const int gcount = min(GT, p.group - g0);
     const int h_base = kvh * p.group + g0;
 
-    const SeqRange r = seq_range<SINKS>(p, b);
+    const SeqRange r = seq_range<MODE>(p, b);
     const int tid = threadIdx.x;
     if (r.n_pages == 0) {  // empty window: zero output (the reference's pre-zeroed buffer)
-        if (split == 0)
+        if (MODE != kBehindPrefix && split == 0)
             for (int idx = tid; idx < gcount * D; idx += kThreads)
                 p.out[((int64_t)b * p.n_heads + h_base) * D + idx] = 0.0f;
         return;
@@ -335,14 +338,14 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
 #pragma unroll
         for (int j = 0; j < PPW; j++) {
             const int pg = (pb + j < pg1) ? pb + j : pb;
-            pid[j] = map_page(p.pm, b, SINKS ? r.v.page(pg) : pg);
+            pid[j] = map_page(p.pm, b, MODE != kWindow ? r.v.page(pg) : pg);
         }
 #pragma unroll
         for (int s = 0; s < NSTEP; s++) {
             const int page = pb + s / 2;
             const int slot = (s & 1) * 8 + tg;
-            const int pos = (SINKS ? r.v.page(page) : page) * 16 + slot;
-            valid[s] = page < pg1 && (SINKS ? r.v.sees(pos) : pos >= r.start && pos < r.end);
+            const int pos = (MODE != kWindow ? r.v.page(page) : page) * 16 + slot;
+            valid[s] = page < pg1 && (MODE != kWindow ? r.v.sees(pos) : pos >= r.start && pos < r.end);
             const int64_t base = pid[s / 2] * p.kv.page_stride + head_off + (int64_t)slot * p.kv.row_stride;
             const uint8_t *kp = p.kv.k + base;
             const uint8_t *vp = p.kv.v + base;
@@ -464,7 +467,7 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
 
     // merge the 4 waves; write the output or this split's partial
     const int64_t unit = ((int64_t)b * p.n_kv_heads + kvh) * p.n_hg + hg;
-    const bool arrive = r.n_splits > 1 && r.n_pages <= p.merge_pages;  // a rule on the window alone
+    const bool arrive = MODE != kBehindPrefix && r.n_splits > 1 && r.n_pages <= p.merge_pages;  // a rule on the window alone
     for (int idx = tid; idx < gcount * D; idx += kThreads) {
         const int g = idx / D;
         const int e = idx - g * D;
@@ -479,7 +482,7 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
             L = fmaf(lds_l[w][g], f, L);
             A = fmaf(lds_acc[w][g][e], f, A);
         }
-        if (r.n_splits == 1) {
+        if (MODE != kBehindPrefix && r.n_splits == 1) {
             p.out[((int64_t)b * p.n_heads + h_base + g) * D + e] = L > 0.0f ? A * (1.0f / L) : A;
         } else {
             const int64_t slot = unit * p.max_splits + split;
@@ -491,7 +494,7 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
     }
     // (m, l) of the split's heads as one whole 128-byte line: sub-line writes cost a
     // read-modify-write in HBM (measured on the Q8_0 kernel's partials: 3-12 us per call)
-    if (r.n_splits > 1 && tid < 8) {
+    if ((MODE == kBehindPrefix || r.n_splits > 1) && tid < 8) {
         float M = -INFINITY, L = 0.0f;
         const int g = tid & 7;
         if (g < GT) {
@@ -532,7 +535,7 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
 // group, q-head g = blockIdx.x). A row of D floats is read by D/4 lanes as
 // float4; the 256 threads form 256/(D/4) split groups that take every
 // NSG-th split, four splits in flight at a time, and are merged through LDS.
-template <int D, int GT, bool SINKS>
+template <int D, int GT, DecodeMode MODE>
 __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const DecodeParams p) {
     constexpr int RL = D / 4;             // lanes per row
     constexpr int NSG = kThreads / RL;    // split groups
@@ -546,8 +549,10 @@ __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const DecodePa
     const int g = blockIdx.x;
     const int gcount = min(GT, p.group - hg * GT);
     if (g >= gcount) return;
-    const SeqRange r = seq_range<SINKS>(p, b);
-    if (r.n_splits <= 1 || r.n_pages <= p.merge_pages) return;  // (one split, or merged in the split kernel)
+    const SeqRange r = seq_range<MODE>(p, b);
+    // (one split, or merged in the split kernel)
+    if (MODE != kBehindPrefix && (r.n_splits <= 1 || r.n_pages <= p.merge_pages)) return;
+    const int n = r.n_splits + (MODE == kBehindPrefix ? prefix_splits(p.pre, r.prefix) : 0);
     const int sg = threadIdx.x / RL;
     const int e4 = threadIdx.x - sg * RL;
     const int64_t unit = ((int64_t)b * p.n_kv_heads + kvh) * p.n_hg + hg;
@@ -555,20 +560,28 @@ __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const DecodePa
 
     float M = -INFINITY, L = 0.0f;
     float4 A = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = sg; s0 < r.n_splits; s0 += NSG * BATCH) {
+    for (int s0 = sg; s0 < n; s0 += NSG * BATCH) {
         float mi[BATCH], li[BATCH];
         float4 ai[BATCH];
 #pragma unroll
         for (int j = 0; j < BATCH; j++) {
             const int s = s0 + j * NSG;
-            const int sc = s < r.n_splits ? s : s0;
+            const int sc = s < n ? s : s0;
             const int64_t slot = (slot0 + sc) * GT + g;
-            const bool in = s < r.n_splits;
-            const float lv = p.part_ml[(slot0 + sc) * 32 + 8 + g];
-            const float4 av = reinterpret_cast<const float4 *>(p.part_acc + slot * D)[e4];
+            const bool in = s < n;
+            const float *ml = p.part_ml + (slot0 + sc) * 32 + g, *acc = p.part_acc + slot * D;
+            int l_at = 8;
+            if (MODE == kBehindPrefix && sc >= r.n_splits) {
+                const int64_t at = ((int64_t)(sc - r.n_splits) * gridDim.z + b) * p.n_heads + kvh * p.group + hg * GT + g;
+                ml = p.pre.ml + 2 * at;
+                acc = p.pre.acc + at * D;
+                l_at = 1;
+            }
+            const float lv = ml[l_at];
+            const float4 av = reinterpret_cast<const float4 *>(acc)[e4];
             // an entry past the last split reloads split s0 and adds nothing
             // (not 0 x its sums: an infinity there would make NaN)
-            mi[j] = in ? p.part_ml[(slot0 + sc) * 32 + g] : -INFINITY;
+            mi[j] = in ? ml[0] : -INFINITY;
             li[j] = in ? lv : 0.0f;
             ai[j] = in ? av : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
@@ -623,18 +636,18 @@ __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const DecodePa
         make_float4(AA.x * inv, AA.y * inv, AA.z * inv, AA.w * inv);
 }
 
-template <int D, int GT, bool SINKS>
+template <int D, int GT, DecodeMode MODE>
 int launch_as(gla_ctx *ctx, const DecodeParams &prm, dim3 grid, bool combine) {
     if (prm.softcap > 0.0f)
-        hipLaunchKernelGGL((decode_split_kernel<D, GT, kStepsPerIter, true, SINKS>), grid, dim3(kThreads), 0,
+        hipLaunchKernelGGL((decode_split_kernel<D, GT, kStepsPerIter, true, MODE>), grid, dim3(kThreads), 0,
                            ctx->stream, prm);
     else
-        hipLaunchKernelGGL((decode_split_kernel<D, GT, kStepsPerIter, false, SINKS>), grid, dim3(kThreads), 0,
+        hipLaunchKernelGGL((decode_split_kernel<D, GT, kStepsPerIter, false, MODE>), grid, dim3(kThreads), 0,
                            ctx->stream, prm);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "decode_split_kernel launch: %s", hipGetErrorString(e));
     if (combine) {
-        hipLaunchKernelGGL((decode_combine_kernel<D, GT, SINKS>), dim3(GT, grid.x, grid.z), dim3(kThreads), 0,
+        hipLaunchKernelGGL((decode_combine_kernel<D, GT, MODE>), dim3(GT, grid.x, grid.z), dim3(kThreads), 0,
                            ctx->stream, prm);
         e = hipGetLastError();
         if (e != hipSuccess)
@@ -645,8 +658,9 @@ int launch_as(gla_ctx *ctx, const DecodeParams &prm, dim3 grid, bool combine) {
 
 template <int D, int GT>
 int launch_typed(gla_ctx *ctx, const DecodeParams &prm, dim3 grid, bool combine) {
-    return prm.n_sinks > 0 ? launch_as<D, GT, true>(ctx, prm, grid, combine)
-                           : launch_as<D, GT, false>(ctx, prm, grid, combine);
+    if (prm.pre.n_groups > 0) return launch_as<D, GT, kBehindPrefix>(ctx, prm, grid, true);
+    if (prm.n_sinks > 0) return launch_as<D, GT, kWindowSinks>(ctx, prm, grid, combine);
+    return launch_as<D, GT, kWindow>(ctx, prm, grid, combine);
 }
 
 // Head-group width: the registers of a lane hold GT*(D/8) q values and as
@@ -725,10 +739,14 @@ int launch_decode(gla_ctx *ctx, const DecodeLaunch &d) {
     prm.merge_pages = merge_pages;
     prm.arrivals = nullptr;
     prm.n_sinks = d.n_sinks;
+    prm.pre = d.pre;
+    const bool behind = decode_mode(d) == kBehindPrefix;
     // Which merges the launch needs: exact from the host lengths, else from
     // the max_kv_len bound.
     bool any_short = false, any_long = false;
-    if (d.kv_len_host) {
+    if (behind) {
+        // all by the combine kernel
+    } else if (d.kv_len_host) {
         for (int b = 0; b < d.n_seqs; b++) {
             const int n = host_pages(d, b);
             const int pps = pps_fixed > 0 ? pps_fixed : split_pages(n);
@@ -748,18 +766,22 @@ int launch_decode(gla_ctx *ctx, const DecodeLaunch &d) {
         int rc = decode_arrivals(ctx, d, (size_t)units, &prm.arrivals);
         if (rc != GLA_OK) return rc;
     }
-    if (max_splits > 1) {
+    if (d.n_seqs > 65535) return set_error(GLA_ERR_INVALID, "decode: n_seqs %d > 65535", d.n_seqs);
+    if (max_splits > 65535) return set_error(GLA_ERR_INVALID, "decode: %d splits per sequence > 65535", max_splits);
+    if (max_splits > 1 || behind) {
         const size_t slots = (size_t)units * max_splits;
         const size_t acc_b = slots * gt * D * sizeof(float);
         const size_t ml_b = slots * 32 * sizeof(float);
         void *scr = nullptr;
-        int rc = decode_scratch(ctx, d, acc_b + ml_b, &scr);
+        int rc = decode_scratch(ctx, d, acc_b + ml_b + prefix_bytes(d), &scr);
         if (rc != GLA_OK) return rc;
         prm.part_acc = (float *)scr;
         prm.part_ml = (float *)((uint8_t *)scr + acc_b);
+        if (behind) {
+            rc = launch_prefix(ctx, d, (uint8_t *)scr + acc_b + ml_b, &prm.pre);
+            if (rc != GLA_OK) return rc;
+        }
     }
-    if (d.n_seqs > 65535) return set_error(GLA_ERR_INVALID, "decode: n_seqs %d > 65535", d.n_seqs);
-    if (max_splits > 65535) return set_error(GLA_ERR_INVALID, "decode: %d splits per sequence > 65535", max_splits);
     dim3 grid(d.n_kv_heads * n_hg, max_splits, d.n_seqs);
     switch (D) {
     case 64:

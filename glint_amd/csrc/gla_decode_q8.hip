@@ -100,7 +100,8 @@ struct Q8Params {
     // past a sequence's end (n_rows > 0; grid (units, n_rows, 1)). Else
     // n_rows = 0 and the grid is (units, max_wg, n_seqs).
     int n_rows;
-    int n_sinks;  // SINKS kernels: first positions seen beside the window
+    int n_sinks;       // kWindowSinks
+    PrefixLaunch pre;  // kBehindPrefix: every workgroup leaves a partial, merged with the prefix's by the combine kernel
     uint16_t rows[kMaxRows];
 };
 
@@ -108,15 +109,17 @@ struct Range {
     int start, end;  // positions [start, end)
     int fp;          // first logical page
     int n_pages;
-    Visible v;       // SINKS kernels (fp is 0: pages are numbered as Visible does)
+    Visible v;       // but for kWindow (fp is 0: pages are numbered as Visible does)
+    int prefix;      // kBehindPrefix: positions that the prefix's partials hold
 };
 
-template <bool SINKS>
+template <DecodeMode MODE>
 __device__ __forceinline__ Range seq_range(const Q8Params &p, int b) {
     Range r;
     int s = p.kv_start[b];
-    if constexpr (SINKS) {
-        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, p.n_sinks, 0);
+    if constexpr (MODE != kWindow) {
+        r.prefix = MODE == kBehindPrefix ? row_prefix(p.pre, b) : 0;
+        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, MODE == kWindowSinks ? p.n_sinks : 0, r.prefix);
         r.start = r.v.start;
         r.end = r.v.end;
         r.fp = 0;
@@ -455,7 +458,7 @@ struct StepConst {
     float sm, kvs, softcap, qcap;
     bool cap;
     int pg0, npg, start, end;
-    Visible v;  // SINKS kernels
+    Visible v;  // but for kWindow
     int kg, ph;
     float pf;  // this lane's piece (0: hi, 1: lo) as a float
 };
@@ -471,7 +474,7 @@ struct StepState {
 // head): S = K.Q, the soft-cap, the window mask and the online softmax.
 // Leaves in pr the probabilities of the lane's four P' positions and in
 // vbad the positions whose V scale must be ignored (bit i).
-template <int D, bool SINKS>
+template <int D, DecodeMode MODE>
 __device__ __forceinline__ void step_qk(const RawK<D> &cur, int step, const StepConst<D> &c, StepState<D> &st,
                                         float (&pr)[4], int &vbad) {
     constexpr int NB = D / 32;
@@ -517,7 +520,7 @@ __device__ __forceinline__ void step_qk(const RawK<D> &cur, int step, const Step
     // on the lane's own page, are flagged so that their V scale is zeroed and
     // a non-finite scale of an unused position cannot reach the output.
     vbad = 0;
-    if constexpr (SINKS) {
+    if constexpr (MODE != kWindow) {
         const int pa = c.v.page(c.pg0 + 2 * step), pb = c.v.page(c.pg0 + 2 * step + 1);
         const bool two = 2 * step + 1 < c.npg;  // (else page 1 repeats page 0's data)
         if (!(c.v.whole(pa) && two && c.v.whole(pb))) {
@@ -612,7 +615,7 @@ __device__ __forceinline__ void step_pv(RawV<D> &cur, const StepConst<D> &c, Ste
 // One wave's chunk: flash attention of the group's q-heads over `ch` pages;
 // leaves O (unnormalised, true scale), m and l of each head at the start of
 // the wave's LDS slot ([kGT][D + 2] floats).
-template <int D, bool SINKS>
+template <int D, DecodeMode MODE>
 __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, int b, int kvh, int h_base,
                                            int gcount, int pg0, int npg, int lane, uint8_t *slot) {
     constexpr int NB = D / 32;  // Q8_0 blocks per head row
@@ -638,7 +641,7 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
     }
     // physical page of chunk page `lane` (clamped into the pool by map_page)
     int pid_l;
-    if constexpr (SINKS) {
+    if constexpr (MODE != kWindow) {
         // (a chunk on one side of the gap is as one without sinks)
         const bool astride = pg0 < r.v.head && pg0 + npg > r.v.head;
         pid_l = p.pm.page_table && p.pm.pt_stride >= 16 && !astride
@@ -758,7 +761,7 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
     c.npg = npg;
     c.start = r.start;
     c.end = r.end;
-    if constexpr (SINKS) c.v = r.v;
+    if constexpr (MODE != kWindow) c.v = r.v;
     c.kg = kg;
     c.ph = ph;
     c.pf = (float)piece;
@@ -781,7 +784,7 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
         }
         float pr[4];
         int vbad;
-        step_qk<D, SINKS>(kr, step, c, st, pr, vbad);
+        step_qk<D, MODE>(kr, step, c, st, pr, vbad);
         // the V half of `step` has landed; only the next K half may be in flight
         if (next)
             wait_vmem<NL>();
@@ -847,7 +850,7 @@ __host__ __device__ __forceinline__ int wg_span(int n, int full, int D) {
 // One workgroup item: (sequence b, its workgroup wg, KV head x head group hx).
 // The 4 waves take 4 consecutive chunks of the unit and merge them in LDS; a
 // unit longer than one workgroup writes one partial per workgroup.
-template <int D, bool SINKS>
+template <int D, DecodeMode MODE>
 __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlotBytesPerD * D], int b, int wg,
                                         int hx) {
     constexpr int kThreads = kWaves * 64;
@@ -861,9 +864,9 @@ __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlo
     const int h_base = kvh * p.group + g0;
     float *out = p.out + ((int64_t)b * p.n_heads + h_base) * D;
 
-    const Range r = seq_range<SINKS>(p, b);
+    const Range r = seq_range<MODE>(p, b);
     if (r.n_pages == 0) {  // empty window: zero output (the reference's pre-zeroed buffer)
-        if (wg == 0)
+        if (MODE != kBehindPrefix && wg == 0)
             for (int idx = tid; idx < gcount * D; idx += kThreads) out[idx] = 0.0f;
         return;
     }
@@ -881,7 +884,7 @@ __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlo
     const int per_wave = ((wg_pages + 2 * kWaves - 1) / (2 * kWaves)) * 2;  // even: a step is two pages
     const int my0 = wave * per_wave;
     if (my0 < wg_pages) {
-        wave_chunk<D, SINKS>(p, r, b, kvh, h_base, gcount, r.fp + wg * span + my0, min(per_wave, wg_pages - my0), lane,
+        wave_chunk<D, MODE>(p, r, b, kvh, h_base, gcount, r.fp + wg * span + my0, min(per_wave, wg_pages - my0), lane,
                       slots[wave]);
     } else if (lane < kGT) {
         float *res = reinterpret_cast<float *>(slots[wave]);
@@ -930,7 +933,7 @@ __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlo
                 A.w = fmaf(res(w, g, d + 3), f, A.w);
             }
         }
-        if (n_wg == 1) {
+        if (MODE != kBehindPrefix && n_wg == 1) {
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
             if (g < gcount)
                 *reinterpret_cast<float4 *>(out + g * D + d) = make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
@@ -941,7 +944,7 @@ __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlo
     // The (m, l) of the partial fill one whole 128-byte line: m[kGT], l[kGT], zeros. (Partial
     // lines, and the partials' rows at a 520-byte stride, measured 3-12 us slower per cfg3 call:
     // sub-line writes cost a read-modify-write in HBM.)
-    if (n_wg > 1 && tid < 8) {
+    if ((MODE == kBehindPrefix || n_wg > 1) && tid < 8) {
         const float Ms = __shfl(Mg, tid & 3), Ls = __shfl(Lg, tid & 3);
         const float v = tid < kGT ? Ms : Ls;
         const float a0 = __shfl(v, 0), a1 = __shfl(v, 1), a2 = __shfl(v, 2), a3 = __shfl(v, 3);
@@ -963,7 +966,7 @@ __device__ __forceinline__ void q8_item(const Q8Params &p, uint8_t (*slots)[kSlo
 // The head index runs fastest, so the workgroups reading the 8 head spans of
 // the same pages are dispatched together and the DRAM rows those pages open
 // are read out while open (measured ~25% over chunk-fastest order).
-template <int D, bool SINKS>
+template <int D, DecodeMode MODE>
 __global__ __launch_bounds__(kWaves * 64) void decode_q8_mfma_kernel(const Q8Params p) {
     // per wave: the streaming slot, later the wave's [kGT][D + 2] result
     __shared__ __attribute__((aligned(16))) uint8_t slots[kWaves][kSlotBytesPerD * D];
@@ -977,7 +980,7 @@ __global__ __launch_bounds__(kWaves * 64) void decode_q8_mfma_kernel(const Q8Par
         b = blockIdx.z;
         wg = blockIdx.y;
     }
-    q8_item<D, SINKS>(p, slots, b, wg, blockIdx.x);
+    q8_item<D, MODE>(p, slots, b, wg, blockIdx.x);
 }
 
 // Merge of the workgroup partials of every unit with more than one
@@ -986,7 +989,7 @@ __global__ __launch_bounds__(kWaves * 64) void decode_q8_mfma_kernel(const Q8Par
 // partials; the per-element arithmetic is that of a scalar merge: eight
 // partials at a time, all loads of a batch in flight together, (M, L, A)
 // absorbing the batch with one rescale).
-template <int D, bool SINKS>
+template <int D, DecodeMode MODE>
 __global__ __launch_bounds__(kGT * D / 4) void decode_q8_combine_kernel(const Q8Params p) {
     const int b = blockIdx.y;
     const int kvh = blockIdx.x / p.n_hg;
@@ -994,10 +997,11 @@ __global__ __launch_bounds__(kGT * D / 4) void decode_q8_combine_kernel(const Q8
     const int g0 = hg * p.hpw;
     const int gcount = min(p.hpw, p.group - g0);
     const int h_base = kvh * p.group + g0;
-    const Range r = seq_range<SINKS>(p, b);
+    const Range r = seq_range<MODE>(p, b);
     const int span = wg_span(r.n_pages, kWaves * p.ch, D);  // pages per workgroup
     const int n_wg = min((r.n_pages + span - 1) / span, p.max_wg);
-    if (n_wg <= 1) return;
+    if (MODE != kBehindPrefix && n_wg <= 1) return;
+    const int n = n_wg + (MODE == kBehindPrefix ? prefix_splits(p.pre, r.prefix) : 0);
     const int g = (4 * (int)threadIdx.x) / D;
     const int d = 4 * (int)threadIdx.x - g * D;
     if (g >= gcount) return;
@@ -1006,18 +1010,26 @@ __global__ __launch_bounds__(kGT * D / 4) void decode_q8_combine_kernel(const Q8
     const float *hp = p.part + unit * p.max_wg * pstride;
     float M = -INFINITY, L = 0.0f;
     float4 A = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i0 = 0; i0 < n_wg; i0 += 8) {
+    for (int i0 = 0; i0 < n; i0 += 8) {
         float mi[8], li[8];
         float4 ai[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const int i = min(i0 + j, n_wg - 1);
-            const bool in = i0 + j < n_wg;
-            const float lv = hp[i * pstride + kGT * D + kGT + g];
-            const float4 av = *reinterpret_cast<const float4 *>(hp + i * pstride + g * D + d);
+            const int i = min(i0 + j, n - 1);
+            const bool in = i0 + j < n;
+            const float *ml = hp + i * pstride + kGT * D + g, *acc = hp + i * pstride + g * D + d;
+            int l_at = kGT;
+            if (MODE == kBehindPrefix && i >= n_wg) {
+                const int64_t at = ((int64_t)(i - n_wg) * gridDim.y + b) * p.n_heads + h_base + g;
+                ml = p.pre.ml + 2 * at;
+                acc = p.pre.acc + at * D + d;
+                l_at = 1;
+            }
+            const float lv = ml[l_at];
+            const float4 av = *reinterpret_cast<const float4 *>(acc);
             // an entry past the last partial reloads the last one and adds
             // nothing (not 0 x its sums: an infinity there would make NaN)
-            mi[j] = in ? hp[i * pstride + kGT * D + g] : -INFINITY;
+            mi[j] = in ? ml[0] : -INFINITY;
             li[j] = in ? lv : 0.0f;
             ai[j] = in ? av : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
@@ -1050,13 +1062,13 @@ __global__ __launch_bounds__(kGT * D / 4) void decode_q8_combine_kernel(const Q8
         make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
 }
 
-template <int D, bool SINKS>
+template <int D, DecodeMode MODE>
 int launch_as(gla_ctx *ctx, const Q8Params &prm, dim3 grid, int n_seqs) {
-    hipLaunchKernelGGL((decode_q8_mfma_kernel<D, SINKS>), grid, dim3(kWaves * 64), 0, ctx->stream, prm);
+    hipLaunchKernelGGL((decode_q8_mfma_kernel<D, MODE>), grid, dim3(kWaves * 64), 0, ctx->stream, prm);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "decode_q8_mfma_kernel launch: %s", hipGetErrorString(e));
-    if (prm.max_wg > 1) {
-        hipLaunchKernelGGL((decode_q8_combine_kernel<D, SINKS>), dim3(prm.n_kv_heads * prm.n_hg, n_seqs),
+    if (MODE == kBehindPrefix || prm.max_wg > 1) {
+        hipLaunchKernelGGL((decode_q8_combine_kernel<D, MODE>), dim3(prm.n_kv_heads * prm.n_hg, n_seqs),
                            dim3(kGT * D / 4), 0, ctx->stream, prm);
         e = hipGetLastError();
         if (e != hipSuccess)
@@ -1067,7 +1079,9 @@ int launch_as(gla_ctx *ctx, const Q8Params &prm, dim3 grid, int n_seqs) {
 
 template <int D>
 int launch_d(gla_ctx *ctx, const Q8Params &prm, dim3 grid, int n_seqs) {
-    return prm.n_sinks > 0 ? launch_as<D, true>(ctx, prm, grid, n_seqs) : launch_as<D, false>(ctx, prm, grid, n_seqs);
+    if (prm.pre.n_groups > 0) return launch_as<D, kBehindPrefix>(ctx, prm, grid, n_seqs);
+    return prm.n_sinks > 0 ? launch_as<D, kWindowSinks>(ctx, prm, grid, n_seqs)
+                           : launch_as<D, kWindow>(ctx, prm, grid, n_seqs);
 }
 
 // Workgroups of decode_q8_mfma_kernel<D> one CU holds at once (0 on error).
@@ -1076,7 +1090,7 @@ int resident_wgs() {
     static int cached = -1;
     if (cached < 0) {
         int n = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_q8_mfma_kernel<D, false>, kWaves * 64, 0) != hipSuccess)
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_q8_mfma_kernel<D, kWindow>, kWaves * 64, 0) != hipSuccess)
             n = 0;
         cached = n;
     }
@@ -1125,7 +1139,7 @@ int launch_decode_q8(gla_ctx *ctx, const DecodeLaunch &d) {
     const int group = d.n_heads / d.n_kv_heads;
     // pages a window can span (a start inside a page adds one), and its sinks'
     const int64_t max_pages = max_window_pages(d);
-    const bool host = d.kv_len_host != nullptr;
+    const bool host = has_host_pages(d);
     auto pages_of = [&](int b) -> int {
         return host ? host_pages(d, b) : (int)max_pages;
     };
@@ -1172,6 +1186,8 @@ int launch_decode_q8(gla_ctx *ctx, const DecodeLaunch &d) {
     prm.max_wg = (int)std::min<int64_t>(max_wg, 1 << 30);
     prm.max_len = d.max_kv_len;
     prm.n_sinks = d.n_sinks;
+    prm.pre = d.pre;
+    const bool behind = decode_mode(d) == kBehindPrefix;
     const bool cap = d.softcap > 0.0f;
     prm.q_mul = cap ? d.scale : d.scale * kLog2e;
     prm.softcap = cap ? d.softcap : 0.0f;
@@ -1179,12 +1195,16 @@ int launch_decode_q8(gla_ctx *ctx, const DecodeLaunch &d) {
     if (d.n_seqs > 65535) return set_error(GLA_ERR_INVALID, "decode: n_seqs %d > 65535", d.n_seqs);
     if (max_wg > 65535)
         return set_error(GLA_ERR_INVALID, "decode: %lld workgroups per sequence > 65535", (long long)max_wg);
-    if (max_wg > 1) {
+    if (max_wg > 1 || behind) {
         const size_t bytes = (size_t)units * max_wg * (kGT * D + 32) * sizeof(float);
         void *scr = nullptr;
-        int rc = decode_scratch(ctx, d, bytes, &scr);
+        int rc = decode_scratch(ctx, d, bytes + prefix_bytes(d), &scr);
         if (rc != GLA_OK) return rc;
         prm.part = (float *)scr;
+        if (behind) {
+            rc = launch_prefix(ctx, d, (uint8_t *)scr + bytes, &prm.pre);
+            if (rc != GLA_OK) return rc;
+        }
     }
     dim3 grid(d.n_kv_heads * n_hg, (unsigned)max_wg, d.n_seqs);
     // With the host lengths, list the workgroups that have pages (plus one per

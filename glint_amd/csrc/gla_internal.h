@@ -335,6 +335,42 @@ inline int host_seq_pages(int start, int len, int max_len, int pos_limit) {
     return e > s ? (int)(((e - 1) >> 4) - (s >> 4) + 1) : 0;
 }
 
+// A batch's groups of rows that share their first positions. The part before a group's
+// last whole page, prefix_positions, is attended by launch_prefix, for all rows of the
+// group at once, in n_splits splits of split_tiles tiles of 32 positions; each leaves
+// (m, l) and O, unnormalised in the log2 domain, of every row:
+//   acc [split][row][head_dim], ml [split][row] {m, l}, row = sequence * n_heads + head.
+struct PrefixLaunch {
+    const int32_t *group_start = nullptr;
+    const int32_t *prefix_len = nullptr;
+    int n_groups = 0;  // 0: the rows share nothing
+    int max_group = 0;
+    int max_prefix = 0;  // at most the storage's positions
+    int max_own = 0;
+    int split_tiles = 0, n_splits = 0;
+    float *acc = nullptr, *ml = nullptr;
+    const int32_t *group_start_host = nullptr, *prefix_len_host = nullptr;
+};
+__host__ __device__ __forceinline__ int prefix_positions(int len, int max_prefix) {
+    return (len < 0 ? 0 : (len > max_prefix ? max_prefix : len)) & ~15;
+}
+__host__ __device__ __forceinline__ int prefix_splits(const PrefixLaunch &p, int positions) {
+    return ((positions + 31) / 32 + p.split_tiles - 1) / p.split_tiles;
+}
+// Positions that row b shares with its group, found by every wave on its own (all lanes
+// call it): the last group that starts at or before b holds it, if it has not ended.
+__device__ __forceinline__ int row_prefix(const PrefixLaunch &p, int b) {
+    const int lane = threadIdx.x & 63;
+    int g = -1;
+    for (int i = 0; i < p.n_groups; i += 64) {
+        const uint64_t before = __ballot(i + lane < p.n_groups && p.group_start[min(i + lane, p.n_groups)] <= b);
+        g += __popcll(before);
+        if (before != ~0ull) break;
+    }
+    if (g < 0 || p.group_start[g + 1] <= b) return 0;
+    return prefix_positions(p.prefix_len[g], p.max_prefix);
+}
+
 // Launchers (return GLA_OK or an error code with the message set).
 struct DecodeLaunch {
     KvLayout kv;
@@ -364,17 +400,44 @@ struct DecodeLaunch {
     size_t arrivals_cap = 0;
     // > 0: the first positions of a sequence that stay visible beside its window
     int n_sinks = 0;
+    // groups of rows that share their first positions (gla_decode_shared)
+    PrefixLaunch pre;
 };
-// Pages a sequence of the launch can have to read, from the bounds alone and from its host lengths.
+// Sets the splits of a launch's prefixes, and what they leave in scratch.
+void plan_prefix(const gla_ctx *ctx, DecodeLaunch *d);
+inline size_t prefix_bytes(const DecodeLaunch &d) {
+    return (size_t)d.pre.n_splits * d.n_seqs * d.n_heads * (d.head_dim + 2) * sizeof(float);
+}
+// Attends d.pre; *pre is d.pre with its partials' places at `scratch` (prefix_bytes).
+int launch_prefix(gla_ctx *ctx, const DecodeLaunch &d, void *scratch, PrefixLaunch *pre);
+// What a decode kernel's sequences read: their window, their window and sinks, or their
+// window behind the prefix that launch_prefix reads. A template argument of the kernels.
+enum DecodeMode { kWindow = 0, kWindowSinks = 1, kBehindPrefix = 2 };
+inline DecodeMode decode_mode(const DecodeLaunch &d) {
+    return d.pre.n_groups > 0 ? kBehindPrefix : (d.n_sinks > 0 ? kWindowSinks : kWindow);
+}
+// Pages a sequence of the launch can have to read, from the bounds alone and from its host
+// lengths, where there are all that it takes.
 inline int max_window_pages(const DecodeLaunch &d) {
     const int window = d.max_kv_len > 0 ? (d.max_kv_len + GLA_PAGE_SIZE - 1) / GLA_PAGE_SIZE + 1 : 1;
     const int sinks = (std::min(d.n_sinks, d.pm.pos_limit) + GLA_PAGE_SIZE - 1) / GLA_PAGE_SIZE;
-    return d.n_sinks > 0 ? window + sinks : window;
+    // (a prefix that ends inside a page leaves up to 15 positions more)
+    const int own = (int)std::min<int64_t>(window, ((int64_t)d.pre.max_own + 2 * GLA_PAGE_SIZE - 2) / GLA_PAGE_SIZE);
+    return d.pre.n_groups > 0 ? std::max(own, 1) : (d.n_sinks > 0 ? window + sinks : window);
+}
+inline bool has_host_pages(const DecodeLaunch &d) {
+    return d.kv_len_host && (d.pre.n_groups == 0 || d.pre.group_start_host);
 }
 inline int host_pages(const DecodeLaunch &d, int b) {
-    if (d.n_sinks > 0)
-        return visible_of(d.kv_start_host[b], d.kv_len_host[b], d.max_kv_len, d.pm.pos_limit, d.n_sinks, 0).n_pages;
-    return host_seq_pages(d.kv_start_host[b], d.kv_len_host[b], d.max_kv_len, d.pm.pos_limit);
+    const int start = d.kv_start_host[b], len = d.kv_len_host[b];
+    if (d.pre.n_groups > 0) {  // (row_prefix on the host)
+        const int32_t *at = d.pre.group_start_host;
+        const int g = (int)(std::upper_bound(at, at + d.pre.n_groups, b) - at) - 1;
+        const int from = g < 0 || at[g + 1] <= b ? 0 : prefix_positions(d.pre.prefix_len_host[g], d.pre.max_prefix);
+        return std::min(visible_of(start, len, d.max_kv_len, d.pm.pos_limit, 0, from).n_pages, max_window_pages(d));
+    }
+    if (d.n_sinks > 0) return visible_of(start, len, d.max_kv_len, d.pm.pos_limit, d.n_sinks, 0).n_pages;
+    return host_seq_pages(start, len, d.max_kv_len, d.pm.pos_limit);
 }
 // Device scratch of a decode launch: d.scratch (no allocation) or the
 // context's buffer for its current stream.
