@@ -809,10 +809,9 @@ int gla_decode_shared(gla_ctx *ctx, const gla_decode_shared_args *a) {
     d.pre.max_own = a->max_own_len;
     d.pre.group_start_host = a->group_start_host;
     d.pre.prefix_len_host = a->prefix_len_host;
-    // rows that share nothing are read one by one
-    if (a->n_groups > 0 && d.pre.max_group > 1 && d.pre.max_prefix > 0) {
+    if (a->n_groups > 0 && d.pre.max_group > 1) {
         d.pre.n_groups = a->n_groups;
-        plan_prefix(ctx, &d);
+        plan_prefix(ctx, &d);  // (or not: short prefixes are read row by row)
     }
     return launch_decode(ctx, d);
     GLA_GUARD_END

@@ -337,8 +337,8 @@ inline int host_seq_pages(int start, int len, int max_len, int pos_limit) {
 
 // A batch's groups of rows that share their first positions. The part before a group's
 // last whole page, prefix_positions, is attended by launch_prefix, for all rows of the
-// group at once, in n_splits splits of split_tiles tiles of 32 positions; each leaves
-// (m, l) and O, unnormalised in the log2 domain, of every row:
+// group at once, in n_splits splits of split_pages pages; each leaves (m, l)
+// and O, unnormalised in the log2 domain, of every row:
 //   acc [split][row][head_dim], ml [split][row] {m, l}, row = sequence * n_heads + head.
 struct PrefixLaunch {
     const int32_t *group_start = nullptr;
@@ -347,7 +347,7 @@ struct PrefixLaunch {
     int max_group = 0;
     int max_prefix = 0;  // at most the storage's positions
     int max_own = 0;
-    int split_tiles = 0, n_splits = 0;
+    int split_pages = 0, n_splits = 0;
     float *acc = nullptr, *ml = nullptr;
     const int32_t *group_start_host = nullptr, *prefix_len_host = nullptr;
 };
@@ -355,7 +355,7 @@ __host__ __device__ __forceinline__ int prefix_positions(int len, int max_prefix
     return (len < 0 ? 0 : (len > max_prefix ? max_prefix : len)) & ~15;
 }
 __host__ __device__ __forceinline__ int prefix_splits(const PrefixLaunch &p, int positions) {
-    return ((positions + 31) / 32 + p.split_tiles - 1) / p.split_tiles;
+    return (positions / 16 + p.split_pages - 1) / p.split_pages;
 }
 // Positions that row b shares with its group, found by every wave on its own (all lanes
 // call it): the last group that starts at or before b holds it, if it has not ended.
@@ -403,8 +403,9 @@ struct DecodeLaunch {
     // groups of rows that share their first positions (gla_decode_shared)
     PrefixLaunch pre;
 };
-// Sets the splits of a launch's prefixes, and what they leave in scratch.
+// Decides whether d->pre is attended apart (n_groups 0 if not) and sets its splits.
 void plan_prefix(const gla_ctx *ctx, DecodeLaunch *d);
+// What launch_prefix leaves in scratch.
 inline size_t prefix_bytes(const DecodeLaunch &d) {
     return (size_t)d.pre.n_splits * d.n_seqs * d.n_heads * (d.head_dim + 2) * sizeof(float);
 }

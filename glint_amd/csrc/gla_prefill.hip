@@ -12,38 +12,29 @@
 //   O^T[d][query]  += V^T . P^T    P^T is packed from the lane's S^T
 //                                  accumulators: V's pieces hold the keys in
 //                                  that order, so no value changes its lane.
-// Two more operators are this code with another value of GLA_PREFILL_MODE, in translation
-// units of their own, so that a plain prefill runs what it would without them:
-//   SINKS (gla_prefill_sinks.hip): rows see the first n_sinks positions beside their
-//     window; the tiles of the sinks come before the window's in every list of tiles
-//     (TileList).
-//   PREFIX (gla_decode_prefix.hip): the rows are the queries of a group of sequences that
-//     decode one token each, the keys the prefix they share, cut in splits; every row
-//     leaves a split's (m, l, O) for the decode's merge instead of an output. Only the
-//     fp32 kernel that converts its own tiles is built.
+// Sinks. The same code once more, with GLA_PREFILL_SINKS 1 (gla_prefill_sinks.hip),
+// is the prefill whose rows see the first n_sinks positions beside their window: the
+// tiles of the sinks come before the window's in every list of tiles (TileList). A
+// compile-time switch, so that a call without sinks runs what it ran before.
 #include <math.h>
 
 #include <algorithm>
 #include <type_traits>
 
 #include "gla_internal.h"
+#include "gla_lanes.h"
 
-#define GLA_PREFILL_PLAIN 0
-#define GLA_PREFILL_SINKS 1
-#define GLA_PREFILL_PREFIX 2
-#ifndef GLA_PREFILL_MODE
-#define GLA_PREFILL_MODE GLA_PREFILL_PLAIN
+#ifndef GLA_PREFILL_SINKS
+#define GLA_PREFILL_SINKS 0
 #endif
 
 namespace gla {
 
 namespace {
 
-constexpr bool kSinks = GLA_PREFILL_MODE == GLA_PREFILL_SINKS;
-constexpr bool kPrefix = GLA_PREFILL_MODE == GLA_PREFILL_PREFIX;
+constexpr bool kSinks = GLA_PREFILL_SINKS;
 
 constexpr int KT = 32;  // keys per tile
-constexpr float kLog2e = 1.4426950408889634f;
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
@@ -64,76 +55,6 @@ struct PrefillParams {
     float softcap;     // > 0: cap * tanh(s / cap)
     int sliding_window;
     int n_sinks;  // kSinks: first positions seen beside the window
-#if GLA_PREFILL_MODE == GLA_PREFILL_PREFIX
-    PrefixLaunch pre;
-    const int32_t *kv_start;  // of the batch's rows, with the decode's clamping
-    const int32_t *kv_len;
-    int max_kv_len;
-    int n_seqs;
-#endif
-};
-
-__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// max of two floats as IEEE-754 maximum (a NaN operand gives NaN): gfx950
-// has v_maximum3_f32, which needs no NaN-quieting max per operand the way
-// fmaxf does after a row swap or a select. Not inline asm: the compiler
-// inserts the wait states an MFMA result needs before a VALU read only for
-// instructions it emits itself, and these maxima read MFMA results directly.
-__device__ __forceinline__ float max2f(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-
-// max / sum over the four 16-lane rows (lane ^ 16, lane ^ 32) with the gfx950
-// row swaps: VALU only, no LDS round trip.
-__device__ __forceinline__ float max_rows4(float x) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = max2f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return max2f(__uint_as_float(c[0]), __uint_as_float(c[1]));
-}
-__device__ __forceinline__ float sum_rows4(float x) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(c[0]) + __uint_as_float(c[1]);
-}
-
-// max / min of unsigned words over the wave, in every lane: DPP rotations within
-// each 16-lane row, then the row swaps.
-template <bool MAX>
-__device__ __forceinline__ uint32_t wave_extreme(uint32_t x) {
-    const auto pick = [](uint32_t a, uint32_t b) { return MAX ? max(a, b) : min(a, b); };
-    x = pick(x, __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, true));  // row_ror 1, 2, 4, 8
-    x = pick(x, __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, true));
-    x = pick(x, __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, true));
-    x = pick(x, __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true));
-    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    x = pick(a[0], a[1]);
-    const auto c = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return pick(c[0], c[1]);
-}
-__device__ __forceinline__ uint32_t umax_rows4(uint32_t x) {
-    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    x = max(a[0], a[1]);
-    const auto c = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return max(c[0], c[1]);
-}
-
-// cap * tanh(x / cap) * log2(e), without the long division sequences: x / cap
-// by the reciprocal of cap and one correction, 1 / (1 + t) by v_rcp_f32 and one
-// Newton step (each then within an ulp).
-struct SoftCap {
-    float cap, inv, out;
-    __device__ __forceinline__ explicit SoftCap(float c) : cap(c), inv(1.0f / c), out(c * kLog2e) {}
-    __device__ __forceinline__ float operator()(float x) const {
-        const float q = x * inv;
-        // past 16 tanh is 1, and an infinite score has no remainder
-        const float y = fabsf(q) < 16.0f ? fmaf(fmaf(-cap, q, x), inv, q) : q;
-        const float t = fast_exp2(-2.0f * kLog2e * fabsf(y));
-        const float d = 1.0f + t;
-        float r = __builtin_amdgcn_rcpf(d);
-        r = fmaf(fmaf(-d, r, 1.0f), r, r);
-        return copysignf((1.0f - t) * r * out, x);
-    }
 };
 
 // Whether key kp is in [lo, hi], or is a sink not past hi.
@@ -199,17 +120,6 @@ struct TileList {
     __device__ __forceinline__ int key0(int i) const { return (first + i + (kSinks && i >= head ? gap : 0)) * KT; }
 };
 
-typedef _Float16 half8p __attribute__((ext_vector_type(8)));
-// max of three floats as one v_maximum3_f32 (as max2f)
-__device__ __forceinline__ float max3f(float a, float b, float c) { return max2f(max2f(a, b), c); }
-// Whether every row of a wave sees the whole tile at k0: the keys up to `hi` are behind
-// its first row, pos_last is its last row's position.
-__device__ __forceinline__ bool inside(const PrefillParams &p, int k0, int klo, int hi, int pos_last) {
-    if (kSinks && k0 + KT <= p.n_sinks) return k0 + KT - 1 <= hi;
-    return k0 >= klo && k0 + KT - 1 <= hi && (p.sliding_window <= 0 || k0 >= window_lo(pos_last, p.sliding_window));
-}
-
-#if GLA_PREFILL_MODE != GLA_PREFILL_PREFIX
 // ---------------------------------------------------------------------------
 // bf16-input variant: Q, K, V and the probabilities are rounded to bf16 and
 // both products run on v_mfma_f32_16x16x32_bf16 with fp32 accumulation; the
@@ -228,6 +138,13 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 template <int D>
 constexpr int kKRowH = D + 8;  // K row in LDS (bf16): 16 bytes of padding
 constexpr int kVtRowH = KT + 8;  // Vt row in LDS (bf16): 32 keys + 16 bytes
+
+// Whether every row of a wave sees the whole tile at k0: the keys up to `hi` are behind
+// its first row, pos_last is its last row's position.
+__device__ __forceinline__ bool inside(const PrefillParams &p, int k0, int klo, int hi, int pos_last) {
+    if (kSinks && k0 + KT <= p.n_sinks) return k0 + KT - 1 <= hi;
+    return k0 >= klo && k0 + KT - 1 <= hi && (p.sliding_window <= 0 || k0 >= window_lo(pos_last, p.sliding_window));
+}
 
 // The 4 keys x 4 dims block of K and of V that one thread stages, as f32.
 struct Block44 {
@@ -366,6 +283,9 @@ __device__ __forceinline__ void bf16_score_init(floatx4 (&sacc)[2][NT]) {
 #pragma unroll
         for (int mt = 0; mt < 2; mt++) sacc[mt][nt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 }
+
+// max of three floats as one v_maximum3_f32 (as max2f)
+__device__ __forceinline__ float max3f(float a, float b, float c) { return max2f(max2f(a, b), c); }
 
 // Online softmax of one 32-key tile of the bf16 kernels (both share it):
 // soft-cap and (MASK) the causal/window mask, the lazy maximum (the reference
@@ -890,8 +810,6 @@ __global__ __launch_bounds__(kBf16sWaves<D> * 64, kBf16sOccupancy<D>) void prefi
     }
 }
 
-#endif  // not PREFIX
-
 // ---------------------------------------------------------------------------
 // fp32 prefill on the f16 matrix cores. Every f32 operand is two f16 pieces
 // after a power-of-two scaling, hi = f16(x) and lo = f16((x - hi) * 2^11): 22
@@ -928,6 +846,7 @@ __global__ __launch_bounds__(kBf16sWaves<D> * 64, kBf16sOccupancy<D>) void prefi
 // differs, 410 with a NaN in V, 430 with a small value, 500 where every tile's keys differ, 1,400 with every
 // 16th dim of V at 2^-34 of the others, 2,200 with eight dims of every key at 2^-30
 // (f32 MFMAs for everything: 1,080).
+typedef _Float16 half8p __attribute__((ext_vector_type(8)));
 
 // instruction groups for the scheduler: MFMAs, LDS reads
 constexpr int kSchedMfma = 0x8, kSchedLds = 0x100;
@@ -1326,7 +1245,6 @@ struct SplitTile {
     }
 };
 
-#if GLA_PREFILL_MODE != GLA_PREFILL_PREFIX
 // The tiles that some query of sequence b attends.
 struct SeqKeys {
     int lo, hi;  // the keys: [lo, hi], hi < 0 if there are none
@@ -1340,19 +1258,6 @@ struct SeqKeys {
 struct SeqTiles : SeqKeys, TileList {
     __device__ __forceinline__ SeqTiles(const PrefillParams &p, int b) : SeqKeys(p, b), TileList(lo, hi, p.n_sinks) {}
 };
-
-#else
-// The prefix's keys [0, hi] and the rows, from `member` on, of group g.
-struct SeqTiles {
-    int lo, hi, member, members, gap = 0, count = 0, first = 0;
-    __device__ __forceinline__ SeqTiles(const PrefillParams &p, int g) {
-        lo = 0;
-        hi = prefix_positions(p.pre.prefix_len[g], p.pre.max_prefix) - 1;
-        member = min(max(p.pre.group_start[g], 0), p.n_seqs);
-        members = min(max(min(p.pre.group_start[g + 1], p.n_seqs) - member, 0), p.pre.max_group);
-    }
-};
-#endif
 
 // Where the tile images of a (sequence, KV head) pair are. `start` null: every
 // pair has `stride` places. Else the attended tiles of all pairs are numbered one
@@ -1379,7 +1284,6 @@ struct Images {
     }
 };
 
-#if GLA_PREFILL_MODE != GLA_PREFILL_PREFIX
 // start[b] of every sequence. One workgroup; a call that has a place for every
 // tile its storage could have it attend does without.
 __global__ __launch_bounds__(1024) void image_start_kernel(const PrefillParams p, int n_seqs, int64_t *start) {
@@ -1544,8 +1448,6 @@ __global__ __launch_bounds__(256) void stage_bf16_kernel(const PrefillParams p, 
     }
 }
 
-#endif  // not PREFIX
-
 // Waves per SIMD the kernel's registers are sized for; LDS holds two tiles of
 // a workgroup: d = 64 32 KB, d = 128 64 KB, d = 256 128 KB. A workgroup that
 // converts its own tiles holds one image and the conversion's buffers, and the
@@ -1568,58 +1470,34 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
     constexpr int LDS = std::max(STAGED ? METAS + 2 * (int)sizeof(TileMeta) : AUX, NW * 16 * SROW * 4);
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
 
-    const int n_hgrp = kPrefix ? 1 : p.group / p.hpw;
+    const int n_hgrp = p.group / p.hpw;
     const int pair = (int)blockIdx.x / n_hgrp;
-    const int item = pair / p.n_kv_heads;  // the sequence, or the group
-    const int kvh = pair - item * p.n_kv_heads;
+    const int b = pair / p.n_kv_heads;
+    const int kvh = pair - b * p.n_kv_heads;
     const int hgrp = (int)blockIdx.x - pair * n_hgrp;
-    const int qblk = kPrefix ? (int)blockIdx.y : p.n_qblocks - 1 - (int)(blockIdx.z * gridDim.y + blockIdx.y);
-    const int waves_per_head = kPrefix ? NW : NW / p.hpw;
+    const int qblk = p.n_qblocks - 1 - (int)(blockIdx.z * gridDim.y + blockIdx.y);
+    const int waves_per_head = NW / p.hpw;
     const int qwg = QW * waves_per_head;
 
-#if GLA_PREFILL_MODE == GLA_PREFILL_PREFIX
-    // row r: query head r % group of the KV head, of sequence r / group of the group
-    const SeqTiles seq(p, item);
-    const int b = seq.member;  // whose pages are read
-    const int q_len = seq.members * p.group;
-    const int qb0 = qblk * qwg;
-    const int all = (seq.hi + KT) / KT, t0 = (int)blockIdx.z * p.pre.split_tiles;
-    if (qb0 >= q_len || t0 >= all) return;
-    const auto row_of = [&](int r) { return (b + r / p.group) * p.n_heads + kvh * p.group + r % p.group; };
-    const auto q_of = [&](const PrefillParams &a, int r) __attribute__((always_inline)) {
-        return a.q + (int64_t)((b + r / a.group) * a.n_heads + kvh * a.group + r % a.group) * D;
-    };
-#else
-    const int b = item;
     const int row0 = p.q_start[b];
     const int q_len = min(max(p.q_start[b + 1] - row0, 0), p.max_q_len);
     const int pos0 = p.pos_offset[b];
     const int qb0 = qblk * qwg;
     if (qblk < 0 || qb0 >= q_len) return;
     const SeqTiles seq(p, b);
-#endif
-    if (!kPrefix && (STAGED ? !im.here(b, kvh, seq.count) : !im.nowhere(b, kvh, seq.count))) return;  // another launch's
+    if (STAGED ? !im.here(b, kvh, seq.count) : !im.nowhere(b, kvh, seq.count)) return;  // another launch's
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lrow = lane & 15;
     const int lgrp = lane >> 4;
-#if GLA_PREFILL_MODE == GLA_PREFILL_PREFIX
-    const int wq0 = qb0 + wave * QW;
-    const int khi = min(seq.hi, (t0 + p.pre.split_tiles) * KT - 1);
-    const int klo = t0 * KT;
-#else
     const int head = kvh * p.group + hgrp * p.hpw + (wave % p.hpw);
     const int wq0 = qb0 + (wave / p.hpw) * QW;
-    const auto q_of = [&](const PrefillParams &a, int r) __attribute__((always_inline)) {
-        return a.q + ((int64_t)(row0 + r) * a.n_heads + head) * D;
-    };
 
     const int q_last = min(q_len, qb0 + qwg) - 1;
     const int khi = min(pos0 + q_last, p.pm.pos_limit - 1);
     const int klo = window_lo(pos0 + qb0, p.sliding_window);
-#endif
     const TileList tiles(klo, khi, p.n_sinks);
     const int tfirst = tiles.first;
     const int n = tiles.count;
@@ -1669,7 +1547,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
     for (int nt = 0; nt < NT; nt++) {
         const int lq = wq0 + nt * 16 + lrow;
         const bool ok = lq < q_len;
-        const float *qp = q_of(p, ok ? lq : 0);
+        const float *qp = p.q + ((int64_t)(row0 + (ok ? lq : 0)) * p.n_heads + head) * D;
         float x[KS][8];
         uint32_t run[KS], top = 0;
 #pragma unroll
@@ -1709,40 +1587,12 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
         weight[nt] = (float)(1 << kScaleP);
         m[nt] = kMLowest;  // finite: the first attended key is an ordinary move of the reference
         const int lq = wq0 + nt * 16 + lrow;
-#if GLA_PREFILL_MODE == GLA_PREFILL_PREFIX
-        qpos[nt] = -1;
-        qlo[nt] = 0;
-        if (lq < q_len) {
-            const int r = b + lq / p.group;
-            const Visible v = visible_of(p.kv_start[r], p.kv_len[r], p.max_kv_len, p.pm.pos_limit, 0, 0);
-            qlo[nt] = v.start;
-            qpos[nt] = v.n_pages ? v.end - 1 : -1;
-        }
-#else
         qpos[nt] = lq < q_len ? pos0 + lq : -1;
         qlo[nt] = window_lo(pos0 + lq, p.sliding_window);
-#endif
     }
-#if GLA_PREFILL_MODE == GLA_PREFILL_PREFIX
-    // keys that some row of the wave attends: [wlo, whi]; that all of them do: [ilo, ihi]
-    int whi = -1, wlo = 0x7fffffff, ihi = khi, ilo = klo;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        whi = max(whi, (int)wave_extreme<true>((uint32_t)(qpos[nt] + 1)) - 1);
-        wlo = min(wlo, (int)wave_extreme<false>((uint32_t)(qpos[nt] < 0 ? 0x7fffffff : qlo[nt])));
-        const bool is_row = wq0 + nt * 16 + lrow < q_len;
-        ihi = min(ihi, (int)wave_extreme<false>((uint32_t)(is_row ? qpos[nt] + 1 : 0x7fffffff)) - 1);
-        ilo = max(ilo, (int)wave_extreme<true>((uint32_t)(is_row ? qlo[nt] : 0)));
-    }
-    whi = __builtin_amdgcn_readfirstlane(whi);
-    wlo = __builtin_amdgcn_readfirstlane(wlo);
-    ihi = __builtin_amdgcn_readfirstlane(ihi);
-    ilo = __builtin_amdgcn_readfirstlane(ilo);
-#else
     // keys this wave's queries attend: [wlo, whi]
     const int whi = min(khi, pos0 + wq0 + QW - 1);
     const int wlo = max(klo, window_lo(pos0 + wq0, p.sliding_window));
-#endif
 
     // The rare path reads the arguments again: held for it over the tiles that
     // need none, they and what follows from them crowd the other registers.
@@ -1762,7 +1612,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const int lq = min(wq0 + nt * 16 + lrow, q_len - 1);  // (a row past the end has no result)
-            qp[nt] = q_of(*a, lq) + lgrp * (D / 4);
+            qp[nt] = a->q + ((int64_t)(row0 + lq) * a->n_heads + head) * D + lgrp * (D / 4);
         }
         floatx4 e[2][NT];
 #pragma unroll
@@ -1904,11 +1754,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
         }
 
         // softmax: as the bf16 kernels' (a lazy maximum), in f32; c undoes the scales
-#if GLA_PREFILL_MODE == GLA_PREFILL_PREFIX
-        const bool interior = k0 >= ilo && k0 + KT - 1 <= ihi;
-#else
         const bool interior = inside(p, k0, klo, min(khi, pos0 + wq0), pos0 + wq0 + QW - 1);
-#endif
 #pragma unroll
         for (int mt = 0; mt < 2; mt++)
 #pragma unroll
@@ -2151,7 +1997,7 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         const float lt = sum_rows4(lpart[nt]);
-        const float inv = kPrefix ? 1.0f : lt > 0.0f ? 1.0f / lt : 0.0f;
+        const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
         const int unit_exp = rexp[nt] == kNoExp ? 0 : rexp[nt] - kTop - kScaleP;
 #pragma unroll
         for (int t = 0; t < DT; t++) {
@@ -2166,96 +2012,11 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
             const int c = (lane % LPR) * 4;
             const floatx4 v = *reinterpret_cast<const floatx4 *>(stage + r * SROW + c);
             const int lq = wq0 + nt * 16 + r;
-            if (lq < q_len) {
-#if GLA_PREFILL_MODE == GLA_PREFILL_PREFIX
-                const int64_t at = (int64_t)blockIdx.z * p.n_seqs * p.n_heads + row_of(lq);
-                *reinterpret_cast<floatx4 *>(p.pre.acc + at * D + c) = v;
-#else
+            if (lq < q_len)
                 __builtin_nontemporal_store(v, reinterpret_cast<floatx4 *>(p.out + ((int64_t)(row0 + lq) * p.n_heads + head) * D + c));
-#endif
-            }
         }
-#if GLA_PREFILL_MODE == GLA_PREFILL_PREFIX
-        const int lq = wq0 + nt * 16 + lrow;
-        if (lgrp == 0 && lq < q_len) {
-            const int64_t at = (int64_t)blockIdx.z * p.n_seqs * p.n_heads + row_of(lq);
-            reinterpret_cast<float2 *>(p.pre.ml)[at] = make_float2(m[nt] == kMLowest ? -INFINITY : m[nt], lt);
-        }
-#endif
     }
 }
-
-#if GLA_PREFILL_MODE == GLA_PREFILL_PREFIX
-
-template <int D, bool Q8, int NT>
-int launch_prefix_as(gla_ctx *ctx, const PrefillParams &prm, dim3 grid) {
-    if (prm.softcap > 0.0f)
-        hipLaunchKernelGGL((prefill_split_kernel<D, Q8, true, false, NT>), grid, dim3(256), 0, ctx->stream, prm, Images{});
-    else
-        hipLaunchKernelGGL((prefill_split_kernel<D, Q8, false, false, NT>), grid, dim3(256), 0, ctx->stream, prm, Images{});
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "prefix kernel launch: %s", hipGetErrorString(e));
-    return GLA_OK;
-}
-
-template <int D>
-int launch_prefix_d(gla_ctx *ctx, bool q8, const PrefillParams &prm, dim3 grid) {
-    return q8 ? launch_prefix_as<D, true, 1>(ctx, prm, grid) : launch_prefix_as<D, false, 1>(ctx, prm, grid);
-}
-
-}  // namespace
-
-// Rows of a workgroup of the prefix kernel.
-constexpr int kPrefixRows = 64;
-
-void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
-    const DecodeLaunch &d = *launch;
-    PrefixLaunch *pre = &launch->pre;
-    const int group = d.n_heads / d.n_kv_heads;
-    const int tiles = (pre->max_prefix + KT - 1) / KT;
-    // row blocks of all groups, at most
-    const int64_t blocks = std::min<int64_t>((int64_t)pre->n_groups * (((int64_t)pre->max_group * group - 1) / kPrefixRows + 1),
-                                             (int64_t)d.n_seqs * group / kPrefixRows + pre->n_groups);
-    const int64_t wgs = blocks * d.n_kv_heads;
-    const int64_t want = std::max<int64_t>(1, 2 * (int64_t)ctx->n_cu / wgs);
-    pre->split_tiles = (int)std::max<int64_t>(2, (tiles + want - 1) / want);
-    pre->n_splits = (tiles + pre->split_tiles - 1) / pre->split_tiles;
-}
-
-int launch_prefix(gla_ctx *ctx, const DecodeLaunch &d, void *scratch, PrefixLaunch *out) {
-    *out = d.pre;
-    out->acc = (float *)scratch;
-    out->ml = out->acc + (size_t)d.pre.n_splits * d.n_seqs * d.n_heads * d.head_dim;
-    const PrefixLaunch &pre = *out;
-    PrefillParams prm{};
-    prm.kv = d.kv;
-    prm.pm = d.pm;
-    prm.q = d.q;
-    prm.n_heads = d.n_heads;
-    prm.n_kv_heads = d.n_kv_heads;
-    prm.group = d.n_heads / d.n_kv_heads;
-    const bool cap = d.softcap > 0.0f;
-    prm.q_mul = cap ? d.scale : d.scale * kLog2e;
-    prm.softcap = cap ? d.softcap : 0.0f;
-    prm.pre = pre;
-    prm.kv_start = d.kv_start;
-    prm.kv_len = d.kv_len;
-    prm.max_kv_len = d.max_kv_len;
-    prm.n_seqs = d.n_seqs;
-    const int blocks = (int)(((int64_t)pre.max_group * prm.group - 1) / kPrefixRows + 1);
-    const dim3 grid(pre.n_groups * d.n_kv_heads, blocks, pre.n_splits);
-    if (blocks > 65535 || pre.n_splits > 65535) return set_error(GLA_ERR_INVALID, "decode: %d row blocks of a group, %d splits", blocks, pre.n_splits);
-    switch (d.head_dim) {
-    case 64:
-        return launch_prefix_d<64>(ctx, d.q8, prm, grid);
-    case 128:
-        return launch_prefix_d<128>(ctx, d.q8, prm, grid);
-    default:
-        return launch_prefix_d<256>(ctx, d.q8, prm, grid);
-    }
-}
-
-#else
 
 // Query blocks of a call whose waves (four to a workgroup) take nt 16-query
 // tiles each.
@@ -2413,7 +2174,7 @@ int launch_f32(gla_ctx *ctx, bool q8, const PrefillParams &prm, int n_seqs, int 
 
 }  // namespace
 
-#if GLA_PREFILL_MODE == GLA_PREFILL_SINKS
+#if GLA_PREFILL_SINKS
 int launch_prefill_sinks(gla_ctx *ctx, const PrefillLaunch &a) {
 #else
 int launch_prefill(gla_ctx *ctx, const PrefillLaunch &a) {
@@ -2496,7 +2257,5 @@ int launch_prefill(gla_ctx *ctx, const PrefillLaunch &a) {
         return launch_f32<256>(ctx, a.q8, prm, a.n_seqs, n_hgrp, n_tiles);
     }
 }
-
-#endif  // not PREFIX
 
 }  // namespace gla
