@@ -6,6 +6,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace gla {
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -32,6 +34,18 @@ __device__ __forceinline__ float sum_rows4(float x) {
     x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
     const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(c[0]) + __uint_as_float(c[1]);
+}
+
+// sum over the 16 lanes of a row (DPP rotations)
+__device__ __forceinline__ float sum_row16(float x) {
+    const auto turned = [](float v, auto control) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(control)::value, 0xf, 0xf, true));
+    };
+    x += turned(x, std::integral_constant<int, 0x121>{});  // row_ror 1, 2, 4, 8
+    x += turned(x, std::integral_constant<int, 0x122>{});
+    x += turned(x, std::integral_constant<int, 0x124>{});
+    x += turned(x, std::integral_constant<int, 0x128>{});
+    return x;
 }
 
 // max / min of unsigned words over the wave, in every lane: DPP rotations within

@@ -1,5 +1,7 @@
 // gla_norm.hip -- norms around a transformer block, its gate and the residual sum, in
-// one pass over the rows (gfx950, HBM-bound; one row: launch and latency).
+// one pass over the rows (gfx950). Many rows are bound by HBM: 7,993 rows of 4,096 with
+// everything, 655 MB, 104 us, 6.3 TB/s (a large copy reaches 5.1). One row is bound by its
+// launch: 2.6 us in a captured step, as an empty kernel's.
 //
 // Math, row by row:
 //   z  = post ? y / sqrt(mean(y^2) + eps) * post : y
@@ -13,6 +15,7 @@
 #include <algorithm>
 
 #include "gla_internal.h"
+#include "gla_lanes.h"
 
 namespace gla {
 
@@ -28,11 +31,12 @@ struct NormParams {
     float eps, scale;
 };
 
-// Sum over the T threads of a row (whole waves); `lds` is used by rows of several waves.
+// Sum over the T threads of a row (whole waves), in every one of them; `lds` is used by
+// rows of several waves.
 template <int T>
 __device__ __forceinline__ float row_sum(float v, float *lds) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    v = sum_row16(v);
+    v = sum_rows4(v);
     if constexpr (T > 64) {
         constexpr int W = T / 64;
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -44,120 +48,138 @@ __device__ __forceinline__ float row_sum(float v, float *lds) {
     return v;
 }
 
-// T threads a row, N pieces of E floats (1 or 4) a thread.
+// A row's pieces i = t, t + T, ... of E floats (1 or 4); those past its end are 0.
 template <int T, int N, int E>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void block_norm_kernel(const NormParams p) {
-    typedef float vec __attribute__((ext_vector_type(E == 4 ? 4 : 2)));  // (E == 1 goes by single floats)
-    constexpr int RPW = T < 256 ? 256 / T : 1;  // rows per workgroup
-    __shared__ float lds[2][T / 64];
-    const int t = threadIdx.x % T;
-    const int pieces = p.dim / E;
-    const auto load = [&](const float *row, int k, float (&v)[E]) {
-        const int i = t + k * T;
+struct Pieces {
+    typedef float vec __attribute__((ext_vector_type(4)));
+    float v[N][E];
+    template <bool ONCE = false>
+    __device__ __forceinline__ void load(const float *row, int t, int pieces) {
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] = 0.0f;
-        if (i < pieces) {
-            if constexpr (E == 4) {
-                const vec w = *reinterpret_cast<const vec *>(row + 4 * i);
+        for (int k = 0; k < N; k++) {
+            const int i = t + k * T;
 #pragma unroll
-                for (int e = 0; e < E; e++) v[e] = w[e];
-            } else {
-                v[0] = row[i];
+            for (int e = 0; e < E; e++) v[k][e] = 0.0f;
+            if (i < pieces) {
+                if constexpr (E == 4) {
+                    const vec *at = reinterpret_cast<const vec *>(row + 4 * i);
+                    const vec w = ONCE ? __builtin_nontemporal_load(at) : *at;
+#pragma unroll
+                    for (int e = 0; e < E; e++) v[k][e] = w[e];
+                } else {
+                    v[k][0] = row[i];
+                }
             }
         }
-    };
-    const auto store = [&](float *row, int k, const float (&v)[E]) {
-        const int i = t + k * T;
-        if (i < pieces) {
-            if constexpr (E == 4)
-                *reinterpret_cast<vec *>(row + 4 * i) = vec{v[0], v[1], v[2], v[3]};
-            else
-                row[i] = v[0];
+    }
+    __device__ __forceinline__ void store(float *row, int t, int pieces) const {
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int i = t + k * T;
+            if (i < pieces) {
+                if constexpr (E == 4)
+                    *reinterpret_cast<vec *>(row + 4 * i) = vec{v[k][0], v[k][1], v[k][2], v[k][3]};
+                else
+                    row[i] = v[k][0];
+            }
         }
-    };
-    const auto squares = [&](const float (&v)[N][E]) {
+    }
+    __device__ __forceinline__ float squares() const {
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < N; k++)
 #pragma unroll
             for (int e = 0; e < E; e++) s = fmaf(v[k][e], v[k][e], s);
         return s;
-    };
-    for (int64_t r = (int64_t)blockIdx.x * RPW + threadIdx.x / T; r < p.n_rows; r += (int64_t)gridDim.x * RPW) {
-        float x[N][E], y[N][E];
+    }
+};
+
+// T threads a row, N pieces of E floats a thread. Everything that a row needs, its weights
+// too, is asked for before the first sum: one round trip to memory and two sums are what a
+// few rows cost. ONCE: the rows' inputs pass the caches by.
+template <int T, int N, int E, bool ONCE>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void block_norm_kernel(const NormParams p) {
+    constexpr int RPW = T < 256 ? 256 / T : 1;  // rows per workgroup
+    __shared__ float lds[2][T / 64];
+    const int t = threadIdx.x % T;
+    const int pieces = p.dim / E;
+    const int64_t r = (int64_t)blockIdx.x * RPW + threadIdx.x / T;
+    if (r >= p.n_rows) return;  // (rows of one wave: a workgroup with rows of several holds one)
+    Pieces<T, N, E> x, y, g, post, pre;
+    x.template load<ONCE>(p.x + r * p.x_stride, t, pieces);
+    if (p.y) y.template load<ONCE>(p.y + r * p.y_stride, t, pieces);
+    if (p.post) post.load(p.post, t, pieces);
+    if (p.gate) {
+        if (ONCE && p.gate_stride)
+            g.template load<ONCE>(p.gate + r * p.gate_stride, t, pieces);
+        else
+            g.load(p.gate + r * p.gate_stride, t, pieces);
+    }
+    if (p.norm_out) pre.load(p.pre, t, pieces);
+    if (p.y) {
+        float f = p.scale;
+        if (p.post) f *= 1.0f / sqrtf(row_sum<T>(y.squares(), lds[0]) / (float)p.dim + p.eps);
 #pragma unroll
-        for (int k = 0; k < N; k++) load(p.x + r * p.x_stride, k, x[k]);
-        if (p.y) {
+        for (int k = 0; k < N; k++)
 #pragma unroll
-            for (int k = 0; k < N; k++) load(p.y + r * p.y_stride, k, y[k]);
-            if (p.gate) {
-                float g[N][E];
-#pragma unroll
-                for (int k = 0; k < N; k++) load(p.gate + r * p.gate_stride, k, g[k]);
-                float f = p.scale;
-                if (p.post) f *= 1.0f / sqrtf(row_sum<T>(squares(y), lds[0]) / (float)p.dim + p.eps);
-#pragma unroll
-                for (int k = 0; k < N; k++)
-#pragma unroll
-                    for (int e = 0; e < E; e++) y[k][e] *= g[k][e] * f;
-            } else {
-                float f = p.scale;
-                if (p.post) f *= 1.0f / sqrtf(row_sum<T>(squares(y), lds[0]) / (float)p.dim + p.eps);
-#pragma unroll
-                for (int k = 0; k < N; k++)
-#pragma unroll
-                    for (int e = 0; e < E; e++) y[k][e] *= f;
+            for (int e = 0; e < E; e++) {
+                const float z = y.v[k][e] * (p.gate ? g.v[k][e] * f : f);
+                x.v[k][e] = p.post ? fmaf(z, post.v[k][e], x.v[k][e]) : x.v[k][e] + z;
             }
-            if (p.post) {
+    }
+    if (p.x_out) x.store(p.x_out + r * p.x_out_stride, t, pieces);
+    if (p.norm_out) {
+        const float f = 1.0f / sqrtf(row_sum<T>(x.squares(), lds[1]) / (float)p.dim + p.eps);
 #pragma unroll
-                for (int k = 0; k < N; k++) {
-                    float w[E];
-                    load(p.post, k, w);
+        for (int k = 0; k < N; k++)
 #pragma unroll
-                    for (int e = 0; e < E; e++) x[k][e] = fmaf(y[k][e], w[e], x[k][e]);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < N; k++)
-#pragma unroll
-                    for (int e = 0; e < E; e++) x[k][e] += y[k][e];
-            }
-        }
-        if (p.x_out) {
-#pragma unroll
-            for (int k = 0; k < N; k++) store(p.x_out + r * p.x_out_stride, k, x[k]);
-        }
-        if (p.norm_out) {
-            const float f = 1.0f / sqrtf(row_sum<T>(squares(x), lds[1]) / (float)p.dim + p.eps);
-#pragma unroll
-            for (int k = 0; k < N; k++) {
-                float w[E];
-                load(p.pre, k, w);
-#pragma unroll
-                for (int e = 0; e < E; e++) x[k][e] *= f * w[e];
-                store(p.norm_out + r * p.norm_out_stride, k, x[k]);
-            }
-        }
-        if constexpr (T > 64) __syncthreads();  // the sums are read: the next row may write them
+            for (int e = 0; e < E; e++) x.v[k][e] *= f * pre.v[k][e];
+        x.store(p.norm_out + r * p.norm_out_stride, t, pieces);
     }
 }
 
-template <int T, int N, int E>
+template <int T, int N, int E, bool ONCE = false>
 int launch_as(gla_ctx *ctx, const NormParams &p) {
     constexpr int RPW = T < 256 ? 256 / T : 1;
-    const int64_t wgs = ((int64_t)p.n_rows + RPW - 1) / RPW;
-    hipLaunchKernelGGL((block_norm_kernel<T, N, E>), dim3((unsigned)std::min<int64_t>(wgs, 1 << 20)),
-                       dim3(T < 256 ? 256 : T), 0, ctx->stream, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "block_norm_kernel launch: %s", hipGetErrorString(e));
+    // (a grid holds fewer than 2^32 threads)
+    constexpr int64_t kMost = (int64_t)1 << 21;
+    for (int64_t r0 = 0; r0 < p.n_rows; r0 += kMost * RPW) {
+        NormParams q = p;
+        q.n_rows = (int)std::min<int64_t>(p.n_rows - r0, kMost * RPW);
+        q.x += r0 * p.x_stride;
+        if (q.y) q.y += r0 * p.y_stride;
+        if (q.gate) q.gate += r0 * p.gate_stride;
+        if (q.x_out) q.x_out += r0 * p.x_out_stride;
+        if (q.norm_out) q.norm_out += r0 * p.norm_out_stride;
+        hipLaunchKernelGGL((block_norm_kernel<T, N, E, ONCE>), dim3((unsigned)((q.n_rows + RPW - 1) / RPW)),
+                           dim3(T < 256 ? 256 : T), 0, ctx->stream, q);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "block_norm_kernel launch: %s", hipGetErrorString(e));
+    }
     return GLA_OK;
 }
 
 template <int E>
 int launch_e(gla_ctx *ctx, const NormParams &p) {
     const int pieces = p.dim / E;
+    // What the call moves, where it is more than the last-level cache holds, would push out of
+    // the caches what the next call reads from them: inputs are then read past them. us a call,
+    // past / through them: 7,993 rows of 4,096, all inputs (655 MB) 104 / 113, without post and
+    // gate (524 MB) 81 / 94; 8,192 of 576 (75 MB) 16.9 / 13.1, 256 of 4,096 (21 MB) 7.4 / 6.2.
+    if constexpr (E == 4) {
+        const int64_t rows = 1 + (p.y != nullptr) + (p.gate && p.gate_stride) + (p.x_out != nullptr) + (p.norm_out != nullptr);
+        if (rows * p.n_rows * p.dim * 4 > (int64_t)256 << 20) {
+            if (pieces <= 256) return launch_as<64, 4, 4, true>(ctx, p);
+            if (pieces <= 1024) return launch_as<256, 4, 4, true>(ctx, p);
+            return launch_as<1024, 4, 4, true>(ctx, p);
+        }
+    }
     if (pieces <= 64) return launch_as<64, 1, E>(ctx, p);
     if (pieces <= 256) return launch_as<64, 4, E>(ctx, p);
+    // As many rows as the device has units, or fewer: the fewest loads a thread. More: several
+    // workgroups a unit. us a captured call, 1,024 / 256 threads a row, both norms and a gate:
+    // 64 rows of 3,584 4.25 / 4.43, 256 of 4,096 6.2 / 6.7, 7,993 of 4,096 118 / 113.
+    if (pieces <= 1024 && p.n_rows <= ctx->n_cu) return launch_as<1024, 1, E>(ctx, p);
     if (pieces <= 1024) return launch_as<256, 4, E>(ctx, p);
     if (pieces <= 4096) return launch_as<1024, 4, E>(ctx, p);
     if constexpr (E == 1) return launch_as<1024, 16, 1>(ctx, p);

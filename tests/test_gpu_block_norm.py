@@ -214,3 +214,23 @@ def test_refusals(backend):
         assert e.value.code == _lib.GLA_ERR_INVALID, bad
     be.block_norm(**{**ok, "x_out": View(t, 100), "x_stride": 200, "x_out_stride": 200})
     be.sync()
+
+
+@pytest.mark.parametrize("n, dim, gate", [(90000, 256, None), (22000, 1000, "rows"), (4100, 5000, "vector")])
+def test_more_than_the_caches_hold(backend, n, dim, gate):
+    """Inputs that are read past the caches (more than 256 MB of rows), in every width's variant."""
+    rng = np.random.default_rng(31)
+    x, y, post, g, pre = inputs(rng, n, dim, True, gate)
+    out, h = run(backend, x, y, post, g, 0.5, pre, 1e-5)
+    at = np.concatenate([np.arange(50), rng.integers(0, n, 400), np.arange(n - 50, n)])
+    want, dx, norm, dh = formula(x[at], y[at], post, g if gate != "rows" else g[at], 0.5, pre, 1e-5)
+    assert np.all(np.abs(out[at] - want) <= dx) and np.all(np.abs(h[at] - norm) <= dh)
+
+
+def test_more_rows_than_a_launch_takes(backend):
+    rng = np.random.default_rng(32)
+    n, dim = 4 * 2 ** 21 + 5, 4
+    x, y, _, _, pre = inputs(rng, n, dim, False, None)
+    out, h = run(backend, x, y, None, None, 1.0, pre, 1e-5)
+    want, dx, norm, dh = formula(x, y, None, None, 1.0, pre, 1e-5)
+    assert np.all(np.abs(out - want) <= dx) and np.all(np.abs(h - norm) <= dh)
