@@ -152,7 +152,7 @@ struct SeqRange {
     int n_pages;
     int pps;         // pages per split
     int n_splits;
-    Visible v;       // but for kWindow (fp is 0: pages are numbered as Visible does)
+    Visible v;       // kWindowSinks (fp is 0: pages are numbered as Visible does)
     int prefix;      // kBehindPrefix: positions that the prefix's partials hold
 };
 
@@ -160,9 +160,8 @@ template <DecodeMode MODE>
 __device__ __forceinline__ SeqRange seq_range(const DecodeParams &p, int b) {
     SeqRange r;
     int s = p.kv_start[b];
-    if constexpr (MODE != kWindow) {
-        r.prefix = MODE == kBehindPrefix ? row_prefix(p.pre, b) : 0;
-        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, MODE == kWindowSinks ? p.n_sinks : 0, r.prefix);
+    if constexpr (MODE == kWindowSinks) {
+        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, p.n_sinks);
         r.start = r.v.start;
         r.end = r.v.end;
         r.fp = 0;
@@ -176,6 +175,10 @@ __device__ __forceinline__ SeqRange seq_range(const DecodeParams &p, int b) {
     len = len < 0 ? 0 : (len > p.max_len ? p.max_len : len);
     int e = s + len;
     if (e > p.pm.pos_limit) e = p.pm.pos_limit;
+    if constexpr (MODE == kBehindPrefix) {
+        r.prefix = row_prefix(p.pre, b);
+        if (s < e && s < r.prefix) s = r.prefix;  // (an empty window stays so)
+    }
     if (s > e) s = e;
     r.start = s;
     r.end = e;
@@ -302,7 +305,9 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
     const int pg1 = split + 1 == r.n_splits ? r.fp + r.n_pages : min(r.fp + r.n_pages, pg0 + r.pps);
 
     const int lane = tid & 63;
-    const int wave = tid >> 6;
+    // (a window with sinks takes more registers to find its pages: with the wave's number in a
+    // scalar they are scalars, and head_dim 256 keeps two waves a SIMD)
+    const int wave = MODE == kWindowSinks ? __builtin_amdgcn_readfirstlane(tid >> 6) : tid >> 6;
     const int tg = lane >> 3;
     const int sub = lane & 7;
 
@@ -338,14 +343,14 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
 #pragma unroll
         for (int j = 0; j < PPW; j++) {
             const int pg = (pb + j < pg1) ? pb + j : pb;
-            pid[j] = map_page(p.pm, b, MODE != kWindow ? r.v.page(pg) : pg);
+            pid[j] = map_page(p.pm, b, MODE == kWindowSinks ? r.v.page(pg) : pg);
         }
 #pragma unroll
         for (int s = 0; s < NSTEP; s++) {
             const int page = pb + s / 2;
             const int slot = (s & 1) * 8 + tg;
-            const int pos = (MODE != kWindow ? r.v.page(page) : page) * 16 + slot;
-            valid[s] = page < pg1 && (MODE != kWindow ? r.v.sees(pos) : pos >= r.start && pos < r.end);
+            const int pos = (MODE == kWindowSinks ? r.v.page(page) : page) * 16 + slot;
+            valid[s] = page < pg1 && (MODE == kWindowSinks ? r.v.sees(pos) : pos >= r.start && pos < r.end);
             const int64_t base = pid[s / 2] * p.kv.page_stride + head_off + (int64_t)slot * p.kv.row_stride;
             const uint8_t *kp = p.kv.k + base;
             const uint8_t *vp = p.kv.v + base;

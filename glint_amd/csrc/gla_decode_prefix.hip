@@ -118,7 +118,7 @@ __device__ __forceinline__ Row row_of(const PrefixParams &p, const Share &s, int
     if (x.ok) {
         const int b = s.member + r / p.group;
         x.at = row_at(p, s, r);
-        const Visible v = visible_of(p.kv_start[b], p.kv_len[b], p.max_kv_len, p.pm.pos_limit, 0, 0);
+        const Visible v = visible_of(p.kv_start[b], p.kv_len[b], p.max_kv_len, p.pm.pos_limit, 0);
         x.lo = v.start;
         x.hi = v.n_pages ? v.end : 0;
     }

@@ -109,7 +109,7 @@ struct Range {
     int start, end;  // positions [start, end)
     int fp;          // first logical page
     int n_pages;
-    Visible v;       // but for kWindow (fp is 0: pages are numbered as Visible does)
+    Visible v;       // kWindowSinks (fp is 0: pages are numbered as Visible does)
     int prefix;      // kBehindPrefix: positions that the prefix's partials hold
 };
 
@@ -117,9 +117,8 @@ template <DecodeMode MODE>
 __device__ __forceinline__ Range seq_range(const Q8Params &p, int b) {
     Range r;
     int s = p.kv_start[b];
-    if constexpr (MODE != kWindow) {
-        r.prefix = MODE == kBehindPrefix ? row_prefix(p.pre, b) : 0;
-        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, MODE == kWindowSinks ? p.n_sinks : 0, r.prefix);
+    if constexpr (MODE == kWindowSinks) {
+        r.v = visible_of(s, p.kv_len[b], p.max_len, p.pm.pos_limit, p.n_sinks);
         r.start = r.v.start;
         r.end = r.v.end;
         r.fp = 0;
@@ -131,6 +130,10 @@ __device__ __forceinline__ Range seq_range(const Q8Params &p, int b) {
     len = len < 0 ? 0 : (len > p.max_len ? p.max_len : len);
     int e = s + len;
     if (e > p.pm.pos_limit) e = p.pm.pos_limit;
+    if constexpr (MODE == kBehindPrefix) {
+        r.prefix = row_prefix(p.pre, b);
+        if (s < e && s < r.prefix) s = r.prefix;  // (an empty window stays so)
+    }
     if (s > e) s = e;
     r.start = s;
     r.end = e;
@@ -458,7 +461,7 @@ struct StepConst {
     float sm, kvs, softcap, qcap;
     bool cap;
     int pg0, npg, start, end;
-    Visible v;  // but for kWindow
+    Visible v;  // kWindowSinks
     int kg, ph;
     float pf;  // this lane's piece (0: hi, 1: lo) as a float
 };
@@ -520,7 +523,7 @@ __device__ __forceinline__ void step_qk(const RawK<D> &cur, int step, const Step
     // on the lane's own page, are flagged so that their V scale is zeroed and
     // a non-finite scale of an unused position cannot reach the output.
     vbad = 0;
-    if constexpr (MODE != kWindow) {
+    if constexpr (MODE == kWindowSinks) {
         const int pa = c.v.page(c.pg0 + 2 * step), pb = c.v.page(c.pg0 + 2 * step + 1);
         const bool two = 2 * step + 1 < c.npg;  // (else page 1 repeats page 0's data)
         if (!(c.v.whole(pa) && two && c.v.whole(pb))) {
@@ -641,7 +644,7 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
     }
     // physical page of chunk page `lane` (clamped into the pool by map_page)
     int pid_l;
-    if constexpr (MODE != kWindow) {
+    if constexpr (MODE == kWindowSinks) {
         // (a chunk on one side of the gap is as one without sinks)
         const bool astride = pg0 < r.v.head && pg0 + npg > r.v.head;
         pid_l = p.pm.page_table && p.pm.pt_stride >= 16 && !astride
@@ -761,7 +764,7 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
     c.npg = npg;
     c.start = r.start;
     c.end = r.end;
-    if constexpr (MODE != kWindow) c.v = r.v;
+    if constexpr (MODE == kWindowSinks) c.v = r.v;
     c.kg = kg;
     c.ph = ph;
     c.pf = (float)piece;

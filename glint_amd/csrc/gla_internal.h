@@ -206,32 +206,33 @@ __device__ __forceinline__ int64_t map_page(const PageMap &pm, int b, int lp) {
 // The pages that a window with sinks touches: of the positions j < end, those with
 // j >= start or j < sinks are seen. Page v of n_pages is the storage's logical
 // page v + (v >= head ? gap : 0): the pages of the sinks, then the window's; every
-// one holds a position that is seen. From `from` on only (a prefix that is read
-// apart; sinks are then 0).
+// one holds a position that is seen.
 struct Visible {
     int start, end, sinks;
     int head, gap, n_pages;
     __host__ __device__ __forceinline__ int page(int v) const { return v + (v >= head ? gap : 0); }
-    __host__ __device__ __forceinline__ bool sees(int pos) const { return pos < end && (pos >= start || pos < sinks); }
+    // (one comparison for both ends of the hole between the sinks and the window: with two, the f32
+    // kernel at head_dim 256 falls to one wave a SIMD)
+    __host__ __device__ __forceinline__ bool sees(int pos) const {
+        return pos < end && (uint32_t)(pos - sinks) >= (uint32_t)(start > sinks ? start - sinks : 0);
+    }
     // every position of a logical page is seen, by the window or by the sinks alone
     __host__ __device__ __forceinline__ bool whole(int page) const {
         return page * 16 + 16 <= end && (page * 16 >= start || page * 16 + 16 <= sinks);
     }
 };
 // With the decode kernels' clamping of start and length (their seq_range).
-__host__ __device__ __forceinline__ Visible visible_of(int start, int len, int max_len, int pos_limit, int n_sinks,
-                                                       int from) {
+__host__ __device__ __forceinline__ Visible visible_of(int start, int len, int max_len, int pos_limit, int n_sinks) {
     Visible r;
-    const int s0 = start < 0 ? 0 : start;
+    const int s = start < 0 ? 0 : start;
     len = len < 0 ? 0 : (len > max_len ? max_len : len);
-    const int64_t e64 = (int64_t)s0 + len;
+    const int64_t e64 = (int64_t)s + len;
     const int e = e64 > pos_limit ? pos_limit : (int)e64;
-    const int s = s0 > from ? s0 : from;
     r.start = s;
     r.end = e;
     r.sinks = n_sinks;
     r.head = r.gap = r.n_pages = 0;
-    if (s0 >= e || s >= e) return r;
+    if (s >= e) return r;
     const int before = ((n_sinks < s ? n_sinks : s) + 15) >> 4;  // pages of the sinks in front of the window
     const int first = s >> 4, last = (e - 1) >> 4;
     if (before >= first) {  // they meet the window's
@@ -326,12 +327,13 @@ int ensure_hstage(gla_ctx *ctx, size_t bytes);
 
 // Pages the window of one sequence spans, with the decode kernels' clamping
 // of its start and length (their seq_range), from the host copies.
-inline int host_seq_pages(int start, int len, int max_len, int pos_limit) {
+inline int host_seq_pages(int start, int len, int max_len, int pos_limit, int from = 0) {
     start = start < 0 ? 0 : start;
     len = len < 0 ? 0 : (len > max_len ? max_len : len);
     int64_t e = (int64_t)start + len;
     if (e > pos_limit) e = pos_limit;
-    const int64_t s = start > e ? e : start;
+    int64_t s = start > e ? e : start;
+    if (s < from) s = from;  // (positions before it are read apart)
     return e > s ? (int)(((e - 1) >> 4) - (s >> 4) + 1) : 0;
 }
 
@@ -435,9 +437,9 @@ inline int host_pages(const DecodeLaunch &d, int b) {
         const int32_t *at = d.pre.group_start_host;
         const int g = (int)(std::upper_bound(at, at + d.pre.n_groups, b) - at) - 1;
         const int from = g < 0 || at[g + 1] <= b ? 0 : prefix_positions(d.pre.prefix_len_host[g], d.pre.max_prefix);
-        return std::min(visible_of(start, len, d.max_kv_len, d.pm.pos_limit, 0, from).n_pages, max_window_pages(d));
+        return std::min(host_seq_pages(start, len, d.max_kv_len, d.pm.pos_limit, from), max_window_pages(d));
     }
-    if (d.n_sinks > 0) return visible_of(start, len, d.max_kv_len, d.pm.pos_limit, d.n_sinks, 0).n_pages;
+    if (d.n_sinks > 0) return visible_of(start, len, d.max_kv_len, d.pm.pos_limit, d.n_sinks).n_pages;
     return host_seq_pages(start, len, d.max_kv_len, d.pm.pos_limit);
 }
 // Device scratch of a decode launch: d.scratch (no allocation) or the
