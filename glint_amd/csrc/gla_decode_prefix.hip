@@ -104,20 +104,15 @@ __device__ __forceinline__ Share share_of(const PrefixParams &p, int tile_rows, 
 struct Row {
     int lo, hi;  // sees lo <= position < hi
     bool ok;
-    int64_t at;  // sequence * n_heads + head
+    int at;  // sequence * n_heads + head (the group's first row, for a row past the group's)
 };
-__device__ __forceinline__ int64_t row_at(const PrefixParams &p, const Share &s, int r) {
-    const int b = s.member + r / p.group;
-    return (int64_t)b * p.n_heads + s.kvh * p.group + r % p.group;
-}
 __device__ __forceinline__ Row row_of(const PrefixParams &p, const Share &s, int r) {
     Row x;
     x.ok = r < s.rows;
     x.lo = x.hi = 0;
-    x.at = 0;
+    const int i = x.ok ? r / p.group : 0, b = s.member + i;
+    x.at = b * p.n_heads + s.kvh * p.group + (x.ok ? r - i * p.group : 0);
     if (x.ok) {
-        const int b = s.member + r / p.group;
-        x.at = row_at(p, s, r);
         const Visible v = visible_of(p.kv_start[b], p.kv_len[b], p.max_kv_len, p.pm.pos_limit, 0);
         x.lo = v.start;
         x.hi = v.n_pages ? v.end : 0;
@@ -161,7 +156,7 @@ constexpr int kMergeFloats = kWaves * 16 * NT * out_row(D);
 // m of the workgroup for this lane's rows; `put` stores the wave's O, times f[nt], in its slot.
 template <int D, int NT, typename Put>
 __device__ __forceinline__ void merge_and_store(const PrefixParams &p, const Share &s, float (&m)[NT], float (&l)[NT],
-                                                float *slots, float (*mls)[2][16 * NT], Put put) {
+                                                float *slots, float (*mls)[2][16 * NT], const int *at, Put put) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int lrow = lane & 15;
     if (lane < 16) {
@@ -191,7 +186,7 @@ __device__ __forceinline__ void merge_and_store(const PrefixParams &p, const Sha
 #pragma unroll
         for (int w = 1; w < kWaves; w++)
             v += *reinterpret_cast<const floatx4 *>(slots + (w * 16 * NT + r) * out_row(D) + c);
-        *reinterpret_cast<floatx4 *>(p.pre.acc + (first + row_at(p, s, s.row0 + r)) * D + c) = v;
+        *reinterpret_cast<floatx4 *>(p.pre.acc + (first + at[r]) * D + c) = v;
     }
     const int r = threadIdx.x;
     if (r < 16 * NT && s.row0 + r < s.rows) {
@@ -203,7 +198,7 @@ __device__ __forceinline__ void merge_and_store(const PrefixParams &p, const Sha
             const float mw = mls[w][0][r];
             sum = fmaf(mls[w][1][r], mw == -INFINITY ? 0.0f : fast_exp2(mw - top), sum);
         }
-        reinterpret_cast<float2 *>(p.pre.ml)[first + row_at(p, s, s.row0 + r)] = make_float2(top, sum);
+        reinterpret_cast<float2 *>(p.pre.ml)[first + at[r]] = make_float2(top, sum);
     }
 }
 
@@ -213,44 +208,17 @@ __device__ __forceinline__ void merge_and_store(const PrefixParams &p, const Sha
 // group kg and step j, which makes K and Q four floats of a row a lane, and the d tiles
 // of O the dims T*64 + m*4 + c, which makes V so.
 template <int D, int NT, bool CAP>
-__global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void prefix_f32_kernel(const PrefixParams p) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefix_f32_kernel(const PrefixParams p) {
     constexpr int KK = D / 16, DT = D / 64;
     constexpr int QFLOATS = NT * KK * 256;
     __shared__ __attribute__((aligned(16))) float lds[std::max(QFLOATS, kMergeFloats<D, NT>)];
     __shared__ float mls[kWaves][2][16 * NT];
+    __shared__ int row_at[16 * NT];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lrow = lane & 15, kg = lane >> 4;
     const Share sh = share_of<false>(p, 16 * NT, wave);
     if (!sh.any) return;
-
-    // the queries, [nt][kk][lane] in the order in which a lane reads them
-    for (int i = threadIdx.x; i < NT * KK * 64; i += kThreads) {
-        const int nt = i / (KK * 64), kk = i / 64 % KK, l = i & 63;
-        const int r = sh.row0 + nt * 16 + (l & 15);
-        floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (r < sh.rows)
-            x = *reinterpret_cast<const floatx4 *>(p.q + row_at(p, sh, r) * D + kk * 16 + (l >> 4) * 4) * p.q_mul;
-        reinterpret_cast<floatx4 *>(lds)[i] = x;
-    }
-    Row rows[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) rows[nt] = row_of(p, sh, sh.row0 + nt * 16 + lrow);
-    const Seen seen = seen_of<NT>(rows);
-    __syncthreads();
-    const floatx4 *qs = reinterpret_cast<const floatx4 *>(lds);
-
-    floatx4 o[DT][4][NT];  // O of d = T*64 + (kg*4 + r)*4 + c in [T][c][nt][r]
-    float m[NT], lpart[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        m[nt] = -INFINITY;
-        lpart[nt] = 0.0f;
-#pragma unroll
-        for (int T = 0; T < DT; T++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) o[T][c][nt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
 
     floatx4 k[KK], v[4][DT];
     const uint32_t koff = (uint32_t)(lrow * p.kv.row_stride + kg * 16);
@@ -269,13 +237,46 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
             for (int T = 0; T < DT; T++)
                 v[r][T] = *reinterpret_cast<const floatx4 *>(at + voff + r * p.kv.row_stride + T * 256);
     };
-
+    // (the first page is on its way while the queries are; a wave without pages reads the group's first)
     const int n = sh.npg;
-    if (n > 0) {
-        const int ids = page_ids(p, sh.member, sh.pg0, n);
-        const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, n - 1)); };
-        load_k(id(0));
-        load_v(id(0));
+    const int ids = page_ids(p, sh.member, n > 0 ? sh.pg0 : 0, max(n, 1));
+    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(n, 1) - 1)); };
+    load_k(id(0));
+    load_v(id(0));
+
+    Row rows[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        rows[nt] = row_of(p, sh, sh.row0 + nt * 16 + lrow);
+        if (threadIdx.x < 16) row_at[nt * 16 + lrow] = rows[nt].at;
+    }
+    // the queries, [nt][kk][lane] in the order in which a lane reads them: a wave takes every fourth kk
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int k4 = 0; k4 < KK / kWaves; k4++) {
+            const int kk = k4 * kWaves + wave;
+            floatx4 x = *reinterpret_cast<const floatx4 *>(p.q + (int64_t)rows[nt].at * D + kk * 16 + kg * 4) * p.q_mul;
+            if (!rows[nt].ok) x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            reinterpret_cast<floatx4 *>(lds)[(nt * KK + kk) * 64 + lane] = x;
+        }
+    const Seen seen = seen_of<NT>(rows);
+    __syncthreads();
+    const floatx4 *qs = reinterpret_cast<const floatx4 *>(lds);
+
+    floatx4 o[DT][4][NT];  // O of d = T*64 + (kg*4 + r)*4 + c in [T][c][nt][r]
+    float m[NT], lpart[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        m[nt] = -INFINITY;
+        lpart[nt] = 0.0f;
+#pragma unroll
+        for (int T = 0; T < DT; T++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[T][c][nt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    {
         for (int i = 0; i < n; i++) {
             const int first = (sh.pg0 + i) * 16;
             const bool inside = seen.all(first, 16);
@@ -327,12 +328,11 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
                 for (int r = 0; r < 4; r++) pr[nt][r] = fast_exp2(x[r] - off);
                 lpart[nt] += (pr[nt][0] + pr[nt][1]) + (pr[nt][2] + pr[nt][3]);
             }
-            // A value that is infinite or NaN reaches only the rows that see its position
-            // (0 times it would not be 0): where some row does not, and there is one, the
-            // rows take turns, each with the values that it sees.
-            bool skip = false, apart = false;
+            // A value that is infinite or NaN reaches only the rows that see its position (0 times
+            // it would not be 0): where some row does not, and there is one, those are left out
+            // of the product and added by themselves.
+            bool apart = false;
             if (!inside) {
-                skip = seen.none(first, 16);
                 float z = rare(0.0f);
 #pragma unroll
                 for (int r = 0; r < 4; r++)
@@ -340,40 +340,57 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
                     for (int T = 0; T < DT; T++)
 #pragma unroll
                         for (int c = 0; c < 4; c++) z = fmaf(v[r][T][c], 0.0f, z);
-                apart = !skip && __ballot(z != z) != 0;
-            }
-            if (apart) {
+                apart = __ballot(z != z) != 0;
+                if (apart) {
+                    const float inf = rare(INFINITY);
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    for (int n16 = 0; n16 < 16; n16++) {
-                        const int lo = __builtin_amdgcn_readlane(rows[nt].lo, n16);
-                        const int hi = __builtin_amdgcn_readlane(rows[nt].hi, n16);
+                    for (int r = 0; r < 4; r++)
 #pragma unroll
                         for (int T = 0; T < DT; T++)
 #pragma unroll
-                            for (int c = 0; c < 4; c++) {
-                                floatx4 x = o[T][c][nt];
+                            for (int c = 0; c < 4; c++) v[r][T][c] = fabsf(v[r][T][c]) < inf ? v[r][T][c] : 0.0f;
+                }
+            }
 #pragma unroll
-                                for (int r = 0; r < 4; r++) {
-                                    const int pos = first + kg * 4 + r;
-                                    const float mine = pos >= lo && pos < hi ? v[r][T][c] : 0.0f;
-                                    x = __builtin_amdgcn_mfma_f32_16x16x4f32(mine, pr[nt][r], x, 0, 0, 0);
-                                }
-                                o[T][c][nt] = lrow == n16 ? x : o[T][c][nt];
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int T = 0; T < DT; T++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            o[T][c][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][T][c], pr[nt][r], o[T][c][nt], 0, 0, 0);
+            if (apart) {
+                const uint8_t *at = p.kv.v + id(i) * p.kv.page_stride + head + kg * 64;
+#pragma unroll 1
+                for (int k4 = 0; k4 < 4; k4++) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int key = 4 * k4 + j, pos = first + key;
+                        float pk[NT];
+                        bool sees[NT];
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            pk[nt] = __shfl(pr[nt][j], k4 * 16 + lrow);
+                            sees[nt] = pos >= rows[nt].lo && pos < rows[nt].hi;
+                        }
+#pragma unroll
+                        for (int T = 0; T < DT; T++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const floatx4 w =
+                                    *reinterpret_cast<const floatx4 *>(at + key * p.kv.row_stride + T * 256 + r * 16);
+#pragma unroll
+                                for (int c = 0; c < 4; c++)
+#pragma unroll
+                                    for (int nt = 0; nt < NT; nt++) {
+                                        const float x = o[T][c][nt][r];
+                                        o[T][c][nt][r] = sees[nt] && !(fabsf(w[c]) < INFINITY) ? fmaf(pk[nt], w[c], x) : x;
+                                    }
+                                asm volatile("" ::: "memory");  // (one row of values at a time in registers)
                             }
                     }
                 }
-            } else if (!skip) {
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int T = 0; T < DT; T++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++)
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++)
-                                o[T][c][nt] =
-                                    __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][T][c], pr[nt][r], o[T][c][nt], 0, 0, 0);
             }
             load_v(id(i + 1));
         }
@@ -381,7 +398,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
     float l[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) l[nt] = sum_rows4(lpart[nt]);
-    merge_and_store<D, NT>(p, sh, m, l, lds, mls, [&](float *slot, const float (&f)[NT]) __attribute__((always_inline)) {
+    merge_and_store<D, NT>(p, sh, m, l, lds, mls, row_at, [&](float *slot, const float (&f)[NT]) __attribute__((always_inline)) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -445,76 +462,59 @@ __device__ __forceinline__ void load_words(const uint8_t *src, uint32_t (&dst)[N
     }
 }
 
+// The f16 pieces of p[j] * scale[j], hi = f16(p * scale) and lo = f16(p * scale - hi), of the
+// f16 scales in the words' high (HIGH) or low halves: 16 mixed multiply-adds, which the
+// compiler writes as products and conversions (24 instructions, and a copy of every word
+// where two tiles use it). The s_nops are wait states that it would count itself: for p,
+// which v_exp_f32 may just have written, for halves written and read, and for the products.
+template <bool HIGH>
+__device__ __forceinline__ void pieces8(const float (&p)[8], const uint32_t (&w)[8], half8 &hi, half8 &lo) {
+    uint32_t h0, h1, h2, h3, l0, l1, l2, l3;
+#define GLA_PIECES(S)                                                                 \
+    asm("s_nop 1\n\t"                                                                \
+        "v_fma_mixlo_f16 %0, %8, %16, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"     \
+        "v_fma_mixlo_f16 %1, %10, %18, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
+        "v_fma_mixlo_f16 %2, %12, %20, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
+        "v_fma_mixlo_f16 %3, %14, %22, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
+        "v_fma_mixhi_f16 %0, %9, %17, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"     \
+        "v_fma_mixhi_f16 %1, %11, %19, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
+        "v_fma_mixhi_f16 %2, %13, %21, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
+        "v_fma_mixhi_f16 %3, %15, %23, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
+        "s_nop 1\n\t"                                                                \
+        "v_fma_mixlo_f16 %4, %8, %16, -%0 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"   \
+        "v_fma_mixlo_f16 %5, %10, %18, -%1 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"  \
+        "v_fma_mixlo_f16 %6, %12, %20, -%2 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"  \
+        "v_fma_mixlo_f16 %7, %14, %22, -%3 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"  \
+        "v_fma_mixhi_f16 %4, %9, %17, -%0 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"   \
+        "v_fma_mixhi_f16 %5, %11, %19, -%1 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"  \
+        "v_fma_mixhi_f16 %6, %13, %21, -%2 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"  \
+        "v_fma_mixhi_f16 %7, %15, %23, -%3 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"  \
+        "s_nop 1"                                                                     \
+        : "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3), "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3) \
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), \
+          "v"(w[0]), "v"(w[1]), "v"(w[2]), "v"(w[3]), "v"(w[4]), "v"(w[5]), "v"(w[6]), "v"(w[7]))
+    if constexpr (HIGH)
+        GLA_PIECES("1");
+    else
+        GLA_PIECES("0");
+#undef GLA_PIECES
+    hi = __builtin_bit_cast(half8, make_uint4(h0, h1, h2, h3));
+    lo = __builtin_bit_cast(half8, make_uint4(l0, l1, l2, l3));
+}
+
 template <int D, int NT, bool CAP>
 __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void prefix_q8_kernel(const PrefixParams p) {
     constexpr int NB = D / 32, NQ = D / 64, ND = D / 16;
     constexpr int QBYTES = NT * NB * 2 * 1024;
     __shared__ __attribute__((aligned(16))) float lds[std::max(QBYTES / 4, kMergeFloats<D, NT>)];
     __shared__ float mls[kWaves][2][16 * NT];
+    __shared__ int row_at[16 * NT];
     __shared__ int qexp[16 * NT];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lrow = lane & 15, kg = lane >> 4;
     const Share sh = share_of<true>(p, 16 * NT, wave);
     if (!sh.any) return;
-
-    // the queries' pieces, [nt][block][piece][lane]: wave w takes the tiles nt = w, w + 4, ...
-    for (int nt = wave; nt < NT; nt += kWaves) {
-        const int r = sh.row0 + nt * 16 + lrow;
-        const bool ok = r < sh.rows;
-        const float *qp = p.q + row_at(p, sh, ok ? r : 0) * D + kg * 8;
-        float x[NB][8], top = 0.0f;
-#pragma unroll
-        for (int blk = 0; blk < NB; blk++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const floatx4 w = *reinterpret_cast<const floatx4 *>(qp + blk * 32 + h * 4) * p.q_mul;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[blk][4 * h + e] = ok ? w[e] : 0.0f;
-                    // (the scale is the finite entries')
-                    const float a = fabsf(x[blk][4 * h + e]);
-                    top = a < INFINITY ? fmaxf(top, a) : top;
-                }
-            }
-        top = max_rows4(top);
-        const int e = pow2_exp(top);
-        const float mul = ldexpf(1.0f, 14 - e);
-        if (kg == 0) qexp[nt * 16 + lrow] = e;
-#pragma unroll
-        for (int blk = 0; blk < NB; blk++) {
-            half8 hi, lo;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float y = x[blk][j] * mul;
-                hi[j] = (_Float16)y;
-                // (an infinite entry's second piece is 0, and its score infinite)
-                lo[j] = __builtin_isinf(y) ? (_Float16)0.0f : (_Float16)(y - (float)hi[j]);
-            }
-            half8 *to = reinterpret_cast<half8 *>(lds) + (nt * NB + blk) * 2 * 64 + lane;
-            to[0] = hi;
-            to[64] = lo;
-        }
-    }
-    Row rows[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) rows[nt] = row_of(p, sh, sh.row0 + nt * 16 + lrow);
-    const Seen seen = seen_of<NT>(rows);
-    __syncthreads();
-    const half8 *qs = reinterpret_cast<const half8 *>(lds);
-    float sm[NT];  // undoes a query's scale
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) sm[nt] = ldexpf(1.0f, qexp[nt * 16 + lrow] - 14);
-
-    floatx4 o[ND][NT];  // O of d = t*16 + kg*4 + r
-    float m[NT], lpart[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        m[nt] = -INFINITY;
-        lpart[nt] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < ND; t++) o[t][nt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
 
     const uint8_t *base = p.kv.k + (int64_t)sh.kvh * p.kv.head_stride;
     uint4 k[2][NQ], v[2][NQ];
@@ -533,18 +533,92 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
         for (int c = 0; c < NQ; c++) v[P][c] = *reinterpret_cast<const uint4 *>(at + 16 * D + off + c * 1024);
         load_words(at + vsoff, vs[P]);
     };
-
+    // (the first pages are on their way while the queries are split; a wave without pages reads the group's first)
     const int n = sh.npg;
+    const int ids = page_ids(p, sh.member, n > 0 ? sh.pg0 : 0, max(n, 1));
+    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(n, 1) - 1)); };
+    load_k(0, id(0));
+    load_k(1, id(1));
+    load_v(0, id(0));
+    load_v(1, id(1));
+
+    Row rows[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        rows[nt] = row_of(p, sh, sh.row0 + nt * 16 + lrow);
+        if (threadIdx.x < 16) row_at[nt * 16 + lrow] = rows[nt].at;
+    }
+    // the queries' pieces, [nt][block][piece][lane]: wave w takes the tiles nt = w, w + 4, ...
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        if (nt % kWaves != wave) continue;
+        const float *qp = p.q + (int64_t)rows[nt].at * D + kg * 8;
+        float x[NB][8], top = 0.0f;
+#pragma unroll
+        for (int blk = 0; blk < NB; blk++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const floatx4 w = *reinterpret_cast<const floatx4 *>(qp + blk * 32 + h * 4) * p.q_mul;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[blk][4 * h + e] = w[e];
+                    top = fmaxf(top, fabsf(w[e]));
+                }
+            }
+        // an infinite entry's second piece is 0 and its score infinite; the scale is the finite entries'
+        const bool infinite = __ballot(top == INFINITY) != 0;
+        if (infinite) {
+            top = rare(0.0f);
+#pragma unroll
+            for (int blk = 0; blk < NB; blk++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float a = fabsf(x[blk][j]);
+                    top = a < INFINITY ? fmaxf(top, a) : top;
+                }
+        }
+        top = max_rows4(top);
+        const int e = pow2_exp(top);
+        const float mul = rows[nt].ok ? ldexpf(1.0f, 14 - e) : 0.0f;
+        if (kg == 0) qexp[nt * 16 + lrow] = e;
+#pragma unroll
+        for (int blk = 0; blk < NB; blk++) {
+            half8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = x[blk][j] * mul;
+                hi[j] = (_Float16)y;
+                lo[j] = (_Float16)(y - (float)hi[j]);
+            }
+            if (infinite) {
+                const float inf = rare(INFINITY);
+#pragma unroll
+                for (int j = 0; j < 8; j++) lo[j] = fabsf(x[blk][j]) == inf ? (_Float16)0.0f : lo[j];
+            }
+            half8 *to = reinterpret_cast<half8 *>(lds) + (nt * NB + blk) * 2 * 64 + lane;
+            to[0] = hi;
+            to[64] = lo;
+        }
+    }
+    const Seen seen = seen_of<NT>(rows);
+    __syncthreads();
+    const half8 *qs = reinterpret_cast<const half8 *>(lds);
+    float sm[NT];  // undoes a query's scale
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) sm[nt] = ldexpf(1.0f, qexp[nt * 16 + lrow] - 14);
+
+    floatx4 o[ND][NT];  // O of d = t*16 + kg*4 + r
+    float m[NT], lpart[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        m[nt] = -INFINITY;
+        lpart[nt] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < ND; t++) o[t][nt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
     float unit = 1.0f;  // of O and of the sums of P
-    float zero = 0.0f;  // (not known to the compiler, which would multiply and convert in two instructions)
-    asm volatile("" : "+s"(zero));
     if (n > 0) {
-        const int ids = page_ids(p, sh.member, sh.pg0, n);
-        const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, n - 1)); };
-        load_k(0, id(0));
-        load_k(1, id(1));
-        load_v(0, id(0));
-        load_v(1, id(1));
         // P' = p * vscale * 2^vexp is below 2^14 (p at most 2^kLazy)
         float vmax = 0.0f;
         const int units = n * (D / 16);  // 16 bytes of V scales each
@@ -603,8 +677,10 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
             uint32_t sees[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                floatx4 x[2] = {s[nt][0] * sm[nt], s[nt][1] * sm[nt]};
+                floatx4 x[2] = {s[nt][0], s[nt][1]};
                 if constexpr (CAP) {
+                    x[0] *= sm[nt];
+                    x[1] *= sm[nt];
                     const SoftCap f(p.softcap);
 #pragma unroll
                     for (int j = 0; j < 8; j++) x[j >> 2][j & 3] = f(x[j >> 2][j & 3]);
@@ -621,8 +697,9 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
                         x[j >> 2][j & 3] = ok ? x[j >> 2][j & 3] : -INFINITY;
                     }
                 }
-                const float mine = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                                         fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+                const float c = CAP ? 1.0f : sm[nt];
+                const float mine = c * fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                                             fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
                 if (__ballot(mine > m[nt] + kLazy)) {
                     const float f = moved(m[nt], mine);
                     lpart[nt] *= f;
@@ -631,7 +708,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
                 }
                 const float off = m[nt] == -INFINITY ? 0.0f : vexp - m[nt];
 #pragma unroll
-                for (int j = 0; j < 8; j++) pr[nt][j] = fast_exp2(x[j >> 2][j & 3] + off);
+                for (int j = 0; j < 8; j++) pr[nt][j] = fast_exp2(fmaf(x[j >> 2][j & 3], c, off));
                 lpart[nt] += ((pr[nt][0] + pr[nt][1]) + (pr[nt][2] + pr[nt][3])) +
                              ((pr[nt][4] + pr[nt][5]) + (pr[nt][6] + pr[nt][7]));
             }
@@ -647,16 +724,14 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    half8 hi, lo;  // of p * vscale: the product's rounding, and what that leaves
+                    half8 hi, lo;
+                    uint32_t w[8];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        // (opaque, or the tiles share one conversion and lose the mixed multiply-add)
-                        uint32_t w[1] = {vs[j >> 2][((j & 3) * NB + blk) >> 1]};
-                        asm volatile("" : "+v"(w[0]));
-                        const float scale = half_at(w, blk & 1);
-                        hi[j] = (_Float16)fmaf(pr[nt][j], scale, zero);
-                        lo[j] = (_Float16)fmaf(pr[nt][j], scale, -(float)hi[j]);
-                    }
+                    for (int j = 0; j < 8; j++) w[j] = vs[j >> 2][((j & 3) * NB + blk) >> 1];
+                    if (blk & 1)
+                        pieces8<true>(pr[nt], w, hi, lo);
+                    else
+                        pieces8<false>(pr[nt], w, hi, lo);
                     // a scale that is infinite or NaN, at a position that the row does not see
                     // (nothing) or sees (infinity has no second piece)
                     if (!plain) {
@@ -682,13 +757,13 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void pr
     float l[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) l[nt] = sum_rows4(lpart[nt]) * unit;
-    merge_and_store<D, NT>(p, sh, m, l, lds, mls, [&](float *slot, const float (&f)[NT]) __attribute__((always_inline)) {
+    merge_and_store<D, NT>(p, sh, m, l, lds, mls, row_at, [&](float *slot, const float (&f)[NT]) __attribute__((always_inline)) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int t = 0; t < ND; t++)
                 *reinterpret_cast<floatx4 *>(slot + (nt * 16 + lrow) * out_row(D) + t * 16 + kg * 4) =
-                    o[t][nt] * unit * f[nt];
+                    o[t][nt] * (unit * f[nt]);
     });
 }
 
@@ -742,13 +817,34 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
     }
     const int64_t tile = 16 * tiles_of(d), group = d.n_heads / d.n_kv_heads;
     const int pages = pre->max_prefix / 16;
-    // row tiles of all groups, at most
+    // workgroups of a launch with splits of n pages: as they are, or from the bounds
+    const bool host = pre->group_start_host && pre->n_groups <= 256;
     const int64_t tiles = std::min<int64_t>(pre->n_groups * ((pre->max_group * group - 1) / tile + 1),
                                             d.n_seqs * group / tile + pre->n_groups);
-    const int64_t want = (d.head_dim == 256 ? 1 : 2) * (int64_t)ctx->n_cu / std::max<int64_t>(1, tiles * d.n_kv_heads);
-    const int64_t each = (pages + std::max<int64_t>(1, want) - 1) / std::max<int64_t>(1, want);
-    // (a wave's pages: an even number, at most 64)
-    pre->split_pages = (int)std::min<int64_t>(std::max<int64_t>((each + 7) / 8 * 8, 8), 256);
+    const auto wgs = [&](int n) {
+        int64_t sum = 0;
+        for (int g = 0; host && g < pre->n_groups; g++) {
+            const int64_t rows = (pre->group_start_host[g + 1] - pre->group_start_host[g]) * group;
+            sum += (rows + tile - 1) / tile * ((prefix_positions(pre->prefix_len_host[g], pre->max_prefix) / 16 + n - 1) / n);
+        }
+        return (host ? sum : tiles * ((pages + n - 1) / n)) * d.n_kv_heads;
+    };
+    // the fewest pages (a wave's: an even number, at most 64) that leave at most `most` workgroups
+    const auto pages_for = [&](int64_t most) {
+        int n = 8;
+        while (n < 256 && wgs(n) > most) n += 8;
+        return n;
+    };
+    // A workgroup for every unit. With Q8_0, whose waves wait for their own vector and matrix
+    // instructions in turn, two, where a split keeps 32 pages; with several groups of f32, whose
+    // unlike lengths leave units idle, two where it keeps 16. Else the waves' set-up and the
+    // combine's splits cost more than they gain. us a call, one / two a unit: behind 8,192
+    // positions 64 rows at 32/8 heads, d = 128, Q8_0 57.0 / 54.9, f32 110 / 112; 16 rows, f32
+    // 40.7 / 43.8; 4 rows, Q8_0 25.0 / 29.9; 24 rows in 3 groups behind up to 4,096 f32 positions
+    // at 16/8, d = 256 79 / 63, 64 rows in one group 78 / 85.
+    const int one = pages_for(ctx->n_cu), least = d.q8 ? 32 : 16;
+    const bool two = d.q8 || pre->n_groups > 1;
+    pre->split_pages = two ? std::max(pages_for(2 * (int64_t)ctx->n_cu), std::min(one, least)) : one;
     pre->n_splits = (pages + pre->split_pages - 1) / pre->split_pages;
 }
 
