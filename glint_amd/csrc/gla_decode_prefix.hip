@@ -794,18 +794,20 @@ int launch_as(gla_ctx *ctx, bool q8, const PrefixParams &prm, dim3 grid) {
 // two more launches than the rows by themselves; what it saves are the bytes that the rows
 // would read again (from L2 mostly) and, with Q8_0, the length of a wave's chain of pages.
 // us a call, apart / row by row, in a captured step with 1-33 positions of each row's own:
-//   f32   9/3 heads, d = 64:   4 rows of 704 14.5 / 9.3, 16 of 2,048 18.7 / 14.2, 16 of 4,096 (94 MB saved) 19.8 / 20.1
-//        32/8 heads, d = 128:  2 rows of 4,096 23.7 / 19.9, 16 of 704 (87 MB) 25.0 / 30.2, 4 of 4,096 (101 MB) 24.2 / 31.3
-//        16/8 heads, d = 256:  8 rows of 704 (81 MB) 26.2 / 22.3, 4 of 2,048 (101 MB) 27.4 / 28.1, 16 of 4,096 36 / 149
-//   Q8_0 32/8 heads, d = 128: 16 rows of 704 (23 MB) 20.2 / 18.3, 8 of 2,048 (31 MB) 22.9 / 26.4, 2 of 4,096 24.4 / 25.1
-//        16/8 heads, d = 256:  8 rows of 704 23.2 / 20.2, 2 of 2,048 26.7 / 41.9
+//   f32   9/3 heads, d = 64:   4 rows of 704 14.0 / 9.3, 16 of 2,048 17.7 / 14.1, 16 of 4,096 (94 MB saved) 19.0 / 20.1
+//        32/8 heads, d = 128:  2 rows of 4,096 22.9 / 19.8, 16 of 704 (87 MB) 24.0 / 30.2, 4 of 4,096 (101 MB) 23.3 / 31.0
+//        16/8 heads, d = 256:  8 rows of 704 (81 MB) 25.9 / 22.3, 4 of 2,048 (101 MB) 26.9 / 28.0, 16 of 4,096 35 / 148
+//   Q8_0  9/3 heads, d = 64:   8 rows of 2,048 18.3 / 17.1, 2 of 4,096 19.0 / 21.0
+//        32/8 heads, d = 128: 16 rows of 704 (23 MB) 19.0 / 18.1, 8 of 2,048 (31 MB) 22.0 / 26.1, 2 of 2,048 18.9 / 19.7,
+//                              2 of 4,096 23.1 / 25.4
+//        16/8 heads, d = 256:  8 rows of 704 21.9 / 20.1, 2 of 2,048 25.1 / 42.0
 static bool pays(const DecodeLaunch &d) {
     const int64_t position = d.kv.page_stride / 16;  // bytes
     if (d.pre.max_prefix == 0) return false;
     if (const char *env = getenv("GLA_DECODE_PREFIX")) return atoi(env) != 0;  // (tuning and tests)
     const int64_t saved = (int64_t)(d.n_seqs - d.pre.n_groups) * d.pre.max_prefix * position;
     if (!d.q8) return saved >= 84000000;
-    return saved >= 28000000 || d.pre.max_prefix >= (d.head_dim == 256 ? 1536 : 4096);
+    return saved >= 28000000 || d.pre.max_prefix >= (d.head_dim == 256 ? 1024 : 2500);
 }
 
 void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {

@@ -72,15 +72,22 @@ struct Pieces {
             }
         }
     }
+    template <bool ONCE>
     __device__ __forceinline__ void store(float *row, int t, int pieces) const {
 #pragma unroll
         for (int k = 0; k < N; k++) {
             const int i = t + k * T;
             if (i < pieces) {
-                if constexpr (E == 4)
-                    *reinterpret_cast<vec *>(row + 4 * i) = vec{v[k][0], v[k][1], v[k][2], v[k][3]};
-                else
+                if constexpr (E == 4) {
+                    vec *at = reinterpret_cast<vec *>(row + 4 * i);
+                    const vec w = {v[k][0], v[k][1], v[k][2], v[k][3]};
+                    if constexpr (ONCE)
+                        __builtin_nontemporal_store(w, at);
+                    else
+                        *at = w;
+                } else {
                     row[i] = v[k][0];
+                }
             }
         }
     }
@@ -96,7 +103,7 @@ struct Pieces {
 
 // T threads a row, N pieces of E floats a thread. Everything that a row needs, its weights
 // too, is asked for before the first sum: one round trip to memory and two sums are what a
-// few rows cost. ONCE: the rows' inputs pass the caches by.
+// few rows cost. ONCE: the rows pass the caches by.
 template <int T, int N, int E, bool ONCE>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void block_norm_kernel(const NormParams p) {
     constexpr int RPW = T < 256 ? 256 / T : 1;  // rows per workgroup
@@ -127,14 +134,14 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_norm_kernel(const Nor
                 x.v[k][e] = p.post ? fmaf(z, post.v[k][e], x.v[k][e]) : x.v[k][e] + z;
             }
     }
-    if (p.x_out) x.store(p.x_out + r * p.x_out_stride, t, pieces);
+    if (p.x_out) x.template store<ONCE>(p.x_out + r * p.x_out_stride, t, pieces);
     if (p.norm_out) {
         const float f = 1.0f / sqrtf(row_sum<T>(x.squares(), lds[1]) / (float)p.dim + p.eps);
 #pragma unroll
         for (int k = 0; k < N; k++)
 #pragma unroll
             for (int e = 0; e < E; e++) x.v[k][e] *= f * pre.v[k][e];
-        x.store(p.norm_out + r * p.norm_out_stride, t, pieces);
+        x.template store<ONCE>(p.norm_out + r * p.norm_out_stride, t, pieces);
     }
 }
 
@@ -162,10 +169,11 @@ int launch_as(gla_ctx *ctx, const NormParams &p) {
 template <int E>
 int launch_e(gla_ctx *ctx, const NormParams &p) {
     const int pieces = p.dim / E;
-    // What the call moves, where it is more than the last-level cache holds, would push out of
-    // the caches what the next call reads from them: inputs are then read past them. us a call,
-    // past / through them: 7,993 rows of 4,096, all inputs (655 MB) 104 / 113, without post and
-    // gate (524 MB) 81 / 94; 8,192 of 576 (75 MB) 16.9 / 13.1, 256 of 4,096 (21 MB) 7.4 / 6.2.
+    // Rows that are more than the last-level cache holds pass it by. us a call on rows that no
+    // cache holds, past / through them: 7,993 rows of 4,096, all inputs (655 MB) 104 / 114,
+    // without post and gate (524 MB) 91 / 96. Fewer go through them, for who wrote and who
+    // reads them: inputs read past them on rows that they hold, 8,192 of 576 (75 MB) 16.9 / 13.1,
+    // 256 of 4,096 (21 MB) 7.4 / 6.2.
     if constexpr (E == 4) {
         const int64_t rows = 1 + (p.y != nullptr) + (p.gate && p.gate_stride) + (p.x_out != nullptr) + (p.norm_out != nullptr);
         if (rows * p.n_rows * p.dim * 4 > (int64_t)256 << 20) {
