@@ -1455,10 +1455,9 @@ __global__ __launch_bounds__(256) void stage_bf16_kernel(const PrefillParams p, 
 template <int D, bool STAGED, int NT>
 constexpr int kSplitOccupancy = !STAGED ? (D == 64 ? 2 : 1) : (D == 64 ? 4 - NT : (D == 128 ? 2 : 1));
 
-template <int D, bool Q8, bool CAP, bool STAGED, int NT>
-__global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill_split_kernel(const PrefillParams p,
-                                                                                                const Images im) {
-    constexpr int NW = 4;
+template <int D, bool Q8, bool CAP, bool STAGED, int NT, int NW = 4>
+__global__ __launch_bounds__(NW * 64, (NW == 8 ? 2 : kSplitOccupancy<D, STAGED, NT>)) void prefill_split_kernel(
+    const PrefillParams p, const Images im) {
     constexpr int QW = 16 * NT;
     constexpr int KS = D / 32;
     constexpr int DT = D / 16;
@@ -2018,10 +2017,10 @@ __global__ __launch_bounds__(256, (kSplitOccupancy<D, STAGED, NT>)) void prefill
     }
 }
 
-// Query blocks of a call whose waves (four to a workgroup) take nt 16-query
+// Query blocks of a call whose waves (nw to a workgroup) take nt 16-query
 // tiles each.
-int wg_blocks(const PrefillParams &prm, int nt) {
-    const int rows = 16 * nt * (4 / prm.hpw);
+int wg_blocks(const PrefillParams &prm, int nt, int nw = 4) {
+    const int rows = 16 * nt * (nw / prm.hpw);
     return (prm.max_q_len + rows - 1) / rows;
 }
 // 16-query tiles per wave of a staged kernel: two share every operand read, one
@@ -2033,6 +2032,16 @@ int wg_blocks(const PrefillParams &prm, int nt) {
 // 76.5; six Gemma-2 prompts (528, half of them empty) f32 96.2 / 104.9.
 int wave_tiles(const gla_ctx *ctx, const PrefillParams &prm, int n_units) {
     return 2 * (int64_t)n_units * wg_blocks(prm, 2) <= 3 * (int64_t)ctx->n_cu ? 1 : 2;
+}
+
+// Waves of a workgroup at head_dim 256, whose tiles leave a CU room for one workgroup: four
+// waves are one a SIMD, eight two, that multiply while the other loads and exponentiates
+// (the same bits). Eight once the workgroups of four are more than the CUs. us per call,
+// four waves of one tile / of two / eight of one, 16/8 heads: 777 and 1,000 rows in a window
+// of 4,096 + 33 620 / 634 / 487, 4 x 2,048 rows, 1,024 + 4 521 / 516 / 430, 4 of 100-700,
+// 512 + 4 105 / 109 / 81; 1,000 rows (256 workgroups) 81 / 147 / 100, 64 rows 205 / 396 / 258.
+bool eight_waves(const gla_ctx *ctx, const PrefillParams &prm, int n_units) {
+    return (int64_t)n_units * wg_blocks(prm, 1) > ctx->n_cu;
 }
 
 template <int D, bool CAP>
@@ -2091,12 +2100,12 @@ template <int D>
 constexpr int kUnstagedRows = D == 256 ? 32 : 64;
 constexpr int kUnstagedTiles = 3;
 
-template <int D, bool Q8, bool CAP, bool STAGED, int NT>
+template <int D, bool Q8, bool CAP, bool STAGED, int NT, int NW = 4>
 int launch_split_as(gla_ctx *ctx, PrefillParams prm, int n_units, const Images &im) {
-    prm.n_qblocks = wg_blocks(prm, NT);
+    prm.n_qblocks = wg_blocks(prm, NT, NW);
     const int y = std::min(prm.n_qblocks, 65535);
-    hipLaunchKernelGGL((prefill_split_kernel<D, Q8, CAP, STAGED, NT>), dim3(n_units, y, (prm.n_qblocks - 1) / y + 1),
-                       dim3(256), 0, ctx->stream, prm, im);
+    hipLaunchKernelGGL((prefill_split_kernel<D, Q8, CAP, STAGED, NT, NW>), dim3(n_units, y, (prm.n_qblocks - 1) / y + 1),
+                       dim3(NW * 64), 0, ctx->stream, prm, im);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "prefill_split_kernel launch: %s", hipGetErrorString(e));
     return GLA_OK;
@@ -2155,8 +2164,13 @@ int launch_split(gla_ctx *ctx, const PrefillParams &prm, int n_seqs, int n_hgrp,
         hipLaunchKernelGGL((stage_split_kernel<D, Q8>), dim3(n_seqs, slices), dim3(256), 0, ctx->stream, prm, im);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "stage_split_kernel launch: %s", hipGetErrorString(e));
-        const int rc = wave_tiles(ctx, prm, n_units) == 1 ? launch_split_as<D, Q8, CAP, true, 1>(ctx, prm, n_units, im)
-                                                          : launch_split_as<D, Q8, CAP, true, 2>(ctx, prm, n_units, im);
+        int rc;
+        if constexpr (kSinks && D == 256)
+            rc = eight_waves(ctx, prm, n_units) ? launch_split_as<D, Q8, CAP, true, 1, 8>(ctx, prm, n_units, im)
+                                                : launch_split_as<D, Q8, CAP, true, 1>(ctx, prm, n_units, im);
+        else
+            rc = wave_tiles(ctx, prm, n_units) == 1 ? launch_split_as<D, Q8, CAP, true, 1>(ctx, prm, n_units, im)
+                                                    : launch_split_as<D, Q8, CAP, true, 2>(ctx, prm, n_units, im);
         if (rc != GLA_OK) return rc;
     }
     return all_placed ? GLA_OK : launch_split_as<D, Q8, CAP, false, 1>(ctx, prm, n_units, im);
