@@ -632,7 +632,7 @@ struct GpuBackend::Staging {
         void *ptr = nullptr;
         size_t bytes = 0;
     };
-    enum { Q, OUT, TABLE, START, LEN, SLOT, QSTART, POSOFF, POS, K, V, N_BUFS };
+    enum { Q, OUT, TABLE, START, LEN, SLOT, QSTART, POSOFF, POS, K, V, GROUP, PREFIX, NORM, POST, PRE, N_BUFS };
     std::shared_ptr<Device> dev;
     Buf bufs[N_BUFS];
 
@@ -788,8 +788,50 @@ Result<Source> source_of(const std::vector<const KvStore *> &stores, const char 
 
 }  // namespace
 
-Result<std::vector<float>> GpuBackend::decode_batch(const std::vector<DecodeSeq> &seqs, const float *q,
-                                                    size_t layer, const AttnShape &shape) {
+namespace {
+
+// Neighbouring sequences of a paged batch that begin with the same pages.
+struct Groups {
+    std::vector<int32_t> start{0}, prefix;  // rows of group g: [start[g], start[g+1]); positions they share
+    int max_group = 0, max_prefix = 0;
+};
+Groups groups_of(const std::vector<DecodeSeq> &seqs, size_t layer) {
+    Groups g;
+    const auto table = [&](size_t b) -> const auto & { return seqs[b].kv->as_paged()->page_table(layer); };
+    for (size_t first = 0; first < seqs.size();) {
+        size_t end = first + 1, pages = 0;
+        for (; end < seqs.size(); end++) {
+            const auto &a = table(first), &b = table(end);
+            size_t n = std::min(end == first + 1 ? a.size() : pages, b.size());
+            n = (size_t)(std::mismatch(a.begin(), a.begin() + (ptrdiff_t)n, b.begin()).first - a.begin());
+            // (a row that shares less than half of what the others do begins another group)
+            if (n == 0 || 2 * n < pages) break;
+            pages = n;
+        }
+        g.start.push_back((int32_t)end);
+        g.prefix.push_back((int32_t)(pages * PAGE_SIZE));
+        g.max_group = std::max(g.max_group, (int)(end - first));
+        g.max_prefix = std::max(g.max_prefix, g.prefix.back());
+        first = end;
+    }
+    return g;
+}
+
+}  // namespace
+
+Result<std::vector<float>> GpuBackend::decode_batch(const std::vector<DecodeSeq> &seqs, const float *q, size_t layer,
+                                                    const AttnShape &shape) {
+    return decode(seqs, q, layer, shape, false);
+}
+
+Result<std::vector<float>> GpuBackend::decode_batch_shared(const std::vector<DecodeSeq> &seqs, const float *q,
+                                                           size_t layer, const AttnShape &shape) {
+    if (shape.n_sinks) return GlintError::gpu_shader_error("decode_batch_shared: n_sinks is for decode_batch");
+    return decode(seqs, q, layer, shape, true);
+}
+
+Result<std::vector<float>> GpuBackend::decode(const std::vector<DecodeSeq> &seqs, const float *q, size_t layer,
+                                              const AttnShape &shape, bool shared) {
     const size_t B = seqs.size();
     const size_t row = (size_t)shape.n_heads * shape.head_dim;
     if (B == 0) return std::vector<float>();
@@ -859,7 +901,29 @@ Result<std::vector<float>> GpuBackend::decode_batch(const std::vector<DecodeSeq>
     a.softcap = shape.softcap;
     a.kv_start_host = start.data();
     a.kv_len_host = len.data();
-    Status s = check(gla_decode(dev_->ctx(), &a), "gla_decode");
+    Status s = Status();
+    if (shared && S.paged) {
+        const Groups g = groups_of(seqs, layer);
+        gla_decode_shared_args sa{};
+        sa.decode = a;
+        sa.n_groups = (int)g.prefix.size();
+        if (!(p = st.put(Staging::GROUP, g.start.data(), g.start.size() * 4))) return p.error();
+        sa.group_start = (const int32_t *)p.value();
+        if (!(p = st.put(Staging::PREFIX, g.prefix.data(), g.prefix.size() * 4))) return p.error();
+        sa.prefix_len = (const int32_t *)p.value();
+        sa.max_group = g.max_group;
+        sa.max_prefix_len = g.max_prefix;
+        for (size_t i = 0; i < g.prefix.size(); i++)
+            for (int32_t b = g.start[i]; b < g.start[i + 1]; b++)
+                sa.max_own_len = std::max(sa.max_own_len, start[b] + len[b] - g.prefix[i]);
+        sa.group_start_host = g.start.data();
+        sa.prefix_len_host = g.prefix.data();
+        s = check(gla_decode_shared(dev_->ctx(), &sa), "gla_decode_shared");
+    } else if (shape.n_sinks) {
+        s = check(gla_decode_sinks(dev_->ctx(), &a, (int)std::min<uint32_t>(shape.n_sinks, INT32_MAX)), "gla_decode_sinks");
+    } else {
+        s = check(gla_decode(dev_->ctx(), &a), "gla_decode");
+    }
     if (!s) return s.error();
     std::vector<float> out(B * row);
     s = check(gla_memcpy_dtoh(dev_->ctx(), out.data(), a.out, out.size() * sizeof(float)), "gla_memcpy_dtoh");
@@ -938,7 +1002,9 @@ Result<std::vector<float>> GpuBackend::prefill_batch(const std::vector<PrefillSe
     a.softcap = shape.softcap;
     a.sliding_window = (int)sliding_window;
     a.precision = precision;
-    Status s = check(gla_prefill(dev_->ctx(), &a), "gla_prefill");
+    Status s = shape.n_sinks ? check(gla_prefill_sinks(dev_->ctx(), &a, (int)std::min<uint32_t>(shape.n_sinks, INT32_MAX)),
+                                     "gla_prefill_sinks")
+                             : check(gla_prefill(dev_->ctx(), &a), "gla_prefill");
     if (!s) return s.error();
     std::vector<float> out(rows * row);
     s = check(gla_memcpy_dtoh(dev_->ctx(), out.data(), a.out, out.size() * sizeof(float)), "gla_memcpy_dtoh");
@@ -1201,6 +1267,55 @@ Result<std::vector<float>> GpuBackend::append_batch(const std::vector<AppendSeq>
     if (!s) return s.error();
     std::vector<float> out(rows * row);
     s = check(gla_memcpy_dtoh(dev_->ctx(), out.data(), a.q_out, out.size() * sizeof(float)), "gla_memcpy_dtoh");
+    if (!s) return s.error();
+    return out;
+}
+
+Result<NormedBlock> GpuBackend::block_norm(const float *x, const float *y, size_t n_rows, size_t dim,
+                                           const BlockNorm &norm) {
+    NormedBlock out;
+    if (n_rows > INT32_MAX || dim > GLA_BLOCK_NORM_MAX_DIM)
+        return GlintError::gpu_shader_error(fmt("block_norm: %zu rows of %zu", n_rows, dim));
+    if (n_rows == 0) return out;
+    const size_t bytes = n_rows * dim * sizeof(float), vec = dim * sizeof(float);
+    gla_block_norm_args a{};
+    a.n_rows = (int)n_rows;
+    a.dim = (int)dim;
+    a.eps = norm.eps;
+    a.scale = norm.scale;
+    Staging &st = *stage_;
+    Result<void *> p = st.put(Staging::Q, x, bytes);
+    if (!p) return p.error();
+    a.x = (const float *)p.value();
+    if (y) {
+        if (!(p = st.put(Staging::K, y, bytes))) return p.error();
+        a.y = (const float *)p.value();
+    }
+    if (norm.post) {
+        if (!(p = st.put(Staging::POST, norm.post, vec))) return p.error();
+        a.post = (const float *)p.value();
+    }
+    if (norm.gate) {
+        if (!(p = st.put(Staging::V, norm.gate, norm.gate_rows ? bytes : vec))) return p.error();
+        a.gate = (const float *)p.value();
+        a.gate_stride = norm.gate_rows ? (int64_t)dim : 0;
+    }
+    if (!(p = st.get(Staging::OUT, bytes))) return p.error();
+    a.x_out = (float *)p.value();
+    if (norm.pre) {
+        if (!(p = st.put(Staging::PRE, norm.pre, vec))) return p.error();
+        a.pre = (const float *)p.value();
+        if (!(p = st.get(Staging::NORM, bytes))) return p.error();
+        a.norm_out = (float *)p.value();
+    }
+    Status s = check(gla_block_norm(dev_->ctx(), &a), "gla_block_norm");
+    if (!s) return s.error();
+    out.x.resize(n_rows * dim);
+    s = check(gla_memcpy_dtoh(dev_->ctx(), out.x.data(), a.x_out, bytes), "gla_memcpy_dtoh");
+    if (s && a.norm_out) {
+        out.normed.resize(n_rows * dim);
+        s = check(gla_memcpy_dtoh(dev_->ctx(), out.normed.data(), a.norm_out, bytes), "gla_memcpy_dtoh");
+    }
     if (!s) return s.error();
     return out;
 }

@@ -435,6 +435,22 @@ struct AttnShape {
     uint32_t head_dim = 0;
     float scale = 0.0f;    // query_pre_attn_scalar or 1/sqrt(head_dim)
     float softcap = 0.0f;  // attn_logit_softcapping; 0: none
+    uint32_t n_sinks = 0;  // first positions that stay visible where a window has left them behind
+};
+
+// The norms around a block (gla_block_norm): post, gate and pre are [dim] host
+// vectors or null, the gate [n_rows][dim] with gate_rows.
+struct BlockNorm {
+    const float *post = nullptr;
+    const float *gate = nullptr;
+    bool gate_rows = false;
+    const float *pre = nullptr;
+    float eps = 1e-6f;
+    float scale = 1.0f;
+};
+struct NormedBlock {
+    std::vector<float> x;       // the residual stream, [n_rows][dim]
+    std::vector<float> normed;  // the next block's input; empty without pre
 };
 
 // GGML Q8_0 weights on the device: the buffer QuantizedTensor::upload_to_gpu
@@ -542,6 +558,12 @@ class GpuBackend {
     // caller keeps its CPU path.
     Result<std::vector<float>> decode_batch(const std::vector<DecodeSeq> &seqs, const float *q, size_t layer,
                                             const AttnShape &shape);
+    // decode_batch of sequences that were forked from common prefixes
+    // (PagedKvCache::fork_from): neighbours whose tables begin with the same
+    // pages are read together (gla_decode_shared), up to rounding the same.
+    // Order the batch by its prefixes. n_sinks is refused.
+    Result<std::vector<float>> decode_batch_shared(const std::vector<DecodeSeq> &seqs, const float *q, size_t layer,
+                                                   const AttnShape &shape);
     // Causal prefill of a batch of prompt chunks whose K/V are written: q
     // [sum n_rows][n_heads*head_dim] host -> same shape. sliding_window 0:
     // none. precision GLA_PREC_BF16 rounds the matrix-product inputs to bf16.
@@ -581,9 +603,16 @@ class GpuBackend {
                                             const float *v, size_t layer, const AttnShape &shape,
                                             const GpuRopePlan *plan);
 
+    // A block's output y joined to the residual stream x, and the sum normed for
+    // the next block (rms_norm and add of src/backend/shaders, with what
+    // models put between them): x, y [n_rows][dim] host; y null: x alone.
+    Result<NormedBlock> block_norm(const float *x, const float *y, size_t n_rows, size_t dim, const BlockNorm &norm);
+
   private:
     explicit GpuBackend(std::shared_ptr<Device> dev);
     struct Staging;
+    Result<std::vector<float>> decode(const std::vector<DecodeSeq> &seqs, const float *q, size_t layer,
+                                      const AttnShape &shape, bool shared);
     std::shared_ptr<Device> dev_;
     std::unique_ptr<Staging> stage_;
 };

@@ -1181,6 +1181,122 @@ DEVICE_TEST(test_rope_rows_through_host_layer) {
     CHECK(!backend().create_rope_plan(spec).ok());
 }
 
+// A window with sinks, decoded and prefilled, over paged caches: the rows see the first
+// n_sinks positions beside their window.
+DEVICE_TEST(test_sinks_match_f64) {
+    const uint32_t H = 4, Hkv = 2, d = 64, sinks = 5;
+    const size_t kv_dim = (size_t)Hkv * d, window = 23, n = 90, chunk = 40;
+    for (gla_kv_dtype dt : {GLA_KV_F32, GLA_KV_Q8_0}) {
+        PagePool shared = backend().create_page_pool(16, Hkv, d, dt).expect("pool");
+        PagedKvCache seq(shared, 1);
+        Rng rng(70 + dt);
+        seq.reserve(n).expect("room");
+        const auto k = rng.normal(n * kv_dim), v = rng.normal(n * kv_dim);
+        seq.write_chunk(0, 0, n, k.data(), v.data());
+        AttnShape shape{H, Hkv, d, 0.125f, 0.0f, sinks};
+        const auto q = rng.normal(chunk * H * d);
+        const auto rows = backend().prefill_batch({{&seq, chunk, n - chunk}}, q.data(), 0, shape, window).expect("prefill");
+        const auto one = backend().decode_batch({{&seq, n - window, window}}, &q[(chunk - 1) * H * d], 0, shape).expect("decode");
+        for (size_t r = 0; r < chunk; r++) {
+            const size_t pos = n - chunk + r;
+            std::vector<std::vector<float>> K, V;
+            for (size_t j = 0; j <= pos; j++)
+                if (j + window > pos || j < sinks) {
+                    K.push_back(seq.k_at(0, j));
+                    V.push_back(seq.v_at(0, j));
+                }
+            for (uint32_t h = 0; h < H; h++) {
+                const size_t o = (r * H + h) * d;
+                const auto want = attend_f64(&q[o], K, V, h / (H / Hkv), d, shape.scale, 0.0);
+                check_close(&rows[o], want, "prefill row " + std::to_string(r));
+                if (r + 1 == chunk) check_close(&one[h * d], want, "decode");
+            }
+        }
+        CHECK(!backend().decode_batch_shared({{&seq, 0, n}}, q.data(), 0, shape).ok());
+    }
+}
+
+// Forks of two prompts and a sequence of its own, decoded with their prefixes read once,
+// by the rule and always, against decode_batch.
+DEVICE_TEST(test_forks_decode_with_their_prefix_read_once) {
+    const uint32_t H = 8, Hkv = 2, d = 128;
+    const size_t kv_dim = (size_t)Hkv * d;
+    for (gla_kv_dtype dt : {GLA_KV_F32, GLA_KV_Q8_0}) {
+        PagePool shared = backend().create_page_pool(80, Hkv, d, dt).expect("pool");
+        Rng rng(5 + dt);
+        const auto write = [&](PagedKvCache &c, size_t to) {
+            for (size_t pos = c.len(); pos < to; pos++) {
+                const auto k = rng.normal(kv_dim), v = rng.normal(kv_dim);
+                c.write(0, pos, k.data(), v.data());
+                c.advance();
+            }
+        };
+        PagedKvCache first(shared, 1), second(shared, 1), own(shared, 1);
+        write(first, 200);
+        write(second, 75);
+        write(own, 50);
+        std::vector<PagedKvCache> forks;
+        for (size_t at : {200u, 193u, 160u}) forks.push_back(first.fork_from(at));
+        for (size_t at : {75u, 64u}) forks.push_back(second.fork_from(at));
+        for (size_t i = 0; i < forks.size(); i++) write(forks[i], forks[i].len() + 3 + 9 * i);
+        std::vector<DecodeSeq> seqs;
+        for (size_t i = 0; i < 3; i++) seqs.push_back({&forks[i], 0, forks[i].len()});
+        seqs.push_back({&own, 0, own.len()});
+        for (size_t i = 3; i < 5; i++) seqs.push_back({&forks[i], 10, forks[i].len() - 10});
+        seqs.push_back({&second, 0, 0});
+        const AttnShape shape{H, Hkv, d, 0.09f, 0.0f};
+        const auto q = rng.normal(seqs.size() * H * d);
+        const auto want = backend().decode_batch(seqs, q.data(), 0, shape).expect("decode");
+        for (const char *apart : {"", "1"}) {
+            if (*apart) setenv("GLA_DECODE_PREFIX", apart, 1);
+            auto r = backend().decode_batch_shared(seqs, q.data(), 0, shape);
+            unsetenv("GLA_DECODE_PREFIX");
+            const auto got = std::move(r).expect("shared");
+            CHECK_EQ(got.size(), want.size());
+            for (size_t i = 0; i < got.size(); i++) CHECK(std::fabs(got[i] - want[i]) <= 1e-5f);
+        }
+        // caches of their own share nothing
+        auto caches = backend().create_kv_caches(2, 1, 32, Hkv, d, dt).expect("caches");
+        std::vector<DecodeSeq> two;
+        for (auto &c : caches) {
+            const auto k = rng.normal(20 * kv_dim), v = rng.normal(20 * kv_dim);
+            c.write_chunk(0, 0, 20, k.data(), v.data());
+            two.push_back({&c, 0, 20});
+        }
+        CHECK(rows_equal(backend().decode_batch_shared(two, q.data(), 0, shape).expect("shared"),
+                         backend().decode_batch(two, q.data(), 0, shape).expect("decode")));
+    }
+}
+
+DEVICE_TEST(test_block_norm) {
+    const size_t n = 3, dim = 100;
+    Rng rng(8);
+    const auto x = rng.normal(n * dim), y = rng.normal(n * dim), post = rng.normal(dim), gate = rng.normal(n * dim), pre = rng.normal(dim);
+    BlockNorm norm{post.data(), gate.data(), true, pre.data(), 1e-5f, 0.5f};
+    const auto got = backend().block_norm(x.data(), y.data(), n, dim, norm).expect("norm");
+    for (size_t r = 0; r < n; r++) {
+        double sy = 0.0, sx = 0.0;
+        std::vector<double> s(dim);
+        for (size_t i = 0; i < dim; i++) sy += (double)y[r * dim + i] * y[r * dim + i];
+        for (size_t i = 0; i < dim; i++) {
+            s[i] = x[r * dim + i] + 0.5 * gate[r * dim + i] * y[r * dim + i] / std::sqrt(sy / dim + 1e-5) * post[i];
+            sx += s[i] * s[i];
+        }
+        for (size_t i = 0; i < dim; i++) {
+            CHECK(std::fabs(got.x[r * dim + i] - s[i]) <= 1e-5);
+            CHECK(std::fabs(got.normed[r * dim + i] - s[i] / std::sqrt(sx / dim + 1e-5) * pre[i]) <= 1e-5);
+        }
+    }
+    norm = BlockNorm{};
+    const auto sum = backend().block_norm(x.data(), y.data(), n, dim, norm).expect("sum");
+    CHECK(sum.normed.empty());
+    for (size_t i = 0; i < n * dim; i++) CHECK(sum.x[i] == x[i] + y[i]);
+    CHECK(!backend().block_norm(x.data(), nullptr, 1, 0, norm).ok());
+    CHECK(!backend().block_norm(x.data(), nullptr, 1, GLA_BLOCK_NORM_MAX_DIM + 1, norm).ok());
+    norm.gate = gate.data();
+    CHECK(!backend().block_norm(x.data(), nullptr, 1, dim, norm).ok());
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
