@@ -191,6 +191,15 @@ __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// Item `at` of a grid row's n, each row beginning with another than the row before.
+// Workgroups go to an XCD's four shader engines in turn: with an even number of items in one
+// order, of which only the first have work in many rows (the longest of a ragged batch, a
+// large group's row tiles), all that work falls to the same engines.
+__device__ __forceinline__ int turned(int at, int n, int row) {
+    const int turn = n % 2 ? 0 : (n % 4 ? row >> 1 : row);
+    return (int)((uint32_t)(at + turn) % (uint32_t)n);
+}
+
 __device__ __forceinline__ int64_t map_page(const PageMap &pm, int b, int lp) {
     int64_t id;
     if (pm.page_table) {

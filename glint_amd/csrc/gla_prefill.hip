@@ -1470,11 +1470,19 @@ __global__ __launch_bounds__(NW * 64, (NW == 8 ? 2 : kSplitOccupancy<D, STAGED, 
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
 
     const int n_hgrp = p.group / p.hpw;
-    const int pair = (int)blockIdx.x / n_hgrp;
+    const int blk = blockIdx.z * gridDim.y + blockIdx.y;
+    int unit = blockIdx.x;
+    if constexpr (kSinks) {
+        // Prompts of 2,048, 541, 760 and 301 rows in a window of 512 + 4 at 32/8 heads, d = 128,
+        // Q8_0, sequences in one order / turned 211 / 130 us, 4 of 2,048 254 / 253.
+        const int per = p.n_kv_heads * n_hgrp, at = unit / per;
+        unit += (turned(at, gridDim.x / per, blk) - at) * per;
+    }
+    const int pair = unit / n_hgrp;
     const int b = pair / p.n_kv_heads;
     const int kvh = pair - b * p.n_kv_heads;
-    const int hgrp = (int)blockIdx.x - pair * n_hgrp;
-    const int qblk = p.n_qblocks - 1 - (int)(blockIdx.z * gridDim.y + blockIdx.y);
+    const int hgrp = unit - pair * n_hgrp;
+    const int qblk = p.n_qblocks - 1 - blk;
     const int waves_per_head = NW / p.hpw;
     const int qwg = QW * waves_per_head;
 
