@@ -841,9 +841,15 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
     };
     // the fewest pages (a wave's: an even number, at most 64) that leave at most `most` workgroups
     const auto pages_for = [&](int64_t most) {
-        int n = 8;
-        while (n < 256 && wgs(n) > most) n += 8;
-        return n;
+        int lo = 1, hi = 32;  // (eights; more pages never make more workgroups)
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (wgs(8 * mid) > most)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        return 8 * lo;
     };
     // A workgroup for every unit. With Q8_0, whose waves wait for their own vector and matrix
     // instructions in turn, two, where a split keeps 32 pages; with several groups of f32, whose
