@@ -26,6 +26,7 @@
 #include <algorithm>
 
 #include "gla_internal.h"
+#include "gla_prefix.h"
 
 namespace gla {
 
@@ -269,8 +270,9 @@ __device__ __forceinline__ void merge_splits_agent(const DecodeParams &p, int64_
     }
 }
 
+// One workgroup item: a split of sequence b, KV head x head group hx.
 template <int D, int GT, int NSTEP, bool CAP, DecodeMode MODE>
-__global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodeParams p) {
+__device__ __forceinline__ void split_item(const DecodeParams &p, int hx, int split, int b) {
     constexpr int EPL = D / 8;       // elements per lane
     constexpr int EPC = 4;           // floats per 16-byte chunk
     constexpr int NCH = EPL / EPC;   // chunks per lane
@@ -280,14 +282,8 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
     __shared__ float lds_m[kWaves][GT];
     __shared__ float lds_l[kWaves][GT];
 
-    // grid (KV head x head group, split, sequence): head index fastest, so
-    // the head spans of the same pages are read together
-    // (24 rows of 1-1,000 positions behind two prefixes of up to 4,096 at 16/8 heads, d = 256 78.4 -> 75.7 us,
-    // with the prefixes' row tiles; windows with sinks are as fast either way)
-    const int split = MODE == kBehindPrefix ? turned(blockIdx.y, gridDim.y, blockIdx.z) : (int)blockIdx.y;
-    const int b = blockIdx.z;
-    const int kvh = blockIdx.x / p.n_hg;
-    const int hg = blockIdx.x - kvh * p.n_hg;
+    const int kvh = hx / p.n_hg;
+    const int hg = hx - kvh * p.n_hg;
     const int g0 = hg * GT;
     const int gcount = min(GT, p.group - g0);
     const int h_base = kvh * p.group + g0;
@@ -538,6 +534,28 @@ __global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodePara
     merge_splits_agent<D, GT>(p, unit * p.max_splits, r.n_splits, gcount, p.out + ((int64_t)b * p.n_heads + h_base) * D);
 }
 
+// Grid (KV head x head group, split, sequence): head index fastest, so the head
+// spans of the same pages are read together.
+template <int D, int GT, int NSTEP, bool CAP, DecodeMode MODE>
+__global__ __launch_bounds__(kThreads) void decode_split_kernel(const DecodeParams p) {
+    split_item<D, GT, NSTEP, CAP, MODE>(p, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+// decode_split_kernel behind prefixes, with their workgroups before its own.
+template <int D, int GT, int NT, bool CAP>
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void decode_prefix_kernel(
+    const DecodeParams p, const prefix::PrefixParams pp, const prefix::Mixed mix) {
+    __shared__ __attribute__((aligned(16))) float lds[prefix::kLdsFloats<D, NT>];
+    prefix::Place w;
+    if (mix.place(w)) {
+        if (w.z >= 0) prefix::f32_item<D, NT, CAP>(pp, w, lds);
+    } else if (w.z >= 0) {
+        // (24 rows of 1-1,000 positions behind two prefixes of up to 4,096 at 16/8 heads, d = 256 78.4 -> 75.7 us,
+        // with the prefixes' row tiles; windows with sinks are as fast either way)
+        split_item<D, GT, kStepsPerIter, CAP, kBehindPrefix>(p, w.x, turned(w.y, mix.oy, w.z), w.z);
+    }
+}
+
 // Log-sum-exp merge of the split partials of one (sequence, kv head, head
 // group, q-head g = blockIdx.x). A row of D floats is read by D/4 lanes as
 // float4; the 256 threads form 256/(D/4) split groups that take every
@@ -663,9 +681,34 @@ int launch_as(gla_ctx *ctx, const DecodeParams &prm, dim3 grid, bool combine) {
     return GLA_OK;
 }
 
+template <int D, int GT, int NT>
+int launch_mixed(gla_ctx *ctx, const DecodeLaunch &d, const DecodeParams &prm, const prefix::PrefixParams &pp, dim3 grid) {
+    prefix::Mixed mix;
+    if (int rc = mix_prefix(d, pp, grid, &mix)) return rc;
+    if (pp.softcap > 0.0f)
+        hipLaunchKernelGGL((decode_prefix_kernel<D, GT, NT, true>), mix.grid(), dim3(kThreads), 0, ctx->stream, prm, pp, mix);
+    else
+        hipLaunchKernelGGL((decode_prefix_kernel<D, GT, NT, false>), mix.grid(), dim3(kThreads), 0, ctx->stream, prm, pp, mix);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "decode_prefix_kernel launch: %s", hipGetErrorString(e));
+    hipLaunchKernelGGL((decode_combine_kernel<D, GT, kBehindPrefix>), dim3(GT, grid.x, grid.z), dim3(kThreads), 0,
+                       ctx->stream, prm);
+    e = hipGetLastError();
+    if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "decode_combine_kernel launch: %s", hipGetErrorString(e));
+    return GLA_OK;
+}
+
 template <int D, int GT>
-int launch_typed(gla_ctx *ctx, const DecodeParams &prm, dim3 grid, bool combine) {
-    if (prm.pre.n_groups > 0) return launch_as<D, GT, kBehindPrefix>(ctx, prm, grid, true);
+int launch_typed(gla_ctx *ctx, const DecodeLaunch &d, const DecodeParams &prm, const prefix::PrefixParams &pp, dim3 grid,
+                 bool combine) {
+    if (prm.pre.n_groups > 0) {
+        if constexpr (D == 256 ? GT == 1 : GT <= 4) {
+            if constexpr (D < 256)
+                if (prefix_tiles(d) == 2) return launch_mixed<D, GT, 2>(ctx, d, prm, pp, grid);
+            return launch_mixed<D, GT, 1>(ctx, d, prm, pp, grid);
+        }
+        return set_error(GLA_ERR_INVALID, "no decode kernel behind a prefix for head_dim %d and head group %d", D, GT);
+    }
     if (prm.n_sinks > 0) return launch_as<D, GT, kWindowSinks>(ctx, prm, grid, combine);
     return launch_as<D, GT, kWindow>(ctx, prm, grid, combine);
 }
@@ -681,20 +724,21 @@ int pick_gt(int d, int group) {
 }
 
 template <int D>
-int launch_d(gla_ctx *ctx, int gt, const DecodeParams &prm, dim3 grid, bool combine) {
+int launch_d(gla_ctx *ctx, int gt, const DecodeLaunch &d, const DecodeParams &prm, const prefix::PrefixParams &pp, dim3 grid,
+             bool combine) {
     switch (gt) {
     case 1:
-        return launch_typed<D, 1>(ctx, prm, grid, combine);
+        return launch_typed<D, 1>(ctx, d, prm, pp, grid, combine);
     case 2:
-        return launch_typed<D, 2>(ctx, prm, grid, combine);
+        return launch_typed<D, 2>(ctx, d, prm, pp, grid, combine);
     case 3:
-        if constexpr (D <= 128) return launch_typed<D, 3>(ctx, prm, grid, combine);
+        if constexpr (D <= 128) return launch_typed<D, 3>(ctx, d, prm, pp, grid, combine);
         break;
     case 4:
-        if constexpr (D <= 128) return launch_typed<D, 4>(ctx, prm, grid, combine);
+        if constexpr (D <= 128) return launch_typed<D, 4>(ctx, d, prm, pp, grid, combine);
         break;
     case 8:
-        if constexpr (D <= 64) return launch_typed<D, 8>(ctx, prm, grid, combine);
+        if constexpr (D <= 64) return launch_typed<D, 8>(ctx, d, prm, pp, grid, combine);
         break;
     }
     return set_error(GLA_ERR_INVALID, "no decode kernel for head_dim %d and head group %d", D, gt);
@@ -706,7 +750,9 @@ int launch_decode(gla_ctx *ctx, const DecodeLaunch &d) {
     if (d.q8) return launch_decode_q8(ctx, d);
     const int D = d.head_dim;
     const int group = d.n_heads / d.n_kv_heads;
-    const int gt = pick_gt(D, group);
+    // (behind a prefix at most four heads, at head_dim 256 one: the kernel for both kinds of workgroups
+    // spills with more; 16 rows of 8-64 behind 4,096 at 16/8 heads, d = 256 33.6 us with two, 29.6 with one)
+    const int gt = pick_gt(D, decode_mode(d) == kBehindPrefix ? std::min(group, D == 256 ? 1 : 4) : group);
     const int n_hg = (group + gt - 1) / gt;
 
     // pages a window can span (a start inside a page adds one), and its sinks'
@@ -722,6 +768,7 @@ int launch_decode(gla_ctx *ctx, const DecodeLaunch &d) {
     const int max_splits = pps_fixed > 0 ? (max_pages + pps_fixed - 1) / pps_fixed : max_splits_upto(max_pages);
 
     DecodeParams prm;
+    prefix::PrefixParams pp;
     prm.kv = d.kv;
     prm.pm = d.pm;
     prm.kv_start = d.kv_start;
@@ -784,19 +831,16 @@ int launch_decode(gla_ctx *ctx, const DecodeLaunch &d) {
         if (rc != GLA_OK) return rc;
         prm.part_acc = (float *)scr;
         prm.part_ml = (float *)((uint8_t *)scr + acc_b);
-        if (behind) {
-            rc = launch_prefix(ctx, d, (uint8_t *)scr + acc_b + ml_b, &prm.pre);
-            if (rc != GLA_OK) return rc;
-        }
+        if (behind) prefix_params(d, (uint8_t *)scr + acc_b + ml_b, &prm.pre, &pp);
     }
     dim3 grid(d.n_kv_heads * n_hg, max_splits, d.n_seqs);
     switch (D) {
     case 64:
-        return launch_d<64>(ctx, gt, prm, grid, any_long);
+        return launch_d<64>(ctx, gt, d, prm, pp, grid, any_long);
     case 128:
-        return launch_d<128>(ctx, gt, prm, grid, any_long);
+        return launch_d<128>(ctx, gt, d, prm, pp, grid, any_long);
     case 256:
-        return launch_d<256>(ctx, gt, prm, grid, any_long);
+        return launch_d<256>(ctx, gt, d, prm, pp, grid, any_long);
     }
     return set_error(GLA_ERR_INVALID, "unsupported head_dim %d", D);
 }

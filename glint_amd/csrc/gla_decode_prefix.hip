@@ -1,821 +1,30 @@
-// gla_decode_prefix.hip -- the part of a batch's decode that groups of its sequences have
-// in common (gfx950, matrix cores): the pages of a group's prefix, multiplied with the
-// queries of all its rows at once.
-//
-// Math, of group g, KV head h and the 16 NT rows (sequence, query head of h) of a row
-// tile, over a split of the prefix's pages:
-//   S^T[key][row] = K . Q^T       s = cap(scale S) log2(e), -inf where a row does not see the key
-//   m = max s, l = sum 2^(s - m), O^T[d][row] = V^T . P^T with P = 2^(s - m)
-// (m, l, O) go to scratch, where the decode's combine kernel merges them with what the
-// row has of its own.
-//
-// Work: a wave takes a quarter of the split's pages by itself, operands straight from
-// global memory into registers (the layouts of both storages are, or allow, the operand
-// order), the next page's in flight while one is multiplied; the waves meet only to merge
-// their (m, l, O) in LDS. Both products keep a row in a column of the tile: a lane's
-// scores are the operand of the second product as they are, and a row's maximum is its
-// four lanes'.
-//
-// What bounds it, the kernel alone: Q8_0 vector issue (65% of the cycles, matrix 21%, in
-// turn): 64 rows at 32/8 heads, d = 128, behind 8,192 positions 39 us, 220 TFLOP/s of the
-// attention's products; f32 the matrix rate from some 48 rows a group on (the same call 91 us,
-// 94 of the 138 TFLOP/s that a library product reaches), HBM and the tiles' re-reads before (24
-// rows in 3 groups behind up to 4,096 positions at 16/8, d = 256 37 us, 180 MB, 4.8 TB/s).
-#include <math.h>
+// gla_decode_prefix.hip -- when and in how many splits a batch's shared prefixes are read
+// apart (host code; the kernels' part is gla_prefix.h).
 #include <stdlib.h>
 
 #include <algorithm>
 
-#include "gla_internal.h"
-#include "gla_lanes.h"
+#include "gla_prefix.h"
 
 namespace gla {
 
-namespace {
-
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef float float2v __attribute__((ext_vector_type(2)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * 64;
-
-struct PrefixParams {
-    KvLayout kv;
-    PageMap pm;
-    PrefixLaunch pre;
-    const float *q;
-    const int32_t *kv_start, *kv_len;  // of the batch's rows
-    int max_kv_len;
-    int n_seqs;
-    int n_heads;
-    int n_kv_heads;
-    int group;
-    float q_mul;    // scale (soft-cap) or scale * log2(e)
-    float softcap;  // > 0: cap * tanh(s / cap)
-};
-
-// x, for a rare block of code to start from: the block stays a branch, where the compiler
-// would compute what is in it every time and select.
-template <typename T>
-__device__ __forceinline__ T rare(T x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
-
-// The reference m of a row's exponents moves only when a score passes it by more than
-// kLazy: p is then at most 2^kLazy, and most pages rescale nothing.
-constexpr float kLazy = 8.0f;
-// Moves m to the maximum of the row's four lanes where that passes it; what the sums are to be multiplied by.
-__device__ __forceinline__ float moved(float &m, float mine) {
-    const float top = max_rows4(mine);
-    const bool up = top > m + kLazy;
-    const float f = up ? fast_exp2(m - top) : 1.0f;
-    m = up ? top : m;
-    return f;
-}
-
-// What a workgroup does, and its wave's share of it.
-struct Share {
-    int kvh;
-    int member;     // the group's first row, whose pages are read
-    int row0, rows; // the tile's first row and the group's number of rows, (sequence, query head) pairs
-    int pg0, npg;   // the wave's pages of the prefix
-    bool any;       // the workgroup has something to do
-};
-// `even`: a wave's pages are taken two at a time.
-template <bool EVEN>
-__device__ __forceinline__ Share share_of(const PrefixParams &p, int tile_rows, int wave) {
-    Share s;
-    const int g = blockIdx.z;
-    // (64 rows in two groups behind up to 8,192 Q8_0 positions at 32/8 heads, d = 128, row tiles in one order / turned 76 / 63 us)
-    const int at = blockIdx.x / p.n_kv_heads;  // (the heads run fastest: a head's row tiles share an L2)
-    s.kvh = blockIdx.x - at * p.n_kv_heads;
-    const int blk = turned(at, gridDim.x / p.n_kv_heads, blockIdx.y);
-    const int pages = prefix_positions(p.pre.prefix_len[g], p.pre.max_prefix) >> 4;
-    s.member = min(max(p.pre.group_start[g], 0), p.n_seqs);
-    const int members = min(max(min(p.pre.group_start[g + 1], p.n_seqs) - s.member, 0), p.pre.max_group);
-    s.rows = members * p.group;
-    s.row0 = blk * tile_rows;
-    const int wg0 = blockIdx.y * p.pre.split_pages;
-    s.any = s.row0 < s.rows && wg0 < pages;
-    const int n = min(p.pre.split_pages, pages - wg0);
-    int each = (n + kWaves - 1) / kWaves;
-    if (EVEN) each = (each + 1) & ~1;
-    s.pg0 = wg0 + wave * each;
-    s.npg = max(min(each, n - wave * each), 0);
-    return s;
-}
-
-// A lane's row of a tile: the positions it sees and where its query is.
-struct Row {
-    int lo, hi;  // sees lo <= position < hi
-    bool ok;
-    int at;  // sequence * n_heads + head (the group's first row, for a row past the group's)
-};
-__device__ __forceinline__ Row row_of(const PrefixParams &p, const Share &s, int r) {
-    Row x;
-    x.ok = r < s.rows;
-    x.lo = x.hi = 0;
-    const int i = x.ok ? r / p.group : 0, b = s.member + i;
-    x.at = b * p.n_heads + s.kvh * p.group + (x.ok ? r - i * p.group : 0);
-    if (x.ok) {
-        const Visible v = visible_of(p.kv_start[b], p.kv_len[b], p.max_kv_len, p.pm.pos_limit, 0);
-        x.lo = v.start;
-        x.hi = v.n_pages ? v.end : 0;
-    }
-    return x;
-}
-
-// Positions that some row of a wave's tile sees, [wlo, whi), and that all do, [ilo, ihi).
-struct Seen {
-    int wlo, whi, ilo, ihi;
-    __device__ __forceinline__ bool none(int first, int n) const { return first >= whi || first + n <= wlo; }
-    __device__ __forceinline__ bool all(int first, int n) const { return first >= ilo && first + n <= ihi; }
-};
-template <int NT>
-__device__ __forceinline__ Seen seen_of(const Row (&rows)[NT]) {
-    constexpr int kMost = 0x7fffffff;
-    int wlo = kMost, whi = 0, ilo = 0, ihi = kMost;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const Row &r = rows[nt];
-        whi = max(whi, (int)wave_extreme<true>((uint32_t)r.hi));
-        wlo = min(wlo, (int)wave_extreme<false>((uint32_t)(r.hi > 0 ? r.lo : kMost)));
-        ihi = min(ihi, (int)wave_extreme<false>((uint32_t)(r.ok ? r.hi : kMost)));
-        ilo = max(ilo, (int)wave_extreme<true>((uint32_t)r.lo));
-    }
-    return {__builtin_amdgcn_readfirstlane(wlo), __builtin_amdgcn_readfirstlane(whi),
-            __builtin_amdgcn_readfirstlane(ilo), __builtin_amdgcn_readfirstlane(ihi)};
-}
-
-// Physical pages of up to 64 pages from logical page pg0 on, one a lane.
-__device__ __forceinline__ int page_ids(const PrefixParams &p, int b, int pg0, int npg) {
-    return (int)map_page(p.pm, b, pg0 + min((int)(threadIdx.x & 63), npg - 1));
-}
-
-// The waves' (m, l) and O, merged and written. A wave's O is in its slot of `slots`
-// ([16 NT][D + 4] floats each), scaled to the workgroup's maximum.
-constexpr int out_row(int D) { return D + 4; }
-template <int D, int NT>
-constexpr int kMergeFloats = kWaves * 16 * NT * out_row(D);
-
-// m of the workgroup for this lane's rows; `put` stores the wave's O, times f[nt], in its slot.
-template <int D, int NT, typename Put>
-__device__ __forceinline__ void merge_and_store(const PrefixParams &p, const Share &s, float (&m)[NT], float (&l)[NT],
-                                                float *slots, float (*mls)[2][16 * NT], const int *at, Put put) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int lrow = lane & 15;
-    if (lane < 16) {
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            mls[wave][0][nt * 16 + lrow] = m[nt];
-            mls[wave][1][nt * 16 + lrow] = l[nt];
-        }
-    }
-    __syncthreads();  // (and every wave is done with the queries, whose place `slots` takes)
-    float f[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        float top = mls[0][0][nt * 16 + lrow];
-#pragma unroll
-        for (int w = 1; w < kWaves; w++) top = fmaxf(top, mls[w][0][nt * 16 + lrow]);
-        // (a wave whose scores were all NaN has m = -inf and NaN sums, which stay NaN)
-        f[nt] = m[nt] == -INFINITY ? 0.0f : fast_exp2(m[nt] - top);
-    }
-    put(slots + wave * 16 * NT * out_row(D), f);
-    __syncthreads();
-    const int64_t first = (int64_t)blockIdx.y * p.n_seqs * p.n_heads;
-    for (int i = threadIdx.x; i < 16 * NT * (D / 4); i += kThreads) {
-        const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
-        if (s.row0 + r >= s.rows) break;
-        floatx4 v = *reinterpret_cast<const floatx4 *>(slots + r * out_row(D) + c);
-#pragma unroll
-        for (int w = 1; w < kWaves; w++)
-            v += *reinterpret_cast<const floatx4 *>(slots + (w * 16 * NT + r) * out_row(D) + c);
-        *reinterpret_cast<floatx4 *>(p.pre.acc + (first + at[r]) * D + c) = v;
-    }
-    const int r = threadIdx.x;
-    if (r < 16 * NT && s.row0 + r < s.rows) {
-        float top = mls[0][0][r], sum = 0.0f;
-#pragma unroll
-        for (int w = 1; w < kWaves; w++) top = fmaxf(top, mls[w][0][r]);
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float mw = mls[w][0][r];
-            sum = fmaf(mls[w][1][r], mw == -INFINITY ? 0.0f : fast_exp2(mw - top), sum);
-        }
-        reinterpret_cast<float2 *>(p.pre.ml)[first + at[r]] = make_float2(top, sum);
-    }
-}
-
-// ---------------------------------------------------------------------------
-// f32 storage, on v_mfma_f32_16x16x4_f32: every product and sum is an f32's, so nothing
-// is scaled or split. Sums of four products run over the dims kk*16 + kg*4 + j, of lane
-// group kg and step j, which makes K and Q four floats of a row a lane, and the d tiles
-// of O the dims T*64 + m*4 + c, which makes V so.
-template <int D, int NT, bool CAP>
-__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefix_f32_kernel(const PrefixParams p) {
-    constexpr int KK = D / 16, DT = D / 64;
-    constexpr int QFLOATS = NT * KK * 256;
-    __shared__ __attribute__((aligned(16))) float lds[std::max(QFLOATS, kMergeFloats<D, NT>)];
-    __shared__ float mls[kWaves][2][16 * NT];
-    __shared__ int row_at[16 * NT];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lrow = lane & 15, kg = lane >> 4;
-    const Share sh = share_of<false>(p, 16 * NT, wave);
-    if (!sh.any) return;
-
-    floatx4 k[KK], v[4][DT];
-    const uint32_t koff = (uint32_t)(lrow * p.kv.row_stride + kg * 16);
-    const uint32_t voff = (uint32_t)(kg * 4 * p.kv.row_stride + lrow * 16);
-    const int64_t head = (int64_t)sh.kvh * p.kv.head_stride;
-    const auto load_k = [&](int64_t page) __attribute__((always_inline)) {
-        const uint8_t *at = p.kv.k + page * p.kv.page_stride + head;
-#pragma unroll
-        for (int kk = 0; kk < KK; kk++) k[kk] = *reinterpret_cast<const floatx4 *>(at + koff + kk * 64);
-    };
-    const auto load_v = [&](int64_t page) __attribute__((always_inline)) {
-        const uint8_t *at = p.kv.v + page * p.kv.page_stride + head;
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int T = 0; T < DT; T++)
-                v[r][T] = *reinterpret_cast<const floatx4 *>(at + voff + r * p.kv.row_stride + T * 256);
-    };
-    // (the first page is on its way while the queries are; a wave without pages reads the group's first)
-    const int n = sh.npg;
-    const int ids = page_ids(p, sh.member, n > 0 ? sh.pg0 : 0, max(n, 1));
-    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(n, 1) - 1)); };
-    load_k(id(0));
-    load_v(id(0));
-
-    Row rows[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        rows[nt] = row_of(p, sh, sh.row0 + nt * 16 + lrow);
-        if (threadIdx.x < 16) row_at[nt * 16 + lrow] = rows[nt].at;
-    }
-    // the queries, [nt][kk][lane] in the order in which a lane reads them: a wave takes every fourth kk
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int k4 = 0; k4 < KK / kWaves; k4++) {
-            const int kk = k4 * kWaves + wave;
-            floatx4 x = *reinterpret_cast<const floatx4 *>(p.q + (int64_t)rows[nt].at * D + kk * 16 + kg * 4) * p.q_mul;
-            if (!rows[nt].ok) x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-            reinterpret_cast<floatx4 *>(lds)[(nt * KK + kk) * 64 + lane] = x;
-        }
-    const Seen seen = seen_of<NT>(rows);
-    __syncthreads();
-    const floatx4 *qs = reinterpret_cast<const floatx4 *>(lds);
-
-    floatx4 o[DT][4][NT];  // O of d = T*64 + (kg*4 + r)*4 + c in [T][c][nt][r]
-    float m[NT], lpart[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        m[nt] = -INFINITY;
-        lpart[nt] = 0.0f;
-#pragma unroll
-        for (int T = 0; T < DT; T++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) o[T][c][nt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    {
-        for (int i = 0; i < n; i++) {
-            const int first = (sh.pg0 + i) * 16;
-            const bool inside = seen.all(first, 16);
-            int qi = lane;
-            asm volatile("" : "+v"(qi));  // (read anew for every page: kept, they would crowd the other registers)
-            floatx4 s[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int kk = 0; kk < KK; kk++) {
-                floatx4 q[NT];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) q[nt] = qs[qi + (nt * KK + kk) * 64];
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        s[nt][j & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[kk][j], q[nt][j], s[nt][j & 1], 0, 0, 0);
-            }
-            load_k(id(i + 1));
-            float pr[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                floatx4 x = s[nt][0] + s[nt][1];
-                if constexpr (CAP) {
-                    const SoftCap f(p.softcap);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) x[r] = f(x[r]);
-                }
-                if (!inside) {
-                    const int pos0 = rare(first + kg * 4);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int pos = pos0 + r;
-                        x[r] = pos >= rows[nt].lo && pos < rows[nt].hi ? x[r] : -INFINITY;
-                    }
-                }
-                const float mine = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                if (__ballot(mine > m[nt] + kLazy)) {
-                    const float f = moved(m[nt], mine);
-                    lpart[nt] *= f;
-#pragma unroll
-                    for (int T = 0; T < DT; T++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) o[T][c][nt] *= f;
-                }
-                const float off = m[nt] == -INFINITY ? 0.0f : m[nt];
-#pragma unroll
-                for (int r = 0; r < 4; r++) pr[nt][r] = fast_exp2(x[r] - off);
-                lpart[nt] += (pr[nt][0] + pr[nt][1]) + (pr[nt][2] + pr[nt][3]);
-            }
-            // A value that is infinite or NaN reaches only the rows that see its position (0 times
-            // it would not be 0): where some row does not, and there is one, those are left out
-            // of the product and added by themselves.
-            bool apart = false;
-            if (!inside) {
-                float z = rare(0.0f);
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int T = 0; T < DT; T++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) z = fmaf(v[r][T][c], 0.0f, z);
-                apart = __ballot(z != z) != 0;
-                if (apart) {
-                    const float inf = rare(INFINITY);
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-#pragma unroll
-                        for (int T = 0; T < DT; T++)
-#pragma unroll
-                            for (int c = 0; c < 4; c++) v[r][T][c] = fabsf(v[r][T][c]) < inf ? v[r][T][c] : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int T = 0; T < DT; T++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-                            o[T][c][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][T][c], pr[nt][r], o[T][c][nt], 0, 0, 0);
-            if (apart) {
-                const uint8_t *at = p.kv.v + id(i) * p.kv.page_stride + head + kg * 64;
-#pragma unroll 1
-                for (int k4 = 0; k4 < 4; k4++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int key = 4 * k4 + j, pos = first + key;
-                        float pk[NT];
-                        bool sees[NT];
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            pk[nt] = __shfl(pr[nt][j], k4 * 16 + lrow);
-                            sees[nt] = pos >= rows[nt].lo && pos < rows[nt].hi;
-                        }
-#pragma unroll
-                        for (int T = 0; T < DT; T++)
-#pragma unroll
-                            for (int r = 0; r < 4; r++) {
-                                const floatx4 w =
-                                    *reinterpret_cast<const floatx4 *>(at + key * p.kv.row_stride + T * 256 + r * 16);
-#pragma unroll
-                                for (int c = 0; c < 4; c++)
-#pragma unroll
-                                    for (int nt = 0; nt < NT; nt++) {
-                                        const float x = o[T][c][nt][r];
-                                        o[T][c][nt][r] = sees[nt] && !(fabsf(w[c]) < INFINITY) ? fmaf(pk[nt], w[c], x) : x;
-                                    }
-                                asm volatile("" ::: "memory");  // (one row of values at a time in registers)
-                            }
-                    }
-                }
-            }
-            load_v(id(i + 1));
-        }
-    }
-    float l[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) l[nt] = sum_rows4(lpart[nt]);
-    merge_and_store<D, NT>(p, sh, m, l, lds, mls, row_at, [&](float *slot, const float (&f)[NT]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int T = 0; T < DT; T++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const floatx4 x = {o[T][0][nt][r], o[T][1][nt][r], o[T][2][nt][r], o[T][3][nt][r]};
-                    *reinterpret_cast<floatx4 *>(slot + (nt * 16 + lrow) * out_row(D) + T * 64 + kg * 16 + r * 4) = x * f[nt];
-                }
-    });
-}
-
-// ---------------------------------------------------------------------------
-// Q8_0 storage, on v_mfma_f32_16x16x32_f16, as the decode of single rows has it
-// (gla_decode_q8.hip): quants are exact in f16; queries, and probabilities times the
-// values' scales, are two f16 pieces (hi = f16(x), lo = f16(x - hi)) after a power-of-two
-// rescale that puts the largest below 2^14. A step is two pages, the depth of one product
-// with V; K's scales are applied to the scores of each block.
-
-// Four stored quants (x + 128, in byte order) -> halves at..at+3 of `o`: 0x64XX is
-// 1024 + XX in f16, so subtracting 1152 leaves x exactly.
-__device__ __forceinline__ void quants4(uint32_t u, half8 &o, int at) {
-    const half2v bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-    const half2v a = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
-    const half2v c = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
-    o[at + 0] = a[0];
-    o[at + 1] = a[1];
-    o[at + 2] = c[0];
-    o[at + 3] = c[1];
-}
-__device__ __forceinline__ uint32_t word(const uint4 &v, int i) {
-    return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w));
-}
-template <int N>
-__device__ __forceinline__ float half_at(const uint32_t (&a)[N], int i) {
-    const uint32_t w = a[i >> 1];
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)((i & 1) ? (w >> 16) : (w & 0xffff)));
-}
-// e with x = m * 2^e, m in [0.5, 1); scaling by 2^(14 - e) maps max|.| below 2^14.
-__device__ __forceinline__ int pow2_exp(float x) {
-    int e = 0;
-    (void)frexpf(x, &e);
-    return e < -100 ? -100 : (e > 100 ? 100 : e);
-}
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t *src, uint32_t (&dst)[N]) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; i++) {
-            const uint4 w = reinterpret_cast<const uint4 *>(src)[i];
-            dst[4 * i] = w.x;
-            dst[4 * i + 1] = w.y;
-            dst[4 * i + 2] = w.z;
-            dst[4 * i + 3] = w.w;
-        }
-    } else {
-        static_assert(N == 2, "8 bytes");
-        const uint2 w = *reinterpret_cast<const uint2 *>(src);
-        dst[0] = w.x;
-        dst[1] = w.y;
-    }
-}
-
-// The f16 pieces of p[j] * scale[j], hi = f16(p * scale) and lo = f16(p * scale - hi), of the
-// f16 scales in the words' high (HIGH) or low halves: 16 mixed multiply-adds, which the
-// compiler writes as products and conversions (24 instructions, and a copy of every word
-// where two tiles use it). The s_nops are wait states that it would count itself: for p,
-// which v_exp_f32 may just have written, for halves written and read, and for the products.
-template <bool HIGH>
-__device__ __forceinline__ void pieces8(const float (&p)[8], const uint32_t (&w)[8], half8 &hi, half8 &lo) {
-    uint32_t h0, h1, h2, h3, l0, l1, l2, l3;
-#define GLA_PIECES(S)                                                                 \
-    asm("s_nop 1\n\t"                                                                \
-        "v_fma_mixlo_f16 %0, %8, %16, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"     \
-        "v_fma_mixlo_f16 %1, %10, %18, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixlo_f16 %2, %12, %20, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixlo_f16 %3, %14, %22, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixhi_f16 %0, %9, %17, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"     \
-        "v_fma_mixhi_f16 %1, %11, %19, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixhi_f16 %2, %13, %21, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixhi_f16 %3, %15, %23, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "s_nop 1\n\t"                                                                \
-        "v_fma_mixlo_f16 %4, %8, %16, -%0 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"   \
-        "v_fma_mixlo_f16 %5, %10, %18, -%1 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixlo_f16 %6, %12, %20, -%2 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixlo_f16 %7, %14, %22, -%3 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixhi_f16 %4, %9, %17, -%0 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"   \
-        "v_fma_mixhi_f16 %5, %11, %19, -%1 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixhi_f16 %6, %13, %21, -%2 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixhi_f16 %7, %15, %23, -%3 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"  \
-        "s_nop 1"                                                                     \
-        : "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3), "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3) \
-        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), \
-          "v"(w[0]), "v"(w[1]), "v"(w[2]), "v"(w[3]), "v"(w[4]), "v"(w[5]), "v"(w[6]), "v"(w[7]))
-    if constexpr (HIGH)
-        GLA_PIECES("1");
-    else
-        GLA_PIECES("0");
-#undef GLA_PIECES
-    hi = __builtin_bit_cast(half8, make_uint4(h0, h1, h2, h3));
-    lo = __builtin_bit_cast(half8, make_uint4(l0, l1, l2, l3));
-}
-
-template <int D, int NT, bool CAP>
-__global__ __launch_bounds__(kThreads, D == 64 ? 3 : (D == 128 ? 2 : 1)) void prefix_q8_kernel(const PrefixParams p) {
-    constexpr int NB = D / 32, NQ = D / 64, ND = D / 16;
-    constexpr int QBYTES = NT * NB * 2 * 1024;
-    __shared__ __attribute__((aligned(16))) float lds[std::max(QBYTES / 4, kMergeFloats<D, NT>)];
-    __shared__ float mls[kWaves][2][16 * NT];
-    __shared__ int row_at[16 * NT];
-    __shared__ int qexp[16 * NT];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lrow = lane & 15, kg = lane >> 4;
-    const Share sh = share_of<true>(p, 16 * NT, wave);
-    if (!sh.any) return;
-
-    const uint8_t *base = p.kv.k + (int64_t)sh.kvh * p.kv.head_stride;
-    uint4 k[2][NQ], v[2][NQ];
-    uint32_t ks[2][2][NB], vs[2][2 * NB];  // 4 positions x the blocks of a parity; x all blocks
-    const uint32_t off = lane * 16, ksoff = (uint32_t)(32 * D + kg * 4 * NB), vsoff = (uint32_t)(33 * D + kg * 8 * NB);
-    const auto load_k = [&](int P, int64_t page) __attribute__((always_inline)) {
-        const uint8_t *at = base + page * p.kv.page_stride;
-#pragma unroll
-        for (int c = 0; c < NQ; c++) k[P][c] = *reinterpret_cast<const uint4 *>(at + off + c * 1024);
-        load_words(at + ksoff, ks[P][0]);
-        load_words(at + ksoff + 16 * NB, ks[P][1]);
-    };
-    const auto load_v = [&](int P, int64_t page) __attribute__((always_inline)) {
-        const uint8_t *at = base + page * p.kv.page_stride;
-#pragma unroll
-        for (int c = 0; c < NQ; c++) v[P][c] = *reinterpret_cast<const uint4 *>(at + 16 * D + off + c * 1024);
-        load_words(at + vsoff, vs[P]);
-    };
-    // (the first pages are on their way while the queries are split; a wave without pages reads the group's first)
-    const int n = sh.npg;
-    const int ids = page_ids(p, sh.member, n > 0 ? sh.pg0 : 0, max(n, 1));
-    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(n, 1) - 1)); };
-    load_k(0, id(0));
-    load_k(1, id(1));
-    load_v(0, id(0));
-    load_v(1, id(1));
-
-    Row rows[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        rows[nt] = row_of(p, sh, sh.row0 + nt * 16 + lrow);
-        if (threadIdx.x < 16) row_at[nt * 16 + lrow] = rows[nt].at;
-    }
-    // the queries' pieces, [nt][block][piece][lane]: wave w takes the tiles nt = w, w + 4, ...
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        if (nt % kWaves != wave) continue;
-        const float *qp = p.q + (int64_t)rows[nt].at * D + kg * 8;
-        float x[NB][8], top = 0.0f;
-#pragma unroll
-        for (int blk = 0; blk < NB; blk++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const floatx4 w = *reinterpret_cast<const floatx4 *>(qp + blk * 32 + h * 4) * p.q_mul;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[blk][4 * h + e] = w[e];
-                    top = fmaxf(top, fabsf(w[e]));
-                }
-            }
-        // an infinite entry's second piece is 0 and its score infinite; the scale is the finite entries'
-        const bool infinite = __ballot(top == INFINITY) != 0;
-        if (infinite) {
-            top = rare(0.0f);
-#pragma unroll
-            for (int blk = 0; blk < NB; blk++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float a = fabsf(x[blk][j]);
-                    top = a < INFINITY ? fmaxf(top, a) : top;
-                }
-        }
-        top = max_rows4(top);
-        const int e = pow2_exp(top);
-        const float mul = rows[nt].ok ? ldexpf(1.0f, 14 - e) : 0.0f;
-        if (kg == 0) qexp[nt * 16 + lrow] = e;
-#pragma unroll
-        for (int blk = 0; blk < NB; blk++) {
-            half8 hi, lo;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float y = x[blk][j] * mul;
-                hi[j] = (_Float16)y;
-                lo[j] = (_Float16)(y - (float)hi[j]);
-            }
-            if (infinite) {
-                const float inf = rare(INFINITY);
-#pragma unroll
-                for (int j = 0; j < 8; j++) lo[j] = fabsf(x[blk][j]) == inf ? (_Float16)0.0f : lo[j];
-            }
-            half8 *to = reinterpret_cast<half8 *>(lds) + (nt * NB + blk) * 2 * 64 + lane;
-            to[0] = hi;
-            to[64] = lo;
-        }
-    }
-    const Seen seen = seen_of<NT>(rows);
-    __syncthreads();
-    const half8 *qs = reinterpret_cast<const half8 *>(lds);
-    float sm[NT];  // undoes a query's scale
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) sm[nt] = ldexpf(1.0f, qexp[nt * 16 + lrow] - 14);
-
-    floatx4 o[ND][NT];  // O of d = t*16 + kg*4 + r
-    float m[NT], lpart[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        m[nt] = -INFINITY;
-        lpart[nt] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < ND; t++) o[t][nt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    float unit = 1.0f;  // of O and of the sums of P
-    if (n > 0) {
-        // P' = p * vscale * 2^vexp is below 2^14 (p at most 2^kLazy)
-        float vmax = 0.0f;
-        const int units = n * (D / 16);  // 16 bytes of V scales each
-        for (int u0 = 0; u0 < units; u0 += 64) {
-            const int u = min(u0 + lane, units - 1);
-            const int64_t page = __shfl(ids, u / (D / 16));
-            uint32_t w[4];
-            load_words(base + page * p.kv.page_stride + 33 * D + u % (D / 16) * 16, w);
-#pragma unroll
-            for (int i = 0; i < 8; i++) vmax = fmaxf(vmax, fabsf(half_at(w, i)));
-        }
-        vmax = wave_max(vmax);
-        const bool vinf = __ballot(vmax == INFINITY) != 0;
-        const int ve = __builtin_amdgcn_readfirstlane(vinf ? 0 : pow2_exp(vmax));
-        constexpr int kTop = 14 - (int)kLazy;
-        const float vexp = (float)(kTop - ve);
-        unit = ldexpf(1.0f, ve - kTop);
-
-        for (int i = 0; i < n; i += 2) {
-            const int first = (sh.pg0 + i) * 16;
-            const bool two = i + 1 < n;
-            const bool plain = two && !vinf && seen.all(first, 32);  // every row sees all, and no scale is infinite
-            int qi = lane;
-            asm volatile("" : "+v"(qi));  // (read anew for every step: kept, they would crowd the other registers)
-            floatx4 s[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int blk = 0; blk < NB; blk++) {
-                half8 a[2];
-#pragma unroll
-                for (int P = 0; P < 2; P++) {
-                    quants4(word(k[P][blk >> 1], (blk & 1) * 2), a[P], 0);
-                    quants4(word(k[P][blk >> 1], (blk & 1) * 2 + 1), a[P], 4);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const half8 qh = qs[qi + (nt * NB + blk) * 128], ql = qs[qi + (nt * NB + blk) * 128 + 64];
-                    floatx4 t[2];
-#pragma unroll
-                    for (int P = 0; P < 2; P++)
-                        t[P] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[P], qh, floatx4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                    for (int P = 0; P < 2; P++) t[P] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[P], ql, t[P], 0, 0, 0);
-#pragma unroll
-                    for (int P = 0; P < 2; P++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            s[nt][P][r] = fmaf(half_at(ks[P][blk & 1], r * (NB / 2) + (blk >> 1)), t[P][r], s[nt][P][r]);
-                }
-            }
-            load_k(0, id(i + 2));
-            load_k(1, id(i + 3));
-
-            float pr[NT][8];
-            uint32_t sees[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                floatx4 x[2] = {s[nt][0], s[nt][1]};
-                if constexpr (CAP) {
-                    x[0] *= sm[nt];
-                    x[1] *= sm[nt];
-                    const SoftCap f(p.softcap);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j >> 2][j & 3] = f(x[j >> 2][j & 3]);
-                }
-                sees[nt] = 0xff;
-                if (!plain) {
-                    const int pos0 = rare(first + kg * 4);
-                    sees[nt] = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int pos = pos0 + (j >> 2) * 16 + (j & 3);
-                        const bool ok = pos >= rows[nt].lo && pos < rows[nt].hi && (j < 4 || two);
-                        sees[nt] |= ok ? 1u << j : 0u;
-                        x[j >> 2][j & 3] = ok ? x[j >> 2][j & 3] : -INFINITY;
-                    }
-                }
-                const float c = CAP ? 1.0f : sm[nt];
-                const float mine = c * fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                                             fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-                if (__ballot(mine > m[nt] + kLazy)) {
-                    const float f = moved(m[nt], mine);
-                    lpart[nt] *= f;
-#pragma unroll
-                    for (int t = 0; t < ND; t++) o[t][nt] *= f;
-                }
-                const float off = m[nt] == -INFINITY ? 0.0f : vexp - m[nt];
-#pragma unroll
-                for (int j = 0; j < 8; j++) pr[nt][j] = fast_exp2(fmaf(x[j >> 2][j & 3], c, off));
-                lpart[nt] += ((pr[nt][0] + pr[nt][1]) + (pr[nt][2] + pr[nt][3])) +
-                             ((pr[nt][4] + pr[nt][5]) + (pr[nt][6] + pr[nt][7]));
-            }
-
-#pragma unroll
-            for (int blk = 0; blk < NB; blk++) {
-                half8 a[2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int t = 2 * blk + h;
-                    quants4(word(v[0][t >> 2], t & 3), a[h], 0);
-                    quants4(word(v[1][t >> 2], t & 3), a[h], 4);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    half8 hi, lo;
-                    uint32_t w[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) w[j] = vs[j >> 2][((j & 3) * NB + blk) >> 1];
-                    if (blk & 1)
-                        pieces8<true>(pr[nt], w, hi, lo);
-                    else
-                        pieces8<false>(pr[nt], w, hi, lo);
-                    // a scale that is infinite or NaN, at a position that the row does not see
-                    // (nothing) or sees (infinity has no second piece)
-                    if (!plain) {
-                        const uint32_t has = rare(sees[nt]);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            lo[j] = (has >> j & 1) == 0 || __builtin_isinf((float)hi[j]) ? (_Float16)0.0f : lo[j];
-                            hi[j] = has >> j & 1 ? hi[j] : (_Float16)0.0f;
-                        }
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        o[2 * blk + h][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[h], hi, o[2 * blk + h][nt], 0, 0, 0);
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        o[2 * blk + h][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[h], lo, o[2 * blk + h][nt], 0, 0, 0);
-                }
-            }
-            load_v(0, id(i + 2));
-            load_v(1, id(i + 3));
-        }
-    }
-    float l[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) l[nt] = sum_rows4(lpart[nt]) * unit;
-    merge_and_store<D, NT>(p, sh, m, l, lds, mls, row_at, [&](float *slot, const float (&f)[NT]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int t = 0; t < ND; t++)
-                *reinterpret_cast<floatx4 *>(slot + (nt * 16 + lrow) * out_row(D) + t * 16 + kg * 4) =
-                    o[t][nt] * (unit * f[nt]);
-    });
-}
-
-// Row tiles of 16 rows a wave.
-int tiles_of(const DecodeLaunch &d) {
-    return d.head_dim < 256 && (int64_t)d.pre.max_group * (d.n_heads / d.n_kv_heads) > 16 ? 2 : 1;
-}
-
-template <int D, int NT>
-int launch_as(gla_ctx *ctx, bool q8, const PrefixParams &prm, dim3 grid) {
-    const bool cap = prm.softcap > 0.0f;
-    if (q8 && cap)
-        hipLaunchKernelGGL((prefix_q8_kernel<D, NT, true>), grid, dim3(kThreads), 0, ctx->stream, prm);
-    else if (q8)
-        hipLaunchKernelGGL((prefix_q8_kernel<D, NT, false>), grid, dim3(kThreads), 0, ctx->stream, prm);
-    else if (cap)
-        hipLaunchKernelGGL((prefix_f32_kernel<D, NT, true>), grid, dim3(kThreads), 0, ctx->stream, prm);
-    else
-        hipLaunchKernelGGL((prefix_f32_kernel<D, NT, false>), grid, dim3(kThreads), 0, ctx->stream, prm);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "prefix kernel launch: %s", hipGetErrorString(e));
-    return GLA_OK;
-}
-
-}  // namespace
-
 // Whether reading the prefixes apart is the faster way, from the launch's bounds. It costs
-// two more launches than the rows by themselves; what it saves are the bytes that the rows
+// a combine and the set-up of more workgroups; what it saves are the bytes that the rows
 // would read again (from L2 mostly) and, with Q8_0, the length of a wave's chain of pages.
 // us a call, apart / row by row, in a captured step with 1-33 positions of each row's own:
-//   f32   9/3 heads, d = 64:   4 rows of 704 14.0 / 9.3, 16 of 2,048 17.7 / 14.1, 16 of 4,096 (94 MB saved) 19.0 / 20.1
-//        32/8 heads, d = 128:  2 rows of 4,096 22.9 / 19.8, 16 of 704 (87 MB) 24.0 / 30.2, 4 of 4,096 (101 MB) 23.3 / 31.0
-//        16/8 heads, d = 256:  8 rows of 704 (81 MB) 25.9 / 22.3, 4 of 2,048 (101 MB) 26.9 / 28.0, 16 of 4,096 35 / 148
-//   Q8_0  9/3 heads, d = 64:   8 rows of 2,048 18.3 / 17.1, 2 of 4,096 19.0 / 21.0
-//        32/8 heads, d = 128: 16 rows of 704 (23 MB) 19.0 / 18.1, 8 of 2,048 (31 MB) 22.0 / 26.1, 2 of 2,048 18.9 / 19.7,
-//                              2 of 4,096 23.1 / 25.4
-//        16/8 heads, d = 256:  8 rows of 704 21.9 / 20.1, 2 of 2,048 25.1 / 42.0
+//   f32   9/3 heads, d = 64:   8 rows of 2,048 (22 MB saved) 12.6 / 10.8, 8 of 4,096 (44 MB) 13.7 / 13.8, 16 of 4,096 14.8 / 20.2
+//        32/8 heads, d = 128:  8 rows of 256 (15 MB) 15.8 / 11.4, 16 of 256 (31 MB) 16.5 / 16.8, 4 of 2,048 (50 MB) 14.9 / 22.5
+//        16/8 heads, d = 256:  4 rows of 704 (35 MB) 19.1 / 14.9, 16 of 256 (63 MB) 18.9 / 17.7, 8 of 704 (81 MB) 20.1 / 22.2
+//   Q8_0  9/3 heads, d = 64:   2 rows of 256 9.9 / 8.1, of 704 10.3 / 10.8, of 4,096 14.4 / 20.9, 16 of 704 11.1 / 11.8
+//        32/8 heads, d = 128:  2 rows of 256 10.8 / 9.6, of 704 11.0 / 13.6, 16 of 256 12.8 / 12.9
+//        16/8 heads, d = 256:  2 rows of 256 13.2 / 13.6, 8 of 256 13.9 / 13.8, 2 of 704 13.4 / 19.9
 static bool pays(const DecodeLaunch &d) {
     const int64_t position = d.kv.page_stride / 16;  // bytes
     if (d.pre.max_prefix == 0) return false;
     if (const char *env = getenv("GLA_DECODE_PREFIX")) return atoi(env) != 0;  // (tuning and tests)
     const int64_t saved = (int64_t)(d.n_seqs - d.pre.n_groups) * d.pre.max_prefix * position;
-    if (!d.q8) return saved >= 84000000;
-    return saved >= 28000000 || d.pre.max_prefix >= (d.head_dim == 256 ? 1024 : 2500);
+    if (!d.q8) return saved >= (d.head_dim == 256 ? 70000000 : 30000000);
+    return d.pre.max_prefix >= (d.head_dim == 64 ? 640 : 448);
 }
 
 void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
@@ -825,7 +34,7 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
         pre->n_groups = 0;
         return;
     }
-    const int64_t tile = 16 * tiles_of(d), group = d.n_heads / d.n_kv_heads;
+    const int64_t tile = 16 * prefix_tiles(d), group = d.n_heads / d.n_kv_heads;
     const int pages = pre->max_prefix / 16;
     // workgroups of a launch with splits of n pages: as they are, or from the bounds
     const bool host = pre->group_start_host && pre->n_groups <= 256;
@@ -851,53 +60,47 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
         }
         return 8 * lo;
     };
-    // A workgroup for every unit. With Q8_0, whose waves wait for their own vector and matrix
-    // instructions in turn, two, where a split keeps 32 pages; with several groups of f32, whose
-    // unlike lengths leave units idle, two where it keeps 16. Else the waves' set-up and the
-    // combine's splits cost more than they gain. us a call, one / two a unit: behind 8,192
-    // positions 64 rows at 32/8 heads, d = 128, Q8_0 57.0 / 54.9, f32 110 / 112; 16 rows, f32
-    // 40.7 / 43.8; 4 rows, Q8_0 25.0 / 29.9; 24 rows in 3 groups behind up to 4,096 f32 positions
-    // at 16/8, d = 256 79 / 63, 64 rows in one group 78 / 85.
-    const int one = pages_for(ctx->n_cu), least = d.q8 ? 32 : 16;
-    const bool two = d.q8 || pre->n_groups > 1;
-    pre->split_pages = two ? std::max(pages_for(2 * (int64_t)ctx->n_cu), std::min(one, least)) : one;
+    // A workgroup for every unit, which leaves room on each for the rows' own: with more the waves'
+    // set-up and the combine's splits cost more than they give. Half as many more for several
+    // groups, whose unlike lengths and part-filled tiles leave units idle. us a call, 1 / 1.5 / 2 a
+    // unit: behind 8,192 positions at 32/8 heads, d = 128, 64 rows of 64-1,000 Q8_0 54.6 / 61 (2), of
+    // 8-64 f32 102 / 109 (2); in groups 96 Q8_0 rows in 3 93 / 88 / 88, 48 f32 rows in 3 133 / 95 / 94,
+    // 64 Q8_0 rows in 4 behind 2,048 32.9 / 27.6 / 29.5; at 16/8, d = 256 24 f32 rows in 3 behind up to
+    // 4,096 64.5 / 63.1 / 67.6, 40 Q8_0 rows in 2 34.8 / 39.0 / 42.0.
+    pre->split_pages = pages_for(pre->n_groups > 1 ? ctx->n_cu + ctx->n_cu / 2 : ctx->n_cu);
     pre->n_splits = (pages + pre->split_pages - 1) / pre->split_pages;
 }
 
-int launch_prefix(gla_ctx *ctx, const DecodeLaunch &d, void *scratch, PrefixLaunch *out) {
+void prefix_params(const DecodeLaunch &d, void *scratch, PrefixLaunch *out, prefix::PrefixParams *prm) {
     *out = d.pre;
     out->acc = (float *)scratch;
     out->ml = out->acc + (size_t)d.pre.n_splits * d.n_seqs * d.n_heads * d.head_dim;
-    PrefixParams prm;
-    prm.kv = d.kv;
-    prm.pm = d.pm;
-    prm.pre = *out;
-    prm.q = d.q;
-    prm.kv_start = d.kv_start;
-    prm.kv_len = d.kv_len;
-    prm.max_kv_len = d.max_kv_len;
-    prm.n_seqs = d.n_seqs;
-    prm.n_heads = d.n_heads;
-    prm.n_kv_heads = d.n_kv_heads;
-    prm.group = d.n_heads / d.n_kv_heads;
+    prm->kv = d.kv;
+    prm->pm = d.pm;
+    prm->pre = *out;
+    prm->q = d.q;
+    prm->kv_start = d.kv_start;
+    prm->kv_len = d.kv_len;
+    prm->max_kv_len = d.max_kv_len;
+    prm->n_seqs = d.n_seqs;
+    prm->n_heads = d.n_heads;
+    prm->n_kv_heads = d.n_kv_heads;
+    prm->group = d.n_heads / d.n_kv_heads;
     const bool cap = d.softcap > 0.0f;
-    prm.q_mul = cap ? d.scale : d.scale * kLog2e;
-    prm.softcap = cap ? d.softcap : 0.0f;
-    const int nt = tiles_of(d);
-    const int64_t blocks = ((int64_t)out->max_group * prm.group - 1) / (16 * nt) + 1;
-    if (blocks * d.n_kv_heads > 0x7fffffff / kThreads || out->n_splits > 65535 || out->n_groups > 65535)
-        return set_error(GLA_ERR_INVALID, "decode: %lld row tiles, %d splits and %d groups of shared prefixes",
-                         (long long)blocks, out->n_splits, out->n_groups);
-    const dim3 grid((unsigned)(blocks * d.n_kv_heads), out->n_splits, out->n_groups);
-    switch (d.head_dim) {
-    case 64:
-        return nt == 2 ? launch_as<64, 2>(ctx, d.q8, prm, grid) : launch_as<64, 1>(ctx, d.q8, prm, grid);
-    case 128:
-        return nt == 2 ? launch_as<128, 2>(ctx, d.q8, prm, grid) : launch_as<128, 1>(ctx, d.q8, prm, grid);
-    case 256:
-        return launch_as<256, 1>(ctx, d.q8, prm, grid);
-    }
-    return set_error(GLA_ERR_INVALID, "unsupported head_dim %d", d.head_dim);
+    prm->q_mul = cap ? d.scale : d.scale * lanes::kLog2e;
+    prm->softcap = cap ? d.softcap : 0.0f;
+    // (more than 2^30 are refused with the grid)
+    const int64_t blocks = ((int64_t)out->max_group * prm->group - 1) / (16 * prefix_tiles(d)) + 1;
+    prm->columns = (int)std::min<int64_t>(blocks * d.n_kv_heads, 1 << 30);
+}
+
+int mix_prefix(const DecodeLaunch &d, const prefix::PrefixParams &prm, dim3 own, prefix::Mixed *mix) {
+    const int64_t n_prefix = (int64_t)prm.columns * d.pre.n_splits * d.pre.n_groups, n_own = (int64_t)own.x * own.y * own.z;
+    if (n_prefix > 1 << 30 || n_own > (1 << 30) - 8)
+        return set_error(GLA_ERR_INVALID, "decode: %lld workgroups for shared prefixes and %lld for the rows behind them",
+                         (long long)n_prefix, (long long)n_own);
+    *mix = {prm.columns, d.pre.n_splits, (int)n_prefix, (int)own.x, (int)own.y, (int)n_own};
+    return GLA_OK;
 }
 
 }  // namespace gla

@@ -54,6 +54,7 @@
 #include <cmath>
 
 #include "gla_internal.h"
+#include "gla_prefix.h"
 
 namespace gla {
 
@@ -986,6 +987,26 @@ __global__ __launch_bounds__(kWaves * 64) void decode_q8_mfma_kernel(const Q8Par
     q8_item<D, MODE>(p, slots, b, wg, blockIdx.x);
 }
 
+// decode_q8_mfma_kernel behind prefixes, with their workgroups among its own.
+template <int D, int NT, bool CAP>
+__global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void decode_q8_prefix_kernel(
+    const Q8Params p, const prefix::PrefixParams pp, const prefix::Mixed mix) {
+    constexpr int kOwnFloats = kWaves * kSlotBytesPerD * D / 4;
+    __shared__ __attribute__((aligned(16))) float lds[std::max(prefix::kLdsFloats<D, NT>, kOwnFloats)];
+    prefix::Place w;
+    if (mix.place(w)) {
+        if (w.z >= 0) prefix::q8_item<D, NT, CAP>(pp, w, lds);
+    } else if (w.z >= 0) {
+        int b = w.z, wg = w.y;
+        if (p.n_rows > 0) {
+            const int e = p.rows[w.y];
+            b = e >> 6;
+            wg = e & 63;
+        }
+        q8_item<D, kBehindPrefix>(p, reinterpret_cast<uint8_t(*)[kSlotBytesPerD * D]>(lds), b, wg, w.x);
+    }
+}
+
 // Merge of the workgroup partials of every unit with more than one
 // workgroup; grid (KV head x head group, sequence), kGT*D/4 threads, each
 // merging four consecutive elements of one head (16-byte loads of the
@@ -1070,7 +1091,7 @@ int launch_as(gla_ctx *ctx, const Q8Params &prm, dim3 grid, int n_seqs) {
     hipLaunchKernelGGL((decode_q8_mfma_kernel<D, MODE>), grid, dim3(kWaves * 64), 0, ctx->stream, prm);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "decode_q8_mfma_kernel launch: %s", hipGetErrorString(e));
-    if (MODE == kBehindPrefix || prm.max_wg > 1) {
+    if (prm.max_wg > 1) {
         hipLaunchKernelGGL((decode_q8_combine_kernel<D, MODE>), dim3(prm.n_kv_heads * prm.n_hg, n_seqs),
                            dim3(kGT * D / 4), 0, ctx->stream, prm);
         e = hipGetLastError();
@@ -1080,9 +1101,33 @@ int launch_as(gla_ctx *ctx, const Q8Params &prm, dim3 grid, int n_seqs) {
     return GLA_OK;
 }
 
+template <int D, int NT>
+int launch_mixed(gla_ctx *ctx, const DecodeLaunch &d, const Q8Params &prm, const prefix::PrefixParams &pp, dim3 grid) {
+    prefix::Mixed mix;
+    if (int rc = mix_prefix(d, pp, grid, &mix)) return rc;
+    if (pp.softcap > 0.0f)
+        hipLaunchKernelGGL((decode_q8_prefix_kernel<D, NT, true>), mix.grid(), dim3(kWaves * 64), 0, ctx->stream,
+                           prm, pp, mix);
+    else
+        hipLaunchKernelGGL((decode_q8_prefix_kernel<D, NT, false>), mix.grid(), dim3(kWaves * 64), 0, ctx->stream,
+                           prm, pp, mix);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "decode_q8_prefix_kernel launch: %s", hipGetErrorString(e));
+    hipLaunchKernelGGL((decode_q8_combine_kernel<D, kBehindPrefix>), dim3(prm.n_kv_heads * prm.n_hg, d.n_seqs),
+                       dim3(kGT * D / 4), 0, ctx->stream, prm);
+    e = hipGetLastError();
+    if (e != hipSuccess) return set_error(GLA_ERR_KERNEL, "decode_q8_combine_kernel launch: %s", hipGetErrorString(e));
+    return GLA_OK;
+}
+
 template <int D>
-int launch_d(gla_ctx *ctx, const Q8Params &prm, dim3 grid, int n_seqs) {
-    if (prm.pre.n_groups > 0) return launch_as<D, kBehindPrefix>(ctx, prm, grid, n_seqs);
+int launch_d(gla_ctx *ctx, const DecodeLaunch &d, const Q8Params &prm, const prefix::PrefixParams &pp, dim3 grid) {
+    const int n_seqs = d.n_seqs;
+    if (prm.pre.n_groups > 0) {
+        if constexpr (D < 256)
+            if (prefix_tiles(d) == 2) return launch_mixed<D, 2>(ctx, d, prm, pp, grid);
+        return launch_mixed<D, 1>(ctx, d, prm, pp, grid);
+    }
     return prm.n_sinks > 0 ? launch_as<D, kWindowSinks>(ctx, prm, grid, n_seqs)
                            : launch_as<D, kWindow>(ctx, prm, grid, n_seqs);
 }
@@ -1174,6 +1219,7 @@ int launch_decode_q8(gla_ctx *ctx, const DecodeLaunch &d) {
     const int64_t units = (int64_t)d.n_seqs * d.n_kv_heads * n_hg;
 
     Q8Params prm;
+    prefix::PrefixParams pp;
     prm.base = d.kv.k;
     prm.page_stride = d.kv.page_stride;
     prm.head_stride = d.kv.head_stride;
@@ -1206,10 +1252,7 @@ int launch_decode_q8(gla_ctx *ctx, const DecodeLaunch &d) {
         int rc = decode_scratch(ctx, d, bytes + prefix_bytes(d), &scr);
         if (rc != GLA_OK) return rc;
         prm.part = (float *)scr;
-        if (behind) {
-            rc = launch_prefix(ctx, d, (uint8_t *)scr + bytes, &prm.pre);
-            if (rc != GLA_OK) return rc;
-        }
+        if (behind) prefix_params(d, (uint8_t *)scr + bytes, &prm.pre, &pp);
     }
     dim3 grid(d.n_kv_heads * n_hg, (unsigned)max_wg, d.n_seqs);
     // With the host lengths, list the workgroups that have pages (plus one per
@@ -1240,11 +1283,11 @@ int launch_decode_q8(gla_ctx *ctx, const DecodeLaunch &d) {
     }
     switch (D) {
     case 64:
-        return launch_d<64>(ctx, prm, grid, d.n_seqs);
+        return launch_d<64>(ctx, d, prm, pp, grid);
     case 128:
-        return launch_d<128>(ctx, prm, grid, d.n_seqs);
+        return launch_d<128>(ctx, d, prm, pp, grid);
     case 256:
-        return launch_d<256>(ctx, prm, grid, d.n_seqs);
+        return launch_d<256>(ctx, d, prm, pp, grid);
     }
     return set_error(GLA_ERR_INVALID, "unsupported head_dim %d", D);
 }

@@ -347,7 +347,7 @@ inline int host_seq_pages(int start, int len, int max_len, int pos_limit, int fr
 }
 
 // A batch's groups of rows that share their first positions. The part before a group's
-// last whole page, prefix_positions, is attended by launch_prefix, for all rows of the
+// last whole page, prefix_positions, is attended for all rows of the
 // group at once, in n_splits splits of split_pages pages; each leaves (m, l)
 // and O, unnormalised in the log2 domain, of every row:
 //   acc [split][row][head_dim], ml [split][row] {m, l}, row = sequence * n_heads + head.
@@ -416,14 +416,24 @@ struct DecodeLaunch {
 };
 // Decides whether d->pre is attended apart (n_groups 0 if not) and sets its splits.
 void plan_prefix(const gla_ctx *ctx, DecodeLaunch *d);
-// What launch_prefix leaves in scratch.
+// What the prefixes' workgroups leave in scratch.
 inline size_t prefix_bytes(const DecodeLaunch &d) {
     return (size_t)d.pre.n_splits * d.n_seqs * d.n_heads * (d.head_dim + 2) * sizeof(float);
 }
-// Attends d.pre; *pre is d.pre with its partials' places at `scratch` (prefix_bytes).
-int launch_prefix(gla_ctx *ctx, const DecodeLaunch &d, void *scratch, PrefixLaunch *pre);
+// Row tiles, of 16 (sequence, query head) pairs of a KV head, that a wave of the prefixes takes.
+inline int prefix_tiles(const DecodeLaunch &d) {
+    return d.head_dim < 256 && (int64_t)d.pre.max_group * (d.n_heads / d.n_kv_heads) > 16 ? 2 : 1;
+}
+namespace prefix {
+struct PrefixParams;
+struct Mixed;
+}  // namespace prefix
+// The kernel arguments of d.pre, whose partials are at `scratch` (prefix_bytes); *pre is d.pre with their places.
+void prefix_params(const DecodeLaunch &d, void *scratch, PrefixLaunch *pre, prefix::PrefixParams *prm);
+// The launch of the prefixes' workgroups with a grid of those of the rows behind them.
+int mix_prefix(const DecodeLaunch &d, const prefix::PrefixParams &prm, dim3 own, prefix::Mixed *mix);
 // What a decode kernel's sequences read: their window, their window and sinks, or their
-// window behind the prefix that launch_prefix reads. A template argument of the kernels.
+// window behind the prefix that is read apart. A template argument of the kernels.
 enum DecodeMode { kWindow = 0, kWindowSinks = 1, kBehindPrefix = 2 };
 inline DecodeMode decode_mode(const DecodeLaunch &d) {
     return d.pre.n_groups > 0 ? kBehindPrefix : (d.n_sinks > 0 ? kWindowSinks : kWindow);

@@ -9,6 +9,7 @@
 #include <type_traits>
 
 namespace gla {
+namespace lanes {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -92,4 +93,5 @@ __device__ __forceinline__ float wave_max(float x) {
     return x;
 }
 
+}  // namespace lanes
 }  // namespace gla

@@ -21,6 +21,8 @@ namespace gla {
 
 namespace {
 
+using namespace lanes;
+
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 struct NormParams {

@@ -32,6 +32,8 @@ namespace gla {
 
 namespace {
 
+using namespace lanes;
+
 constexpr bool kSinks = GLA_PREFILL_SINKS;
 
 constexpr int KT = 32;  // keys per tile
