@@ -19,11 +19,13 @@
 // scores are the operand of the second product as they are, and a row's maximum is its
 // four lanes'.
 //
-// What bounds it, the kernel alone: Q8_0 vector issue (65% of the cycles, matrix 21%, in
+// What bounds it, these workgroups alone: Q8_0 vector issue (65% of the cycles, matrix 21%, in
 // turn): 64 rows at 32/8 heads, d = 128, behind 8,192 positions 39 us, 220 TFLOP/s of the
 // attention's products; f32 the matrix rate from some 48 rows a group on (the same call 91 us,
 // 94 of the 138 TFLOP/s that a library product reaches), HBM and the tiles' re-reads before (24
-// rows in 3 groups behind up to 4,096 positions at 16/8, d = 256 37 us, 180 MB, 4.8 TB/s).
+// rows in 3 groups behind up to 4,096 positions at 16/8, d = 256 37 us, 180 MB, 4.8 TB/s). With the
+// rows' own (64-1,000 positions behind 8,192 Q8_0 49 us, 17-300 in the 3 groups 54 us, 288 MB,
+// 5.4 TB/s).
 #pragma once
 
 #include <math.h>
