@@ -487,43 +487,23 @@ __device__ __forceinline__ void load_words(const uint8_t *src, uint32_t (&dst)[N
 }
 
 // The f16 pieces of p[j] * scale[j], hi = f16(p * scale) and lo = f16(p * scale - hi), of the
-// f16 scales in the words' high (HIGH) or low halves: 16 mixed multiply-adds, which the
-// compiler writes as products and conversions (24 instructions, and a copy of every word
-// where two tiles use it). The s_nops are wait states that it would count itself: for p,
-// which v_exp_f32 may just have written, for halves written and read, and for the products.
+// f16 scales in the words' high (HIGH) or low halves: written so that products and remainders
+// become mixed multiply-adds, which take the halves as they are. 24 instructions where assembly
+// needs 16, but the compiler counts the wait states between the matrix instructions and the
+// registers that these write. Assembly would have to wait for the longest of them every time,
+// which is no faster: 64 rows of 64-1,000 positions behind 8,192 at 32/8 heads, d = 128 53.0 us
+// / this 51.2, of 8-64 47.4 / 45.9, 96 rows in 3 groups 84.0 / 81.8, d = 256 58.5 / 57.9.
 template <bool HIGH>
 __device__ __forceinline__ void pieces8(const float (&p)[8], const uint32_t (&w)[8], half8 &hi, half8 &lo) {
-    uint32_t h0, h1, h2, h3, l0, l1, l2, l3;
-#define GLA_PIECES(S)                                                                 \
-    asm("s_nop 1\n\t"                                                                \
-        "v_fma_mixlo_f16 %0, %8, %16, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"     \
-        "v_fma_mixlo_f16 %1, %10, %18, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixlo_f16 %2, %12, %20, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixlo_f16 %3, %14, %22, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixhi_f16 %0, %9, %17, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"     \
-        "v_fma_mixhi_f16 %1, %11, %19, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixhi_f16 %2, %13, %21, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "v_fma_mixhi_f16 %3, %15, %23, 0 op_sel:[0," S ",0] op_sel_hi:[0,1,0]\n\t"    \
-        "s_nop 1\n\t"                                                                \
-        "v_fma_mixlo_f16 %4, %8, %16, -%0 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"   \
-        "v_fma_mixlo_f16 %5, %10, %18, -%1 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixlo_f16 %6, %12, %20, -%2 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixlo_f16 %7, %14, %22, -%3 op_sel:[0," S ",0] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixhi_f16 %4, %9, %17, -%0 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"   \
-        "v_fma_mixhi_f16 %5, %11, %19, -%1 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixhi_f16 %6, %13, %21, -%2 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"  \
-        "v_fma_mixhi_f16 %7, %15, %23, -%3 op_sel:[0," S ",1] op_sel_hi:[0,1,1]\n\t"  \
-        "s_nop 1"                                                                     \
-        : "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3), "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3) \
-        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), \
-          "v"(w[0]), "v"(w[1]), "v"(w[2]), "v"(w[3]), "v"(w[4]), "v"(w[5]), "v"(w[6]), "v"(w[7]))
-    if constexpr (HIGH)
-        GLA_PIECES("1");
-    else
-        GLA_PIECES("0");
-#undef GLA_PIECES
-    hi = __builtin_bit_cast(half8, make_uint4(h0, h1, h2, h3));
-    lo = __builtin_bit_cast(half8, make_uint4(l0, l1, l2, l3));
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const float s0 = half_at(w, 2 * j + HIGH), s1 = half_at(w, 2 * j + 2 + HIGH);
+        const half2v h = __builtin_convertvector((float2v){fmaf(p[j], s0, 0.0f), fmaf(p[j + 1], s1, 0.0f)}, half2v);
+        hi[j] = h[0];
+        hi[j + 1] = h[1];
+        lo[j] = (_Float16)fmaf(p[j], s0, -(float)h[0]);
+        lo[j + 1] = (_Float16)fmaf(p[j + 1], s1, -(float)h[1]);
+    }
 }
 
 template <int D, int NT, bool CAP>
