@@ -73,12 +73,16 @@ __device__ __forceinline__ T rare(T x) {
 }
 
 // The reference m of a row's exponents moves only when a score passes it by more than
-// kLazy: p is then at most 2^kLazy, and most pages rescale nothing.
-constexpr float kLazy = 8.0f;
+// `lazy`: p is then at most 2^lazy, and most pages rescale nothing. f32 holds any p alike.
+// Q8_0's pieces of p are halves, of which a row that lags wastes the top: p times the largest
+// scale is below 2^14 for p = 1, as in the decode of single rows, and below 2^15.5 for the
+// largest p (a half holds 65,504). With 8 and 2^6 instead 2^-18 of the largest scale was off by
+// 1e-3, and the calls were 1-2% faster.
+constexpr float kLazy = 8.0f, kLazyQ8 = 1.5f;
 // Moves m to the maximum of the row's four lanes where that passes it; what the sums are to be multiplied by.
-__device__ __forceinline__ float moved(float &m, float mine) {
+__device__ __forceinline__ float moved(float &m, float mine, float lazy) {
     const float top = max_rows4(mine);
-    const bool up = top > m + kLazy;
+    const bool up = top > m + lazy;
     const float f = up ? fast_exp2(m - top) : 1.0f;
     m = up ? top : m;
     return f;
@@ -340,7 +344,7 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
                 }
                 const float mine = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
                 if (__ballot(mine > m[nt] + kLazy)) {
-                    const float f = moved(m[nt], mine);
+                    const float f = moved(m[nt], mine, kLazy);
                     lpart[nt] *= f;
 #pragma unroll
                     for (int T = 0; T < DT; T++)
@@ -621,7 +625,7 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
 
     float unit = 1.0f;  // of O and of the sums of P
     if (n > 0) {
-        // P' = p * vscale * 2^vexp is below 2^14 (p at most 2^kLazy)
+        // P' = p * vscale * 2^vexp is below 2^14 for p = 1
         float vmax = 0.0f;
         const int units = n * (D / 16);  // 16 bytes of V scales each
         for (int u0 = 0; u0 < units; u0 += 64) {
@@ -635,9 +639,8 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
         vmax = wave_max(vmax);
         const bool vinf = __ballot(vmax == INFINITY) != 0;
         const int ve = __builtin_amdgcn_readfirstlane(vinf ? 0 : pow2_exp(vmax));
-        constexpr int kTop = 14 - (int)kLazy;
-        const float vexp = (float)(kTop - ve);
-        unit = ldexpf(1.0f, ve - kTop);
+        const float vexp = (float)(14 - ve);
+        unit = ldexpf(1.0f, ve - 14);
 
         for (int i = 0; i < n; i += 2) {
             const int first = (sh.pg0 + i) * 16;
@@ -702,8 +705,8 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
                 const float c = CAP ? 1.0f : sm[nt];
                 const float mine = c * fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                                              fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-                if (__ballot(mine > m[nt] + kLazy)) {
-                    const float f = moved(m[nt], mine);
+                if (__ballot(mine > m[nt] + kLazyQ8)) {
+                    const float f = moved(m[nt], mine, kLazyQ8);
                     lpart[nt] *= f;
 #pragma unroll
                     for (int t = 0; t < ND; t++) o[t][nt] *= f;

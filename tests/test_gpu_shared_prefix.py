@@ -165,6 +165,39 @@ def test_magnitudes(backend, dtype, d):
     assert np.abs(shared(b, q, groups, [400], end * 0, end, scale) - ref).max() <= tol
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_small_blocks_of_values(backend, d):
+    """Q8_0 values whose magnitudes differ from block to block of a head, by up to 2^18: each block's outputs are as near as
+    its own largest value asks. One position of the prefix has nearly all the weight, so that what is lost of the small
+    weights is not averaged away."""
+    rng, n, H, n_kv = np.random.default_rng(11), 32, 8, 2  # (two pages: one wave's step)
+    mul = np.exp2(np.resize([8.0, -10.0, -6.0, 0.0], d // 32)).repeat(32)
+    u = rng.choice([-1.0, 1.0], (n_kv, d))
+    scale = d ** -0.5
+
+    def fill(b):
+        b.k *= np.float32(0.03)
+        b.k[b.at(0, 17)] = (9 * scale * u).reshape(-1)
+        b.v *= np.tile(mul, n_kv).astype(np.float32)
+
+    b, q, groups, end = make(backend, rng, "q8", H, n_kv, d, [5], [n], lambda r: 1 + r, fill=fill)
+    q = (u.repeat(H // n_kv, 0) * rng.uniform(0.97, 1.03, q.shape)).astype(np.float32)
+    ref = want(b, q, end * 0, end, scale)
+    got = shared(b, q, groups, [n], end * 0, end, scale)
+    # Scores: 9 * (1 +- 0.04) at the one position, |s| < 0.5 elsewhere, so that the others' weights are together below
+    # `rest`. A score is off by e as in test_magnitudes (sum |q k| scale < 9.4); a weight by as much, relative, and 2^-20 for
+    # the exponential; that moves an output by 2 e rest twice the block's largest value. Sums of up to n terms: n 2^-24.
+    # A probability times a scale is held in steps of 2^-24 of 2^-13 of the largest scale (two f16 pieces, the largest in
+    # 2^13 .. 2^14, rounded), 127 of them a value, for n positions.
+    e = 2 * (2.0 ** -21 + d * 2.0 ** -24) * 9.4 + 2.0 ** -20
+    rest = (n + 5) * np.exp(0.5 - 8.6)
+    top = np.stack([np.abs(b.v[b.at(r, np.arange(end[r]))]).max(0) for r in range(len(q))]).max(0)
+    top = top.reshape(n_kv, d // 32, 32).max(-1)[np.arange(H) * n_kv // H]  # [H][blocks]
+    tol = (4 * e * rest + n * 2.0 ** -24) * top + n * 2.0 ** -25 * 2.0 ** -13 * top.max(-1, keepdims=True)
+    err = np.abs(got - ref).reshape(len(q), H, d // 32, 32).max(-1)
+    assert np.all(err <= tol), (err / tol).max((0, 1))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "q8"])
 def test_non_finite_data(backend, dtype):
     """A NaN key makes the heads of its group NaN for the rows that see it, an infinite value its dimension; positions that
