@@ -52,6 +52,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "gla_internal.h"
 #include "gla_prefix.h"
@@ -461,6 +462,7 @@ struct StepConst {
     // the true score). P' is p * 2^kvs * vscale, 2^kvs folded into the exp.
     float sm, kvs, softcap, qcap;
     bool cap;
+    bool vinf;  // some V scale of the chunk is infinite
     int pg0, npg, start, end;
     Visible v;  // kWindowSinks
     int kg, ph;
@@ -601,8 +603,13 @@ __device__ __forceinline__ void step_pv(RawV<D> &cur, const StepConst<D> &c, Ste
         const half2v h23 = __builtin_convertvector((float2v){v[2], v[3]}, half2v);
         const half2v e01 = {(_Float16)fmaf(-c.pf, (float)h01[0], v[0]), (_Float16)fmaf(-c.pf, (float)h01[1], v[1])};
         const half2v e23 = {(_Float16)fmaf(-c.pf, (float)h23[0], v[2]), (_Float16)fmaf(-c.pf, (float)h23[1], v[3])};
-        const uint32_t w0 = __builtin_bit_cast(uint32_t, e01);
-        const uint32_t w1 = __builtin_bit_cast(uint32_t, e23);
+        uint32_t w0 = __builtin_bit_cast(uint32_t, e01);
+        uint32_t w1 = __builtin_bit_cast(uint32_t, e23);
+        if (c.vinf) {  // an infinite product is the hi piece as it is, and has no lo piece
+            const half2v z = {(_Float16)0.0f, (_Float16)0.0f}, k01 = c.pf == 0.0f ? h01 : z, k23 = c.pf == 0.0f ? h23 : z;
+            w0 = __builtin_bit_cast(uint32_t, half2v{__builtin_isinf(v[0]) ? k01[0] : e01[0], __builtin_isinf(v[1]) ? k01[1] : e01[1]});
+            w1 = __builtin_bit_cast(uint32_t, half2v{__builtin_isinf(v[2]) ? k23[0] : e23[0], __builtin_isinf(v[3]) ? k23[1] : e23[1]});
+        }
         const uint4 pw = c.ph ? make_uint4(0u, 0u, w0, w1) : make_uint4(w0, w1, 0u, 0u);
         const half8 pa = __builtin_bit_cast(half8, pw);
 #pragma unroll
@@ -678,12 +685,15 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
                                                     (uu % (2 * NB)) * 16);
         }
     };
-    auto scan_max = [&](const uint4 (&w)[4], float vmax) {
+    auto scan_max = [&](const uint4 (&w)[4], float vmax, auto finite) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const uint32_t a[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
 #pragma unroll
-            for (int i = 0; i < 8; i++) vmax = fmaxf(vmax, fabsf(half_at(a, i)));
+            for (int i = 0; i < 8; i++) {
+                const float x = fabsf(half_at(a, i));
+                vmax = finite && x == INFINITY ? vmax : fmaxf(vmax, x);
+            }
         }
         return vmax;
     };
@@ -745,13 +755,25 @@ __device__ __forceinline__ void wave_chunk(const Q8Params &p, const Range &r, in
 
     float inv_vsc;
     {
-        float vmax = scan_max(w0, 0.0f);
+        float vmax = scan_max(w0, 0.0f, std::false_type{});
         for (int u0 = 256; u0 < units; u0 += 256) {
             uint4 w[4];
             scan_loads(u0, w);
-            vmax = scan_max(w, vmax);
+            vmax = scan_max(w, vmax, std::false_type{});
         }
         vmax = wave_max(vmax);
+        // An infinite scale (a wave-uniform branch) has no power of two: it is the finite ones', so
+        // that the chunk's other blocks neither overflow nor lose bits.
+        c.vinf = __ballot(vmax == INFINITY) != 0;
+        if (c.vinf) {
+            vmax = 0.0f;
+            for (int u0 = 0; u0 < units; u0 += 256) {
+                uint4 w[4];
+                scan_loads(u0, w);
+                vmax = scan_max(w, vmax, std::true_type{});
+            }
+            vmax = wave_max(vmax);
+        }
         const int ve = pow2_exp(vmax);
         c.kvs = (float)(14 - ve);
         inv_vsc = ldexpf(1.0f, ve - 14);

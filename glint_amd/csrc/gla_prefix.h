@@ -626,19 +626,27 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
     float unit = 1.0f;  // of O and of the sums of P
     if (n > 0) {
         // P' = p * vscale * 2^vexp is below 2^14 for p = 1
-        float vmax = 0.0f;
         const int units = n * (D / 16);  // 16 bytes of V scales each
-        for (int u0 = 0; u0 < units; u0 += 64) {
-            const int u = min(u0 + lane, units - 1);
-            const int64_t page = __shfl(ids, u / (D / 16));
-            uint32_t w[4];
-            load_words(base + page * p.kv.page_stride + 33 * D + u % (D / 16) * 16, w);
+        const auto largest = [&](auto finite) {
+            float top = 0.0f;
+            for (int u0 = 0; u0 < units; u0 += 64) {
+                const int u = min(u0 + lane, units - 1);
+                const int64_t page = __shfl(ids, u / (D / 16));
+                uint32_t w[4];
+                load_words(base + page * p.kv.page_stride + 33 * D + u % (D / 16) * 16, w);
 #pragma unroll
-            for (int i = 0; i < 8; i++) vmax = fmaxf(vmax, fabsf(half_at(w, i)));
-        }
-        vmax = wave_max(vmax);
+                for (int i = 0; i < 8; i++) {
+                    const float x = fabsf(half_at(w, i));
+                    top = finite && x == INFINITY ? top : fmaxf(top, x);
+                }
+            }
+            return wave_max(top);
+        };
+        float vmax = largest(std::false_type{});
+        // (an infinite scale has no power of two: it is the finite ones', whose positions some rows may see alone)
         const bool vinf = __ballot(vmax == INFINITY) != 0;
-        const int ve = __builtin_amdgcn_readfirstlane(vinf ? 0 : pow2_exp(vmax));
+        if (vinf) vmax = largest(std::true_type{});
+        const int ve = __builtin_amdgcn_readfirstlane(pow2_exp(vmax));
         const float vexp = (float)(14 - ve);
         unit = ldexpf(1.0f, ve - 14);
 
