@@ -93,17 +93,34 @@ struct Place {
     int x, y, z;
 };
 
-// What a workgroup does, and its wave's share of it.
+// A wave's pages of a split's [from, to): its quarter of them (EVEN: taken two at a time).
+struct Pages {
+    int first, n;
+};
+template <bool EVEN>
+__host__ __device__ __forceinline__ Pages wave_pages(int from, int to, int wave) {
+    const int n = to > from ? to - from : 0;
+    int each = (n + kWaves - 1) / kWaves;
+    if (EVEN) each = (each + 1) & ~1;
+    const int left = n - wave * each;
+    return {from + wave * each, left < 0 ? 0 : (left < each ? left : each)};
+}
+// The pages of [from, to) that hold a position of [lo, hi).
+__host__ __device__ __forceinline__ void seen_pages(int &from, int &to, int lo, int hi) {
+    const int first = lo >> 4, end = (hi >> 4) + ((hi & 15) != 0);
+    if (from < first) from = first;
+    if (to > end) to = end;
+}
+
+// What a workgroup does.
 struct Share {
     int kvh;
     int member;     // the group's first row, whose pages are read
     int row0, rows; // the tile's first row and the group's number of rows, (sequence, query head) pairs
-    int pg0, npg;   // the wave's pages of the prefix
+    int from, to;   // the split's pages of the prefix
     bool any;       // the workgroup has something to do
 };
-// `even`: a wave's pages are taken two at a time.
-template <bool EVEN>
-__device__ __forceinline__ Share share_of(const PrefixParams &p, const Place &w, int tile_rows, int wave) {
+__device__ __forceinline__ Share share_of(const PrefixParams &p, const Place &w, int tile_rows) {
     Share s;
     const int g = w.z;
     // (64 rows in two groups behind up to 8,192 Q8_0 positions at 32/8 heads, d = 128, row tiles in one order / turned 76 / 63 us)
@@ -115,13 +132,9 @@ __device__ __forceinline__ Share share_of(const PrefixParams &p, const Place &w,
     const int members = min(max(min(p.pre.group_start[g + 1], p.n_seqs) - s.member, 0), p.pre.max_group);
     s.rows = members * p.group;
     s.row0 = blk * tile_rows;
-    const int wg0 = w.y * p.pre.split_pages;
-    s.any = s.row0 < s.rows && wg0 < pages;
-    const int n = min(p.pre.split_pages, pages - wg0);
-    int each = (n + kWaves - 1) / kWaves;
-    if (EVEN) each = (each + 1) & ~1;
-    s.pg0 = wg0 + wave * each;
-    s.npg = max(min(each, n - wave * each), 0);
+    s.from = w.y * p.pre.split_pages;
+    s.to = min(s.from + p.pre.split_pages, pages);
+    s.any = s.row0 < s.rows && s.from < pages;
     return s;
 }
 
@@ -148,7 +161,6 @@ __device__ __forceinline__ Row row_of(const PrefixParams &p, const Share &s, int
 // Positions that some row of a wave's tile sees, [wlo, whi), and that all do, [ilo, ihi).
 struct Seen {
     int wlo, whi, ilo, ihi;
-    __device__ __forceinline__ bool none(int first, int n) const { return first >= whi || first + n <= wlo; }
     __device__ __forceinline__ bool all(int first, int n) const { return first >= ilo && first + n <= ihi; }
 };
 template <int NT>
@@ -167,9 +179,22 @@ __device__ __forceinline__ Seen seen_of(const Row (&rows)[NT]) {
             __builtin_amdgcn_readfirstlane(ilo), __builtin_amdgcn_readfirstlane(ihi)};
 }
 
-// Physical pages of up to 64 pages from logical page pg0 on, one a lane.
-__device__ __forceinline__ int page_ids(const PrefixParams &p, int b, int pg0, int npg) {
-    return (int)map_page(p.pm, b, pg0 + min((int)(threadIdx.x & 63), npg - 1));
+// A wave's pages again where the rows' windows leave some of the split's unseen; whether it has any then. A
+// page that no row of the tile sees is not read, but for a wave's first, which is asked for before the
+// windows are there. us a call, all pages / these, 32/8 heads, d = 128: 8 rows in windows of 4,096 that begin
+// behind a prefix of 32,768 f32 95.7 / 61.2, Q8_0 48 / 35; 16 in 1,024 that begin in 16,384 54 / 45 and 42 / 29.
+template <bool EVEN>
+__device__ __forceinline__ bool only_seen(const Share &s, const Seen &seen, int wave, Pages &mine) {
+    int from = s.from, to = s.to;
+    seen_pages(from, to, seen.wlo, seen.whi);
+    if (from == s.from && to == s.to) return false;
+    mine = wave_pages<EVEN>(from, to, wave);
+    return mine.n > 0;
+}
+
+// Physical pages of a wave's up to 64, one a lane (without any: the sequence's first).
+__device__ __forceinline__ int page_ids(const PrefixParams &p, int b, const Pages &w) {
+    return (int)map_page(p.pm, b, w.n > 0 ? w.first + min((int)(threadIdx.x & 63), w.n - 1) : 0);
 }
 
 // The waves' (m, l) and O, merged and written. A wave's O is in its slot of `slots`
@@ -245,7 +270,7 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lrow = lane & 15, kg = lane >> 4;
-    const Share sh = share_of<false>(p, w, 16 * NT, wave);
+    const Share sh = share_of(p, w, 16 * NT);
     if (!sh.any) return;
 
     floatx4 k[KK], v[4][DT];
@@ -266,9 +291,9 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
                 v[r][T] = *reinterpret_cast<const floatx4 *>(at + voff + r * p.kv.row_stride + T * 256);
     };
     // (the first page is on its way while the queries are; a wave without pages reads the group's first)
-    const int n = sh.npg;
-    const int ids = page_ids(p, sh.member, n > 0 ? sh.pg0 : 0, max(n, 1));
-    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(n, 1) - 1)); };
+    Pages mine = wave_pages<false>(sh.from, sh.to, wave);
+    int ids = page_ids(p, sh.member, mine);
+    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(mine.n, 1) - 1)); };
     load_k(id(0));
     load_v(id(0));
 
@@ -289,6 +314,12 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
             reinterpret_cast<floatx4 *>(lds)[(nt * KK + kk) * 64 + lane] = x;
         }
     const Seen seen = seen_of<NT>(rows);
+    if (only_seen<false>(sh, seen, wave, mine)) {
+        ids = page_ids(p, sh.member, mine);
+        load_k(id(0));
+        load_v(id(0));
+    }
+    const int n = mine.n;
     __syncthreads();
     const floatx4 *qs = reinterpret_cast<const floatx4 *>(lds);
 
@@ -306,7 +337,7 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
 
     {
         for (int i = 0; i < n; i++) {
-            const int first = (sh.pg0 + i) * 16;
+            const int first = (mine.first + i) * 16;
             const bool inside = seen.all(first, 16);
             int qi = lane;
             asm volatile("" : "+v"(qi));  // (read anew for every page: kept, they would crowd the other registers)
@@ -519,7 +550,7 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lrow = lane & 15, kg = lane >> 4;
-    const Share sh = share_of<true>(p, w, 16 * NT, wave);
+    const Share sh = share_of(p, w, 16 * NT);
     if (!sh.any) return;
 
     const uint8_t *base = p.kv.k + (int64_t)sh.kvh * p.kv.head_stride;
@@ -540,13 +571,16 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
         load_words(at + vsoff, vs[P]);
     };
     // (the first pages are on their way while the queries are split; a wave without pages reads the group's first)
-    const int n = sh.npg;
-    const int ids = page_ids(p, sh.member, n > 0 ? sh.pg0 : 0, max(n, 1));
-    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(n, 1) - 1)); };
-    load_k(0, id(0));
-    load_k(1, id(1));
-    load_v(0, id(0));
-    load_v(1, id(1));
+    Pages mine = wave_pages<true>(sh.from, sh.to, wave);
+    int ids = page_ids(p, sh.member, mine);
+    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(mine.n, 1) - 1)); };
+    const auto load_first = [&]() __attribute__((always_inline)) {
+        load_k(0, id(0));
+        load_k(1, id(1));
+        load_v(0, id(0));
+        load_v(1, id(1));
+    };
+    load_first();
 
     Row rows[NT];
 #pragma unroll
@@ -607,6 +641,11 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
         }
     }
     const Seen seen = seen_of<NT>(rows);
+    if (only_seen<true>(sh, seen, wave, mine)) {
+        ids = page_ids(p, sh.member, mine);
+        load_first();
+    }
+    const int n = mine.n;
     __syncthreads();
     const half8 *qs = reinterpret_cast<const half8 *>(lds);
     float sm[NT];  // undoes a query's scale
@@ -651,7 +690,7 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
         unit = ldexpf(1.0f, ve - 14);
 
         for (int i = 0; i < n; i += 2) {
-            const int first = (sh.pg0 + i) * 16;
+            const int first = (mine.first + i) * 16;
             const bool two = i + 1 < n;
             const bool plain = two && !vinf && seen.all(first, 32);  // every row sees all, and no scale is infinite
             int qi = lane;

@@ -198,6 +198,26 @@ def test_small_blocks_of_values(backend, d):
     assert np.all(err <= tol), (err / tol).max((0, 1))
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prefix_pages_that_no_row_sees(backend, d):
+    """Windows that leave the prefix's first pages out: those are not read, so that values as large as they come there
+    take nothing of the range of those that are seen."""
+    rng, n = np.random.default_rng(13), 400
+
+    def fill(b):
+        b.v *= np.float32(2.0 ** -13)
+        b.v[b.at(0, np.arange(176))] = 1e6 * rng.standard_normal((176, 2 * d))  # (11 pages: waves take two at least)
+
+    b, q, groups, end = make(backend, rng, "q8", 8, 2, d, [5], [n], lambda r: 20 + r, fill=fill)
+    start = np.array([176, 177, 191, 240, 300])
+    ref = want(b, q, start, end, d ** -0.5)
+    top = np.abs(b.v[b.at(0, np.arange(176, n))]).max()
+    for host in ("all", "windows", "none"):
+        got = shared(b, q, groups, [n], start, end - start, d ** -0.5, host=host)
+        # (N(0, 1) data: outputs are averages of some ten values; 1e-4 of the largest, as for values near 1)
+        assert np.abs(got - ref).max() <= 1e-4 * top
+
+
 @pytest.mark.parametrize("dtype", ["f32", "q8"])
 def test_non_finite_data(backend, dtype):
     """A NaN key makes the heads of its group NaN for the rows that see it, an infinite value its dimension; positions that
