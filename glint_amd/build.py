@@ -10,6 +10,7 @@ Outputs (in-tree, git-ignored, shipped with the tree to the GPU box):
     glint_amd/libglint_host.so    C++ host layer over the C ABI (glint_amd/host/glint.hpp)
     glint_amd/_build/test_host    its test program (tests/cpp/test_host.cpp; run by tests/test_host_cpp.py)
     glint_amd/_build/test_pages   the page rules of windows, on the host (tests/cpp/test_pages.hip)
+    glint_amd/_build/test_prefix_plan  the plan of shared prefixes, on the host (tests/cpp/test_prefix_plan.hip)
     oracle/liboracle.so           CPU oracle, built by oracle/Makefile (tests only)
 """
 from __future__ import annotations
@@ -30,6 +31,7 @@ PROBE_LIB = PKG / "libglint_probe.so"
 HOST_LIB = PKG / "libglint_host.so"
 HOST_TEST = BUILD / "test_host"
 PAGES_TEST = BUILD / "test_pages"
+PLAN_TEST = BUILD / "test_prefix_plan"
 ORACLE_DIR = ROOT / "oracle"
 ORACLE_LIB = ORACLE_DIR / "liboracle.so"
 
@@ -103,12 +105,20 @@ def build_host_tests() -> Path:
     return HOST_TEST
 
 
-def build_pages_test() -> Path:
+def _build_host_only(out: Path) -> Path:
     BUILD.mkdir(exist_ok=True)
-    tmp = PAGES_TEST.with_suffix(".tmp")
-    _run([HIPCC, *HIP_FLAGS, "--cuda-host-only", str(ROOT / "tests" / "cpp" / "test_pages.hip"), "-o", str(tmp)])
-    os.replace(tmp, PAGES_TEST)
-    return PAGES_TEST
+    tmp = out.with_suffix(".tmp")
+    _run([HIPCC, *HIP_FLAGS, "--cuda-host-only", str(ROOT / "tests" / "cpp" / f"{out.name}.hip"), "-o", str(tmp)])
+    os.replace(tmp, out)
+    return out
+
+
+def build_pages_test() -> Path:
+    return _build_host_only(PAGES_TEST)
+
+
+def build_plan_test() -> Path:
+    return _build_host_only(PLAN_TEST)
 
 
 def build_synth() -> Path:
@@ -132,6 +142,7 @@ def build_all(jobs: int = 4) -> None:
     build_host()
     build_host_tests()
     build_pages_test()
+    build_plan_test()
 
 
 if __name__ == "__main__":

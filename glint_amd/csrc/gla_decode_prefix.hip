@@ -30,23 +30,40 @@ static bool pays(const DecodeLaunch &d) {
 void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
     const DecodeLaunch &d = *launch;
     PrefixLaunch *pre = &launch->pre;
-    if (!pays(d)) {
+    const bool host = pre->group_start_host != nullptr;
+    if (host) {  // the bounds, as near as they can be
+        pre->max_group = pre->max_prefix = 0;
+        for (int g = 0; g < pre->n_groups; g++) {
+            pre->max_group = std::max(pre->max_group, pre->group_start_host[g + 1] - pre->group_start_host[g]);
+            pre->max_prefix = std::max(pre->max_prefix, std::min(pre->prefix_len_host[g], d.pm.pos_limit) & ~15);
+        }
+    }
+    if (pre->max_group < 2 || !pays(d)) {
         pre->n_groups = 0;
         return;
     }
     const int64_t tile = 16 * prefix_tiles(d), group = d.n_heads / d.n_kv_heads;
     const int pages = pre->max_prefix / 16;
+    int64_t tiles = 0;
+    for (int g = 0; host && g < pre->n_groups; g++)
+        tiles += ((pre->group_start_host[g + 1] - pre->group_start_host[g]) * group + tile - 1) / tile;
+    if (!host)
+        tiles = std::min<int64_t>(pre->n_groups * ((pre->max_group * group - 1) / tile + 1), d.n_seqs * group / tile + pre->n_groups);
+    // The launch has a workgroup for each of these a split, and those find their group: one for every
+    // tile of the largest group a group are thousands too many where groups are unlike. 64 rows behind
+    // 2,048 and 63 pairs behind 64-1,924 at 32/8 heads, d = 128, such / these: f32 365 / 173 us, Q8_0
+    // 146 / 71 (row by row 469 and 80); 8 groups of 1-32 rows behind 100-8,192 known by their bounds alone
+    // 284 / 154 and 109 / 74; 3 of 96 Q8_0 rows behind 8,192 85 / 82.
+    pre->tiles = (int)std::min<int64_t>(tiles, 1 << 30);  // (as many are refused with the grid)
     // workgroups of a launch with splits of n pages: as they are, or from the bounds
-    const bool host = pre->group_start_host && pre->n_groups <= 256;
-    const int64_t tiles = std::min<int64_t>(pre->n_groups * ((pre->max_group * group - 1) / tile + 1),
-                                            d.n_seqs * group / tile + pre->n_groups);
+    const bool few = host && pre->n_groups <= 256;
     const auto wgs = [&](int n) {
         int64_t sum = 0;
-        for (int g = 0; host && g < pre->n_groups; g++) {
+        for (int g = 0; few && g < pre->n_groups; g++) {
             const int64_t rows = (pre->group_start_host[g + 1] - pre->group_start_host[g]) * group;
             sum += (rows + tile - 1) / tile * ((prefix_positions(pre->prefix_len_host[g], pre->max_prefix) / 16 + n - 1) / n);
         }
-        return (host ? sum : tiles * ((pages + n - 1) / n)) * d.n_kv_heads;
+        return (few ? sum : tiles * ((pages + n - 1) / n)) * d.n_kv_heads;
     };
     // the fewest pages (a wave's: an even number, at most 64) that leave at most `most` workgroups
     const auto pages_for = [&](int64_t most) {
@@ -67,7 +84,12 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
     // 8-64 f32 102 / 109 (2); in groups 96 Q8_0 rows in 3 93 / 88 / 88, 48 f32 rows in 3 133 / 95 / 94,
     // 64 Q8_0 rows in 4 behind 2,048 32.9 / 27.6 / 29.5; at 16/8, d = 256 24 f32 rows in 3 behind up to
     // 4,096 64.5 / 63.1 / 67.6, 40 Q8_0 rows in 2 34.8 / 39.0 / 42.0.
-    pre->split_pages = pages_for(pre->n_groups > 1 ? ctx->n_cu + ctx->n_cu / 2 : ctx->n_cu);
+    // Three a unit for several groups known by their bounds alone, of which most may be shorter: 8 Q8_0
+    // groups of 1-32 rows behind 100-8,192, the longest one row's (35 us row by row), 1.5 / 3 / 6 a unit
+    // 74 / 46 / 37, f32 154 / 97 / 77, with the host copies 36 and 65; 32 pairs behind 2,048 each Q8_0 33 /
+    // 37 / 42, f32 109 / 116 / 121.
+    const int units = ctx->n_cu;
+    pre->split_pages = pages_for(pre->n_groups <= 1 ? units : (few ? units + units / 2 : 3 * units));
     pre->n_splits = (pages + pre->split_pages - 1) / pre->split_pages;
 }
 
@@ -90,12 +112,11 @@ void prefix_params(const DecodeLaunch &d, void *scratch, PrefixLaunch *out, pref
     prm->q_mul = cap ? d.scale : d.scale * lanes::kLog2e;
     prm->softcap = cap ? d.softcap : 0.0f;
     // (more than 2^30 are refused with the grid)
-    const int64_t blocks = ((int64_t)out->max_group * prm->group - 1) / (16 * prefix_tiles(d)) + 1;
-    prm->columns = (int)std::min<int64_t>(blocks * d.n_kv_heads, 1 << 30);
+    prm->columns = (int)std::min<int64_t>((int64_t)d.pre.tiles * d.n_kv_heads, 1 << 30);
 }
 
 int mix_prefix(const DecodeLaunch &d, const prefix::PrefixParams &prm, dim3 own, prefix::Mixed *mix) {
-    const int64_t n_prefix = (int64_t)prm.columns * d.pre.n_splits * d.pre.n_groups, n_own = (int64_t)own.x * own.y * own.z;
+    const int64_t n_prefix = (int64_t)prm.columns * d.pre.n_splits, n_own = (int64_t)own.x * own.y * own.z;
     if (n_prefix > 1 << 30 || n_own > (1 << 30) - 8)
         return set_error(GLA_ERR_INVALID, "decode: %lld workgroups for shared prefixes and %lld for the rows behind them",
                          (long long)n_prefix, (long long)n_own);

@@ -358,6 +358,7 @@ struct PrefixLaunch {
     int max_group = 0;
     int max_prefix = 0;  // at most the storage's positions
     int max_own = 0;
+    int tiles = 0;  // row tiles (prefix_tiles) of all groups, at most
     int split_pages = 0, n_splits = 0;
     float *acc = nullptr, *ml = nullptr;
     const int32_t *group_start_host = nullptr, *prefix_len_host = nullptr;

@@ -49,6 +49,18 @@ __device__ __forceinline__ float sum_row16(float x) {
     return x;
 }
 
+// sum over the wave's lanes up to and with this one: DPP shifts within each 16-lane row, then the
+// rows' last lanes into the rows behind them
+__device__ __forceinline__ int sum_to_lane(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15, into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31, into rows 2 and 3
+    return x;
+}
+
 // max / min of unsigned words over the wave, in every lane: DPP rotations within
 // each 16-lane row, then the row swaps.
 template <bool MAX>

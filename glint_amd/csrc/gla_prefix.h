@@ -61,7 +61,7 @@ struct PrefixParams {
     int group;
     float q_mul;    // scale (soft-cap) or scale * log2(e)
     float softcap;  // > 0: cap * tanh(s / cap)
-    int columns;    // KV heads x row tiles of a group
+    int columns;    // KV heads x row tiles of all groups
 };
 
 // x, for a rare block of code to start from: the block stays a branch, where the compiler
@@ -88,10 +88,42 @@ __device__ __forceinline__ float moved(float &m, float mine, float lazy) {
     return f;
 }
 
-// A workgroup's place among the prefixes': KV heads x row tiles, split, group.
+// A workgroup's place among the prefixes' (KV heads x row tiles of all groups, split, 0) or among
+// those of the rows' own pages.
 struct Place {
     int x, y, z;
 };
+
+// Row tile `at` of all groups': its group and its place among that group's tiles.
+struct Tile {
+    int group;  // < 0: there are not as many
+    int at;
+    int first, members;  // the group's rows, clamped into the batch
+};
+__device__ __forceinline__ Tile tile_of(const PrefixParams &p, int tile_rows, int at) {
+    const int lane = threadIdx.x & 63;
+    Tile t;
+    t.group = -1;
+    // (every wave by itself; a launch has fewer than 2^30 tiles, so that the sums stay in 32 bits)
+    for (int i = 0, before = 0; i < p.pre.n_groups; i += 64) {
+        const int g = min(i + lane, p.pre.n_groups - 1);
+        const int first = min(max(p.pre.group_start[g], 0), p.n_seqs);
+        const int members = min(max(min(p.pre.group_start[g + 1], p.n_seqs) - first, 0), p.pre.max_group);
+        const int mine = i + lane < p.pre.n_groups ? (members * p.group + tile_rows - 1) / tile_rows : 0;
+        const int end = before + sum_to_lane(mine);
+        const uint64_t holds = __ballot(end > at);
+        if (holds) {
+            const int l = __builtin_ctzll(holds);
+            t.group = i + l;
+            t.at = at - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(mine, l));
+            t.first = __builtin_amdgcn_readlane(first, l);
+            t.members = __builtin_amdgcn_readlane(members, l);
+            break;
+        }
+        before = __builtin_amdgcn_readlane(end, 63);
+    }
+    return t;
+}
 
 // A wave's pages of a split's [from, to): its quarter of them (EVEN: taken two at a time).
 struct Pages {
@@ -122,19 +154,19 @@ struct Share {
 };
 __device__ __forceinline__ Share share_of(const PrefixParams &p, const Place &w, int tile_rows) {
     Share s;
-    const int g = w.z;
     // (64 rows in two groups behind up to 8,192 Q8_0 positions at 32/8 heads, d = 128, row tiles in one order / turned 76 / 63 us)
     const int at = w.x / p.n_kv_heads;  // (the heads run fastest: a head's row tiles share an L2)
     s.kvh = w.x - at * p.n_kv_heads;
-    const int blk = turned(at, p.columns / p.n_kv_heads, w.y);
-    const int pages = prefix_positions(p.pre.prefix_len[g], p.pre.max_prefix) >> 4;
-    s.member = min(max(p.pre.group_start[g], 0), p.n_seqs);
-    const int members = min(max(min(p.pre.group_start[g + 1], p.n_seqs) - s.member, 0), p.pre.max_group);
-    s.rows = members * p.group;
-    s.row0 = blk * tile_rows;
+    const Tile t = tile_of(p, tile_rows, turned(at, p.columns / p.n_kv_heads, w.y));
+    s.any = t.group >= 0;
+    if (!s.any) return s;
+    const int pages = prefix_positions(p.pre.prefix_len[t.group], p.pre.max_prefix) >> 4;
+    s.member = t.first;
+    s.rows = t.members * p.group;
+    s.row0 = t.at * tile_rows;
     s.from = w.y * p.pre.split_pages;
     s.to = min(s.from + p.pre.split_pages, pages);
-    s.any = s.row0 < s.rows && s.from < pages;
+    s.any = s.from < pages;
     return s;
 }
 
@@ -825,7 +857,7 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
 // 60.3 / 73.2, of 8-64 53.3 / 52.1 / 61.9, 4 rows 24.3 / 18.6 / 20.0; 64 rows in 4 groups behind
 // 2,048 35.3 / 28.1 / 35.9 (the prefixes' are the longest, and all of them are resident).
 struct Mixed {
-    int px, py, n_prefix;  // the prefixes' columns and splits, and their workgroups
+    int px, py, n_prefix;  // the prefixes' columns and splits, and their product
     int ox, oy, n_own;     // those of the rows' own pages
     // (the rows' begin on the same XCD as in a launch of their own)
     __host__ __device__ int own0() const { return (n_prefix + 7) & ~7; }

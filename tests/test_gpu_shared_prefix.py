@@ -198,6 +198,22 @@ def test_small_blocks_of_values(backend, d):
     assert np.all(err <= tol), (err / tol).max((0, 1))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "q8"])
+@pytest.mark.parametrize("n", [64, 65, 128, 300])
+def test_many_groups(backend, dtype, n):
+    """More groups than a wave has lanes, of unlike sizes and prefixes, some of no rows and some that share nothing; rows of no
+    group before and behind them."""
+    rng = np.random.default_rng(n)
+    sizes = rng.integers(0, 4, n)
+    sizes[[0, n // 2, n - 1]] = 2, 9, 3
+    prefix = rng.integers(1, 80, n) * (rng.random(n) < 0.8)
+    prefix[[0, n // 2, n - 1]] = 70, 200, 33
+    b, q, groups, end = make(backend, rng, dtype, 6, 2, 64, sizes, prefix, lambda r: 1 + r % 40, lead=3, trail=2)
+    ref = want(b, q, end * 0, end, 0.125)
+    for host, slack in (("all", 0), ("all", 50), ("windows", 0), ("none", 21)):
+        assert_close(shared(b, q, groups, prefix, end * 0, end, 0.125, host=host, slack=slack), ref)
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_prefix_pages_that_no_row_sees(backend, d):
     """Windows that leave the prefix's first pages out: those are not read, so that values as large as they come there
