@@ -154,7 +154,7 @@ struct SeqRange {
     int pps;         // pages per split
     int n_splits;
     Visible v;       // kWindowSinks (fp is 0: pages are numbered as Visible does)
-    int prefix;      // kBehindPrefix: positions that the prefix's partials hold
+    Splits shared;   // kBehindPrefix: those whose partials hold what the row sees of its group's prefix
 };
 
 template <DecodeMode MODE>
@@ -177,8 +177,9 @@ __device__ __forceinline__ SeqRange seq_range(const DecodeParams &p, int b) {
     int e = s + len;
     if (e > p.pm.pos_limit) e = p.pm.pos_limit;
     if constexpr (MODE == kBehindPrefix) {
-        r.prefix = row_prefix(p.pre, b);
-        if (s < e && s < r.prefix) s = r.prefix;  // (an empty window stays so)
+        const int prefix = row_prefix(p.pre, b);
+        r.shared = prefix_splits(p.pre, prefix, s, e);
+        if (s < e && s < prefix) s = prefix;  // (an empty window stays so)
     }
     if (s > e) s = e;
     r.start = s;
@@ -581,7 +582,7 @@ __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const DecodePa
     const SeqRange r = seq_range<MODE>(p, b);
     // (one split, or merged in the split kernel)
     if (MODE != kBehindPrefix && (r.n_splits <= 1 || r.n_pages <= p.merge_pages)) return;
-    const int n = r.n_splits + (MODE == kBehindPrefix ? prefix_splits(p.pre, r.prefix) : 0);
+    const int n = r.n_splits + (MODE == kBehindPrefix ? r.shared.n : 0);
     const int sg = threadIdx.x / RL;
     const int e4 = threadIdx.x - sg * RL;
     const int64_t unit = ((int64_t)b * p.n_kv_heads + kvh) * p.n_hg + hg;
@@ -601,7 +602,7 @@ __global__ __launch_bounds__(kThreads) void decode_combine_kernel(const DecodePa
             const float *ml = p.part_ml + (slot0 + sc) * 32 + g, *acc = p.part_acc + slot * D;
             int l_at = 8;
             if (MODE == kBehindPrefix && sc >= r.n_splits) {
-                const int64_t at = ((int64_t)(sc - r.n_splits) * gridDim.z + b) * p.n_heads + kvh * p.group + hg * GT + g;
+                const int64_t at = ((int64_t)(sc - r.n_splits + r.shared.first) * gridDim.z + b) * p.n_heads + kvh * p.group + hg * GT + g;
                 ml = p.pre.ml + 2 * at;
                 acc = p.pre.acc + at * D;
                 l_at = 1;

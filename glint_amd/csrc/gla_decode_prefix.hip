@@ -3,6 +3,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <vector>
 
 #include "gla_prefix.h"
 
@@ -27,16 +28,36 @@ static bool pays(const DecodeLaunch &d) {
     return d.pre.max_prefix >= (d.head_dim == 64 ? 640 : 448);
 }
 
+namespace {
+struct Pages {
+    int from, to;
+};
+}  // namespace
+
 void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
     const DecodeLaunch &d = *launch;
     PrefixLaunch *pre = &launch->pre;
     const bool host = pre->group_start_host != nullptr;
-    if (host) {  // the bounds, as near as they can be
-        pre->max_group = pre->max_prefix = 0;
+    // The bounds, as near as the host copies let them be, and the pages of each group's prefix that some row sees.
+    std::vector<Pages> seen;
+    if (host) {
+        seen.resize(pre->n_groups);
+        int max_group = 0, max_prefix = 0;
         for (int g = 0; g < pre->n_groups; g++) {
-            pre->max_group = std::max(pre->max_group, pre->group_start_host[g + 1] - pre->group_start_host[g]);
-            pre->max_prefix = std::max(pre->max_prefix, std::min(pre->prefix_len_host[g], d.pm.pos_limit) & ~15);
+            const int first = pre->group_start_host[g], end = pre->group_start_host[g + 1];
+            const int positions = prefix_positions(pre->prefix_len_host[g], pre->max_prefix);
+            max_group = std::max(max_group, end - first);
+            max_prefix = std::max(max_prefix, positions);
+            int lo = positions, hi = 0;
+            for (int b = first; b < end; b++) {
+                if (d.kv_len_host[b] == 0 || d.kv_start_host[b] >= positions) continue;
+                lo = std::min(lo, (int)d.kv_start_host[b]);
+                hi = std::max(hi, std::min(positions, d.kv_start_host[b] + d.kv_len_host[b]));
+            }
+            seen[g] = {lo / 16, (hi + 15) / 16};
         }
+        pre->max_group = max_group;
+        pre->max_prefix = max_prefix;
     }
     if (pre->max_group < 2 || !pays(d)) {
         pre->n_groups = 0;
@@ -61,7 +82,7 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
         int64_t sum = 0;
         for (int g = 0; few && g < pre->n_groups; g++) {
             const int64_t rows = (pre->group_start_host[g + 1] - pre->group_start_host[g]) * group;
-            sum += (rows + tile - 1) / tile * ((prefix_positions(pre->prefix_len_host[g], pre->max_prefix) / 16 + n - 1) / n);
+            if (seen[g].from < seen[g].to) sum += (rows + tile - 1) / tile * ((seen[g].to - 1) / n - seen[g].from / n + 1);
         }
         return (few ? sum : tiles * ((pages + n - 1) / n)) * d.n_kv_heads;
     };
@@ -90,7 +111,12 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
     // 37 / 42, f32 109 / 116 / 121.
     const int units = ctx->n_cu;
     pre->split_pages = pages_for(pre->n_groups <= 1 ? units : (few ? units + units / 2 : 3 * units));
-    pre->n_splits = (pages + pre->split_pages - 1) / pre->split_pages;
+    int from = pages, to = 0;
+    for (const Pages &p : seen)
+        if (p.from < p.to) from = std::min(from, p.from), to = std::max(to, p.to);
+    if (!host) from = 0, to = pages;
+    pre->first_split = to > from ? from / pre->split_pages : 0;
+    pre->n_splits = to > from ? (to - 1) / pre->split_pages - pre->first_split + 1 : 0;
 }
 
 void prefix_params(const DecodeLaunch &d, void *scratch, PrefixLaunch *out, prefix::PrefixParams *prm) {

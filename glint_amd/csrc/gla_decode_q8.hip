@@ -112,7 +112,7 @@ struct Range {
     int fp;          // first logical page
     int n_pages;
     Visible v;       // kWindowSinks (fp is 0: pages are numbered as Visible does)
-    int prefix;      // kBehindPrefix: positions that the prefix's partials hold
+    Splits shared;   // kBehindPrefix: those whose partials hold what the row sees of its group's prefix
 };
 
 template <DecodeMode MODE>
@@ -133,8 +133,9 @@ __device__ __forceinline__ Range seq_range(const Q8Params &p, int b) {
     int e = s + len;
     if (e > p.pm.pos_limit) e = p.pm.pos_limit;
     if constexpr (MODE == kBehindPrefix) {
-        r.prefix = row_prefix(p.pre, b);
-        if (s < e && s < r.prefix) s = r.prefix;  // (an empty window stays so)
+        const int prefix = row_prefix(p.pre, b);
+        r.shared = prefix_splits(p.pre, prefix, s, e);
+        if (s < e && s < prefix) s = prefix;  // (an empty window stays so)
     }
     if (s > e) s = e;
     r.start = s;
@@ -1047,7 +1048,7 @@ __global__ __launch_bounds__(kGT * D / 4) void decode_q8_combine_kernel(const Q8
     const int span = wg_span(r.n_pages, kWaves * p.ch, D);  // pages per workgroup
     const int n_wg = min((r.n_pages + span - 1) / span, p.max_wg);
     if (MODE != kBehindPrefix && n_wg <= 1) return;
-    const int n = n_wg + (MODE == kBehindPrefix ? prefix_splits(p.pre, r.prefix) : 0);
+    const int n = n_wg + (MODE == kBehindPrefix ? r.shared.n : 0);
     const int g = (4 * (int)threadIdx.x) / D;
     const int d = 4 * (int)threadIdx.x - g * D;
     if (g >= gcount) return;
@@ -1066,7 +1067,7 @@ __global__ __launch_bounds__(kGT * D / 4) void decode_q8_combine_kernel(const Q8
             const float *ml = hp + i * pstride + kGT * D + g, *acc = hp + i * pstride + g * D + d;
             int l_at = kGT;
             if (MODE == kBehindPrefix && i >= n_wg) {
-                const int64_t at = ((int64_t)(i - n_wg) * gridDim.y + b) * p.n_heads + h_base + g;
+                const int64_t at = ((int64_t)(i - n_wg + r.shared.first) * gridDim.y + b) * p.n_heads + h_base + g;
                 ml = p.pre.ml + 2 * at;
                 acc = p.pre.acc + at * D + d;
                 l_at = 1;

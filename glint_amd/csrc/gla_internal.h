@@ -348,9 +348,9 @@ inline int host_seq_pages(int start, int len, int max_len, int pos_limit, int fr
 
 // A batch's groups of rows that share their first positions. The part before a group's
 // last whole page, prefix_positions, is attended for all rows of the
-// group at once, in n_splits splits of split_pages pages; each leaves (m, l)
-// and O, unnormalised in the log2 domain, of every row:
-//   acc [split][row][head_dim], ml [split][row] {m, l}, row = sequence * n_heads + head.
+// group at once, in splits of split_pages pages; each leaves (m, l)
+// and O, unnormalised in the log2 domain, of every row that sees some of it:
+//   acc [split - first_split][row][head_dim], ml [..][row] {m, l}, row = sequence * n_heads + head.
 struct PrefixLaunch {
     const int32_t *group_start = nullptr;
     const int32_t *prefix_len = nullptr;
@@ -359,15 +359,25 @@ struct PrefixLaunch {
     int max_prefix = 0;  // at most the storage's positions
     int max_own = 0;
     int tiles = 0;  // row tiles (prefix_tiles) of all groups, at most
-    int split_pages = 0, n_splits = 0;
+    int split_pages = 0;
+    int first_split = 0, n_splits = 0;  // those before the first are seen by no row
     float *acc = nullptr, *ml = nullptr;
     const int32_t *group_start_host = nullptr, *prefix_len_host = nullptr;
 };
 __host__ __device__ __forceinline__ int prefix_positions(int len, int max_prefix) {
     return (len < 0 ? 0 : (len > max_prefix ? max_prefix : len)) & ~15;
 }
-__host__ __device__ __forceinline__ int prefix_splits(const PrefixLaunch &p, int positions) {
-    return (positions / 16 + p.split_pages - 1) / p.split_pages;
+// The splits, counted from first_split, that hold positions of [start, end) before `positions`.
+struct Splits {
+    int first, n;
+};
+__host__ __device__ __forceinline__ Splits prefix_splits(const PrefixLaunch &p, int positions, int start, int end) {
+    if (end > positions) end = positions;
+    if (start >= end) return {0, 0};
+    int first = (start >> 4) / p.split_pages - p.first_split, last = ((end - 1) >> 4) / p.split_pages - p.first_split;
+    if (first < 0) first = 0;
+    if (last >= p.n_splits) last = p.n_splits - 1;
+    return {first, last < first ? 0 : last - first + 1};
 }
 // Positions that row b shares with its group, found by every wave on its own (all lanes
 // call it): the last group that starts at or before b holds it, if it has not ended.

@@ -164,7 +164,7 @@ __device__ __forceinline__ Share share_of(const PrefixParams &p, const Place &w,
     s.member = t.first;
     s.rows = t.members * p.group;
     s.row0 = t.at * tile_rows;
-    s.from = w.y * p.pre.split_pages;
+    s.from = (w.y + p.pre.first_split) * p.pre.split_pages;
     s.to = min(s.from + p.pre.split_pages, pages);
     s.any = s.from < pages;
     return s;
@@ -211,17 +211,17 @@ __device__ __forceinline__ Seen seen_of(const Row (&rows)[NT]) {
             __builtin_amdgcn_readfirstlane(ilo), __builtin_amdgcn_readfirstlane(ihi)};
 }
 
-// A wave's pages again where the rows' windows leave some of the split's unseen; whether it has any then. A
+// A wave's pages again where the rows' windows leave some of the split's unseen; whether they did. A
 // page that no row of the tile sees is not read, but for a wave's first, which is asked for before the
-// windows are there. us a call, all pages / these, 32/8 heads, d = 128: 8 rows in windows of 4,096 that begin
+// windows are there; a split of which none sees any (`to` <= `from` then) leaves nothing. us a call, all pages / these, 32/8 heads, d = 128: 8 rows in windows of 4,096 that begin
 // behind a prefix of 32,768 f32 95.7 / 61.2, Q8_0 48 / 35; 16 in 1,024 that begin in 16,384 54 / 45 and 42 / 29.
 template <bool EVEN>
-__device__ __forceinline__ bool only_seen(const Share &s, const Seen &seen, int wave, Pages &mine) {
-    int from = s.from, to = s.to;
-    seen_pages(from, to, seen.wlo, seen.whi);
+__device__ __forceinline__ bool only_seen(Share &s, const Seen &seen, int wave, Pages &mine) {
+    const int from = s.from, to = s.to;
+    seen_pages(s.from, s.to, seen.wlo, seen.whi);
     if (from == s.from && to == s.to) return false;
-    mine = wave_pages<EVEN>(from, to, wave);
-    return mine.n > 0;
+    mine = wave_pages<EVEN>(s.from, s.to, wave);
+    return true;
 }
 
 // Physical pages of a wave's up to 64, one a lane (without any: the sequence's first).
@@ -302,7 +302,7 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lrow = lane & 15, kg = lane >> 4;
-    const Share sh = share_of(p, w, 16 * NT);
+    Share sh = share_of(p, w, 16 * NT);
     if (!sh.any) return;
 
     floatx4 k[KK], v[4][DT];
@@ -347,6 +347,7 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
         }
     const Seen seen = seen_of<NT>(rows);
     if (only_seen<false>(sh, seen, wave, mine)) {
+        if (sh.from >= sh.to) return;  // (all waves: they have the same rows)
         ids = page_ids(p, sh.member, mine);
         load_k(id(0));
         load_v(id(0));
@@ -582,7 +583,7 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lrow = lane & 15, kg = lane >> 4;
-    const Share sh = share_of(p, w, 16 * NT);
+    Share sh = share_of(p, w, 16 * NT);
     if (!sh.any) return;
 
     const uint8_t *base = p.kv.k + (int64_t)sh.kvh * p.kv.head_stride;
@@ -674,6 +675,7 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
     }
     const Seen seen = seen_of<NT>(rows);
     if (only_seen<true>(sh, seen, wave, mine)) {
+        if (sh.from >= sh.to) return;  // (all waves: they have the same rows)
         ids = page_ids(p, sh.member, mine);
         load_first();
     }

@@ -98,6 +98,38 @@ int tiles() {
     return 0;
 }
 
+// A row reads the partials of those splits that hold some of what it sees of the prefix, all of them in the launch, and a
+// launch that knows the windows begins with the first that any row sees.
+int windows() {
+    for (bool host : {false, true})
+        for (int own : {1, 30, 500, 4200})
+            for (int window : {0, 16, 200, 1024, 4096})
+                for (const auto &sizes : {std::vector<int>{16}, {5, 20, 2}}) {
+                    std::vector<int32_t> lens{8192, 3000, 900};
+                    lens.resize(sizes.size());
+                    Batch b(kShapes[1], true, sizes, lens, own, host, window);
+                    b.plan();
+                    const PrefixLaunch &pre = b.d.pre;
+                    if (pre.n_groups == 0) continue;
+                    std::set<int> used;
+                    for (int r = 0, g = 0; r < b.d.n_seqs; r++) {
+                        while (b.starts[g + 1] <= r) g++;
+                        const int positions = prefix_positions(b.prefix[g], pre.max_prefix), from = b.start[r];
+                        const Splits mine = prefix_splits(pre, positions, from, from + b.len[r]);
+                        std::set<int> want, got;
+                        for (int j = from; j < positions && j < from + b.len[r]; j++) want.insert(j / 16 / pre.split_pages);
+                        for (int i = mine.first; i < mine.first + mine.n; i++) got.insert(i + pre.first_split);
+                        CHECK(got == want && (mine.n == 0 || (mine.first >= 0 && mine.first + mine.n <= pre.n_splits)),
+                              "row %d of window %d, %d of its own", r, window, own);
+                        used.insert(got.begin(), got.end());
+                    }
+                    if (host)
+                        CHECK(used.empty() ? pre.n_splits == 0 : pre.n_splits == *used.rbegin() - *used.begin() + 1,
+                              "%d splits, window %d, %d of the rows' own", pre.n_splits, window, own);
+                }
+    return 0;
+}
+
 // The pages of a split that hold a position of [lo, hi), shared out to the waves.
 int pages() {
     for (int from : {0, 8, 40})
@@ -124,7 +156,7 @@ int pages() {
 }  // namespace
 
 int main() {
-    if (tiles() || pages()) return 1;
+    if (tiles() || windows() || pages()) return 1;
     printf("plan ok\n");
     return 0;
 }
