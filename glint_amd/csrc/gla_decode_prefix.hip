@@ -9,7 +9,20 @@
 
 namespace gla {
 
-// Whether reading the prefixes apart is the faster way, from the launch's bounds. It costs
+namespace {
+struct Pages {
+    int from, to;
+};
+// What a launch's rows attend, in positions: exactly, from host copies, or as far as its bounds say.
+struct Work {
+    int64_t saved = 0;  // that they would read again, row by row
+    int64_t own = 0;    // behind their prefixes, or in none
+    int64_t total = 0;
+    int longest = 0;    // of a prefix that several rows share, what some row sees
+};
+}  // namespace
+
+// Whether reading the prefixes apart is the faster way. It costs
 // a combine and the set-up of more workgroups; what it saves are the bytes that the rows
 // would read again (from L2 mostly) and, with Q8_0, the length of a wave's chain of pages.
 // us a call, apart / row by row, in a captured step with 1-33 positions of each row's own:
@@ -19,20 +32,22 @@ namespace gla {
 //   Q8_0  9/3 heads, d = 64:   2 rows of 256 9.9 / 8.1, of 704 10.3 / 10.8, of 4,096 14.4 / 20.9, 16 of 704 11.1 / 11.8
 //        32/8 heads, d = 128:  2 rows of 256 10.8 / 9.6, of 704 11.0 / 13.6, 16 of 256 12.8 / 12.9
 //        16/8 heads, d = 256:  2 rows of 256 13.2 / 13.6, 8 of 256 13.9 / 13.8, 2 of 704 13.4 / 19.9
-static bool pays(const DecodeLaunch &d) {
+// It also costs where rows have much of their own, or share nothing: f32 at head_dim 256 reads a row's
+// own positions once a head (a wave holds one, so those of a KV head's others are read again), other
+// f32 kernels lose their merge, and Q8_0 takes rows of no group through the prefixes' tiles. A pair that
+// shares 512 positions among 64 rows of 2,000 f32 at 16/8, d = 256 594 / 373 us, at 32/8, d = 128 254 /
+// 238, Q8_0 52 / 52; 16 rows that see 1,050 of a prefix and 1,000 of their own f32 at 16/8 84 / 78; 64
+// lone rows behind 1,024 beside a pair behind 64 Q8_0 at 32/8 36 / 31, 16 behind 2,048 beside a pair
+// behind as many at 16/8 46 / 75 (5% saved).
+static bool pays(const DecodeLaunch &d, const Work &w) {
     const int64_t position = d.kv.page_stride / 16;  // bytes
-    if (d.pre.max_prefix == 0) return false;
+    if (w.longest == 0) return false;
     if (const char *env = getenv("GLA_DECODE_PREFIX")) return atoi(env) != 0;  // (tuning and tests)
-    const int64_t saved = (int64_t)(d.n_seqs - d.pre.n_groups) * d.pre.max_prefix * position;
-    if (!d.q8) return saved >= (d.head_dim == 256 ? 70000000 : 30000000);
-    return d.pre.max_prefix >= (d.head_dim == 64 ? 640 : 448);
+    if (d.q8) return w.longest >= (d.head_dim == 64 ? 640 : 448) && 64 * w.saved >= w.total;
+    const bool wide = d.head_dim == 256;
+    const int64_t own = wide && d.n_heads > d.n_kv_heads ? w.own : w.own / 10;
+    return (w.saved - own) * position >= (wide ? 70000000 : 30000000);
 }
-
-namespace {
-struct Pages {
-    int from, to;
-};
-}  // namespace
 
 void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
     const DecodeLaunch &d = *launch;
@@ -40,6 +55,7 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
     const bool host = pre->group_start_host != nullptr;
     // The bounds, as near as the host copies let them be, and the pages of each group's prefix that some row sees.
     std::vector<Pages> seen;
+    Work work;
     if (host) {
         seen.resize(pre->n_groups);
         int max_group = 0, max_prefix = 0;
@@ -48,18 +64,36 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
             const int positions = prefix_positions(pre->prefix_len_host[g], pre->max_prefix);
             max_group = std::max(max_group, end - first);
             max_prefix = std::max(max_prefix, positions);
-            int lo = positions, hi = 0;
+            int lo = positions, hi = 0, n = 0;
+            int64_t all = 0;
             for (int b = first; b < end; b++) {
                 if (d.kv_len_host[b] == 0 || d.kv_start_host[b] >= positions) continue;
+                const int to = std::min(positions, d.kv_start_host[b] + d.kv_len_host[b]);
                 lo = std::min(lo, (int)d.kv_start_host[b]);
-                hi = std::max(hi, std::min(positions, d.kv_start_host[b] + d.kv_len_host[b]));
+                hi = std::max(hi, to);
+                all += to - d.kv_start_host[b];
+                n++;
             }
             seen[g] = {lo / 16, (hi + 15) / 16};
+            if (n > 1) {
+                work.saved += std::max<int64_t>(all - (hi - lo), 0);
+                work.longest = std::max(work.longest, hi - lo);
+                work.own -= all;
+            }
         }
+        for (int b = 0; b < d.n_seqs; b++) work.total += d.kv_len_host[b];
+        work.own += work.total;
         pre->max_group = max_group;
         pre->max_prefix = max_prefix;
+    } else if (pre->max_group > 1) {
+        // (half of what a row may have of its own)
+        const int64_t rows = std::max<int64_t>(std::min<int64_t>(d.n_seqs - pre->n_groups, (int64_t)pre->n_groups * (pre->max_group - 1)), 0);
+        work.longest = std::min(pre->max_prefix, d.max_kv_len);
+        work.saved = rows * work.longest;
+        work.own = (int64_t)d.n_seqs * std::min(pre->max_own, d.max_kv_len) / 2;
+        work.total = (int64_t)d.n_seqs * d.max_kv_len;
     }
-    if (pre->max_group < 2 || !pays(d)) {
+    if (!pays(d, work)) {
         pre->n_groups = 0;
         return;
     }

@@ -342,9 +342,12 @@ int gla_prefill_sinks(gla_ctx *ctx, const gla_prefill_args *args, int n_sinks);
  * those of the pages that lie wholly before it are read once for the group, through
  * its first row's pages (the table's row, or the cache's sequence), and multiplied
  * with the queries of all its rows as one matrix product, or by every row for itself
- * where the bounds say that this is faster. Rows in no group share nothing. The results
- * are gla_decode's but for rounding, which depends on the groups and the bounds: not
- * bit-identical to it, nor from one grouping to another.
+ * where the bounds, or the host copies, say that this is faster; what the copies show
+ * exactly the bounds can only guess, and bounds far above what comes make a call slower.
+ * Windows may begin or end inside the prefix or behind it: pages that no row sees are not
+ * read. Rows in no group share nothing. The results are gla_decode's but for rounding,
+ * which depends on the groups, the bounds and the copies: not bit-identical to it, nor
+ * from one grouping to another.
  *
  * Values that the host does not see are clamped into the batch and the storage as
  * gla_decode's are: group starts that fall, or pages that differ where they are said

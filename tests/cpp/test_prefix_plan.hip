@@ -130,6 +130,36 @@ int windows() {
     return 0;
 }
 
+// Whether the prefixes are read apart: what rows share counts, not what they have.
+int rule() {
+    const std::vector<int> lone64(64, 1);
+    for (bool q8 : {false, true})
+        for (bool host : {false, true}) {
+            const auto apart = [&](const Shape &s, const std::vector<int> &sizes, const std::vector<int32_t> &lens, int own,
+                                   int window = 0, int more = 0) {
+                Batch b(s, q8, sizes, lens, own, host, window, more);
+                b.plan();
+                return b.d.pre.n_groups > 0;
+            };
+            for (const Shape &s : kShapes) {
+                CHECK(apart(s, {64}, {8192}, 500), "64 rows behind 8,192");
+                CHECK(apart(s, {10, 4, 10}, {4096, 3000, 2000}, 100), "three groups");
+                CHECK(!apart(s, {4}, {128}, 20), "4 rows behind 128");
+                CHECK(!apart(s, {64}, {8}, 500), "less than a page");
+                CHECK(!apart(s, {2}, {512}, 2000, 0, 62), "a pair among 64 rows of 2,000");
+                CHECK(!apart(s, {1, 1, 1}, {4096, 4096, 4096}, 10), "rows alone behind prefixes");
+                if (host) CHECK(!apart(s, {8}, {32768}, 4200, 4096), "windows behind the prefix");
+            }
+            std::vector<int> sizes(64, 1);
+            sizes.push_back(2);
+            std::vector<int32_t> lens(64, 1024);
+            lens.push_back(64);
+            CHECK(!apart(kShapes[1], sizes, lens, 50), "lone rows and a pair that shares 64");
+            CHECK(apart(kShapes[1], std::vector<int>(32, 2), std::vector<int32_t>(32, 2048), 50), "32 pairs");
+        }
+    return 0;
+}
+
 // The pages of a split that hold a position of [lo, hi), shared out to the waves.
 int pages() {
     for (int from : {0, 8, 40})
@@ -156,7 +186,7 @@ int pages() {
 }  // namespace
 
 int main() {
-    if (tiles() || windows() || pages()) return 1;
+    if (tiles() || rule() || windows() || pages()) return 1;
     printf("plan ok\n");
     return 0;
 }
