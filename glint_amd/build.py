@@ -11,6 +11,7 @@ Outputs (in-tree, git-ignored, shipped with the tree to the GPU box):
     glint_amd/_build/test_host    its test program (tests/cpp/test_host.cpp; run by tests/test_host_cpp.py)
     glint_amd/_build/test_pages   the page rules of windows, on the host (tests/cpp/test_pages.hip)
     glint_amd/_build/test_prefix_plan  the plan of shared prefixes, on the host (tests/cpp/test_prefix_plan.hip)
+    glint_amd/_build/test_prefix_groups  which sequences are read together (tests/cpp/test_prefix_groups.cpp)
     oracle/liboracle.so           CPU oracle, built by oracle/Makefile (tests only)
 """
 from __future__ import annotations
@@ -32,6 +33,7 @@ HOST_LIB = PKG / "libglint_host.so"
 HOST_TEST = BUILD / "test_host"
 PAGES_TEST = BUILD / "test_pages"
 PLAN_TEST = BUILD / "test_prefix_plan"
+GROUPS_TEST = BUILD / "test_prefix_groups"
 ORACLE_DIR = ROOT / "oracle"
 ORACLE_LIB = ORACLE_DIR / "liboracle.so"
 
@@ -113,6 +115,14 @@ def _build_host_only(out: Path) -> Path:
     return out
 
 
+def build_groups_test() -> Path:
+    BUILD.mkdir(exist_ok=True)
+    tmp = GROUPS_TEST.with_suffix(".tmp")
+    _run(["g++", *HOST_FLAGS, "-o", str(tmp), str(ROOT / "tests" / "cpp" / "test_prefix_groups.cpp")])
+    os.replace(tmp, GROUPS_TEST)
+    return GROUPS_TEST
+
+
 def build_pages_test() -> Path:
     return _build_host_only(PAGES_TEST)
 
@@ -143,6 +153,7 @@ def build_all(jobs: int = 4) -> None:
     build_host_tests()
     build_pages_test()
     build_plan_test()
+    build_groups_test()
 
 
 if __name__ == "__main__":

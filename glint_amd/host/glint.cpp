@@ -1,5 +1,6 @@
 // glint.cpp -- the C++ host layer declared in glint.hpp, over include/glint_attn.h.
 #include "glint.hpp"
+#include "prefix_groups.hpp"
 
 #include <algorithm>
 #include <cstdarg>
@@ -788,37 +789,6 @@ Result<Source> source_of(const std::vector<const KvStore *> &stores, const char 
 
 }  // namespace
 
-namespace {
-
-// Neighbouring sequences of a paged batch that begin with the same pages.
-struct Groups {
-    std::vector<int32_t> start{0}, prefix;  // rows of group g: [start[g], start[g+1]); positions they share
-    int max_group = 0, max_prefix = 0;
-};
-Groups groups_of(const std::vector<DecodeSeq> &seqs, size_t layer) {
-    Groups g;
-    const auto table = [&](size_t b) -> const auto & { return seqs[b].kv->as_paged()->page_table(layer); };
-    for (size_t first = 0; first < seqs.size();) {
-        size_t end = first + 1, pages = 0;
-        for (; end < seqs.size(); end++) {
-            const auto &a = table(first), &b = table(end);
-            size_t n = std::min(end == first + 1 ? a.size() : pages, b.size());
-            n = (size_t)(std::mismatch(a.begin(), a.begin() + (ptrdiff_t)n, b.begin()).first - a.begin());
-            // (a row that shares less than half of what the others do begins another group)
-            if (n == 0 || 2 * n < pages) break;
-            pages = n;
-        }
-        g.start.push_back((int32_t)end);
-        g.prefix.push_back((int32_t)(pages * PAGE_SIZE));
-        g.max_group = std::max(g.max_group, (int)(end - first));
-        g.max_prefix = std::max(g.max_prefix, g.prefix.back());
-        first = end;
-    }
-    return g;
-}
-
-}  // namespace
-
 Result<std::vector<float>> GpuBackend::decode_batch(const std::vector<DecodeSeq> &seqs, const float *q, size_t layer,
                                                     const AttnShape &shape) {
     return decode(seqs, q, layer, shape, false);
@@ -903,21 +873,26 @@ Result<std::vector<float>> GpuBackend::decode(const std::vector<DecodeSeq> &seqs
     a.kv_len_host = len.data();
     Status s = Status();
     if (shared && S.paged) {
-        const Groups g = groups_of(seqs, layer);
+        std::vector<const std::vector<int32_t> *> tables;
+        for (const DecodeSeq &seq : seqs) tables.push_back(&seq.kv->as_paged()->page_table(layer));
+        const PrefixGroups g = group_prefixes(tables);
+        std::vector<int32_t> prefix;
+        for (int32_t pages : g.pages) prefix.push_back(pages * (int32_t)PAGE_SIZE);
         gla_decode_shared_args sa{};
         sa.decode = a;
-        sa.n_groups = (int)g.prefix.size();
+        sa.n_groups = (int)prefix.size();
         if (!(p = st.put(Staging::GROUP, g.start.data(), g.start.size() * 4))) return p.error();
         sa.group_start = (const int32_t *)p.value();
-        if (!(p = st.put(Staging::PREFIX, g.prefix.data(), g.prefix.size() * 4))) return p.error();
+        if (!(p = st.put(Staging::PREFIX, prefix.data(), prefix.size() * 4))) return p.error();
         sa.prefix_len = (const int32_t *)p.value();
-        sa.max_group = g.max_group;
-        sa.max_prefix_len = g.max_prefix;
-        for (size_t i = 0; i < g.prefix.size(); i++)
+        for (size_t i = 0; i < prefix.size(); i++) {
+            sa.max_group = std::max(sa.max_group, (int)(g.start[i + 1] - g.start[i]));
+            sa.max_prefix_len = std::max(sa.max_prefix_len, (int)prefix[i]);
             for (int32_t b = g.start[i]; b < g.start[i + 1]; b++)
-                sa.max_own_len = std::max(sa.max_own_len, start[b] + len[b] - g.prefix[i]);
+                sa.max_own_len = std::max(sa.max_own_len, start[b] + len[b] - prefix[i]);
+        }
         sa.group_start_host = g.start.data();
-        sa.prefix_len_host = g.prefix.data();
+        sa.prefix_len_host = prefix.data();
         s = check(gla_decode_shared(dev_->ctx(), &sa), "gla_decode_shared");
     } else if (shape.n_sinks) {
         s = check(gla_decode_sinks(dev_->ctx(), &a, (int)std::min<uint32_t>(shape.n_sinks, INT32_MAX)), "gla_decode_sinks");

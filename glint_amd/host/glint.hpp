@@ -560,8 +560,9 @@ class GpuBackend {
                                             const AttnShape &shape);
     // decode_batch of sequences that were forked from common prefixes
     // (PagedKvCache::fork_from): neighbours whose tables begin with the same
-    // pages are read together (gla_decode_shared), up to rounding the same.
-    // Order the batch by its prefixes. n_sinks is refused.
+    // pages are read together (gla_decode_shared), up to rounding the same, in
+    // the groups that save the most pages. Order the batch by its prefixes.
+    // n_sinks is refused.
     Result<std::vector<float>> decode_batch_shared(const std::vector<DecodeSeq> &seqs, const float *q, size_t layer,
                                                    const AttnShape &shape);
     // Causal prefill of a batch of prompt chunks whose K/V are written: q
