@@ -555,7 +555,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void decode_prefix_kerne
     } else if (w.z >= 0) {
         // KV heads fastest, so that with eight of them a head's groups share an XCD's L2 (24 rows of
         // 17-300 positions in 3 groups behind up to 4,096 at 16/8 heads, d = 256 63.2 -> 60.3 us, 322 ->
-        // 288 MB from HBM); the splits turned (windows with sinks are as fast either way).
+        // 288 MB from HBM, before row tiles were numbered across the groups: 252 MB); the splits turned
+        // (windows with sinks are as fast either way).
         const int hg = w.x / p.n_kv_heads, kvh = w.x - hg * p.n_kv_heads;
         split_item<D, GT, kStepsPerIter, CAP, kBehindPrefix>(p, kvh * p.n_hg + hg, turned(w.y, mix.oy, w.z), w.z);
     }

@@ -1010,7 +1010,7 @@ __global__ __launch_bounds__(kWaves * 64) void decode_q8_mfma_kernel(const Q8Par
     q8_item<D, MODE>(p, slots, b, wg, blockIdx.x);
 }
 
-// decode_q8_mfma_kernel behind prefixes, with their workgroups among its own.
+// decode_q8_mfma_kernel behind prefixes, with their workgroups before its own.
 template <int D, int NT, bool CAP>
 __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void decode_q8_prefix_kernel(
     const Q8Params p, const prefix::PrefixParams pp, const prefix::Mixed mix) {
@@ -1232,7 +1232,7 @@ int launch_decode_q8(gla_ctx *ctx, const DecodeLaunch &d) {
     const int per_cu = D == 64 ? resident_wgs<64>() : (D == 128 ? resident_wgs<128>() : resident_wgs<256>());
     const int64_t slots = (int64_t)std::max(ctx->n_cu, 1) * std::max(per_cu, 1);
     // (behind a prefix, whose kernel fills the device beside it, all heads a wave: 64 rows of
-    // 64-1,000 positions behind 8,192 at 32/8 heads, d = 128, 31 us with two, 16 with four)
+    // 64-1,000 positions behind 8,192 at 32/8 heads, d = 128, the rows' part alone 31 us with two, 16 with four)
     int hpw = decode_mode(d) == kBehindPrefix ? std::min(kGT, group) : choose_hpw(group, wg_total, d.n_kv_heads, slots);
     if (const char *env = getenv("GLA_Q8_HEADS_PER_WAVE")) {
         const int v = atoi(env);

@@ -19,13 +19,13 @@
 // scores are the operand of the second product as they are, and a row's maximum is its
 // four lanes'.
 //
-// What bounds it, these workgroups alone: Q8_0 vector issue (65% of the cycles, matrix 21%, in
-// turn): 64 rows at 32/8 heads, d = 128, behind 8,192 positions 39 us, 220 TFLOP/s of the
-// attention's products; f32 the matrix rate from some 48 rows a group on (the same call 91 us,
-// 94 of the 138 TFLOP/s that a library product reaches), HBM and the tiles' re-reads before (24
-// rows in 3 groups behind up to 4,096 positions at 16/8, d = 256 37 us, 180 MB, 4.8 TB/s). With the
-// rows' own (64-1,000 positions behind 8,192 Q8_0 49 us, 17-300 in the 3 groups 54 us, 288 MB,
-// 5.4 TB/s).
+// What bounds it (whole calls, on clocks that have settled; the first some hundred after a pause
+// are up to a tenth slower): Q8_0 vector issue (68% of the cycles, matrix 19%, in turn): 64 rows of
+// 8-64 positions behind 8,192 at 32/8 heads, d = 128 43.4 us, 198 TFLOP/s of the attention's
+// products, of 64-1,000 47.0; f32 the matrix rate from some 48 rows a group on (64 rows of 8-64 86.8
+// us, 99 of the 138 TFLOP/s that a library product reaches), HBM and the tiles' re-reads before (24
+// rows of 17-300 in 3 groups behind up to 4,096 at 16/8, d = 256 56.6 us, 252 MB, 4.5 TB/s).
+// Two figures of a rule beside the code are of one build and box, in turn, which need not be this one.
 #pragma once
 
 #include <math.h>
@@ -154,7 +154,8 @@ struct Share {
 };
 __device__ __forceinline__ Share share_of(const PrefixParams &p, const Place &w, int tile_rows) {
     Share s;
-    // (64 rows in two groups behind up to 8,192 Q8_0 positions at 32/8 heads, d = 128, row tiles in one order / turned 76 / 63 us)
+    // (row tiles in one order / turned, two groups behind up to 8,192 and 4,096 Q8_0 positions: 64 rows at 32/8 heads,
+    // d = 128 56.9 / 56.2 us, 40 at 16/8, d = 256 37.3 / 36.0; 64 f32 rows in four at 16/8 111.6 / 113.3)
     const int at = w.x / p.n_kv_heads;  // (the heads run fastest: a head's row tiles share an L2)
     s.kvh = w.x - at * p.n_kv_heads;
     const Tile t = tile_of(p, tile_rows, turned(at, p.columns / p.n_kv_heads, w.y));
@@ -854,8 +855,8 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
 }
 
 // The one launch of a batch behind its prefixes: the prefixes' workgroups, then, where those
-// leave room, those of the rows' own pages. us a call, in two launches / in one, with both kinds
-// in turn / in one: Q8_0 behind 8,192 positions at 32/8 heads, d = 128, 64 rows of 64-1,000 64.0 /
+// leave room, those of the rows' own pages. us a call, in two launches / in one / in one with both
+// kinds in turn: Q8_0 behind 8,192 positions at 32/8 heads, d = 128, 64 rows of 64-1,000 64.0 /
 // 60.3 / 73.2, of 8-64 53.3 / 52.1 / 61.9, 4 rows 24.3 / 18.6 / 20.0; 64 rows in 4 groups behind
 // 2,048 35.3 / 28.1 / 35.9 (the prefixes' are the longest, and all of them are resident).
 struct Mixed {
