@@ -86,12 +86,13 @@ void plan_prefix(const gla_ctx *ctx, DecodeLaunch *launch) {
         pre->max_group = max_group;
         pre->max_prefix = max_prefix;
     } else if (pre->max_group > 1) {
-        // (half of what a row may have of its own)
-        const int64_t rows = std::max<int64_t>(std::min<int64_t>(d.n_seqs - pre->n_groups, (int64_t)pre->n_groups * (pre->max_group - 1)), 0);
+        // (what the rows of groups have of their own is between nothing and the bound of every replay: it is
+        // left out, so that it does not hide what they share)
+        const int64_t most = std::min<int64_t>(d.n_seqs, (int64_t)pre->n_groups * pre->max_group);
         work.longest = std::min(pre->max_prefix, d.max_kv_len);
-        work.saved = rows * work.longest;
-        work.own = (int64_t)d.n_seqs * std::min(pre->max_own, d.max_kv_len) / 2;
-        work.total = (int64_t)d.n_seqs * d.max_kv_len;
+        work.saved = std::min<int64_t>(d.n_seqs - pre->n_groups, (int64_t)pre->n_groups * (pre->max_group - 1)) * work.longest;
+        work.own = (d.n_seqs - most) * std::min(pre->max_own, d.max_kv_len);
+        work.total = work.own + most * work.longest;
     }
     if (!pays(d, work)) {
         pre->n_groups = 0;

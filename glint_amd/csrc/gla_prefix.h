@@ -25,7 +25,7 @@
 // products, of 64-1,000 47.0; f32 the matrix rate from some 48 rows a group on (64 rows of 8-64 86.8
 // us, 99 of the 138 TFLOP/s that a library product reaches), HBM and the tiles' re-reads before (24
 // rows of 17-300 in 3 groups behind up to 4,096 at 16/8, d = 256 56.6 us, 252 MB, 4.5 TB/s).
-// Two figures of a rule beside the code are of one build and box, in turn, which need not be this one.
+// Two figures of a rule beside the code were taken in turn on one build, not always this one.
 #pragma once
 
 #include <math.h>
@@ -214,8 +214,9 @@ __device__ __forceinline__ Seen seen_of(const Row (&rows)[NT]) {
 
 // A wave's pages again where the rows' windows leave some of the split's unseen; whether they did. A
 // page that no row of the tile sees is not read, but for a wave's first, which is asked for before the
-// windows are there; a split of which none sees any (`to` <= `from` then) leaves nothing. us a call, all pages / these, 32/8 heads, d = 128: 8 rows in windows of 4,096 that begin
-// behind a prefix of 32,768 f32 95.7 / 61.2, Q8_0 48 / 35; 16 in 1,024 that begin in 16,384 54 / 45 and 42 / 29.
+// windows are there; a split of which none sees any (`to` <= `from` then) leaves nothing. us a call,
+// all pages / these, 32/8 heads, d = 128: 8 rows in windows of 4,096 that begin behind a prefix of
+// 32,768 f32 95.7 / 61.2, Q8_0 48 / 35; 16 in 1,024 that begin in 16,384 54 / 45 and 42 / 29.
 template <bool EVEN>
 __device__ __forceinline__ bool only_seen(Share &s, const Seen &seen, int wave, Pages &mine) {
     const int from = s.from, to = s.to;
@@ -324,9 +325,9 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
                 v[r][T] = *reinterpret_cast<const floatx4 *>(at + voff + r * p.kv.row_stride + T * 256);
     };
     // (the first page is on its way while the queries are; a wave without pages reads the group's first)
-    Pages mine = wave_pages<false>(sh.from, sh.to, wave);
-    int ids = page_ids(p, sh.member, mine);
-    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(mine.n, 1) - 1)); };
+    Pages here = wave_pages<false>(sh.from, sh.to, wave);
+    int ids = page_ids(p, sh.member, here);
+    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(here.n, 1) - 1)); };
     load_k(id(0));
     load_v(id(0));
 
@@ -347,13 +348,13 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
             reinterpret_cast<floatx4 *>(lds)[(nt * KK + kk) * 64 + lane] = x;
         }
     const Seen seen = seen_of<NT>(rows);
-    if (only_seen<false>(sh, seen, wave, mine)) {
+    if (only_seen<false>(sh, seen, wave, here)) {
         if (sh.from >= sh.to) return;  // (all waves: they have the same rows)
-        ids = page_ids(p, sh.member, mine);
+        ids = page_ids(p, sh.member, here);
         load_k(id(0));
         load_v(id(0));
     }
-    const int n = mine.n;
+    const int n = here.n;
     __syncthreads();
     const floatx4 *qs = reinterpret_cast<const floatx4 *>(lds);
 
@@ -371,7 +372,7 @@ __device__ __forceinline__ void f32_item(const PrefixParams &p, const Place &w, 
 
     {
         for (int i = 0; i < n; i++) {
-            const int first = (mine.first + i) * 16;
+            const int first = (here.first + i) * 16;
             const bool inside = seen.all(first, 16);
             int qi = lane;
             asm volatile("" : "+v"(qi));  // (read anew for every page: kept, they would crowd the other registers)
@@ -605,9 +606,9 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
         load_words(at + vsoff, vs[P]);
     };
     // (the first pages are on their way while the queries are split; a wave without pages reads the group's first)
-    Pages mine = wave_pages<true>(sh.from, sh.to, wave);
-    int ids = page_ids(p, sh.member, mine);
-    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(mine.n, 1) - 1)); };
+    Pages here = wave_pages<true>(sh.from, sh.to, wave);
+    int ids = page_ids(p, sh.member, here);
+    const auto id = [&](int i) { return (int64_t)__builtin_amdgcn_readlane(ids, min(i, max(here.n, 1) - 1)); };
     const auto load_first = [&]() __attribute__((always_inline)) {
         load_k(0, id(0));
         load_k(1, id(1));
@@ -675,12 +676,12 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
         }
     }
     const Seen seen = seen_of<NT>(rows);
-    if (only_seen<true>(sh, seen, wave, mine)) {
+    if (only_seen<true>(sh, seen, wave, here)) {
         if (sh.from >= sh.to) return;  // (all waves: they have the same rows)
-        ids = page_ids(p, sh.member, mine);
+        ids = page_ids(p, sh.member, here);
         load_first();
     }
-    const int n = mine.n;
+    const int n = here.n;
     __syncthreads();
     const half8 *qs = reinterpret_cast<const half8 *>(lds);
     float sm[NT];  // undoes a query's scale
@@ -725,7 +726,7 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
         unit = ldexpf(1.0f, ve - 14);
 
         for (int i = 0; i < n; i += 2) {
-            const int first = (mine.first + i) * 16;
+            const int first = (here.first + i) * 16;
             const bool two = i + 1 < n;
             const bool plain = two && !vinf && seen.all(first, 32);  // every row sees all, and no scale is infinite
             int qi = lane;

@@ -150,6 +150,14 @@ int rule() {
                 CHECK(!apart(s, {1, 1, 1}, {4096, 4096, 4096}, 10), "rows alone behind prefixes");
                 if (host) CHECK(!apart(s, {8}, {32768}, 4200, 4096), "windows behind the prefix");
             }
+            if (!host) {  // bounds of every replay: rows whose own part may grow far beyond what they share
+                for (const Shape &s : kShapes) {
+                    Batch b(s, q8, {32}, {2048}, 20, false);
+                    b.d.pre.max_own = b.d.max_kv_len = 32768;
+                    b.plan();
+                    CHECK(b.d.pre.n_groups == 1, "a captured call of 32 rows behind 2,048");
+                }
+            }
             std::vector<int> sizes(64, 1);
             sizes.push_back(2);
             std::vector<int32_t> lens(64, 1024);
