@@ -566,6 +566,12 @@ __device__ __forceinline__ void step_qk(const RawK<D> &cur, int step, const Step
 
 #pragma unroll
     for (int i = 0; i < 4; i++) pr[i] = fast_exp2(fmaf(c.ph ? s1[i] : s0[i], c.sm, off));
+    // kvs - m is rounded to the unit of m, which from 2^22 on would shift the probabilities by as much
+    // (a wave-uniform branch): they overflowed their pieces, and waves whose kvs differ disagreed.
+    if (__ballot(fabsf(m_new * c.sm) >= 0x1p22f)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) pr[i] = fast_exp2(fmaf(c.ph ? s1[i] : s0[i], c.sm, -m_new * c.sm)) * fast_exp2(c.kvs);
+    }
     st.lsum = st.lsum * alpha + ((pr[0] + pr[1]) + (pr[2] + pr[3]));
 
     if (__ballot(alpha != 1.0f)) {

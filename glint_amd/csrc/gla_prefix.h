@@ -76,8 +76,8 @@ __device__ __forceinline__ T rare(T x) {
 // `lazy`: p is then at most 2^lazy, and most pages rescale nothing. f32 holds any p alike.
 // Q8_0's pieces of p are halves, of which a row that lags wastes the top: p times the largest
 // scale is below 2^14 for p = 1, as in the decode of single rows, and below 2^15.5 for the
-// largest p (a half holds 65,504). With 8 and 2^6 instead 2^-18 of the largest scale was off by
-// 1e-3, and the calls were 1-2% faster.
+// largest p (where m's unit rounds m + 1.5 to m + 2, at most 2^16 (1 - 2^-11), a half's largest).
+// With 8 and 2^6 instead 2^-18 of the largest scale was off by 1e-3, and the calls were 1-2% faster.
 constexpr float kLazy = 8.0f, kLazyQ8 = 1.5f;
 // Moves m to the maximum of the row's four lanes where that passes it; what the sums are to be multiplied by.
 __device__ __forceinline__ float moved(float &m, float mine, float lazy) {
@@ -689,16 +689,19 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
     for (int nt = 0; nt < NT; nt++) sm[nt] = ldexpf(1.0f, qexp[nt * 16 + lrow] - 14);
 
     floatx4 o[ND][NT];  // O of d = t*16 + kg*4 + r
-    float m[NT], lpart[NT];
+    float m[NT], moff[NT], lpart[NT];  // p 2^vexp = 2^(s + moff)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         m[nt] = -INFINITY;
-        lpart[nt] = 0.0f;
+        moff[nt] = lpart[nt] = 0.0f;
 #pragma unroll
         for (int t = 0; t < ND; t++) o[t][nt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    float unit = 1.0f;  // of O and of the sums of P
+    // O and the sums of P are in units of 2^-vexp. Where m's own unit is so large that vexp - m would be
+    // rounded to it (an m that keeps p below 2^2 all the same), in units of 1: products of f16 scales fit.
+    int vexp = 0;
+    const auto exp_of = [&](float m) { return fabsf(m) < 0x1p22f ? vexp : min(vexp, 0); };
     if (n > 0) {
         // P' = p * vscale * 2^vexp is below 2^14 for p = 1
         const int units = n * (D / 16);  // 16 bytes of V scales each
@@ -722,8 +725,7 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
         const bool vinf = __ballot(vmax == INFINITY) != 0;
         if (vinf) vmax = largest(std::true_type{});
         const int ve = __builtin_amdgcn_readfirstlane(pow2_exp(vmax));
-        const float vexp = (float)(14 - ve);
-        unit = ldexpf(1.0f, ve - 14);
+        vexp = 14 - ve;
 
         for (int i = 0; i < n; i += 2) {
             const int first = (here.first + i) * 16;
@@ -789,14 +791,15 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
                 const float mine = c * fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                                              fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
                 if (__ballot(mine > m[nt] + kLazyQ8)) {
-                    const float f = moved(m[nt], mine, kLazyQ8);
+                    const int was = exp_of(m[nt]);
+                    const float f = ldexpf(moved(m[nt], mine, kLazyQ8), exp_of(m[nt]) - was);
+                    moff[nt] = m[nt] == -INFINITY ? 0.0f : (float)exp_of(m[nt]) - m[nt];
                     lpart[nt] *= f;
 #pragma unroll
                     for (int t = 0; t < ND; t++) o[t][nt] *= f;
                 }
-                const float off = m[nt] == -INFINITY ? 0.0f : vexp - m[nt];
 #pragma unroll
-                for (int j = 0; j < 8; j++) pr[nt][j] = fast_exp2(fmaf(x[j >> 2][j & 3], c, off));
+                for (int j = 0; j < 8; j++) pr[nt][j] = fast_exp2(fmaf(x[j >> 2][j & 3], c, moff[nt]));
                 lpart[nt] += ((pr[nt][0] + pr[nt][1]) + (pr[nt][2] + pr[nt][3])) +
                              ((pr[nt][4] + pr[nt][5]) + (pr[nt][6] + pr[nt][7]));
             }
@@ -844,14 +847,14 @@ __device__ __forceinline__ void q8_item(const PrefixParams &p, const Place &w, f
     }
     float l[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) l[nt] = sum_rows4(lpart[nt]) * unit;
+    for (int nt = 0; nt < NT; nt++) l[nt] = ldexpf(sum_rows4(lpart[nt]), -exp_of(m[nt]));
     merge_and_store<D, NT>(p, sh, w.y, m, l, lds, mls, row_at, [&](float *slot, const float (&f)[NT]) __attribute__((always_inline)) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int t = 0; t < ND; t++)
                 *reinterpret_cast<floatx4 *>(slot + (nt * 16 + lrow) * out_row(D) + t * 16 + kg * 4) =
-                    o[t][nt] * (unit * f[nt]);
+                    o[t][nt] * ldexpf(f[nt], -exp_of(m[nt]));
     });
 }
 
